@@ -1,0 +1,546 @@
+"""The operators of the paged key-value cache, as measurable cases.
+
+A case is a dict of plain values: `op` names the operator and the rest its
+sizes.  `prepare` makes what a serving program has in hand before the call (on
+the GPU), `run` makes one call: with `own` false in plain torch operations in
+32 bits, with `own` true through the package's entry points.  `work` counts
+what the call cannot do without, `exact` gives the results from the
+definitions in 64 bits.
+
+Layouts: keys [pages, kv_heads, page, dim], values [pages, kv_heads, dim,
+page] (transposed within a page), summaries int8 [pages, kv_heads, dim] with
+scales float32 [pages, kv_heads], a block table int32 [requests, columns] of
+page ids.  A summary's codes are whole numbers by definition, so codes and
+scales are returned as they are held.
+"""
+
+from __future__ import annotations
+
+import math
+import random
+
+import numpy as np
+import torch
+
+own = False
+
+DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def listed():
+    return [
+        # one decoding step's bookkeeping for a small batch (latency)
+        dict(name="plan_decode", op="plan", requests=48, longest=8_192, new=1, page=64),
+        # a large scheduler's step: decoding requests, prompts and idle ones
+        # mixed, small pages
+        dict(name="plan_mixed", op="plan", requests=1_024, longest=16_384, new=63, page=16),
+        # one token for each request of a decoding batch (latency; scattered
+        # writes), a page now and then completed
+        dict(name="append_decode", op="append", requests=64, longest=4_096, new=1, page=64,
+             kv_heads=8, dim=128, dtype="bf16"),
+        # prompts of odd lengths written at once
+        dict(name="append_prompts", op="append", requests=5, longest=20_000, new=4_001, page=16,
+             kv_heads=4, dim=80, dtype="f16"),
+        # the blocks of long conversations scored for each one's new token
+        dict(name="select_decode", op="select", requests=16, longest=131_072, new=1, page=64,
+             kv_heads=8, group=4, dim=128, dtype="bf16", blocks=64),
+        # the same for the tokens of three prompt chunks at the end of long texts
+        dict(name="select_prompts", op="select", requests=3, longest=32_768, new=1_500, page=64,
+             kv_heads=4, group=8, dim=128, dtype="bf16", blocks=16),
+        # an interactive request with a short history (latency)
+        dict(name="attend_one", op="attend", requests=1, longest=777, new=1, page=16, kv_heads=8,
+             group=4, dim=128, dtype="bf16", blocks=0),
+        # a serving batch of ragged lengths (HBM-bound)
+        dict(name="attend_batch", op="attend", requests=64, longest=8_192, new=1, page=64,
+             kv_heads=8, group=4, dim=128, dtype="bf16", blocks=0),
+        # one request with a very long history: all parallelism is its length
+        dict(name="attend_long", op="attend", requests=1, longest=262_144, new=1, page=128,
+             kv_heads=8, group=8, dim=128, dtype="f16", blocks=0),
+        # odd heads and a head size that fills no tile
+        dict(name="attend_odd", op="attend", requests=13, longest=5_001, new=1, page=32, kv_heads=3,
+             group=5, dim=80, dtype="f16", blocks=0),
+        # long conversations that attend to 32 selected blocks
+        dict(name="blocks_decode", op="attend", requests=32, longest=65_536, new=1, page=64,
+             kv_heads=8, group=4, dim=128, dtype="bf16", blocks=32),
+        # every token of three prompt chunks attends to 16 blocks of its own
+        dict(name="blocks_prompts", op="attend", requests=3, longest=32_768, new=1_500, page=64,
+             kv_heads=4, group=8, dim=128, dtype="bf16", blocks=16),
+    ]
+
+
+def _log(rng: random.Random, lo: int, hi: int) -> int:
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng: random.Random):
+    """One more case of the listed ones' ranges (sizes log-uniform, most of
+    them odd, none dearer than the largest listed one)."""
+    op = rng.choice(["plan", "append", "select", "attend", "attend", "blocks", "blocks"])
+    if op == "plan":
+        return dict(op=op, requests=_log(rng, 8, 1_024), longest=_log(rng, 64, 16_384),
+                    new=rng.choice([1, _log(rng, 2, 64)]), page=rng.choice([16, 32, 64, 128]))
+    heads = dict(kv_heads=_log(rng, 1, 8), dim=rng.choice([64, 80, 96, 128, 128, 128, 192, 256]),
+                 dtype=rng.choice(["bf16", "f16"]))
+    page = rng.choice([16, 32, 64, 128])
+    group = rng.choice([1, 2, 3, 4, 5, 7, 8, 12, 16])
+    width = heads["kv_heads"] * heads["dim"]
+    if op == "append":
+        requests = _log(rng, 1, 64)
+        return dict(op=op, requests=requests, longest=_log(rng, 512, 8_192),
+                    new=rng.choice([1, _log(rng, 2, max(2, min(4_000, (1 << 24) // (width * requests))))]),
+                    page=page, **heads)
+    n = _log(rng, 4, 64)
+    if op == "select":
+        requests = _log(rng, 1, 16)
+        longest = _log(rng, 1_024, min(131_072, (1 << 28) // (requests * width) * page))
+        new = rng.choice([1, _log(rng, 2, 1_500)])
+        # the plain form holds a summary for each (token, block, head)
+        new = max(1, min(new, longest, (1 << 30) // (requests * width * (longest // page + 1))))
+        return dict(op=op, requests=requests, longest=longest, new=new, page=page, group=group,
+                    blocks=n, **heads)
+    if op == "attend":
+        longest = _log(rng, 100, 131_072)
+        requests = _log(rng, 1, max(1, min(64, (1 << 28) // (longest * width))))
+        return dict(op=op, requests=requests, longest=longest, new=1, page=page, group=group,
+                    blocks=0, **heads)
+    longest = _log(rng, 2_048, 65_536)
+    requests = _log(rng, 1, max(1, min(32, (1 << 28) // (longest * width))))
+    most = max(1, min(1_500, longest, (1 << 30) // (requests * width * n * page)))
+    return dict(op="attend", requests=requests, longest=longest,
+                new=rng.choice([1, _log(rng, 1, most)]), page=page, group=group, blocks=n, **heads)
+
+
+# ---- sizes: the same for every seed, so that work() knows them -------------------
+
+
+def _lengths(case):
+    """Tokens of each request after the step: the first is the longest, the
+    others between an eighth of it and all of it; in a batch of 8 and more the
+    last place is idle (a padded batch)."""
+    r = random.Random(case["requests"] * 1_000_003 + case["longest"])
+    n = [max(1, int(case["longest"] * (1.0 - 0.875 * r.random()))) for _ in range(case["requests"])]
+    n[0] = case["longest"]
+    if case["requests"] >= 8:
+        n[-1] = 0
+    return n
+
+
+def _counts(case):
+    """New tokens of each request in this step (of its length)."""
+    r = random.Random(case["requests"] * 7_919 + case["new"])
+    if case["new"] == 1:
+        return [min(1, n) for n in _lengths(case)]
+    mixed = [r.choice([case["new"], r.randint(0, case["new"]), 1]) for _ in range(case["requests"])]
+    mixed[0] = case["new"]
+    return [min(n, m) for n, m in zip(_lengths(case), mixed)]
+
+
+def _columns(case):
+    return -(-case["longest"] // case["page"])
+
+
+def _visible(case):
+    """(positions of all new tokens, as one array)"""
+    return np.concatenate([np.arange(n - m, n) for n, m in zip(_lengths(case), _counts(case))])
+
+
+# ---- inputs ------------------------------------------------------------------------
+
+
+def _ints(a, kind=torch.int32):
+    return torch.as_tensor(np.asarray(a), dtype=kind, device="cuda")
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(int(seed))
+    s = dict(case=case)
+    lengths, counts = _lengths(case), _counts(case)
+    requests, page, cols = case["requests"], case["page"], _columns(case)
+    held = [-(-n // page) for n in lengths]
+    pool = sum(held) + requests + 8
+    ids = torch.randperm(pool, generator=g, device="cuda").to(torch.int32)
+
+    if case["op"] == "plan":
+        # the table before the step; the free list holds what the step may
+        # take, and then some
+        past = [n - m for n, m in zip(lengths, counts)]
+        before = [-(-n // page) for n in past]
+        at = np.full((requests, cols), -1, np.int64)
+        used = 0
+        for r, n in enumerate(before):
+            at[r, :n] = np.arange(used, used + n)
+            used += n
+        at = _ints(at, torch.int64)
+        s["table"] = torch.where(at >= 0, ids[at.clamp(min=0)], -1)
+        s["free"] = ids[used:].contiguous()
+        s["past"], s["new"] = _ints(past), _ints(counts)
+        s["cursor"] = torch.zeros((1,), dtype=torch.int32, device="cuda")
+        # a step's batch is padded to a multiple of 64 tokens
+        s["tokens"] = max(64, -(-sum(counts) // 64) * 64)
+        return s
+
+    kv, dim, dtype = case["kv_heads"], case["dim"], DTYPES[case["dtype"]]
+    at = np.full((requests, cols), -1, np.int64)
+    used = 0
+    for r, n in enumerate(held):
+        at[r, :n] = np.arange(used, used + n)
+        used += n
+    at = _ints(at, torch.int64)
+    s["table"] = torch.where(at >= 0, ids[at.clamp(min=0)], -1)
+    who = np.repeat(np.arange(requests), counts)
+    where = _visible(case)
+    tokens = len(who)
+    if case["new"] == 1 and lengths[-1] == 0:  # the idle place stays in the batch
+        who, where = np.append(who, requests - 1), np.append(where, -1)
+        tokens += 1
+    s["requests"], s["positions"] = _ints(who), _ints(where)
+    s["longest"] = case["longest"]
+    group = case.get("group", 1)
+    heads = kv * group
+
+    # subjects: a stretch of text is about one of 64, and so are its keys; the
+    # queries of neighbouring tokens look for one of them
+    subject = 0.6 * torch.randn((64, kv, dim), generator=g, device="cuda")
+    of_page = torch.randint(0, 64, (pool,), generator=g, device="cuda")
+
+    # queries, keys and values of the new tokens are slices of one projection
+    fused = torch.randn((tokens, (heads + 2 * kv) * dim), generator=g, device="cuda")
+    looks = torch.randint(0, 64, (requests, cols * page // 48 + 1), generator=g, device="cuda")
+    spot = looks[s["requests"].long(), s["positions"].clamp(min=0).long() // 48]
+    fused[:, :heads * dim] += subject[spot].repeat_interleave(group, 1).reshape(tokens, -1)
+    fused = fused.to(dtype)
+    s["q"] = fused[:, :heads * dim].view(tokens, heads, dim)
+    s["k"] = fused[:, heads * dim:(heads + kv) * dim].view(tokens, kv, dim)
+    s["v"] = fused[:, (heads + kv) * dim:].view(tokens, kv, dim)
+
+    if case["op"] == "select":
+        # a block's summary: its subject, with what is left of the rest
+        m = subject[of_page] + 0.1 * torch.randn((pool, kv, dim), generator=g, device="cuda")
+        peak = m.abs().amax(2, keepdim=True)
+        s["summaries"] = torch.round(m * (127.0 / peak)).to(torch.int8)
+        s["scales"] = (peak.squeeze(2) / 127.0).contiguous()
+    else:
+        s["keys"] = torch.randn((pool, kv, page, dim), generator=g, device="cuda",
+                                dtype=torch.float32 if pool * kv * page * dim < 1 << 28 else dtype)
+        s["keys"] += subject[of_page].unsqueeze(2).to(s["keys"].dtype)
+        s["keys"] = s["keys"].to(dtype)
+        s["values"] = torch.randn((pool, kv, dim, page), generator=g, device="cuda", dtype=dtype)
+        s["summaries"] = torch.zeros((pool, kv, dim), dtype=torch.int8, device="cuda")
+        s["scales"] = torch.zeros((pool, kv), dtype=torch.float32, device="cuda")
+    if case["op"] == "append":
+        pos = s["positions"].long()
+        pid = s["table"][s["requests"].long(), pos.clamp(min=0) // page].long()
+        s["slots"] = torch.where(pos >= 0, pid * page + pos % page, -1)
+    if case.get("blocks") and case["op"] == "attend":
+        # lists as a score of slowly changing queries gives them: the first
+        # block, the token's own, and what its neighbours mostly take too
+        near = torch.randn((requests, cols * page // 48 + 1, kv, cols), generator=g, device="cuda")
+        score = near[s["requests"].long(), s["positions"].clamp(min=0).long() // 48]
+        score += 0.2 * torch.randn(score.shape, generator=g, device="cuda")
+        own_block = torch.div(s["positions"], page, rounding_mode="floor").view(-1, 1, 1)
+        col = torch.arange(cols, device="cuda")
+        score = torch.where((col == 0) | (col == own_block), 1e9, score)
+        score = torch.where(col <= own_block, score, -math.inf)
+        n = case["blocks"]
+        best, at = torch.topk(score, min(n, cols), dim=2)
+        at = torch.where(best > -math.inf, at, cols).sort(2).values
+        at = torch.nn.functional.pad(at, (0, n - at.shape[2]), value=cols)
+        s["blocks"] = torch.where(at < cols, at, -1).to(torch.int32)
+    return s
+
+
+# ---- the operators in plain operations -------------------------------------------
+
+
+def _plan(s):
+    c, past, new, table, free = s["case"], s["past"].long(), s["new"].long(), s["table"], s["free"]
+    page, cols = c["page"], table.shape[1]
+    have = (past + page - 1) // page
+    want = (past + new + page - 1) // page
+    valid = (past >= 0) & (new >= 0) & (want <= cols)
+    need = torch.where(valid, want - have, 0)
+    upto = torch.cumsum(need, 0)
+    left = len(free) - s["cursor"].long()
+    admitted = valid & ((need == 0) | (upto <= left))
+    first = s["cursor"].long() + upto - need  # of a request's new pages in the free list
+    starts = torch.nn.functional.pad(torch.cumsum(new.clamp(min=0), 0), (1, 0))
+    t = torch.arange(s["tokens"], device=past.device)
+    real = t < starts[-1]
+    r = torch.searchsorted(starts[1:], t, right=True).clamp(max=len(past) - 1)
+    pos = past[r] + t - starts[r]
+    col = (pos // page).clamp(0, cols - 1)
+    fresh = (first[r] + col - have[r]).clamp(0, len(free) - 1)
+    pid = torch.where(col < have[r], table[r, col], free[fresh]).long()
+    ok = real & admitted[r]
+    slots = torch.where(ok & (pid >= 0), pid * page + pos % page, -1)
+    cc = torch.arange(cols, device=past.device)
+    ours = admitted[:, None] & (cc >= have[:, None]) & (cc < want[:, None])
+    at = (first[:, None] + cc - have[:, None]).clamp(0, len(free) - 1)
+    table.copy_(torch.where(ours, free[at], table))
+    taken = torch.where(admitted, upto, 0).amax()
+    return {"slots": slots, "requests": torch.where(real, r, -1).int(),
+            "positions": torch.where(ok, pos, -1).int(), "starts": starts.int(),
+            "lengths": torch.where(admitted, past + new, past).int(),
+            "cursor": (s["cursor"] + taken).int(), "table": table}
+
+
+def _inverse(x):
+    """127 / x, rounded once (a number over a tensor multiplies by a rounded
+    reciprocal), 0 where x holds nothing."""
+    return torch.where(x > 1e-30, torch.full_like(x, 127.0) / x, 0.0)
+
+
+def _append(s):
+    keys, values, slots = s["keys"], s["values"], s["slots"]
+    page = keys.shape[2]
+    there = slots >= 0
+    at = slots[there]
+    pid, off = at // page, at % page
+    keys[pid, :, off] = s["k"][there]
+    values[pid, :, :, off] = s["v"][there]
+    full = pid[off == page - 1]
+    x = keys[full].float()
+    top = x.abs().amax((2, 3))
+    codes = torch.round(x * _inverse(top)[..., None, None])
+    total = codes.sum(2)
+    peak = total.abs().amax(2)
+    s["summaries"][full] = torch.round(total * _inverse(peak)[..., None]).to(torch.int8)
+    s["scales"][full] = torch.where(top > 1e-30, top * (peak / (16129.0 * page)), 0.0)
+    return {"keys": keys, "values": values, "summaries": s["summaries"], "scales": s["scales"]}
+
+
+def _select(s):
+    c, q, table = s["case"], s["q"].float(), s["table"]
+    tokens, kv, n, cols = len(q), c["kv_heads"], c["blocks"], table.shape[1]
+    q = q.view(tokens, kv, -1, c["dim"])
+    top = q.abs().amax((2, 3))
+    codes = torch.round(q * _inverse(top)[..., None, None]).sum(2)
+    codes = torch.round(codes * _inverse(codes.abs().amax(2, keepdim=True)))
+    pages = table[s["requests"].long()].clamp(min=0).long()
+    # products and sums of whole numbers below 2^24: exact in float32
+    dot = torch.matmul(s["summaries"][pages].float().transpose(1, 2), codes.unsqueeze(3)).squeeze(3)
+    score = dot * s["scales"][pages].transpose(1, 2)
+    own_block = torch.div(s["positions"], c["page"], rounding_mode="floor").view(-1, 1, 1)
+    col = torch.arange(cols, device=q.device)
+    score = torch.where((col == 0) | (col == own_block), math.inf, score)
+    score = torch.where(col <= own_block, score, -math.inf)
+    best, at = torch.sort(score, dim=2, descending=True, stable=True)
+    at = torch.where(best > -math.inf, at, cols)[..., :n].sort(2).values
+    at = torch.nn.functional.pad(at, (0, n - at.shape[2]), value=cols)
+    return {"blocks": torch.where(at < cols, at, -1).int()}
+
+
+def _attend(s):
+    c, table, keys, values = s["case"], s["table"], s["keys"], s["values"]
+    q = s["q"].float()
+    tokens, kv, dim, page = len(q), c["kv_heads"], c["dim"], c["page"]
+    q = q.view(tokens, kv, -1, dim)
+    head = torch.arange(kv, device=q.device).view(1, kv, 1)
+    listed_ = s["blocks"].long() if c["blocks"] else \
+        torch.arange(table.shape[1], device=q.device).expand(tokens, kv, -1)
+    who = s["requests"].long().view(-1, 1, 1)
+    pages = torch.where(listed_ >= 0, table[who, listed_.clamp(min=0)].long(), -1)
+    k = keys[pages.clamp(min=0), head].float().view(tokens, kv, -1, dim)
+    v = values[pages.clamp(min=0), head].float().transpose(3, 4).reshape(tokens, kv, -1, dim)
+    at = listed_.unsqueeze(3) * page + torch.arange(page, device=q.device)
+    seen = (pages >= 0).unsqueeze(3) & (at <= s["positions"].view(-1, 1, 1, 1))
+    seen = seen.view(tokens, kv, 1, -1)
+    score = torch.matmul(q, k.transpose(2, 3)) * (1.0 / math.sqrt(dim))
+    score = torch.where(seen, score, -math.inf)
+    top = score.amax(3, keepdim=True)
+    p = torch.exp(score - torch.where(top == -math.inf, 0.0, top))
+    total = p.sum(3, keepdim=True)
+    out = torch.matmul(p, torch.where(seen.transpose(2, 3), v, 0.0))
+    out = torch.where(total > 0, out / total, 0.0)
+    lse = (top + torch.log(total)).view(tokens, -1)
+    return {"out": out.view(tokens, -1, dim).to(s["q"].dtype), "lse": lse}
+
+
+# ---- one call ------------------------------------------------------------------------
+
+
+def _cache(s):
+    """The cache object that a program keeps beside its tensors."""
+    if "cache" not in s:
+        import mlxvs_amd
+
+        zeros = s["summaries"]
+        kv, dim = zeros.shape[1:]
+        keys = s.get("keys")
+        if keys is None:  # select() reads summaries only
+            keys = torch.empty((len(zeros), kv, s["case"]["page"], dim), device=zeros.device,
+                               dtype=s["q"].dtype)
+        values = s.get("values")
+        if values is None:
+            values = keys.view(len(zeros), kv, dim, s["case"]["page"])
+        s["cache"] = mlxvs_amd.PagedKVCache(keys, values, zeros, s["scales"])
+    return s["cache"]
+
+
+def run(state):
+    c = state["case"]
+    op = c["op"]
+    if not own:
+        return {"plan": _plan, "append": _append, "select": _select, "attend": _attend}[op](state)
+    if op == "plan":
+        import mlxvs_amd
+
+        p = state["plan"] = mlxvs_amd.kv_plan(
+            state["past"], state["new"], state["table"], state["free"], state["cursor"], c["page"],
+            state["tokens"], out=state.get("plan"))
+        return {"slots": p.slots, "requests": p.requests, "positions": p.positions,
+                "starts": p.starts, "lengths": p.lengths, "cursor": p.cursor,
+                "table": state["table"]}
+    cache = _cache(state)
+    if op == "append":
+        cache.append(state["k"], state["v"], state["slots"])
+        return {"keys": cache.keys, "values": cache.values, "summaries": cache.summaries,
+                "scales": cache.scales}
+    if op == "select":
+        return {"blocks": cache.select(state["q"], state["table"], state["requests"],
+                                       state["positions"], c["blocks"])}
+    out, lse = cache.attend(state["q"], state["table"], state["requests"], state["positions"],
+                            blocks=state.get("blocks"), longest=state["longest"], lse=True)
+    return {"out": out, "lse": lse}
+
+
+# ---- what a call cannot do without -------------------------------------------------------
+
+
+def work(case):
+    requests, page, cols = case["requests"], case["page"], _columns(case)
+    lengths, counts, where = _lengths(case), _counts(case), _visible(case)
+    tokens = len(where)
+    if case["op"] == "plan":
+        padded = max(64, -(-tokens // 64) * 64)
+        fresh = sum(-(-n // page) - -(-(n - m) // page) for n, m in zip(lengths, counts))
+        return {"bytes": requests * 16 + padded * 16 + fresh * 8, "flops": 0}
+    kv, dim = case["kv_heads"], case["dim"]
+    if case["op"] == "append":
+        full = int((where % page == page - 1).sum())
+        older = sum((n - m) % page for n, m in zip(lengths, counts) if n // page > (n - m) // page)
+        return {"bytes": 8 * tokens * kv * dim + 8 * tokens + 2 * older * kv * dim
+                + full * kv * (dim + 4), "flops": 0}
+    group, n = case["group"], case["blocks"]
+    rows = tokens * kv * group * dim
+    if case["op"] == "select":
+        complete = sum((length - 1) // page for length in lengths if length)
+        pairs = float((where // page).sum())
+        return {"bytes": complete * kv * (dim + 4) + 2 * rows + tokens * kv * n * 4,
+                "flops": 2.0 * pairs * kv * dim}
+    if n:
+        seen = np.minimum(where + 1, np.minimum(n - 1, where // page) * page + where % page + 1)
+        read = min(sum(lengths), int(seen.sum()))
+    else:
+        seen, read = where + 1, sum(lengths)
+    return {"bytes": 4 * read * kv * dim + 4 * rows + 4 * tokens * kv * (group + n) + 4 * requests * cols,
+            "flops": 4.0 * float(seen.sum()) * kv * group * dim}
+
+
+# ---- from the definitions, in 64 bits ------------------------------------------------------
+
+
+def _codes(x):
+    """Whole numbers for the vectors x [..., m, d] (float32): each value over
+    the largest of all m, in 127ths, summed over m, and the sums in 127ths of
+    their largest.  (NumPy: the float32 quotients are part of the definition.)"""
+    f = np.float32
+    top = np.abs(x).max((-1, -2))
+    with np.errstate(divide="ignore", invalid="ignore"):
+        inv = np.where(top > f(1e-30), f(127) / top, f(0)).astype(f)
+        total = np.rint(x * inv[..., None, None]).astype(np.int64).sum(-2)
+        peak = np.abs(total).max(-1)
+        inv = np.where(peak > 0, f(127) / peak.astype(f), f(0)).astype(f)
+    return np.rint(total.astype(f) * inv[..., None]).astype(np.int64), top, peak
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    page = case["page"]
+    table = s["table"].cpu().numpy().copy()
+    if case["op"] == "plan":
+        past, new, free = (s[k].cpu().numpy().tolist() for k in ("past", "new", "free"))
+        slots, who, where, starts, cursor = [], [], [], [0], 0
+        for r, (p, m) in enumerate(zip(past, new)):
+            while -(-p // page) < -(-(p + m) // page) and m:
+                table[r, -(-p // page)] = free[cursor]
+                cursor += 1
+                step = min(m, -(-p // page) * page + page - p)
+                slots += [int(table[r, i // page]) * page + i % page for i in range(p, p + step)]
+                where += range(p, p + step)
+                p, m = p + step, m - step
+            slots += [int(table[r, i // page]) * page + i % page for i in range(p, p + m)]
+            where += range(p, p + m)
+            starts.append(len(slots))
+            who += [r] * (starts[-1] - starts[-2])
+        rest = [-1] * (s["tokens"] - len(slots))
+        return {"slots": np.array(slots + rest, np.int64), "requests": np.array(who + rest, np.int32),
+                "positions": np.array(where + rest, np.int32), "starts": np.array(starts, np.int32),
+                "lengths": np.array(_lengths(case), np.int32), "cursor": np.array([cursor], np.int32),
+                "table": table}
+    if case["op"] == "append":
+        keys, values = s["keys"].clone(), s["values"].clone()
+        codes, scales = s["summaries"].clone(), s["scales"].double()
+        for t, slot in enumerate(s["slots"].tolist()):
+            if slot >= 0:
+                keys[slot // page, :, slot % page] = s["k"][t]
+                values[slot // page, :, :, slot % page] = s["v"][t]
+        full = sorted({slot // page for slot in s["slots"].tolist() if slot >= 0 and slot % page == page - 1})
+        if full:
+            m, top, peak = _codes(keys[full].float().cpu().numpy())
+            codes[full] = torch.as_tensor(m, device="cuda").to(torch.int8)
+            scales[full] = torch.as_tensor(top.astype(np.float64) * peak / (16129.0 * page),
+                                           device="cuda")
+        return {"keys": keys, "values": values, "summaries": codes, "scales": scales}
+    kv, dim, group, n = case["kv_heads"], case["dim"], case["group"], case["blocks"]
+    who, where = s["requests"].tolist(), s["positions"].tolist()
+    if case["op"] == "select":
+        m, scales = s["summaries"].cpu().numpy(), s["scales"].cpu().numpy()
+        q = s["q"].float().cpu().numpy().reshape(len(who), kv, group, dim)
+        codes = _codes(q)[0]
+        out = np.full((len(who), kv, n), -1, np.int32)
+        held = {r: (m[table[r][table[r] >= 0]].astype(np.float32), scales[table[r][table[r] >= 0]])
+                for r in set(who)}
+        for t, (r, p) in enumerate(zip(who, where)):
+            b = p // page
+            if p < 0:
+                continue
+            for h in range(kv):
+                # (whole numbers below 2^24: the float32 product is exact)
+                sc = (held[r][0][:b + 1, h] @ codes[t, h].astype(np.float32)) * held[r][1][:b + 1, h]
+                sc[[0, b]] = np.inf
+                best = np.lexsort((np.arange(b + 1), -sc))[:n]
+                out[t, h, :len(best)] = np.sort(best)
+        return {"blocks": out}
+    q = s["q"].double().view(len(who), kv, group, dim)
+    out = torch.zeros((len(who), kv, group, dim), dtype=torch.float64, device="cuda")
+    lse = torch.full((len(who), kv, group), -math.inf, dtype=torch.float64, device="cuda")
+    heads = torch.arange(kv, device="cuda")
+    pages = s["table"].long()
+    if not n:
+        for t, (r, p) in enumerate(zip(who, where)):
+            if p < 0:
+                continue
+            at = pages[r, :p // page + 1]
+            for h in range(kv):
+                k = s["keys"][at, h].double().reshape(-1, dim)[:p + 1]
+                v = s["values"][at, h].double().transpose(1, 2).reshape(-1, dim)[:p + 1]
+                a = (q[t, h] @ k.T) / math.sqrt(dim)
+                lse[t, h] = torch.logsumexp(a, 1)
+                out[t, h] = torch.softmax(a, 1) @ v
+        return {"out": out.view(len(who), -1, dim), "lse": lse.view(len(who), -1)}
+    step = max(1, (1 << 27) // (kv * n * page * dim))
+    for lo in range(0, len(who), step):
+        b = s["blocks"][lo:lo + step].long()
+        p = s["positions"][lo:lo + step].long().view(-1, 1, 1, 1)
+        at = pages[s["requests"][lo:lo + step].long().view(-1, 1, 1), b.clamp(min=0)].clamp(min=0)
+        k = s["keys"][at, heads.view(1, -1, 1)].double().flatten(2, 3)
+        v = s["values"][at, heads.view(1, -1, 1)].double().transpose(3, 4).flatten(2, 3)
+        off = b.unsqueeze(3) * page + torch.arange(page, device="cuda")
+        hidden = ((b.unsqueeze(3) < 0) | (off > p)).flatten(2).unsqueeze(2)
+        a = torch.matmul(q[lo:lo + step], k.transpose(2, 3).contiguous()) / math.sqrt(dim)
+        a = a.masked_fill(hidden, -math.inf)
+        lse[lo:lo + step] = torch.logsumexp(a, 3)
+        out[lo:lo + step] = torch.matmul(torch.softmax(a, 3).nan_to_num(0.0), v)
+    return {"out": out.view(len(who), -1, dim), "lse": lse.view(len(who), -1)}
