@@ -278,7 +278,7 @@ def _plan(s):
     ours = admitted[:, None] & (cc >= have[:, None]) & (cc < want[:, None])
     at = (first[:, None] + cc - have[:, None]).clamp(0, len(free) - 1)
     table.copy_(torch.where(ours, free[at], table))
-    taken = torch.where(admitted, upto, 0).amax()
+    taken = torch.where(admitted & (need > 0), upto, 0).amax()
     return {"slots": slots, "requests": torch.where(real, r, -1).int(),
             "positions": torch.where(ok, pos, -1).int(), "starts": starts.int(),
             "lengths": torch.where(admitted, past + new, past).int(),
