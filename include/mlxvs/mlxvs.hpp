@@ -232,6 +232,83 @@ MLXVS_API void topk_merge_device(const float* scores, int64_t nq, int64_t t, con
                                  const float* best, int id_offset, bool first, int k,
                                  int32_t* out_ids, float* out_scores, void* stream = nullptr);
 
+/** Element type of a paged key-value cache. */
+enum class KvType { Float16 = 0, BFloat16 = 1 };
+
+/** A paged key-value cache in device memory; layouts and limits as
+ * mlxvs_kv_cache in mlxvs_c.h. */
+struct KvCache {
+  void* keys = nullptr;
+  void* values = nullptr;
+  int8_t* summaries = nullptr;
+  float* scales = nullptr;
+  int64_t pages = 0;
+  int32_t heads = 0;
+  int32_t page_size = 0;
+  int32_t dim = 0;
+  KvType type = KvType::Float16;
+};
+
+/** Queries of tokens and where they stand, as mlxvs_kv_queries. */
+struct KvQueries {
+  const void* q = nullptr;
+  int64_t token_stride = 0;
+  int64_t head_stride = 0;
+  int64_t tokens = 0;
+  int32_t q_heads = 0;
+  int32_t columns = 0;
+  const int32_t* table = nullptr;
+  int64_t table_stride = 0;
+  int64_t requests = 0;
+  const int32_t* token_request = nullptr;
+  const int32_t* positions = nullptr;
+};
+
+/** What kv_plan_device reads and writes, as mlxvs_kv_plan_device's arguments. */
+struct KvPlan {
+  const int32_t* past = nullptr;
+  const int32_t* fresh = nullptr;
+  int64_t requests = 0;
+  int32_t* table = nullptr;
+  int64_t table_stride = 0;
+  int32_t columns = 0;
+  const int32_t* free_pages = nullptr;
+  int64_t free_count = 0;
+  const int32_t* cursor = nullptr;
+  int32_t page_size = 0;
+  int64_t tokens = 0;
+  int64_t* slots = nullptr;
+  int32_t* token_request = nullptr;
+  int32_t* positions = nullptr;
+  int32_t* starts = nullptr;
+  int32_t* lengths = nullptr;
+  int32_t* first = nullptr;
+  int32_t* cursor_out = nullptr;
+};
+
+/** A step's block tables and slot maps (mlxvs_kv_plan_device); enqueues only. */
+MLXVS_API void kv_plan_device(const KvPlan& plan, void* stream = nullptr);
+/** Writes tokens into their slots and summarises the pages they complete
+ * (mlxvs_kv_append_device); enqueues only. */
+MLXVS_API void kv_append_device(const KvCache& cache, const void* k, int64_t k_token_stride,
+                                int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                                int64_t v_head_stride, const int64_t* slots, int64_t tokens,
+                                void* stream = nullptr);
+/** The n best blocks of each token and kv head (mlxvs_kv_select_device);
+ * enqueues only. */
+MLXVS_API void kv_select_device(const KvCache& cache, const KvQueries& queries, int n, int first,
+                                int last, int32_t* blocks, void* workspace,
+                                int64_t workspace_bytes, void* stream = nullptr);
+MLXVS_API int64_t kv_select_workspace(const KvCache& cache, const KvQueries& queries, int n);
+/** Attention over the cache, or over listed blocks of it
+ * (mlxvs_kv_attend_device); enqueues only. */
+MLXVS_API void kv_attend_device(const KvCache& cache, const KvQueries& queries,
+                                const int32_t* blocks, int n, float scale, int64_t longest,
+                                void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                                void* stream = nullptr);
+MLXVS_API int64_t kv_attend_workspace(const KvCache& cache, const KvQueries& queries, int n,
+                                      int64_t longest);
+
 /** Frees the per-device workspace kept between calls. */
 MLXVS_API void release_workspace();
 

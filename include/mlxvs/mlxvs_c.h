@@ -473,6 +473,188 @@ MLXVS_C_API int mlxvs_pairwise_knn(
     float* distances,
     void* stream);
 
+/* ---- the paged key-value cache (extensions) -------------------------------
+ *
+ * A cache of attention keys and values in pages of page_size tokens, and
+ * retrieval over it: a step's block tables and slots from the requests'
+ * lengths (mlxvs_kv_plan_device), the write of its tokens
+ * (mlxvs_kv_append_device), the blocks that a cheap score selects for each of
+ * them (mlxvs_kv_select_device) and their attention, over every block or the
+ * selected ones (mlxvs_kv_attend_device).  All arrays are device memory; the
+ * calls enqueue their work on `stream`, allocate nothing, keep nothing and can
+ * be captured into graphs.  Calls that depend on one another go to one stream
+ * or are ordered by the caller; a workspace serves one call at a time.
+ */
+
+/** Element type of keys, values, queries and outputs. */
+typedef enum {
+  MLXVS_KV_F16 = 0,  /* IEEE binary16 */
+  MLXVS_KV_BF16 = 1, /* bfloat16 */
+} mlxvs_kv_type;
+
+/**
+ * A cache.  page_size: a power of two from 16 to 256; dim: a multiple of 8, at
+ * most 256.  keys [pages][heads][page_size][dim]; values
+ * [pages][heads][dim][page_size], transposed within a page; both 16-byte
+ * aligned.  summaries int8 [pages][heads][dim] with scales float32
+ * [pages][heads] describe complete pages for mlxvs_kv_select_device: code x
+ * scale is the mean of a page's keys (null, both: the cache keeps none).
+ */
+typedef struct {
+  void* keys;
+  void* values;
+  int8_t* summaries;
+  float* scales;
+  int64_t pages;
+  int32_t heads;
+  int32_t page_size;
+  int32_t dim;
+  mlxvs_kv_type type;
+} mlxvs_kv_cache;
+
+/**
+ * Queries of `tokens` tokens and where they stand: q [tokens][q_heads][dim] of
+ * the cache's type, strides in values (multiples of 8; the values of a head
+ * are contiguous; 16-byte aligned), q_heads a multiple of the cache's heads
+ * (query head i reads kv head i / (q_heads / heads)).  table int32
+ * [requests][columns], rows table_stride apart: the page of each block of a
+ * request.  token_request[t] and positions[t] int32: token t belongs to that
+ * request and sees its keys 0 .. position, itself among them; a token with
+ * position -1 (or a request out of range) sees nothing.  A page id outside
+ * [0, pages) stands for a block that is absent.
+ */
+typedef struct {
+  const void* q;
+  int64_t token_stride;
+  int64_t head_stride;
+  int64_t tokens;
+  int32_t q_heads;
+  int32_t columns;
+  const int32_t* table;
+  int64_t table_stride;
+  int64_t requests;
+  const int32_t* token_request;
+  const int32_t* positions;
+} mlxvs_kv_queries;
+
+/**
+ * A step's block tables and slot maps.  Request r holds past[r] tokens and gets
+ * fresh[r] more (0: none).  Its table row has the pages of the tokens it holds;
+ * the pages that the new ones need are taken from free_pages (page ids, used
+ * from entry cursor[0] on) in the requests' order and written into the row.  A
+ * request whose blocks exceed `columns` or whose pages the free list does not
+ * reach is not admitted, nor is any later one that needs pages in the second
+ * case: it takes none.  Written, all int32 but slots:
+ *   slots int64 [tokens], token_request [tokens], positions [tokens]: the new
+ *     tokens in the requests' order: page x page_size + offset, the request,
+ *     the position; slot and position -1 for a request that was not admitted,
+ *     all three -1 past the last token (tokens: the batch's size; tokens past
+ *     it get no entry);
+ *   starts [requests + 1]: each request's first token in the batch;
+ *   lengths [requests]: tokens held after the step;
+ *   first [requests]: a request's first entry of free_pages, -1 if it was not
+ *     admitted (0 if it needs none);
+ *   cursor_out[0]: the first unused entry after the step (may not be cursor).
+ * columns x page_size must be below 2^31.
+ */
+MLXVS_C_API int mlxvs_kv_plan_device(
+    const int32_t* past,
+    const int32_t* fresh,
+    int64_t requests,
+    int32_t* table,
+    int64_t table_stride,
+    int32_t columns,
+    const int32_t* free_pages,
+    int64_t free_count,
+    const int32_t* cursor,
+    int32_t page_size,
+    int64_t tokens,
+    int64_t* slots,
+    int32_t* token_request,
+    int32_t* positions,
+    int32_t* starts,
+    int32_t* lengths,
+    int32_t* first,
+    int32_t* cursor_out,
+    void* stream);
+
+/**
+ * Writes keys and values of tokens into their slots (page x page_size +
+ * offset; outside the cache: skipped), k and v [tokens][heads][dim] with
+ * token and head strides in values (multiples of 8, 16-byte aligned), and then
+ * the summaries of the pages whose last slot is among them (over all their
+ * slots), if the cache keeps summaries.
+ */
+MLXVS_C_API int mlxvs_kv_append_device(
+    const mlxvs_kv_cache* cache,
+    const void* k,
+    int64_t k_token_stride,
+    int64_t k_head_stride,
+    const void* v,
+    int64_t v_token_stride,
+    int64_t v_head_stride,
+    const int64_t* slots,
+    int64_t tokens,
+    void* stream);
+
+/**
+ * The n best blocks of each token and kv head: blocks int32
+ * [tokens][heads][n], ascending, -1 after the last.  Candidates are the blocks
+ * up to the token's own; its own and the last - 1 before it (last >= 1) and the
+ * first `first` of the request are always taken (first + last <= n <= 256),
+ * the others by score, the lowest block among equal ones.  A score is the int8
+ * dot product of a block's summary with the codes of the query (the sum over
+ * the group's heads), times the summary's scale: the same list from every
+ * implementation.  workspace: mlxvs_kv_select_workspace bytes (may be 0).
+ */
+MLXVS_C_API int mlxvs_kv_select_device(
+    const mlxvs_kv_cache* cache,
+    const mlxvs_kv_queries* queries,
+    int32_t n,
+    int32_t first,
+    int32_t last,
+    int32_t* blocks,
+    void* workspace,
+    int64_t workspace_bytes,
+    void* stream);
+
+/** Bytes of workspace of a call with these arguments, -1 if they are invalid
+ * (mlxvs_last_error says why). */
+MLXVS_C_API int64_t mlxvs_kv_select_workspace(const mlxvs_kv_cache* cache,
+                                              const mlxvs_kv_queries* queries, int32_t n);
+
+/**
+ * Attention of the tokens over the cache: out [tokens][q_heads][dim] (the
+ * cache's type, contiguous) and, unless null, lse float32 [tokens][q_heads],
+ * the logarithm of the sum of exponentials.  blocks null: over all of a
+ * request's blocks; else int32 [tokens][heads][n] (n <= 256): over the listed
+ * ones, an entry outside the table or past the token's own block showing
+ * nothing (one listed twice counts twice).  Keys past the token's position
+ * never count, whatever their places hold.  A token that sees nothing: zeros,
+ * lse -inf.  scale > 0 multiplies the scores.  longest: tokens that the longest
+ * request holds, as far as the caller knows (0: all that the table can hold);
+ * it guides how work is split and never what is computed.  workspace:
+ * mlxvs_kv_attend_workspace bytes (may be 0).
+ */
+MLXVS_C_API int mlxvs_kv_attend_device(
+    const mlxvs_kv_cache* cache,
+    const mlxvs_kv_queries* queries,
+    const int32_t* blocks,
+    int32_t n,
+    float scale,
+    int64_t longest,
+    void* out,
+    float* lse,
+    void* workspace,
+    int64_t workspace_bytes,
+    void* stream);
+
+/** Bytes of workspace of a call with these arguments (n 0: over all blocks), -1
+ * if they are invalid. */
+MLXVS_C_API int64_t mlxvs_kv_attend_workspace(const mlxvs_kv_cache* cache,
+                                              const mlxvs_kv_queries* queries, int32_t n,
+                                              int64_t longest);
+
 /**
  * Releases the workspace the library keeps on the current device between
  * calls (it is grown on demand and reused).  Safe to call at any time when

@@ -26,8 +26,10 @@ import numpy as np
 
 __all__ = [
     "IvfFlatIndex",
+    "KvPlan",
     "Metric",
     "NearestNeighbors",
+    "PagedKVCache",
     "all_neighbors",
     "brute_force_knn",
     "brute_force_knn_filtered",
@@ -36,6 +38,7 @@ __all__ = [
     "ivf_flat_extend",
     "ivf_flat_search",
     "kmeans_predict",
+    "kv_plan",
     "library_path",
     "pairwise_knn",
     "topk_merge",
@@ -89,6 +92,11 @@ def _load():
         "mlxvs_hamming_knn_on_stream": [vp, i64, vp, i64, i32, i32, vp, vp, vp],
         "mlxvs_kmeans_predict_on_stream": [vp, i64, vp, i64, i32, i32, i32, vp, vp],
         "mlxvs_topk_merge_on_stream": [vp, i64, i64, vp, vp, i32, i32, i32, vp, vp, vp],
+        "mlxvs_kv_plan_device": [vp, vp, i64, vp, i64, i32, vp, i64, vp, i32, i64, vp, vp, vp, vp,
+                                 vp, vp, vp, vp],
+        "mlxvs_kv_append_device": [vp, vp, i64, i64, vp, i64, i64, vp, i64, vp],
+        "mlxvs_kv_select_device": [vp, vp, i32, i32, i32, vp, vp, i64, vp],
+        "mlxvs_kv_attend_device": [vp, vp, vp, i32, ctypes.c_float, i64, vp, vp, vp, i64, vp],
         "mlxvs_release_workspace": [],
         "mlxvs_profile": [ctypes.c_int],
         "mlxvs_profile_report": [ctypes.c_char_p, i64],
@@ -97,6 +105,11 @@ def _load():
         fn = getattr(lib, name)
         fn.argtypes = args
         fn.restype = ctypes.c_int
+    for name, args in (("mlxvs_kv_select_workspace", [vp, vp, i32]),
+                       ("mlxvs_kv_attend_workspace", [vp, vp, i32, i64])):
+        fn = getattr(lib, name)
+        fn.argtypes = args
+        fn.restype = i64
     lib.mlxvs_last_error.restype = ctypes.c_char_p
     lib.mlxvs_last_error.argtypes = []
     lib.mlxvs_version.restype = ctypes.c_char_p
@@ -553,3 +566,13 @@ def ivf_flat_search_device(centers_ptr, lists, data_ptr, n, indices_ptr, offsets
     _check(_L().mlxvs_ivf_flat_search_device(
         centers_ptr, lists, data_ptr, n, indices_ptr, offsets_ptr, d, int(_metric(metric)),
         queries_ptr, nq, int(k), int(n_probes), ids_ptr, dist_ptr, stream))
+
+
+def __getattr__(name):
+    # the paged key-value cache works on torch tensors: torch is imported only
+    # where it is used
+    if name in ("KvPlan", "PagedKVCache", "kv_plan"):
+        from mlxvs_amd import kvcache
+
+        return getattr(kvcache, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -54,6 +54,19 @@ mlxvs::Metric to_metric(mlxvs_metric m) {
   throw std::invalid_argument("[mlxvs] unknown metric.");
 }
 
+mlxvs::KvCache kv_cache(const mlxvs_kv_cache* c) {
+  require(c != nullptr, "cache must not be NULL.");
+  require(c->type == MLXVS_KV_F16 || c->type == MLXVS_KV_BF16, "unknown type of a cache.");
+  return {c->keys,  c->values,    c->summaries, c->scales, c->pages,
+          c->heads, c->page_size, c->dim,       (mlxvs::KvType)c->type};
+}
+
+mlxvs::KvQueries kv_queries(const mlxvs_kv_queries* q) {
+  require(q != nullptr, "queries must not be NULL.");
+  return {q->q,     q->token_stride, q->head_stride, q->tokens,        q->q_heads,  q->columns,
+          q->table, q->table_stride, q->requests,    q->token_request, q->positions};
+}
+
 void copy_out(const mlxvs::Neighbors& r, int32_t* ids, float* distances) {
   const size_t count = (size_t)r.nq * (size_t)r.k;
   for (size_t i = 0; i < count; ++i) ids[i] = r.ids[i];
@@ -316,6 +329,65 @@ int mlxvs_topk_merge_on_stream(const float* scores, int64_t nq, int64_t t, const
     if (out_scores && !r.second.empty())
       std::memcpy(out_scores, r.second.data(), r.second.size() * sizeof(float));
   });
+}
+
+int mlxvs_kv_plan_device(const int32_t* past, const int32_t* fresh, int64_t requests,
+                         int32_t* table, int64_t table_stride, int32_t columns,
+                         const int32_t* free_pages, int64_t free_count, const int32_t* cursor,
+                         int32_t page_size, int64_t tokens, int64_t* slots,
+                         int32_t* token_request, int32_t* positions, int32_t* starts,
+                         int32_t* lengths, int32_t* first, int32_t* cursor_out, void* stream) {
+  return guarded([&] {
+    mlxvs::kv_plan_device({past, fresh, requests, table, table_stride, columns, free_pages,
+                           free_count, cursor, page_size, tokens, slots, token_request, positions,
+                           starts, lengths, first, cursor_out},
+                          stream);
+  });
+}
+
+int mlxvs_kv_append_device(const mlxvs_kv_cache* cache, const void* k, int64_t k_token_stride,
+                           int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                           int64_t v_head_stride, const int64_t* slots, int64_t tokens,
+                           void* stream) {
+  return guarded([&] {
+    mlxvs::kv_append_device(kv_cache(cache), k, k_token_stride, k_head_stride, v, v_token_stride,
+                            v_head_stride, slots, tokens, stream);
+  });
+}
+
+int mlxvs_kv_select_device(const mlxvs_kv_cache* cache, const mlxvs_kv_queries* queries,
+                           int32_t n, int32_t first, int32_t last, int32_t* blocks,
+                           void* workspace, int64_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    mlxvs::kv_select_device(kv_cache(cache), kv_queries(queries), n, first, last, blocks,
+                            workspace, workspace_bytes, stream);
+  });
+}
+
+int64_t mlxvs_kv_select_workspace(const mlxvs_kv_cache* cache, const mlxvs_kv_queries* queries,
+                                  int32_t n) {
+  int64_t bytes = -1;
+  guarded([&] { bytes = mlxvs::kv_select_workspace(kv_cache(cache), kv_queries(queries), n); });
+  return bytes;
+}
+
+int mlxvs_kv_attend_device(const mlxvs_kv_cache* cache, const mlxvs_kv_queries* queries,
+                           const int32_t* blocks, int32_t n, float scale, int64_t longest,
+                           void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                           void* stream) {
+  return guarded([&] {
+    mlxvs::kv_attend_device(kv_cache(cache), kv_queries(queries), blocks, n, scale, longest, out,
+                            lse, workspace, workspace_bytes, stream);
+  });
+}
+
+int64_t mlxvs_kv_attend_workspace(const mlxvs_kv_cache* cache, const mlxvs_kv_queries* queries,
+                                  int32_t n, int64_t longest) {
+  int64_t bytes = -1;
+  guarded([&] {
+    bytes = mlxvs::kv_attend_workspace(kv_cache(cache), kv_queries(queries), n, longest);
+  });
+  return bytes;
 }
 
 int mlxvs_profile(int enable) {

@@ -30,6 +30,7 @@
 #include "knn_kernels.h"
 #include "mlxvs/mlxvs.hpp"
 #include "plan.h"
+#include "stage.h"
 
 namespace mlxvs {
 namespace {
@@ -2119,6 +2120,14 @@ void release_workspace() {
 }
 
 const char* version() { return "0.16.1"; }
+
+namespace detail {
+void launch_stage(hipStream_t s, const char* stage, hipError_t (*run)(const void*, hipStream_t),
+                  const void* args) {
+  launch(s, stage, [&] { return run(args, s); });
+}
+void need_device() { current_device(); }
+}  // namespace detail
 
 void profile(bool enable) {
   std::lock_guard<std::mutex> g(g_prof_mutex);

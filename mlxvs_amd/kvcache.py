@@ -1,0 +1,322 @@
+"""A paged key-value cache with retrieval over it, on torch tensors.
+
+A model that answers from a long context searches its own cache: the keys are
+the rows, a new token's query the query, blocks of keys the lists.  One step of
+a serving loop:
+
+    plan = kv_plan(past, new, table, free_pages, cursor, page_size, tokens)
+    cache.append(k, v, plan.slots)
+    blocks = cache.select(q, table, plan.requests, plan.positions, 32)
+    out = cache.attend(q, table, plan.requests, plan.positions, blocks=blocks)
+
+(or ``attend`` without ``blocks``: over everything).  Tensors are on one GPU;
+every call runs on torch's current stream there, returns as soon as its work is
+enqueued and can be captured into a graph.  The work is done by libmlxvs_c.so
+(``mlxvs_kv_*`` in include/mlxvs/mlxvs_c.h); without it the calls raise
+ImportError.  Extensions: the reference has no counterpart.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import NamedTuple, Optional
+
+import torch
+
+from mlxvs_amd import _L, _check
+
+_TYPES = {torch.float16: 0, torch.bfloat16: 1}
+
+
+class _Cache(ctypes.Structure):
+    _fields_ = [("keys", ctypes.c_void_p), ("values", ctypes.c_void_p),
+                ("summaries", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+                ("pages", ctypes.c_int64), ("heads", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("dim", ctypes.c_int32), ("type", ctypes.c_int)]
+
+
+class _Queries(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("token_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64), ("tokens", ctypes.c_int64),
+                ("q_heads", ctypes.c_int32), ("columns", ctypes.c_int32),
+                ("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("requests", ctypes.c_int64), ("token_request", ctypes.c_void_p),
+                ("positions", ctypes.c_void_p)]
+
+
+def _need(ok: bool, op: str, what: str) -> None:
+    if not ok:
+        raise ValueError(f"[mlxvs::{op}] {what}")
+
+
+def _ints(x, name: str, op: str, device, dtype=torch.int32, size: Optional[int] = None):
+    """The pointer of a contiguous 1-D tensor of whole numbers."""
+    if not (isinstance(x, torch.Tensor) and x.dtype == dtype and x.dim() == 1
+            and x.is_contiguous() and x.device == device
+            and (size is None or x.shape[0] == size)):
+        of = "" if size is None else f" of {size}"
+        raise ValueError(f"[mlxvs::{op}] {name} must be a contiguous 1-D {dtype} tensor{of} on "
+                         f"{device}.")
+    return x.data_ptr()
+
+
+def _table(table, op: str, device):
+    _need(isinstance(table, torch.Tensor) and table.dtype == torch.int32 and table.dim() == 2
+          and table.device == device and (table.shape[1] <= 1 or table.stride(1) == 1), op,
+          f"table must be an int32 [requests, columns] tensor on {device} with contiguous rows.")
+    return table.data_ptr(), max(table.stride(0), table.shape[1])
+
+
+class _On:
+    """The current stream of a tensor's device, made current meanwhile."""
+
+    def __init__(self, device):
+        self.guard = torch.cuda.device(device) if device.index != torch.cuda.current_device() \
+            else None
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return torch.cuda.current_stream().cuda_stream or None
+
+    def __exit__(self, *a):
+        if self.guard is not None:
+            self.guard.__exit__(*a)
+
+
+class KvPlan(NamedTuple):
+    """A step's bookkeeping (kv_plan): int32 tensors but ``slots`` (int64)."""
+
+    slots: torch.Tensor      # [tokens] page x page_size + offset, -1: none
+    requests: torch.Tensor   # [tokens] the token's request, -1 past the last token
+    positions: torch.Tensor  # [tokens] its position in the request, -1: none
+    starts: torch.Tensor     # [requests + 1] each request's first token
+    lengths: torch.Tensor    # [requests] tokens held after the step
+    first: torch.Tensor      # [requests] its first entry of free_pages, -1: not admitted
+    cursor: torch.Tensor     # [1] the first unused entry of free_pages
+
+
+def kv_plan(past, new, table, free_pages, cursor, page_size, tokens, *, out=None) -> KvPlan:
+    """Block tables and slot maps of a step, from the requests' lengths.
+
+    ``past`` / ``new`` int32 [requests]: tokens that a request holds and gets.
+    ``table`` int32 [requests, columns]: its pages; the pages that new tokens
+    need are taken from ``free_pages`` (int32, from entry ``cursor[0]`` on) in
+    the requests' order and written into it.  ``tokens``: the batch's size; the
+    places past the last token are padding.  A request that the columns or the
+    free list cannot hold is not admitted (``first`` -1, its tokens without
+    slots), nor is a later one that needs pages when the list has run out.
+    ``out``: an earlier plan of the same sizes to write into (its ``cursor`` may
+    not be this call's).  Returns KvPlan; the next step's ``cursor`` is its.
+    """
+    op = "kv_plan"
+    _need(isinstance(past, torch.Tensor) and past.is_cuda, op, "past must be a GPU tensor.")
+    device = past.device
+    requests, tokens = past.numel(), int(tokens)
+    _need(tokens >= 0, op, "tokens must not be negative.")
+    pp = _ints(past, "past", op, device)
+    pn = _ints(new, "new", op, device, size=requests)
+    pf = _ints(free_pages, "free_pages", op, device)
+    pc = _ints(cursor, "cursor", op, device, size=1)
+    pt, stride = _table(table, op, device)
+    _need(table.shape[0] == requests, op, "table must have a row for each request.")
+    with _On(device) as stream:
+        if out is None:
+            i = past.new_empty
+            out = KvPlan(past.new_empty(tokens, dtype=torch.int64), i(tokens), i(tokens),
+                         i(requests + 1), i(requests), i(requests), i(1))
+        else:
+            _need(isinstance(out, KvPlan), op, "out must be a KvPlan.")
+        _check(_L().mlxvs_kv_plan_device(
+            pp, pn, requests, pt, stride, table.shape[1], pf, free_pages.numel(), pc,
+            int(page_size), tokens,
+            _ints(out.slots, "out.slots", op, device, torch.int64, tokens),
+            _ints(out.requests, "out.requests", op, device, size=tokens),
+            _ints(out.positions, "out.positions", op, device, size=tokens),
+            _ints(out.starts, "out.starts", op, device, size=requests + 1),
+            _ints(out.lengths, "out.lengths", op, device, size=requests),
+            _ints(out.first, "out.first", op, device, size=requests),
+            _ints(out.cursor, "out.cursor", op, device, size=1), stream))
+    return out
+
+
+class PagedKVCache:
+    """Attention keys and values in pages, and retrieval over them.
+
+    Args:
+        keys: [pages, kv_heads, page_size, dim], float16 or bfloat16.
+        values: [pages, kv_heads, dim, page_size] (transposed within a page).
+        summaries: int8 [pages, kv_heads, dim], or None: no ``select``.
+        scales: float32 [pages, kv_heads], with ``summaries``.
+
+    ``page_size`` is a power of two from 16 to 256, ``dim`` a multiple of 8 up
+    to 256.  The tensors are used in place and must be contiguous;
+    ``PagedKVCache.empty`` makes them.
+    """
+
+    def __init__(self, keys, values, summaries=None, scales=None):
+        op = "PagedKVCache"
+        _need(isinstance(keys, torch.Tensor) and keys.dim() == 4 and keys.dtype in _TYPES
+              and keys.is_cuda and keys.is_contiguous(), op,
+              "keys must be a contiguous float16 or bfloat16 [pages, kv_heads, page_size, dim] "
+              "GPU tensor.")
+        pages, heads, page, dim = keys.shape
+        _need(isinstance(values, torch.Tensor) and values.shape == (pages, heads, dim, page)
+              and values.dtype == keys.dtype and values.device == keys.device
+              and values.is_contiguous(), op,
+              f"values must be a contiguous {keys.dtype} [pages, kv_heads, dim, page_size] tensor "
+              f"on {keys.device}.")
+        _need(page in (16, 32, 64, 128, 256), op, "page_size must be 16, 32, 64, 128 or 256.")
+        _need(8 <= dim <= 256 and dim % 8 == 0, op, "dim must be a multiple of 8 in [8, 256].")
+        _need((summaries is None) == (scales is None), op, "summaries and scales come together.")
+        if summaries is not None:
+            _need(isinstance(summaries, torch.Tensor) and summaries.shape == (pages, heads, dim)
+                  and summaries.dtype == torch.int8 and summaries.device == keys.device
+                  and summaries.is_contiguous(), op,
+                  f"summaries must be a contiguous int8 [pages, kv_heads, dim] tensor on "
+                  f"{keys.device}.")
+            _need(isinstance(scales, torch.Tensor) and scales.shape == (pages, heads)
+                  and scales.dtype == torch.float32 and scales.device == keys.device
+                  and scales.is_contiguous(), op,
+                  f"scales must be a contiguous float32 [pages, kv_heads] tensor on "
+                  f"{keys.device}.")
+        self.keys, self.values, self.summaries, self.scales = keys, values, summaries, scales
+        self.page_size, self.dim, self.kv_heads = page, dim, heads
+        self._c = _Cache(keys.data_ptr(), values.data_ptr(),
+                         None if summaries is None else summaries.data_ptr(),
+                         None if scales is None else scales.data_ptr(), pages, heads, page, dim,
+                         _TYPES[keys.dtype])
+        self._ref = ctypes.byref(self._c)
+        self._sizes = {}  # workspace bytes of calls by their sizes
+
+    @classmethod
+    def empty(cls, pages, kv_heads, page_size, dim, *, dtype=torch.bfloat16, device="cuda",
+              summaries=True):
+        """A cache of ``pages`` pages that holds nothing yet."""
+        def make(*shape, kind=dtype):
+            return torch.zeros(shape, dtype=kind, device=device)
+
+        return cls(make(pages, kv_heads, page_size, dim), make(pages, kv_heads, dim, page_size),
+                   make(pages, kv_heads, dim, kind=torch.int8) if summaries else None,
+                   make(pages, kv_heads, kind=torch.float32) if summaries else None)
+
+    def _rows(self, x, name: str, op: str, heads: Optional[int] = None):
+        """[tokens, heads, dim] rows as the kernels read them: any token and
+        head strides, 16-byte aligned (a copy where they are not)."""
+        keys = self.keys
+        if not (isinstance(x, torch.Tensor) and x.dim() == 3 and x.dtype == keys.dtype
+                and x.device == keys.device and x.shape[2] == self.dim
+                and (heads is None or x.shape[1] == heads)):
+            raise ValueError(f"[mlxvs::{op}] {name} must be a {keys.dtype} [tokens, heads, "
+                             f"{self.dim}] tensor on {keys.device}.")
+        st = x.stride()
+        if st[2] != 1 or st[0] & 7 or st[1] & 7 or x.data_ptr() & 15:
+            x = x.clone(memory_format=torch.contiguous_format)
+        return x
+
+    def append(self, k, v, slots) -> None:
+        """Write the tokens' keys and values [tokens, kv_heads, dim] into their
+        ``slots`` (int64 [tokens]; -1 or outside the cache: skipped), and the
+        summaries of the pages that this completes."""
+        op = "kv_append"
+        k = self._rows(k, "k", op, self.kv_heads)
+        v = self._rows(v, "v", op, self.kv_heads)
+        tokens = k.shape[0]
+        _need(v.shape[0] == tokens, op, "k and v must have the same tokens.")
+        ps = _ints(slots, "slots", op, k.device, torch.int64, tokens)
+        ks, vs = k.stride(), v.stride()
+        with _On(k.device) as stream:
+            _check(_L().mlxvs_kv_append_device(self._ref, k.data_ptr(), ks[0], ks[1], v.data_ptr(),
+                                               vs[0], vs[1], ps, tokens, stream))
+
+    def _queries(self, q, table, requests, positions, op: str):
+        q = self._rows(q, "q", op)
+        tokens, heads = q.shape[:2]
+        _need(heads >= self.kv_heads and heads % self.kv_heads == 0, op,
+              f"q must have a multiple of {self.kv_heads} heads.")
+        pt, stride = _table(table, op, q.device)
+        st = q.stride()
+        return q, _Queries(q.data_ptr(), st[0], st[1], tokens, heads, table.shape[1], pt, stride,
+                           table.shape[0], _ints(requests, "requests", op, q.device, size=tokens),
+                           _ints(positions, "positions", op, q.device, size=tokens))
+
+    def _workspace(self, size, q, qs, *args):
+        """(tensor, bytes) of scratch memory on the current stream."""
+        key = (size, qs.tokens, qs.q_heads, qs.columns) + args
+        need = self._sizes.get(key)
+        if need is None:
+            need = getattr(_L(), size)(self._ref, ctypes.byref(qs), *args)
+            if need < 0:
+                raise ValueError(_L().mlxvs_last_error().decode())
+            if len(self._sizes) >= 1024:
+                self._sizes.clear()
+            self._sizes[key] = need
+        return (q.new_empty(need, dtype=torch.uint8) if need else None), need
+
+    def select(self, q, table, requests, positions, n, *, first=1, last=1):
+        """The ``n`` best blocks of each token and kv head: int32 [tokens,
+        kv_heads, n], ascending, -1 after the last.
+
+        ``q`` [tokens, q_heads, dim]; ``table`` int32 [requests, columns];
+        ``requests`` / ``positions`` int32 [tokens] (KvPlan's).  Candidates are
+        the blocks up to the token's own.  The ``first`` first ones and the
+        ``last`` latest (its own among them, last >= 1) are always taken, the
+        others by the product of their summary with the query, the lowest
+        block among equal ones.  Scores are whole-number products, so the list
+        is the same from every implementation."""
+        op = "kv_select"
+        n = int(n)
+        _need(self.summaries is not None, op, "the cache keeps no summaries.")
+        q, qs = self._queries(q, table, requests, positions, op)
+        with _On(q.device) as stream:
+            work, size = self._workspace("mlxvs_kv_select_workspace", q, qs, n)
+            out = q.new_empty((q.shape[0], self.kv_heads, n), dtype=torch.int32)
+            _check(_L().mlxvs_kv_select_device(
+                self._ref, ctypes.byref(qs), n, int(first), int(last), out.data_ptr(),
+                None if work is None else work.data_ptr(), size, stream))
+        return out
+
+    def attend(self, q, table, requests, positions, *, blocks=None, scale=None, longest=0,
+               lse=False, out=None):
+        """Attention of the tokens over the cache, [tokens, q_heads, dim].
+
+        A token sees its request's keys 0 .. position, its own among them;
+        ``blocks`` int32 [tokens, kv_heads, n] (n <= 256) limits it to the
+        listed ones.  A token that sees nothing gets zeros.  ``scale``: of the
+        scores, 1 / sqrt(dim) by default.  ``longest``: tokens of the longest
+        request, if the caller knows it (it guides how work is split, never
+        what is computed).  With ``lse`` returns (out, float32 [tokens,
+        q_heads] logarithms of the sums of exponentials)."""
+        op = "kv_attend"
+        q, qs = self._queries(q, table, requests, positions, op)
+        tokens, heads, dim = q.shape
+        n, pb = 0, None
+        if blocks is not None:
+            if not (isinstance(blocks, torch.Tensor) and blocks.dim() == 3
+                    and blocks.dtype == torch.int32 and blocks.is_contiguous()
+                    and blocks.device == q.device and blocks.shape[:2] == (tokens, self.kv_heads)
+                    and blocks.shape[2] >= 1):
+                raise ValueError(f"[mlxvs::{op}] blocks must be a contiguous int32 [tokens, "
+                                 f"kv_heads, n] tensor on {q.device}.")
+            n, pb = blocks.shape[2], blocks.data_ptr()
+        if scale is None:
+            scale = 1.0 / math.sqrt(dim)
+        longest = int(longest)
+        with _On(q.device) as stream:
+            work, size = self._workspace("mlxvs_kv_attend_workspace", q, qs, n, longest)
+            if out is None:
+                out = q.new_empty((tokens, heads, dim))
+            else:
+                _need(isinstance(out, torch.Tensor) and out.shape == q.shape
+                      and out.dtype == q.dtype and out.device == q.device
+                      and out.is_contiguous(), op,
+                      f"out must be a contiguous {q.dtype} [tokens, q_heads, dim] tensor on "
+                      f"{q.device}.")
+            sums = q.new_empty((tokens, heads), dtype=torch.float32) if lse else None
+            if tokens:
+                _check(_L().mlxvs_kv_attend_device(
+                    self._ref, ctypes.byref(qs), pb, n, float(scale), longest, out.data_ptr(),
+                    None if sums is None else sums.data_ptr(),
+                    None if work is None else work.data_ptr(), size, stream))
+        return (out, sums) if lse else out
