@@ -448,6 +448,7 @@ void kv_attend_plan(KvAttendArgs& a) {
   a.splits = 1;
   a.chunk = 64;
   a.waves = 4;
+  if (rows == 0) return;
   if (rows >= 4096) {
     a.waves = 1;
     return;
