@@ -554,7 +554,8 @@ typedef struct {
  *   lengths [requests]: tokens held after the step;
  *   first [requests]: a request's first entry of free_pages, -1 if it was not
  *     admitted (0 if it needs none);
- *   cursor_out[0]: the first unused entry after the step (may not be cursor).
+ *   cursor_out[0]: the first unused entry after the step.
+ * What is written may not overlap what is read, the table apart.
  * columns x page_size must be below 2^31.
  */
 MLXVS_C_API int mlxvs_kv_plan_device(

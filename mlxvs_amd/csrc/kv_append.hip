@@ -20,20 +20,108 @@ namespace {
 
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 
-constexpr int kTile = 16;  // tokens of a workgroup
-
 // Valid slots name a page of the cache; others are skipped.
 __device__ __forceinline__ bool in_cache(const KvCache& c, int64_t slot) {
   return slot >= 0 && (slot >> c.lps) < c.pages;
 }
+__device__ __forceinline__ bool completes(const KvCache& c, int64_t slot) {
+  return in_cache(c, slot) && (slot & (c.page - 1)) == c.page - 1;
+}
 
+template <bool BF16>
+__device__ __forceinline__ float value(uint16_t x) {
+  if constexpr (BF16) return __builtin_bit_cast(float, (uint32_t)x << 16);
+  else return (float)__builtin_bit_cast(_Float16, x);
+}
+template <bool BF16>
+__device__ __forceinline__ float value(const uintx4& v, int j) {
+  return value<BF16>((uint16_t)(v[j / 2] >> (16 * (j & 1))));
+}
+
+template <int THREADS>
+__device__ __forceinline__ float block_max(float x, float* shared) {
+#pragma unroll
+  for (int i = 32; i >= 1; i >>= 1) x = fmaxf(x, __shfl_xor(x, i));
+  if constexpr (THREADS == 64) return x;
+  if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = x;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < THREADS / 64; ++i) x = fmaxf(x, shared[i]);
+  __syncthreads();
+  return x;
+}
+
+struct Sums {
+  int sum[kKvMaxDim];
+  float red[4];
+};
+
+// The summary of a page and head by THREADS threads; row(i) is key i's address.
+template <bool BF16, int THREADS, typename Row>
+__device__ void summarise(const KvCache& c, int64_t at, Sums& s, Row row) {
+  const int tid = threadIdx.x, d = c.dim, chunks = d / 8;
+  const int rows = THREADS / chunks, x = 8 * (tid % chunks);
+  const int i0 = tid < rows * chunks ? tid / chunks : c.page;
+  float top = 0.0f, bad = 0.0f;
+#pragma unroll 4
+  for (int i = i0; i < c.page; i += rows) {
+    const uintx4 v = *(const uintx4*)(row(i) + x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float k = fabsf(value<BF16>(v, j));
+      if (!(k < __builtin_inff())) bad = 1.0f;
+      top = fmaxf(top, k);
+    }
+  }
+  top = block_max<THREADS>(top, s.red);
+  bad = block_max<THREADS>(bad, s.red);
+  // nothing to see (or too small to divide by), or a key that is not finite:
+  // the block counts as the best, so that what is broken is not left out
+  const bool empty = bad != 0.0f || !(top > 1e-30f);
+  const float inv = empty ? 0.0f : 127.0f / top;
+  for (int i = tid; i < d; i += THREADS) s.sum[i] = 0;
+  __syncthreads();
+  if (!empty && i0 < c.page) {
+    // a thread adds up the keys that it has before the threads meet in LDS
+    int part[8] = {};
+#pragma unroll 4
+    for (int i = i0; i < c.page; i += rows) {
+      const uintx4 v = *(const uintx4*)(row(i) + x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) part[j] += (int)rintf(value<BF16>(v, j) * inv);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) atomicAdd(&s.sum[x + j], part[j]);
+  }
+  __syncthreads();
+  float peak = 0.0f;
+  for (int i = tid; i < d; i += THREADS) peak = fmaxf(peak, (float)abs(s.sum[i]));
+  peak = block_max<THREADS>(peak, s.red);
+  const float to = peak > 0.0f ? 127.0f / peak : 0.0f;
+  for (int i = tid; i < d; i += THREADS)
+    c.summaries[at * d + i] = (int8_t)rintf((float)s.sum[i] * to);
+  if (tid == 0)
+    c.scales[at] = bad != 0.0f ? __builtin_inff()
+                   : empty     ? 0.0f
+                               : top * (peak / (16129.0f * (float)c.page));
+  __syncthreads();
+}
+
+// TILE tokens and a head.  FEW: the summaries too, in the same launch: the keys
+// of a completed page that this call writes are read where they come from, so
+// that no workgroup waits for another's stores (each looks all slots through
+// for them, which is why the call's tokens are few).
+constexpr int kFew = 1024;
+
+template <bool BF16, int TILE, bool FEW>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a) {
-  __shared__ uint16_t tile[kTile][kKvMaxDim + 2];
+  __shared__ uint16_t tile[TILE][kKvMaxDim + 2];
   const int h = (int)(blockIdx.x % a.c.heads);
-  const int64_t t0 = (int64_t)(blockIdx.x / a.c.heads) * kTile;
+  const int64_t t0 = (int64_t)(blockIdx.x / a.c.heads) * TILE;
   const int d = a.c.dim, chunks = d / 8;
   const int64_t head = (int64_t)a.c.page * d;
-  const int tokens = (int)min<int64_t>(kTile, a.tokens - t0);
+  const int tokens = (int)min<int64_t>(TILE, a.tokens - t0);
+  const uint16_t* k = (const uint16_t*)a.k + h * a.k_head;
   for (int i = threadIdx.x; i < tokens * chunks; i += 256) {
     const int t = i / chunks, x = 8 * (i % chunks);
     const int64_t slot = a.slots[t0 + t];
@@ -45,111 +133,81 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a) {
     const int64_t page = slot >> a.c.lps;
     const int off = (int)(slot & (a.c.page - 1));
     *(uintx4*)((uint16_t*)a.c.keys + (page * a.c.heads + h) * head + off * d + x) =
-        *(const uintx4*)((const uint16_t*)a.k + (t0 + t) * a.k_token + h * a.k_head + x);
+        *(const uintx4*)(k + (t0 + t) * a.k_token + x);
   }
   __syncthreads();
-  const int t = threadIdx.x % kTile;
-  if (t >= tokens) return;
-  const int64_t slot = a.slots[t0 + t];
-  if (!in_cache(a.c, slot)) return;
-  uint16_t* dst = (uint16_t*)a.c.values + ((slot >> a.c.lps) * a.c.heads + h) * head +
-                  (slot & (a.c.page - 1));
-  for (int i = threadIdx.x / kTile; i < d; i += 256 / kTile) dst[i * a.c.page] = tile[t][i];
-}
-
-template <bool BF16>
-__device__ __forceinline__ float value(uint16_t x) {
-  if constexpr (BF16) return __builtin_bit_cast(float, (uint32_t)x << 16);
-  else return (float)__builtin_bit_cast(_Float16, x);
-}
-
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int i = 32; i >= 1; i >>= 1) x = fmaxf(x, __shfl_xor(x, i));
-  return x;
-}
-
-// One page and head, by one wavefront.
-template <bool BF16>
-__device__ void summarise(const KvCache& c, int64_t page, int h, int* sums) {
-  const int lane = threadIdx.x, d = c.dim, chunks = d / 8;
-  const int64_t at = page * c.heads + h;
-  const uint16_t* keys = (const uint16_t*)c.keys + at * c.page * d;
-  float top = 0.0f;
-  bool finite = true;
-  for (int i = lane; i < c.page * chunks; i += 64) {
-    const uintx4 v = *(const uintx4*)(keys + 8 * i);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float x = fabsf(value<BF16>((uint16_t)(v[j / 2] >> (16 * (j & 1)))));
-      finite &= x < __builtin_inff();
-      top = fmaxf(top, x);
+  const int t = threadIdx.x % TILE;
+  if (t < tokens) {
+    const int64_t slot = a.slots[t0 + t];
+    if (in_cache(a.c, slot)) {
+      uint16_t* dst = (uint16_t*)a.c.values + ((slot >> a.c.lps) * a.c.heads + h) * head +
+                      (slot & (a.c.page - 1));
+      for (int i = threadIdx.x / TILE; i < d; i += 256 / TILE) dst[i * a.c.page] = tile[t][i];
     }
   }
-  top = wave_max(top);
-  finite = __all(finite);
-  // nothing to see (or too small to divide by), or a key that is not finite:
-  // the block counts as the best, so that what is broken is not left out
-  const bool empty = !finite || !(top > 1e-30f);
-  const float inv = empty ? 0.0f : 127.0f / top;
-  for (int i = lane; i < d; i += 64) sums[i] = 0;
-  __syncthreads();
-  if (!empty) {
-    // lanes of one 8-value chunk add what they have before they meet in LDS
-    const int rows = 64 / chunks, x = lane % chunks;
-    if (lane < rows * chunks) {
-      int part[8] = {};
-      for (int i = lane / chunks; i < c.page; i += rows) {
-        const uintx4 v = *(const uintx4*)(keys + i * d + 8 * x);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          part[j] += (int)rintf(value<BF16>((uint16_t)(v[j / 2] >> (16 * (j & 1)))) * inv);
+  if constexpr (FEW) {
+    __shared__ Sums sums;
+    __shared__ int from[256];  // a page's keys: the token that writes it now, or -1
+    for (int i = 0; i < tokens; ++i) {
+      const int64_t slot = a.slots[t0 + i];
+      if (!completes(a.c, slot)) continue;
+      const int64_t page = slot >> a.c.lps;
+      from[threadIdx.x] = -1;
+      __syncthreads();
+      for (int u = threadIdx.x; u < a.tokens; u += 256) {
+        const int64_t other = a.slots[u];
+        if (other >= 0 && other >> a.c.lps == page) from[other & (a.c.page - 1)] = u;
       }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) atomicAdd(&sums[8 * x + j], part[j]);
+      __syncthreads();
+      const int64_t at = page * a.c.heads + h;
+      const uint16_t* held = (const uint16_t*)a.c.keys + at * head;
+      summarise<BF16, 256>(a.c, at, sums, [&](int j) {
+        return from[j] >= 0 ? k + from[j] * a.k_token : held + j * d;
+      });
     }
   }
-  __syncthreads();
-  float peak = 0.0f;
-  for (int i = lane; i < d; i += 64) peak = fmaxf(peak, (float)abs(sums[i]));
-  peak = wave_max(peak);
-  const float to = peak > 0.0f ? 127.0f / peak : 0.0f;
-  for (int i = lane; i < d; i += 64) c.summaries[at * d + i] = (int8_t)rintf((float)sums[i] * to);
-  if (lane == 0)
-    c.scales[at] = !finite ? __builtin_inff()
-                           : empty ? 0.0f : top * (peak / (16129.0f * (float)c.page));
-  __syncthreads();
 }
 
-// A wavefront for `span` tokens and a head.
+// Many tokens: the summaries by a launch of their own, a wavefront for `span`
+// tokens and a head.
 template <bool BF16>
 __global__ __launch_bounds__(64) void kv_summaries_kernel(KvAppendArgs a, int span) {
-  __shared__ int sums[kKvMaxDim];
+  __shared__ Sums sums;
   const int h = (int)(blockIdx.x % a.c.heads);
-  const int64_t t0 = (int64_t)(blockIdx.x / a.c.heads) * span;
-  const int64_t t = t0 + threadIdx.x;
+  const int64_t t = (int64_t)(blockIdx.x / a.c.heads) * span + threadIdx.x;
   const int64_t slot = (int)threadIdx.x < span && t < a.tokens ? a.slots[t] : -1;
-  const bool last = in_cache(a.c, slot) && (slot & (a.c.page - 1)) == a.c.page - 1;
-  for (uint64_t todo = __ballot(last); todo; todo &= todo - 1) {
-    const int from = __builtin_ctzll(todo);
-    summarise<BF16>(a.c, __shfl(slot, from) >> a.c.lps, h, sums);
+  for (uint64_t todo = __ballot(completes(a.c, slot)); todo; todo &= todo - 1) {
+    const int64_t at = (__shfl(slot, __builtin_ctzll(todo)) >> a.c.lps) * a.c.heads + h;
+    const uint16_t* held = (const uint16_t*)a.c.keys + at * a.c.page * a.c.dim;
+    summarise<BF16, 64>(a.c, at, sums, [&](int j) { return held + j * a.c.dim; });
   }
+}
+
+template <bool BF16, int TILE, bool FEW>
+void launch_tile(const KvAppendArgs& a, hipStream_t s) {
+  const int64_t grid = (a.tokens + TILE - 1) / TILE * a.c.heads;
+  kv_append_kernel<BF16, TILE, FEW><<<dim3((unsigned)grid), 256, 0, s>>>(a);
+}
+
+template <bool BF16>
+hipError_t launch_append(const KvAppendArgs& a, hipStream_t s) {
+  constexpr int kSpan = 16;
+  if (a.tokens <= kFew && a.c.summaries) {
+    // (small tiles: a workgroup's summaries follow one another)
+    a.tokens <= 256 ? launch_tile<BF16, 4, true>(a, s) : launch_tile<BF16, 16, true>(a, s);
+    return hipGetLastError();
+  }
+  launch_tile<BF16, 16, false>(a, s);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess || !a.c.summaries) return e;
+  const int64_t grid = (a.tokens + kSpan - 1) / kSpan * a.c.heads;
+  kv_summaries_kernel<BF16><<<dim3((unsigned)grid), 64, 0, s>>>(a, kSpan);
+  return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_kv_append(const KvAppendArgs& a, hipStream_t s) {
-  const int64_t grid = (a.tokens + kTile - 1) / kTile * a.c.heads;
-  kv_append_kernel<<<dim3((unsigned)grid), 256, 0, s>>>(a);
-  return hipGetLastError();
-}
-
-hipError_t launch_kv_summaries(const KvAppendArgs& a, hipStream_t s) {
-  const int span = a.tokens > 1024 ? 16 : 1;
-  const int64_t grid = (a.tokens + span - 1) / span * a.c.heads;
-  if (a.c.bf16) kv_summaries_kernel<true><<<dim3((unsigned)grid), 64, 0, s>>>(a, span);
-  else kv_summaries_kernel<false><<<dim3((unsigned)grid), 64, 0, s>>>(a, span);
-  return hipGetLastError();
+  return a.c.bf16 ? launch_append<true>(a, s) : launch_append<false>(a, s);
 }
 
 }  // namespace mlxvs::kern

@@ -56,8 +56,6 @@ struct KvAppendArgs {
   int64_t tokens;
 };
 hipError_t launch_kv_append(const KvAppendArgs& a, hipStream_t s);
-// The summaries of the pages whose last slot is among `slots`.
-hipError_t launch_kv_summaries(const KvAppendArgs& a, hipStream_t s);
 
 // Queries of tokens and where they stand.
 struct KvQueries {
@@ -95,8 +93,8 @@ struct KvAttendArgs {
   int splits;       // parts of a row's keys, joined by a second launch if more than one
   int chunk;        // keys of a part (a multiple of 64; the last part takes the rest)
   int waves;        // wavefronts that share a part (1: a row each, no parts)
-  float* part_o;    // [tokens][heads][splits][group][dim]
-  float* part_ml;   // [tokens][heads][splits][group][2]
+  float* part_o;    // [tokens][heads][group][splits][dim]
+  float* part_ml;   // [tokens][heads][group][splits][2]
 };
 void kv_attend_plan(KvAttendArgs& a);  // sets splits, chunk and waves
 int64_t kv_attend_workspace(const KvAttendArgs& a);

@@ -118,6 +118,11 @@ void kv_plan_device(const KvPlan& p, void* stream) {
         "slots, token_request and positions must not be NULL.");
   check(p.starts && p.cursor && p.cursor_out, "starts, cursor and cursor_out must not be NULL.");
   check(p.cursor != p.cursor_out, "cursor_out must not be cursor.");
+  const auto apart = [&](const int32_t* x) {
+    return p.lengths + p.requests <= x || x + p.requests <= p.lengths;
+  };
+  check(p.requests == 0 || (apart(p.past) && apart(p.fresh)),
+        "lengths must not overlap past or fresh.");
   check_grid((p.tokens + 255) / 256 + (p.requests + 3) / 4, 256, check);
   detail::need_device();
   const kern::KvPlanArgs a{p.past,      p.fresh,         p.table,     p.free_pages, p.cursor,
@@ -143,9 +148,6 @@ void kv_append_device(const KvCache& cache, const void* k, int64_t k_token_strid
   detail::need_device();
   detail::launch_stage<kern::KvAppendArgs, kern::launch_kv_append>((hipStream_t)stream,
                                                                    "kv_append", a);
-  if (a.c.summaries)
-    detail::launch_stage<kern::KvAppendArgs, kern::launch_kv_summaries>((hipStream_t)stream,
-                                                                        "kv_summaries", a);
 }
 
 int64_t kv_select_workspace(const KvCache& cache, const KvQueries& queries, int n) {

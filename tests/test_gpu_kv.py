@@ -180,7 +180,7 @@ def test_append(engine, heads, page, dim, dtype):
     check_append(cache, k, v, slots)
 
 
-@pytest.mark.parametrize("tokens", [1, 15, 16, 17, 1500])
+@pytest.mark.parametrize("tokens", [1, 15, 16, 17, 256, 257, 1024, 1025, 1500])
 def test_append_in_any_order(engine, tokens):
     # slots in no order: a page's last slot may come before its others
     rng = np.random.default_rng(tokens)

@@ -97,7 +97,7 @@ def test_arguments_that_are_refused(engine):
 
 def plan(lib, **k):
     f = dict(past=P, fresh=P, requests=3, table=P, stride=5, columns=5, free=P, count=9, cursor=P,
-             page=16, tokens=8, slots=P, who=P, where=P, starts=P, lengths=P, first=P, out=P + 4)
+             page=16, tokens=8, slots=P, who=P, where=P, starts=P, lengths=P + 12, first=P, out=P + 4)
     f.update(k)
     return lib.mlxvs_kv_plan_device(*f.values(), None)
 
@@ -107,7 +107,7 @@ def plan(lib, **k):
     dict(columns=-1), dict(columns=1 << 28, stride=1 << 28), dict(free=None), dict(count=-1),
     dict(cursor=None), dict(page=15), dict(tokens=-1), dict(slots=None), dict(who=None),
     dict(where=None), dict(starts=None), dict(lengths=None), dict(first=None), dict(out=None),
-    dict(out=P)])
+    dict(out=P), dict(lengths=P), dict(lengths=P + 8)])
 def test_plans_that_are_refused(engine, bad):
     lib = engine._L()
     assert plan(lib, **bad) == INVALID
