@@ -28,6 +28,7 @@
 namespace mlxvs::kern {
 namespace {
 
+typedef float floatx2 __attribute__((ext_vector_type(2)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
@@ -74,9 +75,9 @@ __device__ __forceinline__ uintx4 keep(uintx4 v, int n) {
   return v;
 }
 
-// DP: head size rounded up to a multiple of 32.  WAVES: wavefronts that share
-// a row's part (1: a row each).  P16: pages of 16 keys, two to a 32-key pair.
-template <int DP, bool BF16, bool LIST, int WAVES, bool P16>
+// DP: head size rounded up to a multiple of 32.  LIST: over listed blocks.  P16:
+// pages of 16 keys, two to a 32-key pair.
+template <int DP, bool BF16, bool LIST, bool P16>
 struct Attend {
   using T = std::conditional_t<BF16, __bf16, _Float16>;
   using Tx8 = std::conditional_t<BF16, bf16x8, halfx8>;
@@ -249,10 +250,12 @@ __device__ __forceinline__ float lse_of(float m, float l, float scale, float bia
   return fmaf(m, scale, kLn2 * (__log2f(l) - bias));
 }
 
-// Rows of many tokens (or heads): a wavefront each, no parts.
+// Many rows: a wavefront each, no parts.
+constexpr int64_t kManyRows = 4096;
+
 template <int DP, bool BF16, bool LIST, bool P16>
 __global__ __launch_bounds__(256, 2) void kv_attend_rows_kernel(KvAttendArgs a) {
-  using A = Attend<DP, BF16, LIST, 1, P16>;
+  using A = Attend<DP, BF16, LIST, P16>;
   const int tiles = (a.q.group + kColumns - 1) / kColumns;
   const int64_t row = blockIdx.x;
   const int mt = (int)(row % tiles);
@@ -289,21 +292,22 @@ __global__ __launch_bounds__(256, 2) void kv_attend_rows_kernel(KvAttendArgs a) 
 }
 
 // Few rows: a part of a row's keys for each workgroup, its steps dealt to the
-// wavefronts in turn.
-template <int DP, bool BF16, bool LIST, bool P16>
-__global__ __launch_bounds__(256, 2) void kv_attend_parts_kernel(KvAttendArgs a) {
-  constexpr int W = 4;
-  using A = Attend<DP, BF16, LIST, W, P16>;
-  __shared__ float so[W][kColumns][DP + 4];
-  __shared__ float sm[W][kColumns], sl[W][kColumns];
+// W wavefronts in turn.
+template <int DP, bool BF16, bool LIST, bool P16, int W>
+__global__ __launch_bounds__(64 * W, 2) void kv_attend_parts_kernel(KvAttendArgs a) {
+  constexpr int H = 4;  // wavefronts whose sums meet in LDS at a time
+  using A = Attend<DP, BF16, LIST, P16>;
+  __shared__ float so[H][kColumns][DP + 4];
+  __shared__ float sm[H][kColumns], sl[H][kColumns];
   const int tiles = (a.q.group + kColumns - 1) / kColumns;
-  int64_t b = blockIdx.x;
-  const int part = (int)(b % a.splits);
-  b /= a.splits;
-  const int mt = (int)(b % tiles);
-  b /= tiles;
+  // first parts first: a row's later ones may be empty, and workgroups go round
+  // the 8 XCDs
+  const int mt = (int)(blockIdx.x % tiles);
+  int64_t b = blockIdx.x / tiles;
   const int h = (int)(b % a.c.heads);
-  const int64_t t = b / a.c.heads;
+  b /= a.c.heads;
+  const int64_t t = b % a.q.tokens;
+  const int part = (int)(b / a.q.tokens);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   A w(a, threadIdx.x & 63);
   const int r = a.q.token_request[t], pos = a.q.positions[t];
@@ -323,27 +327,48 @@ __global__ __launch_bounds__(256, 2) void kv_attend_parts_kernel(KvAttendArgs a)
     for (int64_t k = k0 + wave * A::kKeys; k < stop; k += W * A::kKeys) w.step(h, (int)k);
     k0 = stop;
   }
-  const float l = column_sum(w.l);
-  if (w.grp == 0) {
-    sm[wave][w.col] = w.m;
-    sl[wave][w.col] = l;
-  }
+  w.l = column_sum(w.l);
+  const float c = a.scale * kLog2e;
+  const auto put = [&](int x) {
+    if (w.grp == 0) {
+      sm[x][w.col] = w.m;
+      sl[x][w.col] = w.l;
+    }
 #pragma unroll
-  for (int i = 0; i < A::kTiles; ++i) *(floatx4*)&so[wave][w.col][16 * i + 4 * w.grp] = w.o[i];
+    for (int i = 0; i < A::kTiles; ++i) *(floatx4*)&so[x][w.col][16 * i + 4 * w.grp] = w.o[i];
+  };
+  if constexpr (W > H) {
+    static_assert(W == 2 * H, "pairs of wavefronts");
+    if (wave >= H) put(wave - H);
+    __syncthreads();
+    if (wave < H) {
+      const float m = sm[wave][w.col], top = fmaxf(w.m, m);
+      const float safe = top == -__builtin_inff() ? 0.0f : top;
+      const float f0 = __builtin_amdgcn_exp2f((w.m - safe) * c);
+      const float f1 = __builtin_amdgcn_exp2f((m - safe) * c);
+      w.m = top;
+      w.l = w.l * f0 + sl[wave][w.col] * f1;
+#pragma unroll
+      for (int i = 0; i < A::kTiles; ++i)
+        w.o[i] = w.o[i] * f0 + *(const floatx4*)&so[wave][w.col][16 * i + 4 * w.grp] * f1;
+      put(wave);  // (in the places that this lane has read)
+    }
+  } else {
+    put(wave);
+  }
   __syncthreads();
   const int groups = min(kColumns, a.q.group - mt * kColumns);
   const int quads = a.c.dim / 4;
-  const float c = a.scale * kLog2e;
-  for (int i = threadIdx.x; i < groups * quads; i += 256) {
+  for (int i = threadIdx.x; i < groups * quads; i += 64 * W) {
     const int g = i / quads, d = 4 * (i % quads);
     float top = sm[0][g];
 #pragma unroll
-    for (int x = 1; x < W; ++x) top = fmaxf(top, sm[x][g]);
+    for (int x = 1; x < H; ++x) top = fmaxf(top, sm[x][g]);
     const float safe = top == -__builtin_inff() ? 0.0f : top;
     float sum = 0.0f;
     floatx4 o = {0, 0, 0, 0};
 #pragma unroll
-    for (int x = 0; x < W; ++x) {
+    for (int x = 0; x < H; ++x) {
       const float f = __builtin_amdgcn_exp2f((sm[x][g] - safe) * c);
       sum = fmaf(sl[x][g], f, sum);
       o += *(const floatx4*)&so[x][g][d] * f;
@@ -359,52 +384,62 @@ __global__ __launch_bounds__(256, 2) void kv_attend_parts_kernel(KvAttendArgs a)
       *(typename A::Tx4*)((typename A::T*)a.out + at * a.c.dim + d) = x;
       if (a.lse && d == 0) a.lse[at] = lse_of(top, sum, a.scale, A::kBias);
     } else {
-      const int64_t at = (head * a.splits + part) * a.q.group + gg;
+      const int64_t at = (head * a.q.group + gg) * a.splits + part;
       *(floatx4*)(a.part_o + at * a.c.dim + d) = o;
-      if (d == 0) {
-        a.part_ml[2 * at] = top;
-        a.part_ml[2 * at + 1] = sum;
-      }
+      if (d == 0) *(floatx2*)(a.part_ml + 2 * at) = floatx2{top, sum};
     }
   }
 }
 
 // Joins the parts of a row: out = sum_s w_s O_s / sum_s w_s l_s, w_s = 2^((m_s -
-// max) c), always in the parts' order.
+// max) c).  Threads of one quarter of values take the parts in turn, and their
+// sums are added in order: the same result on every run.
 template <bool BF16>
-__global__ __launch_bounds__(64) void kv_attend_join_kernel(KvAttendArgs a) {
+__global__ __launch_bounds__(256) void kv_attend_join_kernel(KvAttendArgs a) {
   using T = std::conditional_t<BF16, __bf16, _Float16>;
   using Tx4 = std::conditional_t<BF16, bf16x4, halfx4>;
+  __shared__ floatx4 so[256];
+  __shared__ float ss[256], sm[4];
+  const int tid = threadIdx.x;
   const int64_t at = blockIdx.x;  // (token, query head)
-  const int g = (int)(at % a.q.group);
-  const int64_t head = at / a.q.group;
   const float c = a.scale * kLog2e;
-  const int64_t first = head * a.splits * a.q.group + g;
+  const float* ml = a.part_ml + 2 * at * a.splits;
   float top = -__builtin_inff();
-  for (int s = threadIdx.x; s < a.splits; s += 64)
-    top = fmaxf(top, a.part_ml[2 * (first + (int64_t)s * a.q.group)]);
+  for (int s = tid; s < a.splits; s += 256) top = fmaxf(top, ml[2 * s]);
 #pragma unroll
   for (int x = 32; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+  if ((tid & 63) == 0) sm[tid >> 6] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
   const float safe = top == -__builtin_inff() ? 0.0f : top;
-  const int d = 4 * threadIdx.x;
+  const int quads = a.c.dim / 4, lanes = 256 / quads;
+  const int mine = tid / quads, d = 4 * (tid % quads);
   float sum = 0.0f;
   floatx4 o = {0, 0, 0, 0};
-  for (int s = 0; s < a.splits; ++s) {
-    const int64_t p = first + (int64_t)s * a.q.group;
-    const float m = a.part_ml[2 * p], l = a.part_ml[2 * p + 1];
-    if (m == -__builtin_inff() && l == 0.0f) continue;
-    const float f = __builtin_amdgcn_exp2f((m - safe) * c);
-    sum = fmaf(l, f, sum);
-    if (d < a.c.dim) o += *(const floatx4*)(a.part_o + p * a.c.dim + d) * f;
+  if (mine < lanes) {
+    const float* po = a.part_o + at * a.splits * a.c.dim + d;
+#pragma unroll 4
+    for (int s = mine; s < a.splits; s += lanes) {
+      const floatx2 p = *(const floatx2*)(ml + 2 * s);
+      const float f = __builtin_amdgcn_exp2f((p[0] - safe) * c);
+      sum = fmaf(p[1], f, sum);
+      o += *(const floatx4*)(po + (int64_t)s * a.c.dim) * f;
+    }
+  }
+  so[tid] = o;
+  ss[tid] = sum;
+  __syncthreads();
+  if (tid >= quads) return;
+  for (int x = 1; x < min(lanes, a.splits); ++x) {
+    o += so[x * quads + tid];
+    sum += ss[x * quads + tid];
   }
   const float inv = 1.0f / sum;
-  if (d < a.c.dim) {
-    Tx4 x;
+  Tx4 x;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = (T)(sum == 0.0f ? 0.0f : o[j] * inv);
-    *(Tx4*)((T*)a.out + at * a.c.dim + d) = x;
-  }
-  if (a.lse && threadIdx.x == 0) a.lse[at] = lse_of(top, sum, a.scale, BF16 ? 0.0f : 14.0f);
+  for (int j = 0; j < 4; ++j) x[j] = (T)(sum == 0.0f ? 0.0f : o[j] * inv);
+  *(Tx4*)((T*)a.out + at * a.c.dim + d) = x;
+  if (a.lse && tid == 0) a.lse[at] = lse_of(top, sum, a.scale, BF16 ? 0.0f : 14.0f);
 }
 
 template <int DP, bool BF16, bool LIST, bool P16>
@@ -414,8 +449,9 @@ void launch_one(const KvAttendArgs& a, hipStream_t s) {
     const int64_t grid = (a.q.tokens + 3) / 4 * a.c.heads * tiles;
     kv_attend_rows_kernel<DP, BF16, LIST, P16><<<dim3((unsigned)grid), 256, 0, s>>>(a);
   } else {
-    const int64_t grid = a.q.tokens * a.c.heads * tiles * a.splits;
-    kv_attend_parts_kernel<DP, BF16, LIST, P16><<<dim3((unsigned)grid), 256, 0, s>>>(a);
+    const dim3 grid((unsigned)(a.q.tokens * a.c.heads * tiles * a.splits));
+    if (a.waves == 8) kv_attend_parts_kernel<DP, BF16, LIST, P16, 8><<<grid, 512, 0, s>>>(a);
+    else kv_attend_parts_kernel<DP, BF16, LIST, P16, 4><<<grid, 256, 0, s>>>(a);
   }
 }
 
@@ -449,15 +485,26 @@ void kv_attend_plan(KvAttendArgs& a) {
   a.chunk = 64;
   a.waves = 4;
   if (rows == 0) return;
-  if (rows >= 4096) {
+  if (rows >= kManyRows) {
     a.waves = 1;
     return;
   }
-  const int64_t want = std::max<int64_t>(1, (1024 + rows - 1) / rows);
-  int64_t chunk = (most + want - 1) / want;
-  chunk = std::max<int64_t>(256, (chunk + 255) / 256 * 256);
-  a.chunk = (int)std::min<int64_t>(chunk, 1 << 30);
-  a.splits = (int)std::max<int64_t>(1, (most + a.chunk - 1) / a.chunk);
+  // As many parts as fill the card (2 workgroups a CU: chunks of 4,096 instead
+  // of 1,024 keys 187 / 199 us on one request of 262,144 tokens and 8 kv heads),
+  // but no longer ones than 1,024 keys where requests differ in length (64
+  // ragged requests of up to 8,192 tokens, 8 kv heads: 247 us with 1,024, 260
+  // with 4,096).  Rows of up to 1,024 keys stay whole: the launch that joins
+  // parts costs more than the wait (777 keys, 8 heads: 13.1 us whole, 15.3 in
+  // four), and so do lists where there is a row for every CU (256 rows of 2,048
+  // keys: 51.5 us whole, 55.4 in two).
+  const bool whole = most <= 1024 || (a.n && rows >= 256);
+  int64_t chunk = (most * rows / 512 + 255) / 256 * 256;
+  if (a.q.tokens > 1 && !a.n) chunk = std::min<int64_t>(chunk, 1024);
+  chunk = std::max<int64_t>(512, std::min<int64_t>(chunk, 1 << 30));
+  if (!whole) a.splits = (int)((most + chunk - 1) / chunk);
+  a.chunk = whole ? 1 << 30 : (int)chunk;
+  // eight wavefronts share a part where there is no second workgroup for a CU
+  if (rows * a.splits <= 256) a.waves = 8;
 }
 
 int64_t kv_attend_workspace(const KvAttendArgs& a) {
@@ -475,8 +522,8 @@ hipError_t launch_kv_attend(const KvAttendArgs& a, hipStream_t s) {
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   if (a.splits > 1) {
     const unsigned grid = (unsigned)(a.q.tokens * a.c.heads * a.q.group);
-    if (a.c.bf16) kv_attend_join_kernel<true><<<grid, 64, 0, s>>>(a);
-    else kv_attend_join_kernel<false><<<grid, 64, 0, s>>>(a);
+    if (a.c.bf16) kv_attend_join_kernel<true><<<grid, 256, 0, s>>>(a);
+    else kv_attend_join_kernel<false><<<grid, 256, 0, s>>>(a);
   }
   return hipGetLastError();
 }
