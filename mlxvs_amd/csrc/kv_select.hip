@@ -27,8 +27,6 @@ typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
 
 constexpr uint32_t kAlways = 0xFFFFFFFFu;
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
 constexpr int kLdsCols = 8192;  // ranks of a row that stay in LDS (32 KB)
 
 template <bool BF16>
@@ -36,6 +34,9 @@ __device__ __forceinline__ float value(uint16_t x) {
   if constexpr (BF16) return __builtin_bit_cast(float, (uint32_t)x << 16);
   else return (float)__builtin_bit_cast(_Float16, x);
 }
+
+// Bits set, signed: counts are subtracted and compared.
+__device__ __forceinline__ int bits(uint64_t x) { return (int)__popcll(x); }
 
 __device__ __forceinline__ uint32_t rank_of(int dot, float scale) {
   // a summary that is not finite ranks first (a broken block is not left out)
@@ -45,6 +46,7 @@ __device__ __forceinline__ uint32_t rank_of(int dot, float scale) {
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
+template <int THREADS>
 __device__ __forceinline__ float block_max(float x, float* shared) {
 #pragma unroll
   for (int i = 32; i >= 1; i >>= 1) x = fmaxf(x, __shfl_xor(x, i));
@@ -52,95 +54,122 @@ __device__ __forceinline__ float block_max(float x, float* shared) {
   __syncthreads();
   float y = shared[0];
 #pragma unroll
-  for (int i = 1; i < kWaves; ++i) y = fmaxf(y, shared[i]);
+  for (int i = 1; i < THREADS / 64; ++i) y = fmaxf(y, shared[i]);
   __syncthreads();
   return y;
 }
 
 // The codes of a (token, head)'s query, zeros past dim.  A query that holds
 // nothing, or a value that is not finite, has codes 0.
-template <bool BF16>
+template <bool BF16, int THREADS>
 __device__ void query_codes(const KvSelectArgs& a, int64_t t, int h, int8_t* codes,
                             float* shared) {
   const int d = threadIdx.x, g = a.q.group;
   const uint16_t* q = (const uint16_t*)a.q.q + t * a.q.q_token + (int64_t)h * g * a.q.q_head + d;
   float top = 0.0f, bad = 0.0f;
-  if (d < a.c.dim)
+  if (d < a.c.dim) {
+#pragma unroll 4
     for (int i = 0; i < g; ++i) {
       const float x = fabsf(value<BF16>(q[i * a.q.q_head]));
       if (!(x < __builtin_inff())) bad = 1.0f;
       top = fmaxf(top, x);
     }
-  top = block_max(top, shared);
-  bad = block_max(bad, shared);
+  }
+  top = block_max<THREADS>(top, shared);
+  bad = block_max<THREADS>(bad, shared);
   const float inv = bad == 0.0f && top > 1e-30f ? 127.0f / top : 0.0f;
   int sum = 0;
-  if (d < a.c.dim && inv != 0.0f)
+  if (d < a.c.dim && inv != 0.0f) {
+#pragma unroll 4
     for (int i = 0; i < g; ++i) sum += (int)rintf(value<BF16>(q[i * a.q.q_head]) * inv);
-  const float peak = block_max((float)abs(sum), shared);
+  }
+  const float peak = block_max<THREADS>((float)abs(sum), shared);
   const float to = peak > 0.0f ? 127.0f / peak : 0.0f;
-  codes[d] = (int8_t)rintf((float)sum * to);
+  if (d < kKvMaxDim) codes[d] = (int8_t)rintf((float)sum * to);
   __syncthreads();
 }
 
 // Ranks of the columns [c0, c1) of a row into ranks[0 ..], lanes of a page's
-// group adding up their parts of its dot product.  CH: bytes a lane loads.
-template <int CH>
+// group adding up their parts of its dot product.  The page ids pass through
+// ranks first, so that a thread has kAhead summaries in flight at a time.  CH:
+// bytes a lane loads.
+constexpr int kAhead = 4;
+
+template <int CH, int THREADS>
 __device__ void rank_columns(const KvSelectArgs& a, int h, int r, int own, int c0, int c1,
                              const int8_t* codes, uint32_t* ranks) {
-  const int d = a.c.dim, chunks = d / CH;
+  const int d = a.c.dim, chunks = d / CH, count = c1 - c0;
+  for (int i = threadIdx.x; i < count; i += THREADS)
+    ranks[i] = (uint32_t)a.q.table[(int64_t)r * a.q.table_stride + c0 + i];
   int lanes = 1;
   while (lanes < chunks) lanes *= 2;
-  const int at = threadIdx.x % lanes, per = kThreads / lanes;
+  const int at = threadIdx.x % lanes, per = THREADS / lanes;
   uint32_t q[CH / 4];
 #pragma unroll
-  for (int i = 0; i < CH / 4; ++i) q[i] = at < chunks ? *(const uint32_t*)(codes + CH * at + 4 * i) : 0;
-  for (int j0 = c0; j0 < c1; j0 += per) {
-    const int j = j0 + (int)threadIdx.x / lanes;
-    const int p = j < c1 ? a.q.table[(int64_t)r * a.q.table_stride + j] : -1;
-    const bool there = p >= 0 && p < a.c.pages;
-    const int64_t row = ((int64_t)p * a.c.heads + h);
-    int dot = 0;
-    if (there && at < chunks) {
-      const int8_t* m = a.c.summaries + row * d + CH * at;
-      if constexpr (CH == 16) {
-        const uintx4 v = *(const uintx4*)m;
+  for (int i = 0; i < CH / 4; ++i)
+    q[i] = at < chunks ? *(const uint32_t*)(codes + CH * at + 4 * i) : 0;
+  __syncthreads();
+  for (int j0 = threadIdx.x / lanes; j0 - (int)threadIdx.x / lanes < count; j0 += kAhead * per) {
+    uint32_t v[kAhead][CH / 4];
+    float scale[kAhead];
+    bool there[kAhead];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) dot = __builtin_amdgcn_sdot4((int)v[i], (int)q[i], dot, false);
-      } else {
-        const uintx2 v = *(const uintx2*)m;
+    for (int u = 0; u < kAhead; ++u) {
+      const int j = j0 + u * per;
+      const int p = j < count ? (int)ranks[j] : -1;
+      there[u] = p >= 0 && p < a.c.pages;
+      const int64_t row = (int64_t)p * a.c.heads + h;
+      scale[u] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) dot = __builtin_amdgcn_sdot4((int)v[i], (int)q[i], dot, false);
+      for (int i = 0; i < CH / 4; ++i) v[u][i] = 0;
+      if (there[u]) {
+        if (at < chunks) {
+          const int8_t* m = a.c.summaries + row * d + CH * at;
+          if constexpr (CH == 16) *(uintx4*)v[u] = *(const uintx4*)m;
+          else *(uintx2*)v[u] = *(const uintx2*)m;
+        }
+        if (at == 0) scale[u] = a.c.scales[row];
       }
     }
-    for (int x = 1; x < lanes; x *= 2) dot += __shfl_xor(dot, x);
-    if (at == 0 && j < c1) {
-      uint32_t k = 0;
-      if (there) k = j < a.first || j > own - a.last ? kAlways : rank_of(dot, a.c.scales[row]);
-      ranks[j - c0] = k;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      int dot = 0;
+#pragma unroll
+      for (int i = 0; i < CH / 4; ++i) dot = __builtin_amdgcn_sdot4((int)v[u][i], (int)q[i], dot, false);
+      for (int x = 1; x < lanes; x *= 2) dot += __shfl_xor(dot, x);
+      const int j = j0 + u * per, c = c0 + j;
+      // (the group's other lanes have read the page id: they are of one wavefront)
+      if (at == 0 && j < count)
+        ranks[j] = !there[u]                          ? 0
+                   : c < a.first || c > own - a.last ? kAlways
+                                                      : rank_of(dot, scale[u]);
     }
   }
 }
 
+template <int THREADS>
 struct Select {
   uint32_t hist[256];
-  int gt[kWaves], eq[kWaves];
+  int gt[THREADS / 64], eq[THREADS / 64];
   uint32_t prefix;
   int left;
 };
 
 // The n largest of ranks[0 .. count), the lowest columns among equal ones,
 // ascending by column into out, -1 after.
-__device__ void take_best(const uint32_t* ranks, int count, int n, int32_t* out, Select& s) {
+template <int THREADS>
+__device__ void take_best(const uint32_t* ranks, int count, int n, int32_t* out,
+                          Select<THREADS>& s) {
+  constexpr int kWaves = THREADS / 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   // the n-th largest rank, 8 bits at a time
   uint32_t prefix = 0;
   int left = n;
   if (count > n) {
     for (int shift = 24; shift >= 0; shift -= 8) {
-      s.hist[threadIdx.x] = 0;
+      if (threadIdx.x < 256) s.hist[threadIdx.x] = 0;
       __syncthreads();
-      for (int i = threadIdx.x; i < count; i += kThreads) {
+      for (int i = threadIdx.x; i < count; i += THREADS) {
         const uint32_t k = ranks[i];
         if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)))
           atomicAdd(&s.hist[(k >> shift) & 255], 1u);
@@ -180,8 +209,8 @@ __device__ void take_best(const uint32_t* ranks, int count, int n, int32_t* out,
   int gt = 0, eq = 0;
   for (int i = from + lane; i - lane < to; i += 64) {
     const uint32_t k = i < to ? ranks[i] : 0;
-    gt += __popcll(__ballot(few ? k > 0 : k > prefix));
-    if (!few) eq += __popcll(__ballot(i < to && k == prefix && k > 0));
+    gt += bits(__ballot(few ? k > 0 : k > prefix));
+    if (!few) eq += bits(__ballot(i < to && k == prefix && k > 0));
   }
   if (lane == 0) {
     s.gt[wave] = gt;
@@ -198,11 +227,11 @@ __device__ void take_best(const uint32_t* ranks, int count, int n, int32_t* out,
     const uint32_t k = i < to ? ranks[i] : 0;
     const bool up = few ? k > 0 : k > prefix, tie = !few && i < to && k == prefix && k > 0;
     const uint64_t tied = __ballot(tie);
-    const bool take = up || (tie && ties + __popcll(tied & below) < left);
+    const bool take = up || (tie && ties + bits(tied & below) < left);
     const uint64_t taken = __ballot(take);
-    if (take) out[at + __popcll(taken & below)] = i;
-    at += __popcll(taken);
-    ties += __popcll(tied);
+    if (take) out[at + bits(taken & below)] = i;
+    at += bits(taken);
+    ties += bits(tied);
   }
   int all = 0, tied = 0;
   for (int w = 0; w < kWaves; ++w) {
@@ -210,7 +239,7 @@ __device__ void take_best(const uint32_t* ranks, int count, int n, int32_t* out,
     tied += s.eq[w];
   }
   all += min(tied, left);
-  for (int i = all + threadIdx.x; i < n; i += kThreads) out[i] = -1;
+  for (int i = all + threadIdx.x; i < n; i += THREADS) out[i] = -1;
 }
 
 // Columns of a row that may be listed: up to its own block's.
@@ -222,21 +251,21 @@ __device__ __forceinline__ int columns(const KvSelectArgs& a, int64_t t, int* r,
 }
 
 // A row's ranks in LDS, then its list.
-template <bool BF16, int CH>
-__global__ __launch_bounds__(kThreads) void kv_select_kernel(KvSelectArgs a) {
+template <bool BF16, int CH, int THREADS>
+__global__ __launch_bounds__(THREADS) void kv_select_kernel(KvSelectArgs a) {
   extern __shared__ uint32_t ranks[];
-  __shared__ Select s;
+  __shared__ Select<THREADS> s;
   __shared__ __align__(16) int8_t codes[kKvMaxDim];
-  __shared__ float red[kWaves];
+  __shared__ float red[THREADS / 64];
   const int h = (int)(blockIdx.x % a.c.heads);
   const int64_t t = blockIdx.x / a.c.heads;
   int r, own;
   const int count = columns(a, t, &r, &own);
   if (count > a.n) {  // (else every candidate is taken, whatever its score)
-    query_codes<BF16>(a, t, h, codes, red);
-    rank_columns<CH>(a, h, r, own, 0, count, codes, ranks);
+    query_codes<BF16, THREADS>(a, t, h, codes, red);
+    rank_columns<CH, THREADS>(a, h, r, own, 0, count, codes, ranks);
   } else {
-    for (int j = threadIdx.x; j < count; j += kThreads) {
+    for (int j = threadIdx.x; j < count; j += THREADS) {
       const int p = a.q.table[(int64_t)r * a.q.table_stride + j];
       ranks[j] = p >= 0 && p < a.c.pages ? kAlways : 0;
     }
@@ -249,9 +278,10 @@ constexpr int kPartCols = 1024;
 
 // Long rows: ranks to the workspace, a stretch of columns a workgroup ...
 template <bool BF16, int CH>
-__global__ __launch_bounds__(kThreads) void kv_select_ranks_kernel(KvSelectArgs a, int parts) {
+__global__ __launch_bounds__(256) void kv_select_ranks_kernel(KvSelectArgs a, int parts) {
   __shared__ __align__(16) int8_t codes[kKvMaxDim];
-  __shared__ float red[kWaves];
+  __shared__ float red[4];
+  __shared__ uint32_t ranks[kPartCols];
   const int part = (int)(blockIdx.x % parts);
   const int64_t row = blockIdx.x / parts;
   const int h = (int)(row % a.c.heads);
@@ -260,44 +290,260 @@ __global__ __launch_bounds__(kThreads) void kv_select_ranks_kernel(KvSelectArgs 
   const int count = columns(a, t, &r, &own);
   const int c0 = part * kPartCols, c1 = min(count, c0 + kPartCols);
   if (c0 >= c1) return;
-  query_codes<BF16>(a, t, h, codes, red);
-  rank_columns<CH>(a, h, r, own, c0, c1, codes, a.keys + row * a.q.cols + c0);
+  query_codes<BF16, 256>(a, t, h, codes, red);
+  rank_columns<CH, 256>(a, h, r, own, c0, c1, codes, ranks);
+  __syncthreads();
+  uint32_t* out = a.keys + row * a.q.cols;
+  for (int i = threadIdx.x; i < c1 - c0; i += 256) out[c0 + i] = ranks[i];
 }
 
 // ... and the lists from there.
-__global__ __launch_bounds__(kThreads) void kv_select_lists_kernel(KvSelectArgs a) {
-  __shared__ Select s;
+__global__ __launch_bounds__(1024) void kv_select_lists_kernel(KvSelectArgs a) {
+  __shared__ Select<1024> s;
   const int64_t row = blockIdx.x;
   int r, own;
   const int count = columns(a, row / a.c.heads, &r, &own);
   take_best(a.keys + row * a.q.cols, count, a.n, a.blocks + row * a.n, s);
 }
 
-bool in_lds(const KvSelectArgs& a) {
-  return a.q.cols <= kLdsCols && (a.q.cols <= 4096 || a.q.tokens * a.c.heads >= 256);
+// Prompts: 16 tokens and a head a workgroup.  Scores are an int8 product of 16
+// blocks' summaries and the 16 tokens' codes on the 16x16x64 MFMA, ranks go to
+// LDS, and each wavefront lists the best of 4 tokens: the n-th largest rank bit
+// by bit, counting with ballots, no barrier.  NR: ranks a lane holds.
+typedef int intx4 __attribute__((ext_vector_type(4)));
+constexpr int kTile = 16;
+
+__device__ __forceinline__ intx4 mfma_i8(uintx4 x, uintx4 y, intx4 c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(intx4, x),
+                                               __builtin_bit_cast(intx4, y), c, 0, 0, 0);
+#else
+  return c;
+#endif
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int i = 32; i >= 1; i >>= 1) x = fmaxf(x, __shfl_xor(x, i));
+  return x;
+}
+
+// query_codes of one wavefront: two neighbouring values a lane (KD / 128 times).
+template <bool BF16, int KD>
+__device__ void wave_query_codes(const KvSelectArgs& a, int64_t t, int h, int8_t* codes) {
+  constexpr int P = (KD + 127) / 128;
+  const int lane = threadIdx.x & 63, g = a.q.group;
+  const uint16_t* q = (const uint16_t*)a.q.q + t * a.q.q_token + (int64_t)h * g * a.q.q_head;
+  float top = 0.0f;
+  bool good = true;
+  for (int i = 0; i < g; ++i) {
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const int d = 2 * (lane + 64 * p);
+      if (d >= a.c.dim) continue;
+      const uint32_t x = *(const uint32_t*)(q + i * a.q.q_head + d);
+      const float u = fabsf(value<BF16>((uint16_t)x)), v = fabsf(value<BF16>((uint16_t)(x >> 16)));
+      good &= u < __builtin_inff() && v < __builtin_inff();
+      top = fmaxf(top, fmaxf(u, v));
+    }
+  }
+  top = wave_max(top);
+  const float inv = __all(good) && top > 1e-30f ? 127.0f / top : 0.0f;
+  int s0[P] = {}, s1[P] = {};
+  float peak = 0.0f;
+  if (inv != 0.0f) {
+    for (int i = 0; i < g; ++i) {
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        const int d = 2 * (lane + 64 * p);
+        if (d >= a.c.dim) continue;
+        const uint32_t x = *(const uint32_t*)(q + i * a.q.q_head + d);
+        s0[p] += (int)rintf(value<BF16>((uint16_t)x) * inv);
+        s1[p] += (int)rintf(value<BF16>((uint16_t)(x >> 16)) * inv);
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < P; ++p) peak = fmaxf(peak, fmaxf((float)abs(s0[p]), (float)abs(s1[p])));
+  }
+  peak = wave_max(peak);
+  const float to = peak > 0.0f ? 127.0f / peak : 0.0f;
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int d = 2 * (lane + 64 * p);
+    if (d < KD) {
+      const int x = (int)rintf((float)s0[p] * to), y = (int)rintf((float)s1[p] * to);
+      *(uint16_t*)(codes + d) = (uint16_t)((x & 255) | (y & 255) << 8);
+    }
+  }
+}
+
+template <bool BF16, int KD, int NR>
+__global__ __launch_bounds__(256) void kv_select_tile_kernel(KvSelectArgs a) {
+  constexpr int S = 64 * NR + 4;  // (rows 4 banks apart)
+  extern __shared__ __align__(16) uint32_t ranks[];  // [kTile][S]
+  __shared__ __align__(16) int8_t codes[kTile][KD + 16];
+  __shared__ int req[kTile], cnt[kTile], own[kTile];
+  const int h = (int)(blockIdx.x % a.c.heads);
+  const int64_t t0 = (int64_t)(blockIdx.x / a.c.heads) * kTile;
+  const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (threadIdx.x < kTile) {
+    int r = -1, o = -1, n = 0;
+    if (t0 + threadIdx.x < a.q.tokens) n = columns(a, t0 + threadIdx.x, &r, &o);
+    req[threadIdx.x] = r;
+    own[threadIdx.x] = o;
+    cnt[threadIdx.x] = n;
+  }
+  for (int i = wave; i < kTile; i += 4)
+    wave_query_codes<BF16, KD>(a, min(t0 + i, a.q.tokens - 1), h, codes[i]);
+  __syncthreads();
+  uintx4 q[KD / 64];
+#pragma unroll
+  for (int i = 0; i < KD / 64; ++i) q[i] = *(const uintx4*)&codes[col][64 * i + 16 * grp];
+  const int myreq = req[col], mycnt = cnt[col], myown = own[col];
+  // the requests of the tile one after another (most often there is one)
+  for (uint64_t todo = __ballot(mycnt > 0) & 0xFFFF; todo;) {
+    const int r = __builtin_amdgcn_readlane(myreq, __builtin_ctzll(todo));
+    const bool mine = mycnt > 0 && myreq == r;
+    int most = mine ? mycnt : 0;
+#pragma unroll
+    for (int x = 1; x < 16; x *= 2) most = max(most, __shfl_xor(most, x));
+    todo &= ~__ballot(mine);
+    const int32_t* table = a.q.table + (int64_t)r * a.q.table_stride;
+    for (int j0 = 16 * wave; j0 < most; j0 += 64) {
+      const int p = j0 + col < most ? table[j0 + col] : -1;
+      const bool there = p >= 0 && p < a.c.pages;
+      const int64_t row = (int64_t)p * a.c.heads + h;
+      intx4 dot = {0, 0, 0, 0};
+      const int8_t* m = a.c.summaries + row * a.c.dim + 16 * grp;
+      float scale = 0.0f;
+      if (there) scale = a.c.scales[row];
+#pragma unroll
+      for (int i = 0; i < KD / 64; ++i) {
+        uintx4 v = {};
+        if (there && 64 * i + 16 * grp < a.c.dim) v = *(const uintx4*)(m + 64 * i);
+        dot = mfma_i8(v, q[i], dot);
+      }
+      const uint32_t present = (uint32_t)__ballot(there);
+      uintx4 k;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = j0 + 4 * grp + i;
+        const float s = __shfl(scale, 4 * grp + i);
+        k[i] = !(present >> (4 * grp + i) & 1)           ? 0
+               : j < a.first || j > myown - a.last ? kAlways
+                                                         : rank_of(dot[i], s);
+      }
+      if (mine) *(uintx4*)&ranks[col * S + j0 + 4 * grp] = k;
+    }
+  }
+  __syncthreads();
+  const uint64_t below = (uint64_t(1) << lane) - 1;
+  for (int i = wave; i < kTile; i += 4) {
+    const int64_t t = t0 + i;
+    if (t >= a.q.tokens) break;
+    const int count = cnt[i];
+    uint32_t k[NR];
+#pragma unroll
+    for (int x = 0; x < NR; ++x)
+      k[x] = 64 * x + lane < count ? ranks[i * S + 64 * x + lane] : 0;
+    // cut: all ranks from it on are taken, the first `ties` of those equal to
+    // it only
+    uint32_t cut = 1;
+    int ties = 64 * NR;
+    if (count > a.n) {
+      cut = 0;
+      int upto = 0;  // ranks at or above cut
+      for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t c = cut | 1u << bit;
+        int n = 0;
+#pragma unroll
+        for (int x = 0; x < NR; ++x) n += bits(__ballot(k[x] >= c));
+        if (n >= a.n) {
+          cut = c;
+          upto = n;
+          if (n == a.n) break;
+        }
+      }
+      if (cut == 0) cut = 1;  // (absent blocks: fewer candidates than n)
+      else if (upto > a.n) {
+        int above = 0;
+#pragma unroll
+        for (int x = 0; x < NR; ++x) above += bits(__ballot(k[x] > cut));
+        ties = a.n - above;
+      }
+    }
+    int32_t* out = a.blocks + (t * a.c.heads + h) * a.n;
+    int at = 0;
+#pragma unroll
+    for (int x = 0; x < NR; ++x) {
+      const uint64_t tied = __ballot(k[x] == cut);
+      const bool take = k[x] > cut || (k[x] == cut && bits(tied & below) < ties);
+      const uint64_t taken = __ballot(take);
+      if (take) out[at + bits(taken & below)] = 64 * x + lane;
+      at += bits(taken);
+      ties -= bits(tied);
+    }
+    for (int x = at + lane; x < a.n; x += 64) out[x] = -1;
+  }
+}
+
+// Ways to list (measured in us a call): a row a workgroup, its ranks in LDS; in
+// two launches over the workspace where rows are few and long; 16 tokens a
+// workgroup where a request has many.
+enum class Way { kRow, kParts, kTile };
+
+constexpr int kTileCols = 64 * 14;  // ranks of 16 tokens in 58 KB of LDS
+
+Way way_of(const KvSelectArgs& a) {
+  if (a.c.dim % 16 == 0 && a.q.cols <= kTileCols && a.q.tokens >= 8 * a.q.requests)
+    return Way::kTile;
+  if (a.q.cols <= 4096 || (a.q.cols <= kLdsCols && a.q.tokens * a.c.heads >= 256))
+    return Way::kRow;
+  return Way::kParts;
+}
+
+template <bool BF16, int KD>
+void launch_tile(const KvSelectArgs& a, hipStream_t s) {
+  const unsigned grid = (unsigned)((a.q.tokens + kTile - 1) / kTile * a.c.heads);
+  if (a.q.cols <= 256)
+    kv_select_tile_kernel<BF16, KD, 4><<<grid, 256, kTile * (64 * 4 + 4) * 4, s>>>(a);
+  else if (a.q.cols <= 512)
+    kv_select_tile_kernel<BF16, KD, 8><<<grid, 256, kTile * (64 * 8 + 4) * 4, s>>>(a);
+  else
+    kv_select_tile_kernel<BF16, KD, 14><<<grid, 256, kTile * (64 * 14 + 4) * 4, s>>>(a);
 }
 
 template <bool BF16, int CH>
 void launch_select(const KvSelectArgs& a, hipStream_t s) {
   const unsigned rows = (unsigned)(a.q.tokens * a.c.heads);
-  if (in_lds(a)) {
-    kv_select_kernel<BF16, CH><<<rows, kThreads, a.q.cols * 4, s>>>(a);
-    return;
+  switch (way_of(a)) {
+    case Way::kTile:
+      if (a.c.dim <= 64) launch_tile<BF16, 64>(a, s);
+      else if (a.c.dim <= 128) launch_tile<BF16, 128>(a, s);
+      else launch_tile<BF16, 256>(a, s);
+      return;
+    case Way::kRow:
+      if (rows < 512) kv_select_kernel<BF16, CH, 1024><<<rows, 1024, a.q.cols * 4, s>>>(a);
+      else kv_select_kernel<BF16, CH, 256><<<rows, 256, a.q.cols * 4, s>>>(a);
+      return;
+    case Way::kParts:
+      const int parts = (a.q.cols + kPartCols - 1) / kPartCols;
+      kv_select_ranks_kernel<BF16, CH><<<rows * parts, 256, 0, s>>>(a, parts);
+      kv_select_lists_kernel<<<rows, 1024, 0, s>>>(a);
   }
-  const int parts = (a.q.cols + kPartCols - 1) / kPartCols;
-  kv_select_ranks_kernel<BF16, CH><<<rows * parts, kThreads, 0, s>>>(a, parts);
-  kv_select_lists_kernel<<<rows, kThreads, 0, s>>>(a);
 }
 
 }  // namespace
 
 int64_t kv_select_workspace(const KvSelectArgs& a) {
-  return in_lds(a) ? 0 : a.q.tokens * a.c.heads * a.q.cols * 4;
+  return way_of(a) == Way::kParts ? a.q.tokens * a.c.heads * a.q.cols * 4 : 0;
 }
 
 int64_t kv_select_grid(const KvSelectArgs& a) {
+  // (in workgroups of 256)
   const int64_t rows = a.q.tokens * a.c.heads;
-  return in_lds(a) ? rows : rows * ((a.q.cols + kPartCols - 1) / kPartCols);
+  return way_of(a) == Way::kParts ? rows * ((a.q.cols + kPartCols - 1) / kPartCols) : 4 * rows;
 }
 
 hipError_t launch_kv_select(const KvSelectArgs& a, hipStream_t s) {

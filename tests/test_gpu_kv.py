@@ -286,6 +286,27 @@ def test_select_for_the_tokens_of_prompts(engine, tokens):
         check_select(engine, q, codes, scales, table, who, positions, page, n)
 
 
+@pytest.mark.parametrize("cols,heads,group,d", [(255, 2, 3, 80), (300, 1, 16, 16), (512, 2, 2, 256),
+                                                (513, 1, 5, 64), (896, 2, 1, 128), (897, 1, 2, 48),
+                                                (300, 1, 2, 72)])
+def test_select_for_prompts_among_many_blocks(engine, cols, heads, group, d):
+    rng = np.random.default_rng(cols)
+    codes, scales = summaries(rng, 950, heads, d)
+    scales[5], scales[9] = np.inf, 0.0
+    codes[100:200] = codes[100]  # ties
+    scales[100:200] = scales[100]
+    table = rng.integers(-3, 960, (2, cols)).astype(np.int32)
+    tokens = 45
+    who = np.repeat([0, 1, 0, 7], [17, 20, 7, 1])
+    positions = rng.integers(0, cols * 16, tokens)
+    positions[:20] = cols * 16 - 1 - np.arange(20)
+    positions[30] = -1
+    q = dev(rng.standard_normal((tokens, heads * group, d), np.float32)).half()
+    q[3, 0, 1], q[4] = float("inf"), 0.0
+    for n in (2, 33, 256):
+        check_select(engine, q, codes, scales, table, who, positions, 16, n)
+
+
 @pytest.mark.parametrize("cols", [4096, 4097, 9000])
 def test_select_among_many_blocks(engine, cols):
     rng = np.random.default_rng(cols)
