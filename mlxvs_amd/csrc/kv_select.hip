@@ -46,6 +46,16 @@ __device__ __forceinline__ uint32_t rank_of(int dot, float scale) {
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
+// |x|, infinity for what is not finite (a NaN would get lost in a maximum).
+__device__ __forceinline__ float finite_abs(float x) {
+  x = fabsf(x);
+  return x < __builtin_inff() ? x : __builtin_inff();
+}
+// The factor that takes values of at most `top` to codes, 0 where there is none.
+__device__ __forceinline__ float to_codes(float top) {
+  return top > 1e-30f && top < __builtin_inff() ? 127.0f / top : 0.0f;
+}
+
 template <int THREADS>
 __device__ __forceinline__ float block_max(float x, float* shared) {
 #pragma unroll
@@ -66,21 +76,16 @@ __device__ void query_codes(const KvSelectArgs& a, int64_t t, int h, int8_t* cod
                             float* shared) {
   const int d = threadIdx.x, g = a.q.group;
   const uint16_t* q = (const uint16_t*)a.q.q + t * a.q.q_token + (int64_t)h * g * a.q.q_head + d;
-  float top = 0.0f, bad = 0.0f;
+  float top = 0.0f;
   if (d < a.c.dim) {
-#pragma unroll 4
-    for (int i = 0; i < g; ++i) {
-      const float x = fabsf(value<BF16>(q[i * a.q.q_head]));
-      if (!(x < __builtin_inff())) bad = 1.0f;
-      top = fmaxf(top, x);
-    }
+#pragma unroll 8
+    for (int i = 0; i < g; ++i) top = fmaxf(top, finite_abs(value<BF16>(q[i * a.q.q_head])));
   }
   top = block_max<THREADS>(top, shared);
-  bad = block_max<THREADS>(bad, shared);
-  const float inv = bad == 0.0f && top > 1e-30f ? 127.0f / top : 0.0f;
+  const float inv = to_codes(top);
   int sum = 0;
   if (d < a.c.dim && inv != 0.0f) {
-#pragma unroll 4
+#pragma unroll 8
     for (int i = 0; i < g; ++i) sum += (int)rintf(value<BF16>(q[i * a.q.q_head]) * inv);
   }
   const float peak = block_max<THREADS>((float)abs(sum), shared);
@@ -93,7 +98,7 @@ __device__ void query_codes(const KvSelectArgs& a, int64_t t, int h, int8_t* cod
 // group adding up their parts of its dot product.  The page ids pass through
 // ranks first, so that a thread has kAhead summaries in flight at a time.  CH:
 // bytes a lane loads.
-constexpr int kAhead = 4;
+constexpr int kAhead = 8;
 
 template <int CH, int THREADS>
 __device__ void rank_columns(const KvSelectArgs& a, int h, int r, int own, int c0, int c1,
@@ -308,7 +313,7 @@ __global__ __launch_bounds__(1024) void kv_select_lists_kernel(KvSelectArgs a) {
 
 // Prompts: 16 tokens and a head a workgroup.  Scores are an int8 product of 16
 // blocks' summaries and the 16 tokens' codes on the 16x16x64 MFMA, ranks go to
-// LDS, and each wavefront lists the best of 4 tokens: the n-th largest rank bit
+// LDS, and each wavefront lists the best of 2 tokens: the n-th largest rank bit
 // by bit, counting with ballots, no barrier.  NR: ranks a lane holds.
 typedef int intx4 __attribute__((ext_vector_type(4)));
 constexpr int kTile = 16;
@@ -328,57 +333,71 @@ __device__ __forceinline__ float wave_max(float x) {
   return x;
 }
 
-// query_codes of one wavefront: two neighbouring values a lane (KD / 128 times).
-template <bool BF16, int KD>
-__device__ void wave_query_codes(const KvSelectArgs& a, int64_t t, int h, int8_t* codes) {
-  constexpr int P = (KD + 127) / 128;
+// query_codes of a wavefront's tokens t0, t0 + step, ..: two neighbouring values
+// a lane (KD / 128 times), the loads of all tokens and eight heads in flight.
+template <bool BF16, int KD, int NT>
+__device__ void wave_query_codes(const KvSelectArgs& a, int64_t t0, int step, int h,
+                                 int8_t* codes, int stride) {
+  constexpr int P = (KD + 127) / 128, HEADS = 8;
   const int lane = threadIdx.x & 63, g = a.q.group;
-  const uint16_t* q = (const uint16_t*)a.q.q + t * a.q.q_token + (int64_t)h * g * a.q.q_head;
-  float top = 0.0f;
-  bool good = true;
-  for (int i = 0; i < g; ++i) {
+  const uint16_t* q[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+    q[t] = (const uint16_t*)a.q.q + min(t0 + t * step, a.q.tokens - 1) * a.q.q_token +
+           (int64_t)h * g * a.q.q_head;
+  const auto each = [&](auto&& f) {
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       const int d = 2 * (lane + 64 * p);
       if (d >= a.c.dim) continue;
-      const uint32_t x = *(const uint32_t*)(q + i * a.q.q_head + d);
-      const float u = fabsf(value<BF16>((uint16_t)x)), v = fabsf(value<BF16>((uint16_t)(x >> 16)));
-      good &= u < __builtin_inff() && v < __builtin_inff();
-      top = fmaxf(top, fmaxf(u, v));
-    }
-  }
-  top = wave_max(top);
-  const float inv = __all(good) && top > 1e-30f ? 127.0f / top : 0.0f;
-  int s0[P] = {}, s1[P] = {};
-  float peak = 0.0f;
-  if (inv != 0.0f) {
-    for (int i = 0; i < g; ++i) {
+      for (int i0 = 0; i0 < g; i0 += HEADS) {
+        uint32_t x[NT][HEADS];
 #pragma unroll
-      for (int p = 0; p < P; ++p) {
-        const int d = 2 * (lane + 64 * p);
-        if (d >= a.c.dim) continue;
-        const uint32_t x = *(const uint32_t*)(q + i * a.q.q_head + d);
-        s0[p] += (int)rintf(value<BF16>((uint16_t)x) * inv);
-        s1[p] += (int)rintf(value<BF16>((uint16_t)(x >> 16)) * inv);
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < HEADS; ++i)  // (past the last head: zeros, which add nothing)
+            x[t][i] = i0 + i < g ? *(const uint32_t*)(q[t] + (i0 + i) * a.q.q_head + d) : 0;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < HEADS; ++i)
+            f(t, p, value<BF16>((uint16_t)x[t][i]), value<BF16>((uint16_t)(x[t][i] >> 16)));
       }
     }
+  };
+  float inv[NT] = {}, peak[NT] = {};
+  int s0[NT][P] = {}, s1[NT][P] = {};
+  each([&](int t, int, float u, float v) {
+    inv[t] = fmaxf(inv[t], fmaxf(finite_abs(u), finite_abs(v)));
+  });
 #pragma unroll
-    for (int p = 0; p < P; ++p) peak = fmaxf(peak, fmaxf((float)abs(s0[p]), (float)abs(s1[p])));
-  }
-  peak = wave_max(peak);
-  const float to = peak > 0.0f ? 127.0f / peak : 0.0f;
+  for (int t = 0; t < NT; ++t) inv[t] = to_codes(wave_max(inv[t]));
+  each([&](int t, int p, float u, float v) {
+    // (a factor of 0 belongs to values that may not be finite)
+    s0[t][p] += inv[t] != 0.0f ? (int)rintf(u * inv[t]) : 0;
+    s1[t][p] += inv[t] != 0.0f ? (int)rintf(v * inv[t]) : 0;
+  });
 #pragma unroll
-  for (int p = 0; p < P; ++p) {
-    const int d = 2 * (lane + 64 * p);
-    if (d < KD) {
-      const int x = (int)rintf((float)s0[p] * to), y = (int)rintf((float)s1[p] * to);
-      *(uint16_t*)(codes + d) = (uint16_t)((x & 255) | (y & 255) << 8);
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+      peak[t] = fmaxf(peak[t], fmaxf((float)abs(s0[t][p]), (float)abs(s1[t][p])));
+    peak[t] = wave_max(peak[t]);
+    const float to = peak[t] > 0.0f ? 127.0f / peak[t] : 0.0f;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const int d = 2 * (lane + 64 * p);
+      if (d < KD) {
+        const int x = (int)rintf((float)s0[t][p] * to), y = (int)rintf((float)s1[t][p] * to);
+        *(uint16_t*)(codes + t * step * stride + d) = (uint16_t)((x & 255) | (y & 255) << 8);
+      }
     }
   }
 }
 
 template <bool BF16, int KD, int NR>
-__global__ __launch_bounds__(256) void kv_select_tile_kernel(KvSelectArgs a) {
+__global__ __launch_bounds__(512) void kv_select_tile_kernel(KvSelectArgs a) {
+  constexpr int W = 8;
   constexpr int S = 64 * NR + 4;  // (rows 4 banks apart)
   extern __shared__ __align__(16) uint32_t ranks[];  // [kTile][S]
   __shared__ __align__(16) int8_t codes[kTile][KD + 16];
@@ -394,8 +413,7 @@ __global__ __launch_bounds__(256) void kv_select_tile_kernel(KvSelectArgs a) {
     own[threadIdx.x] = o;
     cnt[threadIdx.x] = n;
   }
-  for (int i = wave; i < kTile; i += 4)
-    wave_query_codes<BF16, KD>(a, min(t0 + i, a.q.tokens - 1), h, codes[i]);
+  wave_query_codes<BF16, KD, kTile / W>(a, t0 + wave, W, h, codes[wave], KD + 16);
   __syncthreads();
   uintx4 q[KD / 64];
 #pragma unroll
@@ -410,7 +428,8 @@ __global__ __launch_bounds__(256) void kv_select_tile_kernel(KvSelectArgs a) {
     for (int x = 1; x < 16; x *= 2) most = max(most, __shfl_xor(most, x));
     todo &= ~__ballot(mine);
     const int32_t* table = a.q.table + (int64_t)r * a.q.table_stride;
-    for (int j0 = 16 * wave; j0 < most; j0 += 64) {
+    #pragma unroll 2
+    for (int j0 = 16 * wave; j0 < most; j0 += 16 * W) {
       const int p = j0 + col < most ? table[j0 + col] : -1;
       const bool there = p >= 0 && p < a.c.pages;
       const int64_t row = (int64_t)p * a.c.heads + h;
@@ -439,7 +458,7 @@ __global__ __launch_bounds__(256) void kv_select_tile_kernel(KvSelectArgs a) {
   }
   __syncthreads();
   const uint64_t below = (uint64_t(1) << lane) - 1;
-  for (int i = wave; i < kTile; i += 4) {
+  for (int i = wave; i < kTile; i += W) {
     const int64_t t = t0 + i;
     if (t >= a.q.tokens) break;
     const int count = cnt[i];
@@ -507,11 +526,11 @@ template <bool BF16, int KD>
 void launch_tile(const KvSelectArgs& a, hipStream_t s) {
   const unsigned grid = (unsigned)((a.q.tokens + kTile - 1) / kTile * a.c.heads);
   if (a.q.cols <= 256)
-    kv_select_tile_kernel<BF16, KD, 4><<<grid, 256, kTile * (64 * 4 + 4) * 4, s>>>(a);
+    kv_select_tile_kernel<BF16, KD, 4><<<grid, 512, kTile * (64 * 4 + 4) * 4, s>>>(a);
   else if (a.q.cols <= 512)
-    kv_select_tile_kernel<BF16, KD, 8><<<grid, 256, kTile * (64 * 8 + 4) * 4, s>>>(a);
+    kv_select_tile_kernel<BF16, KD, 8><<<grid, 512, kTile * (64 * 8 + 4) * 4, s>>>(a);
   else
-    kv_select_tile_kernel<BF16, KD, 14><<<grid, 256, kTile * (64 * 14 + 4) * 4, s>>>(a);
+    kv_select_tile_kernel<BF16, KD, 14><<<grid, 512, kTile * (64 * 14 + 4) * 4, s>>>(a);
 }
 
 template <bool BF16, int CH>
