@@ -94,62 +94,233 @@ __device__ void query_codes(const KvSelectArgs& a, int64_t t, int h, int8_t* cod
   __syncthreads();
 }
 
-// Ranks of the columns [c0, c1) of a row into ranks[0 ..], lanes of a page's
-// group adding up their parts of its dot product.  The page ids pass through
-// ranks first, so that a thread has kAhead summaries in flight at a time.  CH:
-// bytes a lane loads.
-constexpr int kAhead = 8;
+typedef int intx4 __attribute__((ext_vector_type(4)));
 
-template <int CH, int THREADS>
-__device__ void rank_columns(const KvSelectArgs& a, int h, int r, int own, int c0, int c1,
-                             const int8_t* codes, uint32_t* ranks) {
-  const int d = a.c.dim, chunks = d / CH, count = c1 - c0;
-  for (int i = threadIdx.x; i < count; i += THREADS)
-    ranks[i] = (uint32_t)a.q.table[(int64_t)r * a.q.table_stride + c0 + i];
-  int lanes = 1;
-  while (lanes < chunks) lanes *= 2;
-  const int at = threadIdx.x % lanes, per = THREADS / lanes;
-  uint32_t q[CH / 4];
+__device__ __forceinline__ intx4 mfma_i8(uintx4 x, uintx4 y, intx4 c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(intx4, x),
+                                               __builtin_bit_cast(intx4, y), c, 0, 0, 0);
+#else
+  return c;
+#endif
+}
+
+__device__ __forceinline__ float wave_max(float x) {
 #pragma unroll
-  for (int i = 0; i < CH / 4; ++i)
-    q[i] = at < chunks ? *(const uint32_t*)(codes + CH * at + 4 * i) : 0;
-  __syncthreads();
-  for (int j0 = threadIdx.x / lanes; j0 - (int)threadIdx.x / lanes < count; j0 += kAhead * per) {
-    uint32_t v[kAhead][CH / 4];
-    float scale[kAhead];
-    bool there[kAhead];
+  for (int i = 32; i >= 1; i >>= 1) x = fmaxf(x, __shfl_xor(x, i));
+  return x;
+}
+
+// query_codes of a wavefront's tokens t0, t0 + step, ..: two neighbouring values
+// a lane (KD / 128 times), the loads of all tokens and eight heads in flight.
+template <bool BF16, int KD, int NT>
+__device__ void wave_query_codes(const KvSelectArgs& a, int64_t t0, int step, int h,
+                                 int8_t* codes, int stride) {
+  constexpr int P = (KD + 127) / 128, HEADS = 8;
+  const int lane = threadIdx.x & 63, g = a.q.group;
+  const uint16_t* q[NT];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int j = j0 + u * per;
-      const int p = j < count ? (int)ranks[j] : -1;
-      there[u] = p >= 0 && p < a.c.pages;
-      const int64_t row = (int64_t)p * a.c.heads + h;
-      scale[u] = 0.0f;
+  for (int t = 0; t < NT; ++t)
+    q[t] = (const uint16_t*)a.q.q + min(t0 + t * step, a.q.tokens - 1) * a.q.q_token +
+           (int64_t)h * g * a.q.q_head;
+  const auto each = [&](auto&& f) {
 #pragma unroll
-      for (int i = 0; i < CH / 4; ++i) v[u][i] = 0;
-      if (there[u]) {
-        if (at < chunks) {
-          const int8_t* m = a.c.summaries + row * d + CH * at;
-          if constexpr (CH == 16) *(uintx4*)v[u] = *(const uintx4*)m;
-          else *(uintx2*)v[u] = *(const uintx2*)m;
-        }
-        if (at == 0) scale[u] = a.c.scales[row];
+    for (int p = 0; p < P; ++p) {
+      const int d = 2 * (lane + 64 * p);
+      if (d >= a.c.dim) continue;
+      for (int i0 = 0; i0 < g; i0 += HEADS) {
+        uint32_t x[NT][HEADS];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < HEADS; ++i)  // (past the last head: zeros, which add nothing)
+            x[t][i] = i0 + i < g ? *(const uint32_t*)(q[t] + (i0 + i) * a.q.q_head + d) : 0;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < HEADS; ++i)
+            f(t, p, value<BF16>((uint16_t)x[t][i]), value<BF16>((uint16_t)(x[t][i] >> 16)));
       }
     }
+  };
+  float inv[NT] = {}, peak[NT] = {};
+  int s0[NT][P] = {}, s1[NT][P] = {};
+  each([&](int t, int, float u, float v) {
+    inv[t] = fmaxf(inv[t], fmaxf(finite_abs(u), finite_abs(v)));
+  });
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      int dot = 0;
+  for (int t = 0; t < NT; ++t) inv[t] = to_codes(wave_max(inv[t]));
+  each([&](int t, int p, float u, float v) {
+    // (a factor of 0 belongs to values that may not be finite)
+    s0[t][p] += inv[t] != 0.0f ? (int)rintf(u * inv[t]) : 0;
+    s1[t][p] += inv[t] != 0.0f ? (int)rintf(v * inv[t]) : 0;
+  });
 #pragma unroll
-      for (int i = 0; i < CH / 4; ++i) dot = __builtin_amdgcn_sdot4((int)v[u][i], (int)q[i], dot, false);
-      for (int x = 1; x < lanes; x *= 2) dot += __shfl_xor(dot, x);
-      const int j = j0 + u * per, c = c0 + j;
-      // (the group's other lanes have read the page id: they are of one wavefront)
-      if (at == 0 && j < count)
-        ranks[j] = !there[u]                          ? 0
-                   : c < a.first || c > own - a.last ? kAlways
-                                                      : rank_of(dot, scale[u]);
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+      peak[t] = fmaxf(peak[t], fmaxf((float)abs(s0[t][p]), (float)abs(s1[t][p])));
+    peak[t] = wave_max(peak[t]);
+    const float to = peak[t] > 0.0f ? 127.0f / peak[t] : 0.0f;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const int d = 2 * (lane + 64 * p);
+      if (d < KD) {
+        const int x = (int)rintf((float)s0[t][p] * to), y = (int)rintf((float)s1[t][p] * to);
+        *(uint16_t*)(codes + t * step * stride + d) = (uint16_t)((x & 255) | (y & 255) << 8);
+      }
     }
   }
+}
+
+// Scores of 16 columns' blocks a step, by one wavefront: their summaries are the
+// rows of the 16x16x64 int8 MFMA (lane l: 16 bytes of the block of column l %
+// 16), the codes of 16 queries, or one sixteen times, its columns.  KD: head
+// size rounded up to a multiple of 64.  A16: rows of summaries are 16-byte
+// aligned (else 8).  AHEAD steps are in flight at a time, each `stride` columns
+// and `heads` heads past the one before; those from `steps` on are empty.
+template <int KD, bool A16, int AHEAD>
+struct BlockScores {
+  uintx4 v[AHEAD][KD / 64];
+  float scale[AHEAD];
+  uint32_t present[AHEAD];  // bit m: column m of the step has a page
+
+  __device__ __forceinline__ void load(const KvSelectArgs& a, int h, const int32_t* table, int j0,
+                                       int stride, int count, int heads = 0, int steps = AHEAD) {
+    const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+    int p[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int j = j0 + u * stride + col;
+      p[u] = j < count && u < steps ? table[j] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const bool there = p[u] >= 0 && p[u] < a.c.pages;
+      const int64_t row = (int64_t)p[u] * a.c.heads + h + u * heads;
+      const int8_t* m = a.c.summaries + row * a.c.dim;
+      scale[u] = 0.0f;
+      if (there) scale[u] = a.c.scales[row];
+#pragma unroll
+      for (int i = 0; i < KD / 64; ++i) {
+        const int at = 64 * i + 16 * grp;
+        v[u][i] = uintx4{};
+        if constexpr (A16) {
+          if (there && at < a.c.dim) v[u][i] = *(const uintx4*)(m + at);
+        } else {
+          if (there && at < a.c.dim) *(uintx2*)&v[u][i] = *(const uintx2*)(m + at);
+          if (there && at + 8 < a.c.dim) *((uintx2*)&v[u][i] + 1) = *(const uintx2*)(m + at + 8);
+        }
+      }
+      present[u] = (uint32_t)__ballot(there);
+    }
+  }
+
+  // The ranks of step u under one query, its codes in all 16 columns: columns j0
+  // .. of a row of `count`, up to the block `own`.
+  __device__ __forceinline__ void put(const KvSelectArgs& a, int u, const uintx4 (&codes)[KD / 64],
+                                      int own, int j0, int count, uint32_t* ranks) const {
+    const intx4 d = dots(u, codes);
+    // the 16 columns of the product are alike: lane l ranks row 4 grp + l % 4
+    const int lane = threadIdx.x & 63, i = lane & 3, m = 4 * (lane >> 4) + i, j = j0 + m;
+    const float s = __shfl(scale[u], m);
+    const int dot = i & 2 ? (i & 1 ? d[3] : d[2]) : (i & 1 ? d[1] : d[0]);
+    if ((lane & 15) < 4 && j < count)
+      ranks[j] = !(present[u] >> m & 1)              ? 0
+                 : j < a.first || j > own - a.last ? kAlways
+                                                     : rank_of(dot, s);
+  }
+
+  // Row 4 grp + i of step u: its dot product with the lane's column of codes.
+  __device__ __forceinline__ intx4 dots(int u, const uintx4 (&codes)[KD / 64]) const {
+    intx4 d = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < KD / 64; ++i) d = mfma_i8(v[u][i], codes[i], d);
+    return d;
+  }
+};
+
+template <int KD>
+__device__ __forceinline__ void load_codes(uintx4 (&q)[KD / 64], const int8_t* codes) {
+#pragma unroll
+  for (int i = 0; i < KD / 64; ++i)
+    q[i] = *(const uintx4*)(codes + 64 * i + 16 * ((threadIdx.x & 63) >> 4));
+}
+
+// Ranks of the columns [0, count) of one query into LDS.  make() leaves its
+// codes in `codes` (it waits for the workgroup) while the first summaries are
+// on their way.
+template <int KD, bool A16, int AHEAD, int THREADS, typename Make>
+__device__ void rank_row(const KvSelectArgs& a, int h, int own, const int32_t* table, int count,
+                         const int8_t* codes, uint32_t* ranks, Make make) {
+  constexpr int STRIDE = 16 * (THREADS / 64);
+  int j0 = 16 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  BlockScores<KD, A16, AHEAD> b;
+  b.load(a, h, table, j0, STRIDE, count);
+  make();
+  uintx4 q[KD / 64];
+  load_codes<KD>(q, codes);
+  while (j0 < count) {
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) b.put(a, u, q, own, j0 + u * STRIDE, count, ranks);
+    j0 += AHEAD * STRIDE;
+    if (j0 < count) b.load(a, h, table, j0, STRIDE, count);
+  }
+}
+
+// The n largest of a wavefront's ranks (64 x + lane: k[x]), the lowest columns
+// among equal ones, ascending by column into out, -1 after.  The n-th largest
+// is found bit by bit, counting with ballots: no barrier.
+template <int NR>
+__device__ void wave_take_best(const uint32_t (&k)[NR], int count, int n, int32_t* out) {
+  const int lane = threadIdx.x & 63;
+  // all ranks from `cut` on are taken, of those equal to it the first `ties`
+  uint32_t cut = 1;
+  int ties = 64 * NR;
+  if (count > n) {
+    cut = 0;
+    int upto = 0;  // ranks at or above cut
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t c = cut | 1u << bit;
+      int m = 0;
+#pragma unroll
+      for (int x = 0; x < NR; ++x) m += bits(__ballot(k[x] >= c));
+      if (m >= n) {
+        cut = c;
+        upto = m;
+        if (m == n) break;
+      }
+    }
+    if (cut == 0) {
+      cut = 1;  // (absent blocks: fewer candidates than n)
+    } else if (upto > n) {
+      int above = 0;
+#pragma unroll
+      for (int x = 0; x < NR; ++x) above += bits(__ballot(k[x] > cut));
+      ties = n - above;
+    }
+  }
+  const uint64_t below = (uint64_t(1) << lane) - 1;
+  int at = 0;
+#pragma unroll
+  for (int x = 0; x < NR; ++x) {
+    const uint64_t tied = __ballot(k[x] == cut);
+    const bool take = k[x] > cut || (k[x] == cut && bits(tied & below) < ties);
+    const uint64_t taken = __ballot(take);
+    if (take) out[at + bits(taken & below)] = 64 * x + lane;
+    at += bits(taken);
+    ties -= bits(tied);
+  }
+  for (int x = at + lane; x < n; x += 64) out[x] = -1;
+}
+
+template <int NR>
+__device__ void wave_take_best(const uint32_t* ranks, int count, int n, int32_t* out) {
+  const int lane = threadIdx.x & 63;
+  uint32_t k[NR];
+#pragma unroll
+  for (int x = 0; x < NR; ++x) k[x] = 64 * x + lane < count ? ranks[64 * x + lane] : 0;
+  wave_take_best(k, count, n, out);
 }
 
 template <int THREADS>
@@ -248,15 +419,18 @@ __device__ void take_best(const uint32_t* ranks, int count, int n, int32_t* out,
 }
 
 // Columns of a row that may be listed: up to its own block's.
-__device__ __forceinline__ int columns(const KvSelectArgs& a, int64_t t, int* r, int* own) {
+__device__ __forceinline__ int columns_of(const KvSelectArgs& a, int64_t t, int* r, int* own) {
   *r = a.q.token_request[t];
   const int pos = a.q.positions[t];
   *own = pos >= 0 ? pos >> a.c.lps : -1;
   return *r >= 0 && *r < a.q.requests ? min(*own + 1, a.q.cols) : 0;
 }
 
+// Steps in flight (registers: 16 bytes a step and 64 values).
+constexpr int ahead(int kd) { return kd == 256 ? 4 : 8; }
+
 // A row's ranks in LDS, then its list.
-template <bool BF16, int CH, int THREADS>
+template <bool BF16, int KD, bool A16, int THREADS>
 __global__ __launch_bounds__(THREADS) void kv_select_kernel(KvSelectArgs a) {
   extern __shared__ uint32_t ranks[];
   __shared__ Select<THREADS> s;
@@ -265,13 +439,15 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(KvSelectArgs a) {
   const int h = (int)(blockIdx.x % a.c.heads);
   const int64_t t = blockIdx.x / a.c.heads;
   int r, own;
-  const int count = columns(a, t, &r, &own);
+  const int count = columns_of(a, t, &r, &own);
+  const int32_t* table = a.q.table + (int64_t)r * a.q.table_stride;
   if (count > a.n) {  // (else every candidate is taken, whatever its score)
-    query_codes<BF16, THREADS>(a, t, h, codes, red);
-    rank_columns<CH, THREADS>(a, h, r, own, 0, count, codes, ranks);
+    rank_row<KD, A16, ahead(KD), THREADS>(
+        a, h, own, table, count, codes, ranks,
+        [&] { query_codes<BF16, THREADS>(a, t, h, codes, red); });
   } else {
     for (int j = threadIdx.x; j < count; j += THREADS) {
-      const int p = a.q.table[(int64_t)r * a.q.table_stride + j];
+      const int p = table[j];
       ranks[j] = p >= 0 && p < a.c.pages ? kAlways : 0;
     }
   }
@@ -279,126 +455,62 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(KvSelectArgs a) {
   take_best(ranks, count, a.n, a.blocks + (t * a.c.heads + h) * a.n, s);
 }
 
-constexpr int kPartCols = 1024;
+// Long rows: ranks to the workspace, 128 columns of up to 8 heads a workgroup
+// (a page's summaries and scales lie side by side over its heads), 16 columns a
+// wavefront ...
+constexpr int kPartCols = 128, kPartHeads = 8;
 
-// Long rows: ranks to the workspace, a stretch of columns a workgroup ...
-template <bool BF16, int CH>
-__global__ __launch_bounds__(256) void kv_select_ranks_kernel(KvSelectArgs a, int parts) {
-  __shared__ __align__(16) int8_t codes[kKvMaxDim];
-  __shared__ float red[4];
-  __shared__ uint32_t ranks[kPartCols];
+template <bool BF16, int KD, bool A16>
+__global__ __launch_bounds__(512) void kv_select_ranks_kernel(KvSelectArgs a, int parts) {
+  __shared__ __align__(16) int8_t codes[kPartHeads][KD + 16];
   const int part = (int)(blockIdx.x % parts);
-  const int64_t row = blockIdx.x / parts;
-  const int h = (int)(row % a.c.heads);
-  const int64_t t = row / a.c.heads;
+  const int sets = (a.c.heads + kPartHeads - 1) / kPartHeads;
+  const int h0 = (int)(blockIdx.x / parts % sets) * kPartHeads;
+  const int64_t t = blockIdx.x / parts / sets;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int heads = min(kPartHeads, a.c.heads - h0);
   int r, own;
-  const int count = columns(a, t, &r, &own);
-  const int c0 = part * kPartCols, c1 = min(count, c0 + kPartCols);
-  if (c0 >= c1) return;
-  query_codes<BF16, 256>(a, t, h, codes, red);
-  rank_columns<CH, 256>(a, h, r, own, c0, c1, codes, ranks);
+  const int count = columns_of(a, t, &r, &own);
+  if (part * kPartCols >= count) return;
+  const int j0 = part * kPartCols + 16 * wave;
+  BlockScores<KD, A16, kPartHeads> b;
+  b.load(a, h0, a.q.table + (int64_t)r * a.q.table_stride, j0, 0, count, 1, heads);
+  if (wave < heads) wave_query_codes<BF16, KD, 1>(a, t, 0, h0 + wave, codes[wave], 0);
   __syncthreads();
-  uint32_t* out = a.keys + row * a.q.cols;
-  for (int i = threadIdx.x; i < c1 - c0; i += 256) out[c0 + i] = ranks[i];
+#pragma unroll
+  for (int u = 0; u < kPartHeads; ++u) {
+    if (u >= heads) break;
+    uintx4 q[KD / 64];
+    load_codes<KD>(q, codes[u]);
+    b.put(a, u, q, own, j0, count, a.keys + (t * a.c.heads + h0 + u) * a.q.cols);
+  }
 }
 
-// ... and the lists from there.
-__global__ __launch_bounds__(1024) void kv_select_lists_kernel(KvSelectArgs a) {
+// ... and the lists from there, by way of LDS if they fit.
+__global__ __launch_bounds__(1024) void kv_select_lists_kernel(KvSelectArgs a, bool lds) {
+  extern __shared__ uint32_t held[];
   __shared__ Select<1024> s;
   const int64_t row = blockIdx.x;
   int r, own;
-  const int count = columns(a, row / a.c.heads, &r, &own);
-  take_best(a.keys + row * a.q.cols, count, a.n, a.blocks + row * a.n, s);
+  const int count = columns_of(a, row / a.c.heads, &r, &own);
+  const uint32_t* ranks = a.keys + row * a.q.cols;
+  if (lds) {
+#pragma unroll 8
+    for (int i = threadIdx.x; i < count; i += 1024) held[i] = ranks[i];
+    __syncthreads();
+  }
+  take_best(lds ? held : ranks, count, a.n, a.blocks + row * a.n, s);
 }
 
 // Prompts: 16 tokens and a head a workgroup.  Scores are an int8 product of 16
 // blocks' summaries and the 16 tokens' codes on the 16x16x64 MFMA, ranks go to
-// LDS, and each wavefront lists the best of 2 tokens: the n-th largest rank bit
-// by bit, counting with ballots, no barrier.  NR: ranks a lane holds.
-typedef int intx4 __attribute__((ext_vector_type(4)));
+// LDS, and each wavefront lists the best of 2 tokens.  NR: ranks a lane holds.
 constexpr int kTile = 16;
 
-__device__ __forceinline__ intx4 mfma_i8(uintx4 x, uintx4 y, intx4 c) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(intx4, x),
-                                               __builtin_bit_cast(intx4, y), c, 0, 0, 0);
-#else
-  return c;
-#endif
-}
-
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int i = 32; i >= 1; i >>= 1) x = fmaxf(x, __shfl_xor(x, i));
-  return x;
-}
-
-// query_codes of a wavefront's tokens t0, t0 + step, ..: two neighbouring values
-// a lane (KD / 128 times), the loads of all tokens and eight heads in flight.
-template <bool BF16, int KD, int NT>
-__device__ void wave_query_codes(const KvSelectArgs& a, int64_t t0, int step, int h,
-                                 int8_t* codes, int stride) {
-  constexpr int P = (KD + 127) / 128, HEADS = 8;
-  const int lane = threadIdx.x & 63, g = a.q.group;
-  const uint16_t* q[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-    q[t] = (const uint16_t*)a.q.q + min(t0 + t * step, a.q.tokens - 1) * a.q.q_token +
-           (int64_t)h * g * a.q.q_head;
-  const auto each = [&](auto&& f) {
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-      const int d = 2 * (lane + 64 * p);
-      if (d >= a.c.dim) continue;
-      for (int i0 = 0; i0 < g; i0 += HEADS) {
-        uint32_t x[NT][HEADS];
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int i = 0; i < HEADS; ++i)  // (past the last head: zeros, which add nothing)
-            x[t][i] = i0 + i < g ? *(const uint32_t*)(q[t] + (i0 + i) * a.q.q_head + d) : 0;
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int i = 0; i < HEADS; ++i)
-            f(t, p, value<BF16>((uint16_t)x[t][i]), value<BF16>((uint16_t)(x[t][i] >> 16)));
-      }
-    }
-  };
-  float inv[NT] = {}, peak[NT] = {};
-  int s0[NT][P] = {}, s1[NT][P] = {};
-  each([&](int t, int, float u, float v) {
-    inv[t] = fmaxf(inv[t], fmaxf(finite_abs(u), finite_abs(v)));
-  });
-#pragma unroll
-  for (int t = 0; t < NT; ++t) inv[t] = to_codes(wave_max(inv[t]));
-  each([&](int t, int p, float u, float v) {
-    // (a factor of 0 belongs to values that may not be finite)
-    s0[t][p] += inv[t] != 0.0f ? (int)rintf(u * inv[t]) : 0;
-    s1[t][p] += inv[t] != 0.0f ? (int)rintf(v * inv[t]) : 0;
-  });
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-      peak[t] = fmaxf(peak[t], fmaxf((float)abs(s0[t][p]), (float)abs(s1[t][p])));
-    peak[t] = wave_max(peak[t]);
-    const float to = peak[t] > 0.0f ? 127.0f / peak[t] : 0.0f;
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-      const int d = 2 * (lane + 64 * p);
-      if (d < KD) {
-        const int x = (int)rintf((float)s0[t][p] * to), y = (int)rintf((float)s1[t][p] * to);
-        *(uint16_t*)(codes + t * step * stride + d) = (uint16_t)((x & 255) | (y & 255) << 8);
-      }
-    }
-  }
-}
-
-template <bool BF16, int KD, int NR>
+template <bool BF16, int KD, bool A16, int NR>
 __global__ __launch_bounds__(512) void kv_select_tile_kernel(KvSelectArgs a) {
-  constexpr int W = 8;
-  constexpr int S = 64 * NR + 4;  // (rows 4 banks apart)
+  constexpr int W = 8, S = 64 * NR + 4;  // (rows 4 banks apart)
+  constexpr int AHEAD = KD == 256 ? 2 : 4;
   extern __shared__ __align__(16) uint32_t ranks[];  // [kTile][S]
   __shared__ __align__(16) int8_t codes[kTile][KD + 16];
   __shared__ int req[kTile], cnt[kTile], own[kTile];
@@ -408,7 +520,7 @@ __global__ __launch_bounds__(512) void kv_select_tile_kernel(KvSelectArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (threadIdx.x < kTile) {
     int r = -1, o = -1, n = 0;
-    if (t0 + threadIdx.x < a.q.tokens) n = columns(a, t0 + threadIdx.x, &r, &o);
+    if (t0 + threadIdx.x < a.q.tokens) n = columns_of(a, t0 + threadIdx.x, &r, &o);
     req[threadIdx.x] = r;
     own[threadIdx.x] = o;
     cnt[threadIdx.x] = n;
@@ -416,8 +528,7 @@ __global__ __launch_bounds__(512) void kv_select_tile_kernel(KvSelectArgs a) {
   wave_query_codes<BF16, KD, kTile / W>(a, t0 + wave, W, h, codes[wave], KD + 16);
   __syncthreads();
   uintx4 q[KD / 64];
-#pragma unroll
-  for (int i = 0; i < KD / 64; ++i) q[i] = *(const uintx4*)&codes[col][64 * i + 16 * grp];
+  load_codes<KD>(q, codes[col]);
   const int myreq = req[col], mycnt = cnt[col], myown = own[col];
   // the requests of the tile one after another (most often there is one)
   for (uint64_t todo = __ballot(mycnt > 0) & 0xFFFF; todo;) {
@@ -428,129 +539,80 @@ __global__ __launch_bounds__(512) void kv_select_tile_kernel(KvSelectArgs a) {
     for (int x = 1; x < 16; x *= 2) most = max(most, __shfl_xor(most, x));
     todo &= ~__ballot(mine);
     const int32_t* table = a.q.table + (int64_t)r * a.q.table_stride;
-    #pragma unroll 2
-    for (int j0 = 16 * wave; j0 < most; j0 += 16 * W) {
-      const int p = j0 + col < most ? table[j0 + col] : -1;
-      const bool there = p >= 0 && p < a.c.pages;
-      const int64_t row = (int64_t)p * a.c.heads + h;
-      intx4 dot = {0, 0, 0, 0};
-      const int8_t* m = a.c.summaries + row * a.c.dim + 16 * grp;
-      float scale = 0.0f;
-      if (there) scale = a.c.scales[row];
+    for (int j0 = 16 * wave; j0 < most; j0 += 16 * W * AHEAD) {
+      BlockScores<KD, A16, AHEAD> b;
+      b.load(a, h, table, j0, 16 * W, most);
 #pragma unroll
-      for (int i = 0; i < KD / 64; ++i) {
-        uintx4 v = {};
-        if (there && 64 * i + 16 * grp < a.c.dim) v = *(const uintx4*)(m + 64 * i);
-        dot = mfma_i8(v, q[i], dot);
-      }
-      const uint32_t present = (uint32_t)__ballot(there);
-      uintx4 k;
+      for (int u = 0; u < AHEAD; ++u) {
+        const intx4 d = b.dots(u, q);
+        uintx4 k;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = j0 + 4 * grp + i;
-        const float s = __shfl(scale, 4 * grp + i);
-        k[i] = !(present >> (4 * grp + i) & 1)           ? 0
-               : j < a.first || j > myown - a.last ? kAlways
-                                                         : rank_of(dot[i], s);
+        for (int i = 0; i < 4; ++i) {
+          const int m = 4 * grp + i, j = j0 + 16 * W * u + m;
+          const float s = __shfl(b.scale[u], m);
+          k[i] = !(b.present[u] >> m & 1)              ? 0
+                 : j < a.first || j > myown - a.last ? kAlways
+                                                       : rank_of(d[i], s);
+        }
+        const int j = j0 + 16 * W * u + 4 * grp;
+        if (mine && j < 64 * NR) *(uintx4*)&ranks[col * S + j] = k;
       }
-      if (mine) *(uintx4*)&ranks[col * S + j0 + 4 * grp] = k;
     }
   }
   __syncthreads();
-  const uint64_t below = (uint64_t(1) << lane) - 1;
-  for (int i = wave; i < kTile; i += W) {
-    const int64_t t = t0 + i;
-    if (t >= a.q.tokens) break;
-    const int count = cnt[i];
-    uint32_t k[NR];
-#pragma unroll
-    for (int x = 0; x < NR; ++x)
-      k[x] = 64 * x + lane < count ? ranks[i * S + 64 * x + lane] : 0;
-    // cut: all ranks from it on are taken, the first `ties` of those equal to
-    // it only
-    uint32_t cut = 1;
-    int ties = 64 * NR;
-    if (count > a.n) {
-      cut = 0;
-      int upto = 0;  // ranks at or above cut
-      for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t c = cut | 1u << bit;
-        int n = 0;
-#pragma unroll
-        for (int x = 0; x < NR; ++x) n += bits(__ballot(k[x] >= c));
-        if (n >= a.n) {
-          cut = c;
-          upto = n;
-          if (n == a.n) break;
-        }
-      }
-      if (cut == 0) cut = 1;  // (absent blocks: fewer candidates than n)
-      else if (upto > a.n) {
-        int above = 0;
-#pragma unroll
-        for (int x = 0; x < NR; ++x) above += bits(__ballot(k[x] > cut));
-        ties = a.n - above;
-      }
-    }
-    int32_t* out = a.blocks + (t * a.c.heads + h) * a.n;
-    int at = 0;
-#pragma unroll
-    for (int x = 0; x < NR; ++x) {
-      const uint64_t tied = __ballot(k[x] == cut);
-      const bool take = k[x] > cut || (k[x] == cut && bits(tied & below) < ties);
-      const uint64_t taken = __ballot(take);
-      if (take) out[at + bits(taken & below)] = 64 * x + lane;
-      at += bits(taken);
-      ties -= bits(tied);
-    }
-    for (int x = at + lane; x < a.n; x += 64) out[x] = -1;
-  }
+  for (int i = wave; i < kTile && t0 + i < a.q.tokens; i += W)
+    wave_take_best<NR>(ranks + i * S, cnt[i], a.n, a.blocks + ((t0 + i) * a.c.heads + h) * a.n);
 }
 
-// Ways to list (measured in us a call): a row a workgroup, its ranks in LDS; in
-// two launches over the workspace where rows are few and long; 16 tokens a
-// workgroup where a request has many.
+// Ways to list: a row a workgroup, its ranks in LDS; over the workspace in two
+// launches where rows are long; 16 tokens a workgroup where requests have many.
+// A launch is a chain of five dependent accesses, about 10 us whatever its size:
+// one token of 8 heads takes 31.4 us by rows and 20.4 in two launches at 4,096
+// columns, 20.0 and 19.3 at 2,048, 11.3 and 13.5 at 512.
 enum class Way { kRow, kParts, kTile };
 
 constexpr int kTileCols = 64 * 14;  // ranks of 16 tokens in 58 KB of LDS
 
 Way way_of(const KvSelectArgs& a) {
-  if (a.c.dim % 16 == 0 && a.q.cols <= kTileCols && a.q.tokens >= 8 * a.q.requests)
-    return Way::kTile;
-  if (a.q.cols <= 4096 || (a.q.cols <= kLdsCols && a.q.tokens * a.c.heads >= 256))
-    return Way::kRow;
-  return Way::kParts;
+  if (a.q.cols <= kTileCols && a.q.tokens >= 8 * a.q.requests) return Way::kTile;
+  return a.q.cols <= 2048 ? Way::kRow : Way::kParts;
 }
 
-template <bool BF16, int KD>
+template <bool BF16, int KD, bool A16, int NR>
 void launch_tile(const KvSelectArgs& a, hipStream_t s) {
   const unsigned grid = (unsigned)((a.q.tokens + kTile - 1) / kTile * a.c.heads);
-  if (a.q.cols <= 256)
-    kv_select_tile_kernel<BF16, KD, 4><<<grid, 512, kTile * (64 * 4 + 4) * 4, s>>>(a);
-  else if (a.q.cols <= 512)
-    kv_select_tile_kernel<BF16, KD, 8><<<grid, 512, kTile * (64 * 8 + 4) * 4, s>>>(a);
-  else
-    kv_select_tile_kernel<BF16, KD, 14><<<grid, 512, kTile * (64 * 14 + 4) * 4, s>>>(a);
+  kv_select_tile_kernel<BF16, KD, A16, NR><<<grid, 512, kTile * (64 * NR + 4) * 4, s>>>(a);
 }
 
-template <bool BF16, int CH>
+template <bool BF16, int KD, bool A16>
 void launch_select(const KvSelectArgs& a, hipStream_t s) {
   const unsigned rows = (unsigned)(a.q.tokens * a.c.heads);
   switch (way_of(a)) {
     case Way::kTile:
-      if (a.c.dim <= 64) launch_tile<BF16, 64>(a, s);
-      else if (a.c.dim <= 128) launch_tile<BF16, 128>(a, s);
-      else launch_tile<BF16, 256>(a, s);
+      if (a.q.cols <= 256) launch_tile<BF16, KD, A16, 4>(a, s);
+      else if (a.q.cols <= 512) launch_tile<BF16, KD, A16, 8>(a, s);
+      else launch_tile<BF16, KD, A16, 14>(a, s);
       return;
     case Way::kRow:
-      if (rows < 512) kv_select_kernel<BF16, CH, 1024><<<rows, 1024, a.q.cols * 4, s>>>(a);
-      else kv_select_kernel<BF16, CH, 256><<<rows, 256, a.q.cols * 4, s>>>(a);
+      if (rows < 512) kv_select_kernel<BF16, KD, A16, 1024><<<rows, 1024, a.q.cols * 4, s>>>(a);
+      else kv_select_kernel<BF16, KD, A16, 256><<<rows, 256, a.q.cols * 4, s>>>(a);
       return;
     case Way::kParts:
       const int parts = (a.q.cols + kPartCols - 1) / kPartCols;
-      kv_select_ranks_kernel<BF16, CH><<<rows * parts, 256, 0, s>>>(a, parts);
-      kv_select_lists_kernel<<<rows, 1024, 0, s>>>(a);
+      const int sets = (a.c.heads + kPartHeads - 1) / kPartHeads;
+      const bool lds = a.q.cols <= kLdsCols;
+      kv_select_ranks_kernel<BF16, KD, A16>
+          <<<(unsigned)(a.q.tokens * sets * parts), 512, 0, s>>>(a, parts);
+      kv_select_lists_kernel<<<rows, 1024, lds ? a.q.cols * 4 : 0, s>>>(a, lds);
   }
+}
+
+template <bool BF16>
+void launch_dim(const KvSelectArgs& a, hipStream_t s) {
+  const bool a16 = a.c.dim % 16 == 0;
+  if (a.c.dim <= 64) a16 ? launch_select<BF16, 64, true>(a, s) : launch_select<BF16, 64, false>(a, s);
+  else if (a.c.dim <= 128) a16 ? launch_select<BF16, 128, true>(a, s) : launch_select<BF16, 128, false>(a, s);
+  else a16 ? launch_select<BF16, 256, true>(a, s) : launch_select<BF16, 256, false>(a, s);
 }
 
 }  // namespace
@@ -562,14 +624,12 @@ int64_t kv_select_workspace(const KvSelectArgs& a) {
 int64_t kv_select_grid(const KvSelectArgs& a) {
   // (in workgroups of 256)
   const int64_t rows = a.q.tokens * a.c.heads;
-  return way_of(a) == Way::kParts ? rows * ((a.q.cols + kPartCols - 1) / kPartCols) : 4 * rows;
+  return way_of(a) == Way::kParts
+             ? 2 * rows * ((a.q.cols + kPartCols - 1) / kPartCols) : 4 * rows;
 }
 
 hipError_t launch_kv_select(const KvSelectArgs& a, hipStream_t s) {
-  if (a.c.dim % 16 == 0)
-    a.c.bf16 ? launch_select<true, 16>(a, s) : launch_select<false, 16>(a, s);
-  else
-    a.c.bf16 ? launch_select<true, 8>(a, s) : launch_select<false, 8>(a, s);
+  a.c.bf16 ? launch_dim<true>(a, s) : launch_dim<false>(a, s);
   return hipGetLastError();
 }
 

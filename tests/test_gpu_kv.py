@@ -307,7 +307,7 @@ def test_select_for_prompts_among_many_blocks(engine, cols, heads, group, d):
         check_select(engine, q, codes, scales, table, who, positions, 16, n)
 
 
-@pytest.mark.parametrize("cols", [4096, 4097, 9000])
+@pytest.mark.parametrize("cols", [2048, 2049, 4096, 8192, 8193, 9000])
 def test_select_among_many_blocks(engine, cols):
     rng = np.random.default_rng(cols)
     codes, scales = summaries(rng, 700, 1, 16)
@@ -316,6 +316,16 @@ def test_select_among_many_blocks(engine, cols):
     positions = np.array([cols * 16 - 1, 5000, (cols - 1) * 16])
     for n in (2, 256):
         check_select(engine, q, codes, scales, table, np.array([0, 0, 1]), positions, 16, n)
+
+
+@pytest.mark.parametrize("heads,group,d", [(9, 2, 80), (3, 3, 72), (8, 1, 256), (1, 2, 128)])
+def test_select_among_many_blocks_of_several_heads(engine, heads, group, d):
+    rng = np.random.default_rng(heads)
+    codes, scales = summaries(rng, 90, heads, d)
+    table = rng.integers(-1, 95, (2, 2100)).astype(np.int32)
+    q = dev(rng.standard_normal((3, heads * group, d), np.float32)).bfloat16()
+    check_select(engine, q, codes, scales, table, np.array([1, 0, 1]),
+                 np.array([2100 * 16 - 1, 16 * 16, 2050 * 16]), 16, 11)
 
 
 def test_select_ties_go_to_the_lowest_block(engine):
