@@ -55,14 +55,29 @@ __device__ __forceinline__ floatx4 mfma(halfx8 a, halfx8 b, floatx4 c) {
 #endif
 }
 
-// The maximum over the lanes of one column (l, l ^ 16, l ^ 32, l ^ 48).
+// The maximum over the lanes of one column (l, l ^ 16, l ^ 32, l ^ 48).  The lane
+// swaps are VALU instructions: a shuffle would wait for LDS.  (Written out: the
+// builtins' two results are taken for one where both operands are one value.
+// The instruction reads other lanes' registers two wait states after a write.)
 __device__ __forceinline__ float column_max(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
+#if defined(__HIP_DEVICE_COMPILE__)
+  float y = x;
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+  x = y = fmaxf(x, y);
+  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+  x = fmaxf(x, y);
+#endif
+  return x;
 }
 __device__ __forceinline__ float column_sum(float x) {
   x += __shfl_xor(x, 16);
   return x + __shfl_xor(x, 32);
+}
+
+// An entry of a block table, by a scalar load: the same for a whole wavefront, and
+// not written while the kernel runs.
+__device__ __forceinline__ int table_entry(const int32_t* table, int i) {
+  return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)(table + i);
 }
 
 // The first `n` of 8 values (n <= 0: none), zeros after.
@@ -75,8 +90,18 @@ __device__ __forceinline__ uintx4 keep(uintx4 v, int n) {
   return v;
 }
 
-// DP: head size rounded up to a multiple of 32.  LIST: over listed blocks.  P16:
-// pages of 16 keys, two to a 32-key pair.
+// Head sizes are rounded up to one of these; a kernel for DP has more values than
+// the next smaller one holds, so that only the last of them need a check.
+constexpr int kSizes[] = {64, 96, 128, 192, 256};
+constexpr int sure_values(int dp) {
+  int below = 0;
+  for (int s : kSizes)
+    if (s < dp) below = s;
+  return below;
+}
+
+// DP: head size rounded up.  LIST: over listed blocks.  P16: pages of 16 keys,
+// two to a 32-key pair.
 template <int DP, bool BF16, bool LIST, bool P16>
 struct Attend {
   using T = std::conditional_t<BF16, __bf16, _Float16>;
@@ -144,7 +169,7 @@ struct Attend {
 
   // The step of kKeys keys from key `k` (of the row's listed keys) on.
   __device__ __forceinline__ void step(int h, int k) {
-    const int ps = a.c.page, lps = a.c.lps;
+    const int ps = P16 ? 16 : a.c.page, lps = P16 ? 4 : a.c.lps;
     const int64_t head = (int64_t)ps * d;  // values of a (page, head)
     uintx4 kf[2 * kPairs][kChunks], vf[kPairs][kTiles];
     int n8[kPairs];  // of this lane's 8 keys of a pair, those that show
@@ -184,14 +209,15 @@ struct Attend {
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
           kf[2 * p + u][i] = uintx4{};
-          if (32 * i + 8 * grp < d) kf[2 * p + u][i] = *(const uintx4*)(kp[p] + 4 * u * d + 32 * i);
+          if (32 * i + 32 <= sure_values(DP) || 32 * i + 8 * grp < d)
+            kf[2 * p + u][i] = *(const uintx4*)(kp[p] + 4 * u * d + 32 * i);
         }
 #pragma unroll
     for (int p = 0; p < kPairs; ++p)
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) {
         vf[p][i] = uintx4{};
-        if (16 * i + col < d) vf[p][i] = *(const uintx4*)(vp[p] + 16 * i * ps);
+        if (16 * i + 16 <= sure_values(DP) || 16 * i + col < d) vf[p][i] = *(const uintx4*)(vp[p] + 16 * i * ps);
       }
 
     floatx4 s[2 * kPairs];
@@ -250,49 +276,400 @@ __device__ __forceinline__ float lse_of(float m, float l, float scale, float bia
   return fmaf(m, scale, kLn2 * (__log2f(l) - bias));
 }
 
-// Many rows: a wavefront each, no parts.
-constexpr int64_t kManyRows = 4096;
-
-template <int DP, bool BF16, bool LIST, bool P16>
-__global__ __launch_bounds__(256, 2) void kv_attend_rows_kernel(KvAttendArgs a) {
-  using A = Attend<DP, BF16, LIST, P16>;
-  const int tiles = (a.q.group + kColumns - 1) / kColumns;
-  const int64_t row = blockIdx.x;
-  const int mt = (int)(row % tiles);
-  const int h = (int)(row / tiles % a.c.heads);
-  const int64_t t = row / tiles / a.c.heads * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (t >= a.q.tokens) return;
-  A w(a, threadIdx.x & 63);
-  w.start(t, h, mt);
-  const int r = a.q.token_request[t], pos = a.q.positions[t];
-  if (r >= 0 && r < a.q.requests && pos >= 0) {
-    const int end = LIST ? a.n : min(pos >> a.c.lps, a.q.cols - 1) + 1;
-    for (int e = 0; e < end; e += 64) {
-      w.entries(t, h, r, pos, e, end);
-      const int64_t k1 = (int64_t)min(end, e + 64) << a.c.lps;
-      for (int64_t k = (int64_t)e << a.c.lps; k < k1; k += A::kKeys) w.step(h, (int)k);
-    }
-  }
-  const float l = column_sum(w.l);
-  const int g = mt * kColumns + w.col;
-  if (g >= a.q.group) return;
-  const float inv = 1.0f / l;
-  const int64_t at = t * a.c.heads * a.q.group + h * a.q.group + g;
-#pragma unroll
-  for (int i = 0; i < A::kTiles; ++i) {
-    const int d = 16 * i + 4 * w.grp;
-    if (d < a.c.dim) {
-      typename A::Tx4 x;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = (typename A::T)(l == 0.0f ? 0.0f : w.o[i][j] * inv);
-      *(typename A::Tx4*)((typename A::T*)a.out + at * a.c.dim + d) = x;
-    }
-  }
-  if (a.lse && w.grp == 0) a.lse[at] = lse_of(w.m, l, a.scale, A::kBias);
+// The smallest / largest value of the 16 lanes of a row (lanes 16 g .. 16 g + 15).
+template <int CTRL>
+__device__ __forceinline__ int row_ror(int x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_update_dpp(x, x, CTRL, 0xF, 0xF, false);
+#else
+  return x;
+#endif
+}
+__device__ __forceinline__ int row_min(int x) {
+  x = min(x, row_ror<0x128>(x));
+  x = min(x, row_ror<0x124>(x));
+  x = min(x, row_ror<0x122>(x));
+  return min(x, row_ror<0x121>(x));
+}
+__device__ __forceinline__ int row_max(int x) {
+  x = max(x, row_ror<0x128>(x));
+  x = max(x, row_ror<0x124>(x));
+  x = max(x, row_ror<0x122>(x));
+  return max(x, row_ror<0x121>(x));
 }
 
-// Few rows: a part of a row's keys for each workgroup, its steps dealt to the
-// W wavefronts in turn.
+// Tokens of prompts: a wavefront for as many neighbouring tokens as fill NT
+// tiles of 16 columns with their heads of a kv head (two tokens of 8 heads in a
+// tile).  Neighbours look at much the same blocks: their lists are merged block
+// by block, always the lowest of the tokens' next ones, so that a block that
+// several of them take is loaded once and multiplied by all their heads, and
+// keys that a column's token does not see get no weight.  What bounds it is
+// loads from L2 and the Infinity Cache: with a wavefront for each token 3,001
+// tokens of 16 blocks, 4 kv heads of 8, read 6.3 GB in 680 us.
+//
+// Lists in any order are right: each entry is taken once, whatever it meets.
+//
+// A weight of 0 does not hide a value that is not finite.  Values past every
+// token's keys are masked; one that only some of the tokens see would reach the
+// others' sums as NaN, so a wavefront whose sums are not finite does its tokens
+// over, one at a time.
+extern __shared__ int kv_lists[];  // [tokens][n + 1]
+
+template <int DP, bool BF16, bool LIST, bool P16, int NT>
+struct AttendShared {
+  using T = std::conditional_t<BF16, __bf16, _Float16>;
+  using Tx8 = std::conditional_t<BF16, bf16x8, halfx8>;
+  using Tx4 = std::conditional_t<BF16, bf16x4, halfx4>;
+  static constexpr int kChunks = DP / 32, kTiles = DP / 16;
+  static constexpr float kBias = BF16 ? 0.0f : 14.0f;
+  static constexpr int kNone = 0x7FFFFFFF;
+
+  const KvAttendArgs& a;
+  const int lane, col, grp, h;
+  const float c;
+  Tx8 q[NT][kChunks];
+  floatx4 o[NT][kTiles];
+  float m[NT], l[NT];
+  int pos[NT];               // of the column's token
+  // the column's place in its token's list (in LDS; without lists, counting
+  // up) and its next block
+  int at[NT], next[NT];
+  bool on[NT];
+
+  __device__ __forceinline__ AttendShared(const KvAttendArgs& args, int ln, int head)
+      : a(args), lane(ln), col(ln & 15), grp(ln >> 4), h(head), c(args.scale * kLog2e) {}
+
+  __device__ __forceinline__ void reset() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) o[n][i] = floatx4{0, 0, 0, 0};
+      m[n] = -__builtin_inff();
+      l[n] = 0.0f;
+    }
+  }
+
+  __device__ __forceinline__ int entry(int n) const {
+    if (!on[n]) return kNone;
+    if constexpr (LIST) return kv_lists[at[n]];
+    return at[n] <= min(pos[n] >> a.c.lps, a.q.cols - 1) ? at[n] : kNone;
+  }
+
+  // The lowest next block of the columns that are on (kNone: no more), and how
+  // many of its keys each column sees.
+  __device__ __forceinline__ int advance(int (&seen)[NT]) {
+    int b = next[0];
+#pragma unroll
+    for (int n = 1; n < NT; ++n) b = min(b, next[n]);
+    b = __builtin_amdgcn_readfirstlane(row_min(b));
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const bool hit = next[n] == b && b != kNone;
+      seen[n] = hit ? min(a.c.page, pos[n] + 1 - (b << a.c.lps)) : 0;
+      if (hit) {
+        ++at[n];
+        next[n] = entry(n);
+      }
+    }
+    return b;
+  }
+
+  // What one look at the lists gives: the keys of a block (of two pages of 16).
+  struct Unit {
+    const T *k, *v;  // this lane's K row and V^T row of its first 32 keys
+    int lim[NT];     // of those, and this lane's 8, the first that a column sees
+    int top;         // keys that any column sees
+    bool all;        // every column sees all
+  };
+  // blocks looked up ahead, so that their pages are known in time
+  static constexpr int kBlocks = P16 ? 2 : 1;
+  int block[kBlocks], page[kBlocks], seen[kBlocks][NT];
+
+  __device__ __forceinline__ void look(const int32_t* table) {
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i) {
+      block[i] = advance(seen[i]);
+      page[i] = table_entry(table, block[i] == kNone ? 0 : block[i]);
+    }
+  }
+
+  // The next unit whose pages are there; false: no more.
+  __device__ __forceinline__ bool unit(const int32_t* table, Unit& u) {
+    const int ps = P16 ? 16 : a.c.page, d = a.c.dim;
+    const int64_t head = (int64_t)ps * d;
+    while (block[0] != kNone) {
+      bool there[kBlocks], some = false;
+      int p[kBlocks];
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i) {
+        there[i] = block[i] != kNone && page[i] >= 0 && page[i] < a.c.pages;
+        some |= there[i];
+        p[i] = there[i] ? page[i] : 0;  // (an absent page is read as page 0 and not seen)
+      }
+      if (some) {
+        const int row = 8 * (col >> 2);  // this lane's K rows start here
+        int64_t pk = p[0], pv = p[0];
+        if constexpr (P16) {
+          pk = row < 16 ? p[0] : p[1];
+          pv = grp < 2 ? p[0] : p[1];
+        }
+        u.k = (const T*)a.c.keys + (pk * a.c.heads + h) * head +
+              ((P16 ? row & 15 : row) + (col & 3)) * d + 8 * grp;
+        u.v = (const T*)a.c.values + (pv * a.c.heads + h) * head + col * ps +
+              (P16 ? (8 * grp) & 15 : 8 * grp);
+        int top = 0;
+        u.all = true;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          int s = there[0] ? seen[0][n] : 0;
+          if constexpr (P16) {
+            const int s1 = there[1] ? seen[1][n] : 0;
+            top = max(top, s1 > 0 ? 16 + s1 : s);
+            u.all &= s == 16 && s1 == 16;
+            u.lim[n] = (grp < 2 ? s : s1) - ((8 * grp) & 15);
+          } else {
+            top = max(top, s);
+            u.all &= s == ps;
+            u.lim[n] = s - 8 * grp;
+          }
+        }
+        u.top = __builtin_amdgcn_readfirstlane(row_max(top));
+        u.all = __all(u.all);
+      }
+      look(table);
+      if (some) return true;
+    }
+    return false;
+  }
+
+  // Loads without conditions, so that the waits count them: values past the
+  // head's are read in a place of its own and masked (K), or make sums that
+  // nobody stores (V).
+  __device__ __forceinline__ void load_k(uintx4 (&kf)[2][kChunks], const T* kp) const {
+    const int d = a.c.dim;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        int at = 32 * i;
+        if (32 * i + 32 > sure_values(DP) && 32 * i + 8 * grp >= d) at = -8 * grp;
+        kf[u][i] = *(const uintx4*)(kp + 4 * u * d + at);
+      }
+  }
+  __device__ __forceinline__ Tx8 k_row(const uintx4 (&kf)[kChunks], int i) const {
+    uintx4 x = kf[i];
+    if (32 * i + 32 > sure_values(DP) && 32 * i + 8 * grp >= a.c.dim) x = uintx4{};
+    return __builtin_bit_cast(Tx8, x);
+  }
+  __device__ __forceinline__ void load_v(uintx4 (&vf)[kTiles], const T* vp) const {
+    const int d = a.c.dim, ps = P16 ? 16 : a.c.page;
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+      int row = 16 * i;
+      if (16 * i + 16 > sure_values(DP) && 16 * i + col >= d) row = -col;
+      vf[i] = *(const uintx4*)(vp + row * ps);
+    }
+  }
+
+  // All blocks of the columns that are on, of request r, 32 keys a step; the K
+  // rows of the next step are on their way while this one's weights are made.
+  __device__ __forceinline__ void run(int r) {
+    const int d = a.c.dim;
+    const int32_t* table = a.q.table + (int64_t)r * a.q.table_stride;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) next[n] = entry(n);
+    look(table);
+    Unit u;
+    if (!unit(table, u)) return;
+    uintx4 kf[2][kChunks], vf[kTiles];
+    load_k(kf, u.k);
+    int off = 0;
+    for (bool more = true; more;) {
+      load_v(vf, u.v + off);
+      floatx4 s[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          s[n][x] = floatx4{0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < kChunks; ++i)
+            s[n][x] = mfma(k_row(kf[x], i), q[n][i], s[n][x]);
+        }
+      // this step's limits, then the next step
+      int n8[NT], most = 0;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        n8[n] = u.lim[n] - off;
+        most = max(most, n8[n]);
+      }
+      const bool all = u.all;
+      off += 32;
+      if (off >= u.top) {
+        off = 0;
+        more = unit(table, u);
+      }
+      load_k(kf, u.k + off * d);  // (after the last step: its own once more)
+      Tx8 pr[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if (!all) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i >= n8[n]) s[n][i / 4][i % 4] = -__builtin_inff();
+        }
+        float top = m[n];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, s[n][i / 4][i % 4]);
+        top = column_max(top);
+        if (__any(top > m[n])) {
+          const float w = top == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((m[n] - top) * c);
+          l[n] *= w;
+#pragma unroll
+          for (int i = 0; i < kTiles; ++i) o[n][i] *= w;
+          m[n] = top;
+        }
+        const float base = kBias - (m[n] == -__builtin_inff() ? 0.0f : m[n]) * c;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(s[n][i / 4][i % 4], c, base));
+          l[n] += x;
+          pr[n][i] = (T)x;
+        }
+      }
+      if (!all) {
+        most = row_max(most);
+        if (__any(most < 8)) {
+#pragma unroll
+          for (int i = 0; i < kTiles; ++i) vf[i] = keep(vf[i], most);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i)
+          o[n][i] = mfma(__builtin_bit_cast(Tx8, vf[i]), pr[n], o[n][i]);
+    }
+  }
+};
+
+template <int DP>
+constexpr int kColumnTiles = DP <= 128 ? 2 : 1;  // (registers: two wavefronts a SIMD)
+
+// Tokens that share a wavefront, and wavefronts that share a token's heads.
+struct Sharing {
+  int tokens, tiles;
+};
+__host__ __device__ __forceinline__ Sharing sharing(int group, int columns) {
+  if (group <= columns) return {columns / group, 1};
+  return {1, (group + columns - 1) / columns};
+}
+
+template <int DP, bool BF16, bool LIST, bool P16>
+__global__ __launch_bounds__(64, 2) void kv_attend_shared_kernel(KvAttendArgs a) {
+  constexpr int NT = kColumnTiles<DP>;
+  using A = AttendShared<DP, BF16, LIST, P16, NT>;
+  const int group = a.q.group, lane = threadIdx.x;
+  const Sharing sh = sharing(group, kColumns * NT);
+  const int mt = (int)(blockIdx.x % sh.tiles);
+  const int h = (int)(blockIdx.x / sh.tiles % a.c.heads);
+  const int64_t t0 = (int64_t)(blockIdx.x / sh.tiles / a.c.heads) * sh.tokens;
+  const int tokens = (int)min<int64_t>(sh.tokens, a.q.tokens - t0);
+  A w(a, lane, h);
+  // lane i: token t0 + i
+  int myreq = -1, mypos = -1;
+  if (lane < tokens) {
+    myreq = a.q.token_request[t0 + lane];
+    mypos = a.q.positions[t0 + lane];
+  }
+  const bool sees = myreq >= 0 && myreq < a.q.requests && mypos >= 0;
+  if constexpr (LIST) {
+    // the tokens' lists, without the entries that show nothing
+    for (int i = 0; i < tokens; ++i) {
+      const int own = __shfl(sees ? mypos >> a.c.lps : -1, i);
+      const int32_t* from = a.blocks + ((t0 + i) * a.c.heads + h) * a.n;
+      int at = i * (a.n + 1);
+      for (int e = lane; e - lane < a.n; e += 64) {
+        const int b = e < a.n ? from[e] : -1;
+        const bool take = b >= 0 && b < a.q.cols && b <= own;
+        const uint64_t taken = __ballot(take);
+        if (take) kv_lists[at + (int)__popcll(taken & ((uint64_t(1) << lane) - 1))] = b;
+        at += (int)__popcll(taken);
+      }
+      if (lane == 0) kv_lists[at] = A::kNone;
+    }
+    __syncthreads();
+  }
+  int tok[NT], g[NT];
+  bool mine[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int x = mt * kColumns * NT + kColumns * n + w.col;  // column
+    tok[n] = x / group;
+    g[n] = x % group;
+    mine[n] = tok[n] < tokens;
+    if (!mine[n]) tok[n] = 0;
+    w.pos[n] = __shfl(mypos, tok[n]);
+    const auto* src = (const typename A::T*)a.q.q + (t0 + tok[n]) * a.q.q_token +
+                      (int64_t)(h * group + g[n]) * a.q.q_head;
+#pragma unroll
+    for (int i = 0; i < A::kChunks; ++i) {
+      uintx4 x4 = {};
+      if (mine[n] && 32 * i + 8 * w.grp < a.c.dim) x4 = *(const uintx4*)(src + 32 * i + 8 * w.grp);
+      w.q[n][i] = __builtin_bit_cast(typename A::Tx8, x4);
+    }
+  }
+  // first all tokens together, a request after another; then, if that left
+  // sums that are not finite, each token by itself
+  for (int alone = -1; alone < tokens; ++alone) {
+    w.reset();
+    uint64_t todo = __ballot(sees);
+    if (alone >= 0) todo &= uint64_t(1) << alone;
+    while (todo) {
+      const int r = __builtin_amdgcn_readlane(myreq, __builtin_ctzll(todo));
+      const uint64_t with = todo & __ballot(myreq == r);
+      todo &= ~with;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        w.on[n] = mine[n] && (with >> tok[n] & 1);
+        w.at[n] = LIST ? tok[n] * (a.n + 1) : 0;
+      }
+      w.run(r);
+    }
+    bool good = true;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < A::kTiles; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          good &= fabsf(w.o[n][i][j]) < __builtin_inff() || 16 * i + 4 * w.grp >= a.c.dim;
+    if (alone < 0 && !__all(good) && tokens > 1) continue;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float l = column_sum(w.l[n]);
+      if (!mine[n] || (alone >= 0 && tok[n] != alone)) continue;
+      const float inv = 1.0f / l;
+      const int64_t at = ((t0 + tok[n]) * a.c.heads + h) * group + g[n];
+#pragma unroll
+      for (int i = 0; i < A::kTiles; ++i) {
+        const int d = 16 * i + 4 * w.grp;
+        if (d < a.c.dim) {
+          typename A::Tx4 x;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            x[j] = (typename A::T)(l == 0.0f ? 0.0f : w.o[n][i][j] * inv);
+          *(typename A::Tx4*)((typename A::T*)a.out + at * a.c.dim + d) = x;
+        }
+      }
+      if (a.lse && w.grp == 0) a.lse[at] = lse_of(w.m[n], l, a.scale, A::kBias);
+    }
+    if (alone < 0) break;
+  }
+}
+
+// A part of a row's keys for each workgroup, its steps dealt to the W wavefronts
+// in turn.
 template <int DP, bool BF16, bool LIST, bool P16, int W>
 __global__ __launch_bounds__(64 * W, 2) void kv_attend_parts_kernel(KvAttendArgs a) {
   constexpr int H = 4;  // wavefronts whose sums meet in LDS at a time
@@ -442,17 +819,26 @@ __global__ __launch_bounds__(256) void kv_attend_join_kernel(KvAttendArgs a) {
   if (a.lse && tid == 0) a.lse[at] = lse_of(top, sum, a.scale, BF16 ? 0.0f : 14.0f);
 }
 
+int column_tiles(int dim) { return dim <= 128 ? kColumnTiles<128> : kColumnTiles<256>; }
+
+int64_t shared_grid(const KvAttendArgs& a) {
+  const Sharing sh = sharing(a.q.group, kColumns * column_tiles(a.c.dim));
+  return (a.q.tokens + sh.tokens - 1) / sh.tokens * a.c.heads * sh.tiles;
+}
+
 template <int DP, bool BF16, bool LIST, bool P16>
 void launch_one(const KvAttendArgs& a, hipStream_t s) {
-  const int tiles = (a.q.group + kColumns - 1) / kColumns;
   if (a.waves == 1) {
-    const int64_t grid = (a.q.tokens + 3) / 4 * a.c.heads * tiles;
-    kv_attend_rows_kernel<DP, BF16, LIST, P16><<<dim3((unsigned)grid), 256, 0, s>>>(a);
-  } else {
-    const dim3 grid((unsigned)(a.q.tokens * a.c.heads * tiles * a.splits));
-    if (a.waves == 8) kv_attend_parts_kernel<DP, BF16, LIST, P16, 8><<<grid, 512, 0, s>>>(a);
-    else kv_attend_parts_kernel<DP, BF16, LIST, P16, 4><<<grid, 256, 0, s>>>(a);
+    const Sharing sh = sharing(a.q.group, kColumns * kColumnTiles<DP>);
+    const size_t lds = LIST ? sizeof(int) * sh.tokens * (a.n + 1) : 0;
+    kv_attend_shared_kernel<DP, BF16, LIST, P16>
+        <<<dim3((unsigned)shared_grid(a)), 64, lds, s>>>(a);
+    return;
   }
+  const int tiles = (a.q.group + kColumns - 1) / kColumns;
+  const dim3 grid((unsigned)(a.q.tokens * a.c.heads * tiles * a.splits));
+  if (a.waves == 8) kv_attend_parts_kernel<DP, BF16, LIST, P16, 8><<<grid, 512, 0, s>>>(a);
+  else kv_attend_parts_kernel<DP, BF16, LIST, P16, 4><<<grid, 256, 0, s>>>(a);
 }
 
 template <int DP, bool BF16>
@@ -485,7 +871,8 @@ void kv_attend_plan(KvAttendArgs& a) {
   a.chunk = 64;
   a.waves = 4;
   if (rows == 0) return;
-  if (rows >= kManyRows) {
+  // tokens of prompts share wavefronts, if that leaves enough of them
+  if (a.q.tokens >= 4 * a.q.requests && shared_grid(a) >= 1024) {
     a.waves = 1;
     return;
   }
@@ -513,8 +900,9 @@ int64_t kv_attend_workspace(const KvAttendArgs& a) {
 }
 
 int64_t kv_attend_grid(const KvAttendArgs& a) {
-  return std::max(a.q.tokens * a.c.heads * a.q.group,
-                  (a.q.tokens + 3) * a.c.heads * ((a.q.group + kColumns - 1) / kColumns) * a.splits);
+  if (a.waves == 1) return shared_grid(a);
+  const int64_t rows = a.q.tokens * a.c.heads * ((a.q.group + kColumns - 1) / kColumns);
+  return std::max(a.q.tokens * a.c.heads * a.q.group, rows * a.splits * a.waves / 4);
 }
 
 hipError_t launch_kv_attend(const KvAttendArgs& a, hipStream_t s) {
