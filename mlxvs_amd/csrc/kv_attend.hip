@@ -16,7 +16,7 @@
 //
 // P is rounded to the cache's type for the second product (the values' own
 // precision; a sum of roundings that averages out), its sum is not; under f16
-// P is scaled by 2^14 so that small terms of long sums stay normal numbers.
+// P is scaled up so that small terms of long sums stay normal numbers.
 // Scores, maxima, sums and the output are float32.
 #include <hip/hip_runtime.h>
 
@@ -24,6 +24,7 @@
 #include <type_traits>
 
 #include "kv_cache.h"
+#include "lds_stage.h"
 
 namespace mlxvs::kern {
 namespace {
@@ -100,6 +101,44 @@ constexpr int sure_values(int dp) {
   return below;
 }
 
+// The weights of a lane's scores, exp2(c s + bias - c max) rounded to T, with the
+// running maximum m and this lane's sum l of its column, and the column's sums o
+// scaled if the maximum moves.  It is let be until scores pass it by more than
+// kSlack: weights are then up to 2^kSlack, and the sums are moved rarely.
+constexpr float kSlack = 8.0f;
+// log2 of what weights are scaled by: under f16 they stay below its largest
+// number, and small terms of long sums normal ones
+template <typename T>
+constexpr float kBiasOf = std::is_same_v<T, _Float16> ? 7.0f : 0.0f;
+
+template <int S, int TILES, typename T8>
+__device__ __forceinline__ void weights(floatx4 (&s)[2 * S], float& m, float& l, float c, float twice,
+                                        floatx4 (&o)[TILES], T8 (&p)[S]) {
+  using T = std::conditional_t<std::is_same_v<T8, bf16x8>, __bf16, _Float16>;
+  float top = m;
+#pragma unroll
+  for (int u = 0; u < 2 * S; ++u)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = fmaxf(top, s[u][i]);
+  top = column_max(top);
+  if (__any((top - m) * c > kSlack)) {  // (from nothing seen: infinity)
+    const float w = top == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((m - top) * c);
+    l *= w;
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) o[i] *= w;
+    m = top;
+  }
+  const float low = kBiasOf<T> + twice - (m == -__builtin_inff() ? 0.0f : m) * c;
+#pragma unroll
+  for (int u = 0; u < S; ++u)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = __builtin_amdgcn_exp2f(fmaf(s[2 * u + i / 4][i % 4], c, low));
+      l += x;
+      p[u][i] = (T)x;
+    }
+}
+
 // DP: head size rounded up.  LIST: over listed blocks.  P16: pages of 16 keys,
 // two to a 32-key pair.
 template <int DP, bool BF16, bool LIST, bool P16>
@@ -111,7 +150,7 @@ struct Attend {
   static constexpr int kTiles = DP / 16;            // rows of V^T
   static constexpr int kPairs = DP <= 128 ? 2 : 1;  // 32-key pairs a step
   static constexpr int kKeys = 32 * kPairs;
-  static constexpr float kBias = BF16 ? 0.0f : 14.0f;  // log2 of P's scale
+  static constexpr float kBias = kBiasOf<T>;
 
   const KvAttendArgs& a;
   const int lane, col, grp;
@@ -239,30 +278,8 @@ struct Attend {
         for (int i = 0; i < kTiles; ++i) vf[p][i] = keep(vf[p][i], n8[p]);
       }
     }
-    float top = m;
-#pragma unroll
-    for (int u = 0; u < 2 * kPairs; ++u)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) top = fmaxf(top, s[u][i]);
-    top = column_max(top);
-    if (__any(top > m)) {
-      // (a column that has seen nothing: 2^(-inf))
-      const float w = top == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((m - top) * c);
-      l *= w;
-#pragma unroll
-      for (int i = 0; i < kTiles; ++i) o[i] *= w;
-      m = top;
-    }
-    const float base = kBias - (m == -__builtin_inff() ? 0.0f : m) * c;
     Tx8 pr[kPairs];
-#pragma unroll
-    for (int p = 0; p < kPairs; ++p)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float x = __builtin_amdgcn_exp2f(fmaf(s[2 * p + i / 4][i % 4], c, base));
-        l += x;
-        pr[p][i] = (T)x;
-      }
+    weights<kPairs>(s, m, l, c, 0.0f, o, pr);
 #pragma unroll
     for (int p = 0; p < kPairs; ++p)
 #pragma unroll
@@ -298,46 +315,133 @@ __device__ __forceinline__ int row_max(int x) {
   return max(x, row_ror<0x121>(x));
 }
 
-// Tokens of prompts: a wavefront for as many neighbouring tokens as fill NT
+// Tokens of prompts.  A wavefront has as many neighbouring tokens as fill NT
 // tiles of 16 columns with their heads of a kv head (two tokens of 8 heads in a
-// tile).  Neighbours look at much the same blocks: their lists are merged block
-// by block, always the lowest of the tokens' next ones, so that a block that
-// several of them take is loaded once and multiplied by all their heads, and
-// keys that a column's token does not see get no weight.  What bounds it is
-// loads from L2 and the Infinity Cache: with a wavefront for each token 3,001
-// tokens of 16 blocks, 4 kv heads of 8, read 6.3 GB in 680 us.
+// tile), a workgroup four wavefronts.  Neighbours look at much the same blocks:
+// the workgroup walks the union of its tokens' blocks, each loaded once, and a
+// wavefront multiplies those that a token of its own takes; keys that a column's
+// token does not see get no weight.
 //
-// Lists in any order are right: each entry is taken once, whatever it meets.
+// What bounds it otherwise is loads: a wavefront's MFMA operands straight from
+// the cache are 16 bytes of 16 different rows to 16 neighbouring lanes, a row a
+// cycle, 64 cycles a load (3,001 tokens of 16 blocks, 4 kv heads of 8, with a
+// wavefront for each token: 6.3 GB in 680 us; with four tokens that share one:
+// 2.2 GB in 322 us, the same rate).  So tiles of keys and values go to LDS by
+// direct loads of neighbouring chunks, a tile ahead of the products, and the
+// operands come from there, in chunks that are swapped by row so that 8 lanes
+// read from 8 different sets of banks.
+//
+// Lists in any order are right: one that does not ascend is sorted first, and a
+// block listed twice counts twice.
 //
 // A weight of 0 does not hide a value that is not finite.  Values past every
 // token's keys are masked; one that only some of the tokens see would reach the
-// others' sums as NaN, so a wavefront whose sums are not finite does its tokens
+// others' sums as NaN, so a workgroup whose sums are not finite does its tokens
 // over, one at a time.
-extern __shared__ int kv_lists[];  // [tokens][n + 1]
+constexpr int kColumnTiles = 1;
 
-template <int DP, bool BF16, bool LIST, bool P16, int NT>
+constexpr int kSharedWaves = 4;
+constexpr int kListInts = 3840;  // of all lists of a workgroup (two workgroups a CU)
+constexpr int kWindow = 2048;    // blocks whose union is made at a time
+
+// Tokens that share a wavefront, and wavefronts that share a token's heads.
+struct Sharing {
+  int tokens, tiles;
+};
+__host__ __device__ __forceinline__ Sharing sharing(int group, int columns, int n) {
+  if (group > columns) return {1, (group + columns - 1) / columns};
+  const int most = kListInts / kSharedWaves / (n + 1);
+  const int tokens = columns / group;
+  return {tokens < most ? tokens : most, 1};
+}
+
+// 16 bytes a lane from `from` to lds + 16 lane.
+__device__ __forceinline__ void copy16_to_lds(const void* from, void* lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                   (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+#endif
+}
+
+// PK: pages of 16 keys, two to a tile of 32, or tiles of 32 or 64 keys of larger
+// ones.
+template <int DP, bool BF16, bool LIST, int PK>
 struct AttendShared {
   using T = std::conditional_t<BF16, __bf16, _Float16>;
   using Tx8 = std::conditional_t<BF16, bf16x8, halfx8>;
   using Tx4 = std::conditional_t<BF16, bf16x4, halfx4>;
+  static constexpr int NT = kColumnTiles;
+  static constexpr int kKeys = PK == 64 ? 64 : 32;  // of a tile
   static constexpr int kChunks = DP / 32, kTiles = DP / 16;
-  static constexpr float kBias = BF16 ? 0.0f : 14.0f;
+  static constexpr float kBias = kBiasOf<T>;
   static constexpr int kNone = 0x7FFFFFFF;
+  // copies of a wavefront, 1 KB each, of a tile's keys or values
+  static constexpr int kCopies = (kKeys * DP * 2 + 1024 * kSharedWaves - 1) / (1024 * kSharedWaves);
+  static constexpr int kTileBytes = kCopies * 1024 * kSharedWaves;
+  static constexpr int kBlocks = PK == 16 ? 2 : 1;
+
+  // Two buffers with names of their own: loads into one are not taken to alias
+  // reads of the other (which would wait for them).
+  struct Buffer {
+    char *k, *v;
+  };
+  struct Shared {
+    int lists[LIST ? kListInts : 1];
+    uint32_t window[kWindow / 32];
+    int lowest, again, furthest;
+  };
 
   const KvAttendArgs& a;
-  const int lane, col, grp, h;
+  Shared& sh;
+  const int lane, wave, col, grp, h;
+  const int d, ps, nc;  // values, keys of a page, 16-byte chunks of a K row
   const float c;
   Tx8 q[NT][kChunks];
   floatx4 o[NT][kTiles];
   float m[NT], l[NT];
-  int pos[NT];               // of the column's token
-  // the column's place in its token's list (in LDS; without lists, counting
-  // up) and its next block
-  int at[NT], next[NT];
+  int pos[NT];           // of the column's token
+  int at[NT], next[NT];  // its place in its list, and the block there
   bool on[NT];
+  // what this lane copies, in bytes from a tile's start (bit 31: of the second page)
+  uint32_t from_k[kCopies], from_v[kCopies];
+  int at_k[2][kChunks], at_v;            // where this lane's operands are, in bytes
 
-  __device__ __forceinline__ AttendShared(const KvAttendArgs& args, int ln, int head)
-      : a(args), lane(ln), col(ln & 15), grp(ln >> 4), h(head), c(args.scale * kLog2e) {}
+  __device__ __forceinline__ int swap_of_k(int row) const {
+    row &= 31;  // (alike in both halves of a tile)
+    return (nc & (nc - 1)) == 0 ? (row ^ (row >> 3)) & (nc - 1) : 0;
+  }
+  __device__ __forceinline__ static int swap_of_v(int row) {
+    return kKeys == 64 ? row & 7 : (row ^ (row >> 2)) & 3;
+  }
+
+  __device__ __forceinline__ AttendShared(const KvAttendArgs& args, Shared& s, int head)
+      : a(args), sh(s), lane(threadIdx.x & 63),
+        wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), col(lane & 15), grp(lane >> 4),
+        h(head), d(args.c.dim), ps(PK == 16 ? 16 : args.c.page), nc(d / 8),
+        c(args.scale * kLog2e) {
+    constexpr int nv = kKeys / 8;
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const int x = 64 * (wave + kSharedWaves * i) + lane;
+      // (past the head's values: the tile's start, which nobody reads there)
+      const int rk = x / nc, ck = (x % nc) ^ swap_of_k(rk);
+      const int rv = x / nv, cv = (x % nv) ^ swap_of_v(rv);
+      from_k[i] = rk < kKeys ? 2 * (rk * d + 8 * ck) : 0;
+      from_v[i] = rv < d ? 2 * (rv * ps + 8 * cv) : 0;
+      if constexpr (PK == 16) {
+        if (rk < kKeys && rk >= 16) from_k[i] = (2 * ((rk - 16) * d + 8 * ck)) | 1u << 31;
+        if (rv < d && cv >= 2) from_v[i] = (2 * (rv * ps + 8 * (cv - 2))) | 1u << 31;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int r = 8 * (col >> 2) + 4 * u + (col & 3);
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i)  // (past the head's values: any, and masked)
+        at_k[u][i] = 16 * (r * nc + (4 * i + grp < nc ? (4 * i + grp) ^ swap_of_k(r) : 0));
+    }
+    at_v = col * kKeys * 2 + 16 * (grp ^ swap_of_v(col));
+  }
 
   __device__ __forceinline__ void reset() {
 #pragma unroll
@@ -349,233 +453,370 @@ struct AttendShared {
     }
   }
 
+  // The block at the column's place of its list.
   __device__ __forceinline__ int entry(int n) const {
     if (!on[n]) return kNone;
-    if constexpr (LIST) return kv_lists[at[n]];
+    if constexpr (LIST) return sh.lists[at[n]];
     return at[n] <= min(pos[n] >> a.c.lps, a.q.cols - 1) ? at[n] : kNone;
   }
 
-  // The lowest next block of the columns that are on (kNone: no more), and how
-  // many of its keys each column sees.
-  __device__ __forceinline__ int advance(int (&seen)[NT]) {
-    int b = next[0];
+  // How many keys of block b each column sees, and how often it has it listed.
+  // Blocks before b that it has listed (their pages are absent) are passed by.
+  __device__ __forceinline__ void look(int b, int (&seen)[NT], int (&times)[NT]) {
 #pragma unroll
-    for (int n = 1; n < NT; ++n) b = min(b, next[n]);
-    b = __builtin_amdgcn_readfirstlane(row_min(b));
+    for (int n = 0; n < NT; ++n) times[n] = 0;
+    bool some = true;
+    while (some) {
+      bool moved = false;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const bool hit = next[n] == b && b != kNone;
-      seen[n] = hit ? min(a.c.page, pos[n] + 1 - (b << a.c.lps)) : 0;
-      if (hit) {
-        ++at[n];
-        next[n] = entry(n);
-      }
+      for (int n = 0; n < NT; ++n)
+        if (next[n] <= b) {
+          times[n] += next[n] == b;
+          ++at[n];
+          next[n] = entry(n);
+          moved = true;
+        }
+      some = __any(moved);
     }
-    return b;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) seen[n] = times[n] ? min(ps, pos[n] + 1 - (b << a.c.lps)) : 0;
   }
 
-  // What one look at the lists gives: the keys of a block (of two pages of 16).
-  struct Unit {
-    const T *k, *v;  // this lane's K row and V^T row of its first 32 keys
-    int lim[NT];     // of those, and this lane's 8, the first that a column sees
-    int top;         // keys that any column sees
-    bool all;        // every column sees all
-  };
-  // blocks looked up ahead, so that their pages are known in time
-  static constexpr int kBlocks = P16 ? 2 : 1;
-  int block[kBlocks], page[kBlocks], seen[kBlocks][NT];
+  // ---- the union of the workgroup's blocks, the same on every wavefront ----------
+  uint32_t bits;      // lists: blocks 32 lane .. of the window
+  int base, floor;    // the window's first block, the one past its last
+  int counter;        // without lists: the next block
+  int last;           // the furthest position of the workgroup's tokens
 
-  __device__ __forceinline__ void look(const int32_t* table) {
+  __device__ __forceinline__ int next_block() {
+    if constexpr (!LIST) {
+      return counter <= min(last >> a.c.lps, a.q.cols - 1) ? counter++ : kNone;
+    } else {
+      const uint64_t some = __ballot(bits != 0);
+      if (!some) return kNone;
+      const int i = __builtin_ctzll(some);
+      const uint32_t w = __builtin_amdgcn_readlane(bits, i);
+      if (lane == i) bits &= bits - 1;
+      return base + 32 * i + __builtin_ctz(w);
+    }
+  }
+
+  struct Tile {
+    int block[kBlocks], page[kBlocks], off;
+  };
+  const int32_t* table;
+
+  // The next tile; false: no more.
+  __device__ __forceinline__ bool next_tile(Tile& t) {
+    if constexpr (PK != 16) {
+      t.off += kKeys;
+      if (t.off < ps && t.off < last + 1 - (t.block[0] << a.c.lps)) return true;
+    }
+    t.off = 0;
+    while (true) {
+      bool some = false;
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i) {
+        t.block[i] = block[i];
+        t.page[i] = block[i] == kNone || page[i] < 0 || page[i] >= a.c.pages ? -1 : page[i];
+        some |= t.page[i] >= 0;
+      }
+      find();
+      if (some) return true;
+      if (t.block[kBlocks - 1] == kNone) return false;
+    }
+  }
+
+  // The blocks after that, looked up a tile ahead.
+  int block[kBlocks], page[kBlocks];
+
+  __device__ __forceinline__ void find() {
 #pragma unroll
     for (int i = 0; i < kBlocks; ++i) {
-      block[i] = advance(seen[i]);
+      block[i] = next_block();
       page[i] = table_entry(table, block[i] == kNone ? 0 : block[i]);
     }
   }
 
-  // The next unit whose pages are there; false: no more.
-  __device__ __forceinline__ bool unit(const int32_t* table, Unit& u) {
-    const int ps = P16 ? 16 : a.c.page, d = a.c.dim;
+  // Copies a tile's keys and values into a buffer.
+  __device__ __forceinline__ void copy(const Tile& t, Buffer to_) {
+    const char *k[kBlocks], *v[kBlocks];
     const int64_t head = (int64_t)ps * d;
-    while (block[0] != kNone) {
-      bool there[kBlocks], some = false;
-      int p[kBlocks];
 #pragma unroll
-      for (int i = 0; i < kBlocks; ++i) {
-        there[i] = block[i] != kNone && page[i] >= 0 && page[i] < a.c.pages;
-        some |= there[i];
-        p[i] = there[i] ? page[i] : 0;  // (an absent page is read as page 0 and not seen)
-      }
-      if (some) {
-        const int row = 8 * (col >> 2);  // this lane's K rows start here
-        int64_t pk = p[0], pv = p[0];
-        if constexpr (P16) {
-          pk = row < 16 ? p[0] : p[1];
-          pv = grp < 2 ? p[0] : p[1];
-        }
-        u.k = (const T*)a.c.keys + (pk * a.c.heads + h) * head +
-              ((P16 ? row & 15 : row) + (col & 3)) * d + 8 * grp;
-        u.v = (const T*)a.c.values + (pv * a.c.heads + h) * head + col * ps +
-              (P16 ? (8 * grp) & 15 : 8 * grp);
-        int top = 0;
-        u.all = true;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          int s = there[0] ? seen[0][n] : 0;
-          if constexpr (P16) {
-            const int s1 = there[1] ? seen[1][n] : 0;
-            top = max(top, s1 > 0 ? 16 + s1 : s);
-            u.all &= s == 16 && s1 == 16;
-            u.lim[n] = (grp < 2 ? s : s1) - ((8 * grp) & 15);
-          } else {
-            top = max(top, s);
-            u.all &= s == ps;
-            u.lim[n] = s - 8 * grp;
-          }
-        }
-        u.top = __builtin_amdgcn_readfirstlane(row_max(top));
-        u.all = __all(u.all);
-      }
-      look(table);
-      if (some) return true;
+    for (int i = 0; i < kBlocks; ++i) {
+      // (an absent page of a pair is read as page 0 and not seen)
+      const int64_t p = ((int64_t)max(0, t.page[i]) * a.c.heads + h) * head;
+      k[i] = (const char*)a.c.keys + 2 * (p + (PK == 16 ? 0 : t.off * d));
+      v[i] = (const char*)a.c.values + 2 * (p + (PK == 16 ? 0 : t.off));
     }
-    return false;
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const int to = 1024 * (wave + kSharedWaves * i);
+      const char *fk = k[0] + from_k[i], *fv = v[0] + from_v[i];
+      if constexpr (PK == 16) {
+        fk = (from_k[i] >> 31 ? k[1] : k[0]) + (from_k[i] & 0x7FFFFFFF);
+        fv = (from_v[i] >> 31 ? v[1] : v[0]) + (from_v[i] & 0x7FFFFFFF);
+      }
+      copy16_to_lds(fk, to_.k + to);
+      copy16_to_lds(fv, to_.v + to);
+    }
   }
 
-  // Loads without conditions, so that the waits count them: values past the
-  // head's are read in a place of its own and masked (K), or make sums that
-  // nobody stores (V).
-  __device__ __forceinline__ void load_k(uintx4 (&kf)[2][kChunks], const T* kp) const {
-    const int d = a.c.dim;
+  // Zeros in the place of values past the workgroup's furthest token, or of an
+  // absent page of a pair: a weight of 0 would not hide what is not finite.
+  __device__ __forceinline__ void clear(const Tile& t, Buffer in) {
+    constexpr int nv = kKeys / 8, kPer = PK == 16 ? 2 : nv;  // chunks of a row, of a page's
+    bool some = false;
+    int shown[kBlocks];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int i = 0; i < kBlocks; ++i) {
+      shown[i] = t.block[i] == kNone || t.page[i] < 0 ? 0 : last + 1 - (t.block[i] << a.c.lps) - t.off;
+      some |= shown[i] < 8 * kPer;
+    }
+    if (!some) return;
+    for (int x = threadIdx.x; x < d * nv; x += 64 * kSharedWaves) {
+      const int row = x / nv, chunk = (x % nv) ^ swap_of_v(row);
+      const int left = shown[chunk / kPer] - 8 * (chunk % kPer);
+      if (left < 8) *(uintx4*)(in.v + 16 * x) = keep(*(const uintx4*)(in.v + 16 * x), left);
+    }
+    __syncthreads();
+  }
+
+  // 32 keys of a buffer, from key `k0` of the tile on: of this lane's 8 keys
+  // column tile n sees the first n8[n].  `twice`: log2 of how often a block is
+  // listed.
+  __device__ __forceinline__ void step(Buffer from, int k0, const int (&n8)[NT], bool all,
+                                       const float (&twice)[NT]) {
+    floatx4 s[NT][2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      uintx4 kf[kChunks];
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
-        int at = 32 * i;
-        if (32 * i + 32 > sure_values(DP) && 32 * i + 8 * grp >= d) at = -8 * grp;
-        kf[u][i] = *(const uintx4*)(kp + 4 * u * d + at);
+        kf[i] = *(const uintx4*)(from.k + k0 * nc * 16 + at_k[u][i]);
+        if (32 * i + 32 > sure_values(DP) && 32 * i + 8 * grp >= d) kf[i] = uintx4{};
       }
-  }
-  __device__ __forceinline__ Tx8 k_row(const uintx4 (&kf)[kChunks], int i) const {
-    uintx4 x = kf[i];
-    if (32 * i + 32 > sure_values(DP) && 32 * i + 8 * grp >= a.c.dim) x = uintx4{};
-    return __builtin_bit_cast(Tx8, x);
-  }
-  __device__ __forceinline__ void load_v(uintx4 (&vf)[kTiles], const T* vp) const {
-    const int d = a.c.dim, ps = P16 ? 16 : a.c.page;
 #pragma unroll
-    for (int i = 0; i < kTiles; ++i) {
-      int row = 16 * i;
-      if (16 * i + 16 > sure_values(DP) && 16 * i + col >= d) row = -col;
-      vf[i] = *(const uintx4*)(vp + row * ps);
+      for (int n = 0; n < NT; ++n) {
+        s[n][u] = floatx4{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i)
+          s[n][u] = mfma(__builtin_bit_cast(Tx8, kf[i]), q[n][i], s[n][u]);
+      }
+    }
+    uintx4 vf[kTiles];
+    // (32 keys on, a chunk's place differs in one bit)
+    const char* v = from.v + (at_v ^ (k0 ? 64 : 0));
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) vf[i] = *(const uintx4*)(v + i * 32 * kKeys);
+    Tx8 pr[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      if (!all) hide(s[n], n8[n]);
+      Tx8 one[1];
+      weights<1>(s[n], m[n], l[n], c, twice[n], o[n], one);
+      pr[n] = one[0];
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i)
+        o[n][i] = mfma(__builtin_bit_cast(Tx8, vf[i]), pr[n], o[n][i]);
+  }
+
+  // A lane's 8 scores of which its column sees the first n.
+  __device__ __forceinline__ static void hide(floatx4 (&s)[2], int n) {
+    if (__any(n > 0 && n < 8)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i >= n) s[i / 4][i % 4] = -__builtin_inff();
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i / 4][i % 4] = n > 0 ? s[i / 4][i % 4] : -__builtin_inff();
     }
   }
 
-  // All blocks of the columns that are on, of request r, 32 keys a step; the K
-  // rows of the next step are on their way while this one's weights are made.
-  __device__ __forceinline__ void run(int r) {
-    const int d = a.c.dim;
-    const int32_t* table = a.q.table + (int64_t)r * a.q.table_stride;
+  // The steps of a tile in a buffer that this wavefront's tokens see; seen and
+  // times are kept over the tiles of a block.
+  int seen[kBlocks][NT], times[kBlocks][NT];
+
+  __device__ __forceinline__ void use(const Tile& t, Buffer from) {
+    if (t.off == 0) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) next[n] = entry(n);
-    look(table);
-    Unit u;
-    if (!unit(table, u)) return;
-    uintx4 kf[2][kChunks], vf[kTiles];
-    load_k(kf, u.k);
-    int off = 0;
-    for (bool more = true; more;) {
-      load_v(vf, u.v + off);
-      floatx4 s[NT][2];
+      for (int i = 0; i < kBlocks; ++i) {
+        if (t.block[i] != kNone) look(t.block[i], seen[i], times[i]);
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          s[n][x] = floatx4{0, 0, 0, 0};
-#pragma unroll
-          for (int i = 0; i < kChunks; ++i)
-            s[n][x] = mfma(k_row(kf[x], i), q[n][i], s[n][x]);
-        }
-      // this step's limits, then the next step
-      int n8[NT], most = 0;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        n8[n] = u.lim[n] - off;
-        most = max(most, n8[n]);
+        for (int n = 0; n < NT; ++n)
+          if (t.page[i] < 0) seen[i][n] = 0;
       }
-      const bool all = u.all;
-      off += 32;
-      if (off >= u.top) {
-        off = 0;
-        more = unit(table, u);
+    }
+    int top = 0, n8[NT];
+    float twice[NT];
+    bool all = true;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int s0 = seen[0][n] - t.off;
+      if constexpr (PK == 16) {
+        const int s1 = seen[1][n];
+        top = max(top, s1 > 0 ? 16 + s1 : s0);
+        all &= s0 == 16 && s1 == 16;
+        n8[n] = (grp < 2 ? s0 : s1) - ((8 * grp) & 15);
+        twice[n] = __log2f((float)max(1, grp < 2 ? times[0][n] : times[1][n]));
+      } else {
+        top = max(top, s0);
+        all &= s0 >= kKeys;
+        n8[n] = s0 - 8 * grp;
+        twice[n] = __log2f((float)max(1, times[0][n]));
       }
-      load_k(kf, u.k + off * d);  // (after the last step: its own once more)
-      Tx8 pr[NT];
+    }
+    top = __builtin_amdgcn_readfirstlane(row_max(top));
+    if (top <= 0) return;
+    all = __all(all);
+#pragma unroll 1
+    for (int k0 = 0; k0 < min(top, kKeys); k0 += 32) {
+      int left[NT];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        if (!all) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i >= n8[n]) s[n][i / 4][i % 4] = -__builtin_inff();
-        }
-        float top = m[n];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, s[n][i / 4][i % 4]);
-        top = column_max(top);
-        if (__any(top > m[n])) {
-          const float w = top == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((m[n] - top) * c);
-          l[n] *= w;
-#pragma unroll
-          for (int i = 0; i < kTiles; ++i) o[n][i] *= w;
-          m[n] = top;
-        }
-        const float base = kBias - (m[n] == -__builtin_inff() ? 0.0f : m[n]) * c;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float x = __builtin_amdgcn_exp2f(fmaf(s[n][i / 4][i % 4], c, base));
-          l[n] += x;
-          pr[n][i] = (T)x;
-        }
-      }
-      if (!all) {
-        most = row_max(most);
-        if (__any(most < 8)) {
-#pragma unroll
-          for (int i = 0; i < kTiles; ++i) vf[i] = keep(vf[i], most);
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i)
-          o[n][i] = mfma(__builtin_bit_cast(Tx8, vf[i]), pr[n], o[n][i]);
+      for (int n = 0; n < NT; ++n) left[n] = n8[n] - k0;
+      step(from, k0, left, all, twice);
     }
   }
+
+  uint64_t todo, with;  // tokens of this wavefront: to come, and of the request at hand
+  bool open;            // the request at hand may have blocks left
+
+  // Goes to the next request that some wavefront's tokens have; false: none.
+  // Every wavefront of the workgroup comes here, and into window().
+  __device__ __forceinline__ bool request(int myreq, const int (&tok)[NT], const bool (&mine)[NT],
+                                          int stride) {
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      sh.again = kNone;
+      sh.furthest = -1;
+    }
+    __syncthreads();
+    int r = todo >> lane & 1 ? myreq : kNone;
+#pragma unroll
+    for (int x = 32; x >= 1; x >>= 1) r = min(r, __shfl_xor(r, x));
+    if (lane == 0 && r != kNone) atomicMin(&sh.again, r);
+    __syncthreads();
+    r = __builtin_amdgcn_readfirstlane(sh.again);
+    if (r == kNone) return false;
+    with = todo & __ballot(myreq == r);
+    todo &= ~with;
+    table = a.q.table + (int64_t)r * a.q.table_stride;
+    int far = -1;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      on[n] = mine[n] && (with >> tok[n] & 1);
+      at[n] = LIST ? (first_list + tok[n]) * stride : 0;
+      next[n] = entry(n);
+      if (on[n]) far = max(far, pos[n]);
+    }
+    far = row_max(far);
+    if (lane == 0 && far >= 0) atomicMax(&sh.furthest, far);
+    __syncthreads();
+    last = __builtin_amdgcn_readfirstlane(sh.furthest);
+    base = counter = floor = 0;
+    return open = true;
+  }
+
+  // Makes the union of the request's next blocks, from the lowest that some token
+  // has listed on; false: none are left.
+  __device__ __forceinline__ bool window(int stride) {
+    if constexpr (!LIST) {
+      const bool was = open;
+      open = false;
+      return was;
+    }
+    // past the last window, whatever of it was absent: every window is a later one
+    if (floor > 0) {
+      int seen[NT], times[NT];
+      look(floor - 1, seen, times);
+    }
+    __syncthreads();
+    if (threadIdx.x < kWindow / 32) sh.window[threadIdx.x] = 0;
+    if (threadIdx.x == 0) sh.lowest = kNone;
+    __syncthreads();
+    int low = next[0];
+#pragma unroll
+    for (int n = 1; n < NT; ++n) low = min(low, next[n]);
+    low = row_min(low);
+    if (lane == 0 && low != kNone) atomicMin(&sh.lowest, low);
+    __syncthreads();
+    base = __builtin_amdgcn_readfirstlane(sh.lowest);
+    if (base == kNone) return open = false;
+    base &= ~(kWindow - 1);
+    floor = base + kWindow;
+    for (uint64_t left = with; left; left &= left - 1) {
+      const int* list = sh.lists + (first_list + __builtin_ctzll(left)) * stride;
+      for (int e = lane; e < stride; e += 64) {
+        const int b = list[e];
+        if (b == kNone) break;
+        if (b >= base && b - base < kWindow) atomicOr(&sh.window[(b - base) >> 5], 1u << (b & 31));
+      }
+    }
+    __syncthreads();
+    bits = sh.window[lane];
+    return true;
+  }
+
+  // All blocks of this wavefront's tokens `todo`.
+  __device__ __forceinline__ void run(int myreq, const int (&tok)[NT], const bool (&mine)[NT],
+                                      int stride, Buffer b0, Buffer b1) {
+    Tile now;
+    bool more = false;
+    open = false;
+    const auto turn = [&](Buffer from, Buffer to) {
+      Tile then = now;
+      more = next_tile(then);
+      dma_barrier();  // this tile is there, and the other buffer is free
+      mfma_settle();
+      if (more) copy(then, to);
+      clear(now, from);
+      use(now, from);
+      now = then;
+    };
+    // (one loop around the sums, so that they stay in one set of registers)
+    while (true) {
+      if (!more) {
+        while (true) {
+          if (!open && !request(myreq, tok, mine, stride)) return;
+          if (!window(stride)) continue;
+          now.off = 1 << 30;  // (past any block)
+          now.block[0] = 0;
+          find();
+          more = next_tile(now);
+          if (more) break;
+        }
+        __syncthreads();  // (the last tile's buffer is free)
+        copy(now, b0);
+      }
+      turn(b0, b1);
+      if (more) turn(b1, b0);
+    }
+  }
+
+  // The first of the workgroup's lists that is this wavefront's.
+  int first_list;
 };
 
-template <int DP>
-constexpr int kColumnTiles = DP <= 128 ? 2 : 1;  // (registers: two wavefronts a SIMD)
-
-// Tokens that share a wavefront, and wavefronts that share a token's heads.
-struct Sharing {
-  int tokens, tiles;
-};
-__host__ __device__ __forceinline__ Sharing sharing(int group, int columns) {
-  if (group <= columns) return {columns / group, 1};
-  return {1, (group + columns - 1) / columns};
-}
-
-template <int DP, bool BF16, bool LIST, bool P16>
-__global__ __launch_bounds__(64, 2) void kv_attend_shared_kernel(KvAttendArgs a) {
-  constexpr int NT = kColumnTiles<DP>;
-  using A = AttendShared<DP, BF16, LIST, P16, NT>;
-  const int group = a.q.group, lane = threadIdx.x;
-  const Sharing sh = sharing(group, kColumns * NT);
-  const int mt = (int)(blockIdx.x % sh.tiles);
-  const int h = (int)(blockIdx.x / sh.tiles % a.c.heads);
-  const int64_t t0 = (int64_t)(blockIdx.x / sh.tiles / a.c.heads) * sh.tokens;
-  const int tokens = (int)min<int64_t>(sh.tokens, a.q.tokens - t0);
-  A w(a, lane, h);
+template <int DP, bool BF16, bool LIST, int PK>
+__global__ __launch_bounds__(64 * kSharedWaves, DP <= 192 ? 2 : 1) void kv_attend_shared_kernel(KvAttendArgs a) {
+  using A = AttendShared<DP, BF16, LIST, PK>;
+  constexpr int NT = A::NT;
+  __shared__ typename A::Shared sh;
+  __shared__ __align__(16) char k0[A::kTileBytes], v0[A::kTileBytes], k1[A::kTileBytes],
+      v1[A::kTileBytes];
+  const int group = a.q.group;
+  const Sharing share = sharing(group, kColumns * NT, a.n);
+  // wavefronts go through the head tiles of a set of tokens, then to the next
+  const int h = (int)(blockIdx.x % a.c.heads);
+  A w(a, sh, h);
+  const int lane = w.lane;
+  const int64_t unit = (int64_t)(blockIdx.x / a.c.heads) * kSharedWaves + w.wave;
+  const int mt = (int)(unit % share.tiles);
+  const int64_t t0 = unit / share.tiles * share.tokens;
+  const int tokens = (int)max<int64_t>(0, min<int64_t>(share.tokens, a.q.tokens - t0));
   // lane i: token t0 + i
   int myreq = -1, mypos = -1;
   if (lane < tokens) {
@@ -583,22 +824,43 @@ __global__ __launch_bounds__(64, 2) void kv_attend_shared_kernel(KvAttendArgs a)
     mypos = a.q.positions[t0 + lane];
   }
   const bool sees = myreq >= 0 && myreq < a.q.requests && mypos >= 0;
+  const int stride = a.n + 1;
+  w.first_list = w.wave * share.tokens;
   if constexpr (LIST) {
-    // the tokens' lists, without the entries that show nothing
+    // the tokens' lists, without the entries that show nothing, ascending
     for (int i = 0; i < tokens; ++i) {
       const int own = __shfl(sees ? mypos >> a.c.lps : -1, i);
       const int32_t* from = a.blocks + ((t0 + i) * a.c.heads + h) * a.n;
-      int at = i * (a.n + 1);
+      int* list = sh.lists + (w.first_list + i) * stride;
+      int at = 0, before = -1;
+      bool ascends = true;
       for (int e = lane; e - lane < a.n; e += 64) {
         const int b = e < a.n ? from[e] : -1;
         const bool take = b >= 0 && b < a.q.cols && b <= own;
         const uint64_t taken = __ballot(take);
-        if (take) kv_lists[at + (int)__popcll(taken & ((uint64_t(1) << lane) - 1))] = b;
+        const uint64_t mine = taken & ((uint64_t(1) << lane) - 1);
+        if (take) list[at + (int)__popcll(mine)] = b;
+        const int left = __shfl(b, mine ? 63 - __builtin_clzll(mine) : 0);
+        ascends &= !take || b >= (mine ? left : before);
+        if (taken) before = __shfl(b, 63 - __builtin_clzll(taken));
         at += (int)__popcll(taken);
       }
-      if (lane == 0) kv_lists[at] = A::kNone;
+      if (lane == 0) list[at] = A::kNone;
+      if (!__all(ascends)) {
+        // each entry's place is the number of those below it, or equal and before
+        int b[kKvMaxBlocks / 64], to[kKvMaxBlocks / 64];
+#pragma unroll
+        for (int x = 0; x < kKvMaxBlocks / 64; ++x) {
+          const int e = lane + 64 * x;
+          b[x] = e < at ? list[e] : A::kNone;
+          to[x] = 0;
+          for (int y = 0; y < at; ++y) to[x] += list[y] < b[x] || (list[y] == b[x] && y < e);
+        }
+#pragma unroll
+        for (int x = 0; x < kKvMaxBlocks / 64; ++x)
+          if (lane + 64 * x < at) list[to[x]] = b[x];
+      }
     }
-    __syncthreads();
   }
   int tok[NT], g[NT];
   bool mine[NT];
@@ -621,21 +883,14 @@ __global__ __launch_bounds__(64, 2) void kv_attend_shared_kernel(KvAttendArgs a)
   }
   // first all tokens together, a request after another; then, if that left
   // sums that are not finite, each token by itself
-  for (int alone = -1; alone < tokens; ++alone) {
+  const int all_tokens = share.tokens * kSharedWaves;
+  for (int turn = -1; turn < all_tokens; ++turn) {
+    const int alone = turn < 0 ? -1 : turn - w.first_list;  // of this wavefront's
     w.reset();
-    uint64_t todo = __ballot(sees);
-    if (alone >= 0) todo &= uint64_t(1) << alone;
-    while (todo) {
-      const int r = __builtin_amdgcn_readlane(myreq, __builtin_ctzll(todo));
-      const uint64_t with = todo & __ballot(myreq == r);
-      todo &= ~with;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        w.on[n] = mine[n] && (with >> tok[n] & 1);
-        w.at[n] = LIST ? tok[n] * (a.n + 1) : 0;
-      }
-      w.run(r);
-    }
+    w.todo = __ballot(sees);
+    if (turn >= 0) w.todo &= alone >= 0 && alone < share.tokens ? uint64_t(1) << alone : 0;
+    w.run(myreq, tok, mine, stride, {k0, v0}, {k1, v1});
+    mfma_settle();
     bool good = true;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -644,11 +899,11 @@ __global__ __launch_bounds__(64, 2) void kv_attend_shared_kernel(KvAttendArgs a)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           good &= fabsf(w.o[n][i][j]) < __builtin_inff() || 16 * i + 4 * w.grp >= a.c.dim;
-    if (alone < 0 && !__all(good) && tokens > 1) continue;
+    if (turn < 0 && __syncthreads_or(!good)) continue;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const float l = column_sum(w.l[n]);
-      if (!mine[n] || (alone >= 0 && tok[n] != alone)) continue;
+      if (!mine[n] || (turn >= 0 && tok[n] != alone)) continue;
       const float inv = 1.0f / l;
       const int64_t at = ((t0 + tok[n]) * a.c.heads + h) * group + g[n];
 #pragma unroll
@@ -664,7 +919,7 @@ __global__ __launch_bounds__(64, 2) void kv_attend_shared_kernel(KvAttendArgs a)
       }
       if (a.lse && w.grp == 0) a.lse[at] = lse_of(w.m[n], l, a.scale, A::kBias);
     }
-    if (alone < 0) break;
+    if (turn < 0) break;
   }
 }
 
@@ -816,39 +1071,42 @@ __global__ __launch_bounds__(256) void kv_attend_join_kernel(KvAttendArgs a) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) x[j] = (T)(sum == 0.0f ? 0.0f : o[j] * inv);
   *(Tx4*)((T*)a.out + at * a.c.dim + d) = x;
-  if (a.lse && tid == 0) a.lse[at] = lse_of(top, sum, a.scale, BF16 ? 0.0f : 14.0f);
+  if (a.lse && tid == 0) a.lse[at] = lse_of(top, sum, a.scale, kBiasOf<T>);
 }
 
-int column_tiles(int dim) { return dim <= 128 ? kColumnTiles<128> : kColumnTiles<256>; }
-
 int64_t shared_grid(const KvAttendArgs& a) {
-  const Sharing sh = sharing(a.q.group, kColumns * column_tiles(a.c.dim));
-  return (a.q.tokens + sh.tokens - 1) / sh.tokens * a.c.heads * sh.tiles;
+  const Sharing sh = sharing(a.q.group, kColumns * kColumnTiles, a.n);
+  const int64_t units = (a.q.tokens + sh.tokens - 1) / sh.tokens * sh.tiles;
+  return (units + kSharedWaves - 1) / kSharedWaves * a.c.heads;
 }
 
 template <int DP, bool BF16, bool LIST, bool P16>
-void launch_one(const KvAttendArgs& a, hipStream_t s) {
-  if (a.waves == 1) {
-    const Sharing sh = sharing(a.q.group, kColumns * kColumnTiles<DP>);
-    const size_t lds = LIST ? sizeof(int) * sh.tokens * (a.n + 1) : 0;
-    kv_attend_shared_kernel<DP, BF16, LIST, P16>
-        <<<dim3((unsigned)shared_grid(a)), 64, lds, s>>>(a);
-    return;
-  }
+void launch_parts(const KvAttendArgs& a, hipStream_t s) {
   const int tiles = (a.q.group + kColumns - 1) / kColumns;
   const dim3 grid((unsigned)(a.q.tokens * a.c.heads * tiles * a.splits));
   if (a.waves == 8) kv_attend_parts_kernel<DP, BF16, LIST, P16, 8><<<grid, 512, 0, s>>>(a);
   else kv_attend_parts_kernel<DP, BF16, LIST, P16, 4><<<grid, 256, 0, s>>>(a);
 }
 
+template <int DP, bool BF16, bool LIST>
+void launch_listed(const KvAttendArgs& a, hipStream_t s) {
+  if (a.waves == 1) {
+    const dim3 grid((unsigned)shared_grid(a));
+    constexpr int kThreads = 64 * kSharedWaves;
+    // (tiles of 64 keys while two workgroups of them fit a CU)
+    constexpr int kLarge = DP <= 128 ? 64 : 32;
+    if (a.c.page == 16) kv_attend_shared_kernel<DP, BF16, LIST, 16><<<grid, kThreads, 0, s>>>(a);
+    else if (a.c.page == 32) kv_attend_shared_kernel<DP, BF16, LIST, 32><<<grid, kThreads, 0, s>>>(a);
+    else kv_attend_shared_kernel<DP, BF16, LIST, kLarge><<<grid, kThreads, 0, s>>>(a);
+    return;
+  }
+  if (a.c.page == 16) launch_parts<DP, BF16, LIST, true>(a, s);
+  else launch_parts<DP, BF16, LIST, false>(a, s);
+}
+
 template <int DP, bool BF16>
 void launch_dim(const KvAttendArgs& a, hipStream_t s) {
-  const bool p16 = a.c.page == 16;
-  if (a.blocks) {
-    p16 ? launch_one<DP, BF16, true, true>(a, s) : launch_one<DP, BF16, true, false>(a, s);
-  } else {
-    p16 ? launch_one<DP, BF16, false, true>(a, s) : launch_one<DP, BF16, false, false>(a, s);
-  }
+  a.blocks ? launch_listed<DP, BF16, true>(a, s) : launch_listed<DP, BF16, false>(a, s);
 }
 
 template <bool BF16>
@@ -872,7 +1130,7 @@ void kv_attend_plan(KvAttendArgs& a) {
   a.waves = 4;
   if (rows == 0) return;
   // tokens of prompts share wavefronts, if that leaves enough of them
-  if (a.q.tokens >= 4 * a.q.requests && shared_grid(a) >= 1024) {
+  if (a.q.tokens >= 4 * a.q.requests && shared_grid(a) >= 256) {
     a.waves = 1;
     return;
   }

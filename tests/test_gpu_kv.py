@@ -467,6 +467,78 @@ def test_attend_of_many_rows(engine, dtype, listed):
         check_attend(cache, dtype, q, table, who, positions, blocks=blocks)
 
 
+SHARED = [(128, 2, 16, 64, 70), (64, 5, 32, 80, 60), (64, 16, 64, 128, 24), (40, 20, 128, 96, 33),
+          (64, 8, 256, 256, 40), (64, 4, 64, 192, 50), (128, 1, 16, 248, 66), (64, 8, 64, 40, 50),
+          (96, 3, 32, 128, 60), (64, 7, 16, 128, 40), (32, 33, 16, 96, 25)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("heads,group,page,dim,tokens", SHARED)
+def test_attend_of_tokens_that_share_wavefronts(engine, heads, group, page, dim, tokens, dtype):
+    # neighbouring tokens of one request, of others, idle ones; everything, lists
+    # as select gives them, lists in any order with gaps and repeats
+    rng = np.random.default_rng(heads + dim)
+    cols = max(3, 200 // page)
+    cache = make_cache(engine, 2 * cols + 2, heads, page, dim, dtype, rng)
+    table = tables(rng, 2 * cols + 2, 2, cols)
+    table[1, 1] = -1  # an absent page
+    who = np.repeat([0, 1, 0, 5, 1], [tokens - 15, 5, 4, 1, 5])
+    positions = np.minimum(cols * page - 1, np.arange(tokens) * 3 + 7)
+    positions[[2, tokens - 3]] = -1
+    positions[-1] = 0
+    q = dev(rng.standard_normal((tokens, heads * group, dim), np.float32)).to(DTYPES[dtype])
+    check_attend(cache, dtype, q, table, who, positions)
+    n = 5
+    blocks = np.full((tokens, heads, n), -1)
+    for t in range(tokens):
+        for h in range(heads):
+            b = np.unique(rng.integers(0, max(1, positions[t] // page + 1), n))
+            blocks[t, h, :len(b)] = b
+    check_attend(cache, dtype, q, table, who, positions, blocks=blocks)
+    blocks = rng.integers(-2, cols + 2, (tokens, heads, 9))
+    check_attend(cache, dtype, q, table, who, positions, blocks=blocks)
+
+
+@pytest.mark.parametrize("n", [70, 256])
+def test_attend_over_long_lists_of_many_tokens(engine, n):
+    rng = np.random.default_rng(n)
+    heads, group, page, dim, cols, tokens = 96, 8, 16, 16, 2300, 24
+    cache = make_cache(engine, 300, heads, page, dim, "bf16", rng)
+    table = rng.integers(0, 300, (2, cols)).astype(np.int32)
+    who, positions = np.zeros(tokens, int), rng.integers(30_000, cols * page, tokens)
+    q = dev(rng.standard_normal((tokens, heads * group, dim), np.float32)).bfloat16()
+    blocks = np.sort(rng.integers(0, cols, (tokens, heads, n)), 2)
+    blocks[::3] = rng.permuted(blocks[::3], axis=2)
+    check_attend(cache, "bf16", q, table, who, positions, blocks=blocks)
+
+
+@pytest.mark.parametrize("listed", [False, True])
+@pytest.mark.parametrize("page", [16, 64])
+def test_what_only_later_tokens_see_does_not_reach_earlier_ones(engine, page, listed):
+    rng = np.random.default_rng(page)
+    heads, group, dim, cols, tokens = 64, 8, 64, 8, 40
+    cache = make_cache(engine, cols, heads, page, dim, "bf16", rng)
+    clean = make_cache(engine, cols, heads, page, dim, "bf16", rng)
+    clean.keys.copy_(cache.keys)
+    clean.values.copy_(cache.values)
+    table = np.arange(cols, dtype=np.int32)[None].repeat(2, 0)
+    who, positions = np.zeros(tokens, int), np.arange(tokens) + 2 * page
+    bad = 2 * page + 17  # (a key that tokens from the 17th on see)
+    cache.values[bad // page, :, 5, bad % page] = float("nan")
+    cache.values[bad // page, :, 9, bad % page] = float("inf")
+    cache.keys[7] = float("nan")
+    cache.values[7] = float("nan")
+    q = dev(rng.standard_normal((tokens, heads * group, dim), np.float32)).bfloat16()
+    blocks = np.tile(np.array([0, 1, 2, 3, 4, 5, 7], np.int32), (tokens, heads, 1)) if listed else None
+    want = check_attend(clean, "bf16", q, table, who, positions, blocks=blocks)
+    got = cache.attend(q, dev(table), dev(who, torch.int32), dev(positions, torch.int32),
+                       blocks=None if blocks is None else dev(blocks))
+    assert torch.equal(got[:17], want[:17])
+    others = [i for i in range(dim) if i not in (5, 9)]
+    assert torch.equal(got[17:][..., others], want[17:][..., others])
+    assert got[17:, :, 5].isnan().all() and got[17:, :, 9].isinf().all()
+
+
 @pytest.mark.parametrize("tokens", [1, 3, 17])
 def test_attend_over_a_long_cache(engine, tokens):
     # many parts that are joined; a request much shorter than the longest
