@@ -102,17 +102,17 @@ constexpr int sure_values(int dp) {
 }
 
 // log2 of what weights are scaled by: under f16 small terms of long sums stay
-// normal numbers (the largest weight is 2^14)
+// normal numbers (the largest weight is 2^14).
 template <typename T>
 constexpr float kBiasOf = std::is_same_v<T, _Float16> ? 14.0f : 0.0f;
 
-// The weights of a lane's scores, exp2(c s + bias + twice - c max) rounded to T,
+// The weights of a lane's scores, exp2(c s + bias - c max) rounded to T,
 // with the running maximum m and this lane's sum l of its column, and the
 // column's sums o scaled where the maximum moves.  (Letting the maximum lag by up
 // to 2^8 spares most of that: 3% on prompts; but then the largest weights, which
 // are whole otherwise, get rounded too: error against 64 bits 2.2e-3, not 2.0e-3.)
 template <int S, int TILES, typename T8>
-__device__ __forceinline__ void weights(floatx4 (&s)[2 * S], float& m, float& l, float c, float twice,
+__device__ __forceinline__ void weights(floatx4 (&s)[2 * S], float& m, float& l, float c, float bias,
                                         floatx4 (&o)[TILES], T8 (&p)[S]) {
   using T = std::conditional_t<std::is_same_v<T8, bf16x8>, __bf16, _Float16>;
   float top = m;
@@ -128,7 +128,7 @@ __device__ __forceinline__ void weights(floatx4 (&s)[2 * S], float& m, float& l,
     for (int i = 0; i < TILES; ++i) o[i] *= w;
     m = top;
   }
-  const float low = kBiasOf<T> + twice - (m == -__builtin_inff() ? 0.0f : m) * c;
+  const float low = bias - (m == -__builtin_inff() ? 0.0f : m) * c;
 #pragma unroll
   for (int u = 0; u < S; ++u)
 #pragma unroll
@@ -279,7 +279,7 @@ struct Attend {
       }
     }
     Tx8 pr[kPairs];
-    weights<kPairs>(s, m, l, c, 0.0f, o, pr);
+    weights<kPairs>(s, m, l, c, kBias, o, pr);
 #pragma unroll
     for (int p = 0; p < kPairs; ++p)
 #pragma unroll
@@ -373,11 +373,15 @@ struct AttendShared {
   static constexpr int NT = kColumnTiles;
   static constexpr int kKeys = PK == 64 ? 64 : 32;  // of a tile
   static constexpr int kChunks = DP / 32, kTiles = DP / 16;
-  static constexpr float kBias = kBiasOf<T>;
+  // (room for a block that is listed 256 times)
+  static constexpr float kBias = BF16 ? 0.0f : 7.0f;
   static constexpr int kNone = 0x7FFFFFFF;
-  // copies of a wavefront, 1 KB each, of a tile's keys or values
-  static constexpr int kCopies = (kKeys * DP * 2 + 1024 * kSharedWaves - 1) / (1024 * kSharedWaves);
-  static constexpr int kTileBytes = kCopies * 1024 * kSharedWaves;
+  // K rows lie at a power of two of 16-byte chunks in LDS, V^T rows densely; 1 KB
+  // copies, dealt to the wavefronts
+  static constexpr int kRow = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;
+  static constexpr int kPerCopy = 1024 * kSharedWaves;
+  static constexpr int kCopiesK = kKeys * kRow * 16 / kPerCopy;
+  static constexpr int kCopiesV = (kKeys * DP * 2 + kPerCopy - 1) / kPerCopy;
   static constexpr int kBlocks = PK == 16 ? 2 : 1;
 
   // Two buffers with names of their own: loads into one are not taken to alias
@@ -394,7 +398,7 @@ struct AttendShared {
   const KvAttendArgs& a;
   Shared& sh;
   const int lane, wave, col, grp, h;
-  const int d, ps, nc;  // values, keys of a page, 16-byte chunks of a K row
+  const int d, ps;  // values, keys of a page
   const float c;
   Tx8 q[NT][kChunks];
   floatx4 o[NT][kTiles];
@@ -403,12 +407,14 @@ struct AttendShared {
   int at[NT], next[NT];  // its place in its list, and the block there
   bool on[NT];
   // what this lane copies, in bytes from a tile's start (bit 31: of the second page)
-  uint32_t from_k[kCopies], from_v[kCopies];
-  int at_k[2][kChunks], at_v;            // where this lane's operands are, in bytes
+  uint32_t from_k[kCopiesK], from_v[kCopiesV];
+  int at_k, at_v;  // where this lane's first operands are, in bytes
 
-  __device__ __forceinline__ int swap_of_k(int row) const {
+  // Chunks of a row are swapped so that the 8 lanes that read together, rows 0 to
+  // 3 and 8 to 11 or neighbours, find 8 sets of banks.
+  __device__ __forceinline__ static int swap_of_k(int row) {
     row &= 31;  // (alike in both halves of a tile)
-    return (nc & (nc - 1)) == 0 ? (row ^ (row >> 3)) & (nc - 1) : 0;
+    return (row ^ (row >> 3)) & (kRow - 1);
   }
   __device__ __forceinline__ static int swap_of_v(int row) {
     return kKeys == 64 ? row & 7 : (row ^ (row >> 2)) & 3;
@@ -417,29 +423,27 @@ struct AttendShared {
   __device__ __forceinline__ AttendShared(const KvAttendArgs& args, Shared& s, int head)
       : a(args), sh(s), lane(threadIdx.x & 63),
         wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), col(lane & 15), grp(lane >> 4),
-        h(head), d(args.c.dim), ps(PK == 16 ? 16 : args.c.page), nc(d / 8),
-        c(args.scale * kLog2e) {
+        h(head), d(args.c.dim), ps(PK == 16 ? 16 : args.c.page), c(args.scale * kLog2e) {
     constexpr int nv = kKeys / 8;
+    // (past the head's values: the tile's start, for chunks that nobody uses)
 #pragma unroll
-    for (int i = 0; i < kCopies; ++i) {
+    for (int i = 0; i < kCopiesK; ++i) {
       const int x = 64 * (wave + kSharedWaves * i) + lane;
-      // (past the head's values: the tile's start, which nobody reads there)
-      const int rk = x / nc, ck = (x % nc) ^ swap_of_k(rk);
-      const int rv = x / nv, cv = (x % nv) ^ swap_of_v(rv);
-      from_k[i] = rk < kKeys ? 2 * (rk * d + 8 * ck) : 0;
-      from_v[i] = rv < d ? 2 * (rv * ps + 8 * cv) : 0;
-      if constexpr (PK == 16) {
-        if (rk < kKeys && rk >= 16) from_k[i] = (2 * ((rk - 16) * d + 8 * ck)) | 1u << 31;
-        if (rv < d && cv >= 2) from_v[i] = (2 * (rv * ps + 8 * (cv - 2))) | 1u << 31;
-      }
+      const int row = x / kRow, chunk = (x % kRow) ^ swap_of_k(row);
+      const bool second = PK == 16 && row >= 16;
+      from_k[i] = 8 * chunk < d ? 2 * ((second ? row - 16 : row) * d + 8 * chunk) : 0;
+      if (second) from_k[i] |= 1u << 31;
     }
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int r = 8 * (col >> 2) + 4 * u + (col & 3);
-#pragma unroll
-      for (int i = 0; i < kChunks; ++i)  // (past the head's values: any, and masked)
-        at_k[u][i] = 16 * (r * nc + (4 * i + grp < nc ? (4 * i + grp) ^ swap_of_k(r) : 0));
+    for (int i = 0; i < kCopiesV; ++i) {
+      const int x = 64 * (wave + kSharedWaves * i) + lane;
+      const int row = x / nv, chunk = (x % nv) ^ swap_of_v(row);
+      const bool second = PK == 16 && chunk >= 2;
+      from_v[i] = row < d ? 2 * (row * ps + 8 * (second ? chunk - 2 : chunk)) : 0;
+      if (second) from_v[i] |= 1u << 31;
     }
+    const int r = 8 * (col >> 2) + (col & 3);
+    at_k = 16 * (r * kRow + (grp ^ swap_of_k(r)));
     at_v = col * kKeys * 2 + 16 * (grp ^ swap_of_v(col));
   }
 
@@ -549,17 +553,16 @@ struct AttendShared {
       k[i] = (const char*)a.c.keys + 2 * (p + (PK == 16 ? 0 : t.off * d));
       v[i] = (const char*)a.c.values + 2 * (p + (PK == 16 ? 0 : t.off));
     }
+    const auto place = [](const char* const (&page)[kBlocks], uint32_t at) {
+      if constexpr (PK == 16) return (at >> 31 ? page[1] : page[0]) + (at & 0x7FFFFFFF);
+      else return page[0] + at;
+    };
 #pragma unroll
-    for (int i = 0; i < kCopies; ++i) {
-      const int to = 1024 * (wave + kSharedWaves * i);
-      const char *fk = k[0] + from_k[i], *fv = v[0] + from_v[i];
-      if constexpr (PK == 16) {
-        fk = (from_k[i] >> 31 ? k[1] : k[0]) + (from_k[i] & 0x7FFFFFFF);
-        fv = (from_v[i] >> 31 ? v[1] : v[0]) + (from_v[i] & 0x7FFFFFFF);
-      }
-      copy16_to_lds(fk, to_.k + to);
-      copy16_to_lds(fv, to_.v + to);
-    }
+    for (int i = 0; i < kCopiesK; ++i)
+      copy16_to_lds(place(k, from_k[i]), to_.k + 1024 * (wave + kSharedWaves * i));
+#pragma unroll
+    for (int i = 0; i < kCopiesV; ++i)
+      copy16_to_lds(place(v, from_v[i]), to_.v + 1024 * (wave + kSharedWaves * i));
   }
 
   // Zeros in the place of values past the workgroup's furthest token, or of an
@@ -593,7 +596,8 @@ struct AttendShared {
       uintx4 kf[kChunks];
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
-        kf[i] = *(const uintx4*)(from.k + k0 * nc * 16 + at_k[u][i]);
+        // (a row 4 further on, and each 4 chunks, differ in one bit of the swap)
+        kf[i] = *(const uintx4*)(from.k + 16 * kRow * (k0 + 4 * u) + (at_k ^ (64 * (i ^ u))));
         if (32 * i + 32 > sure_values(DP) && 32 * i + 8 * grp >= d) kf[i] = uintx4{};
       }
 #pragma unroll
@@ -614,7 +618,7 @@ struct AttendShared {
     for (int n = 0; n < NT; ++n) {
       if (!all) hide(s[n], n8[n]);
       Tx8 one[1];
-      weights<1>(s[n], m[n], l[n], c, twice[n], o[n], one);
+      weights<1>(s[n], m[n], l[n], c, kBias + twice[n], o[n], one);
       pr[n] = one[0];
     }
 #pragma unroll
@@ -805,8 +809,8 @@ __global__ __launch_bounds__(64 * kSharedWaves, DP <= 192 ? 2 : 1) void kv_atten
   using A = AttendShared<DP, BF16, LIST, PK>;
   constexpr int NT = A::NT;
   __shared__ typename A::Shared sh;
-  __shared__ __align__(16) char k0[A::kTileBytes], v0[A::kTileBytes], k1[A::kTileBytes],
-      v1[A::kTileBytes];
+  __shared__ __align__(16) char k0[A::kCopiesK * A::kPerCopy], k1[A::kCopiesK * A::kPerCopy],
+      v0[A::kCopiesV * A::kPerCopy], v1[A::kCopiesV * A::kPerCopy];
   const int group = a.q.group;
   const Sharing share = sharing(group, kColumns * NT, a.n);
   // wavefronts go through the head tiles of a set of tokens, then to the next

@@ -512,6 +512,19 @@ def test_attend_over_long_lists_of_many_tokens(engine, n):
     check_attend(cache, "bf16", q, table, who, positions, blocks=blocks)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("tokens", [2, 40])
+def test_a_block_that_is_listed_256_times(engine, tokens, dtype):
+    rng = np.random.default_rng(tokens)
+    heads, group, page, dim, cols = 64, 8, 16, 32, 5
+    cache = make_cache(engine, cols, heads, page, dim, dtype, rng)
+    table = np.arange(cols, dtype=np.int32)[None]
+    q = dev(rng.standard_normal((tokens, heads * group, dim), np.float32)).to(DTYPES[dtype])
+    blocks = np.full((tokens, heads, 256), 3)
+    blocks[::2, :, 100:] = rng.integers(0, cols, (1, 1, 156))
+    check_attend(cache, dtype, q, table, np.zeros(tokens, int), np.full(tokens, 70), blocks=blocks)
+
+
 @pytest.mark.parametrize("listed", [False, True])
 @pytest.mark.parametrize("page", [16, 64])
 def test_what_only_later_tokens_see_does_not_reach_earlier_ones(engine, page, listed):
