@@ -110,7 +110,10 @@ __device__ void summarise(const KvCache& c, int64_t at, Sums& s, Row row) {
 // TILE tokens and a head.  FEW: the summaries too, in the same launch: the keys
 // of a completed page that this call writes are read where they come from, so
 // that no workgroup waits for another's stores (each looks all slots through
-// for them, which is why the call's tokens are few).
+// for them, which is why the call's tokens are few).  In one and two launches
+// (8 kv heads of 128 values, pages of 64): 256 requests' tokens 9.6 and 16.6 us,
+// 1,024 requests' 21.8 and 23.9; one request's 1,024 tokens 9.4 and 9.6, 2,048
+// 12.5 and 11.2.
 constexpr int kFew = 1024;
 
 template <bool BF16, int TILE, bool FEW>
@@ -193,8 +196,10 @@ template <bool BF16>
 hipError_t launch_append(const KvAppendArgs& a, hipStream_t s) {
   constexpr int kSpan = 16;
   if (a.tokens <= kFew && a.c.summaries) {
-    // (small tiles: a workgroup's summaries follow one another)
-    a.tokens <= 256 ? launch_tile<BF16, 4, true>(a, s) : launch_tile<BF16, 16, true>(a, s);
+    // Small tiles: a workgroup's summaries follow one another.  By 4 and 16: 64
+    // requests' tokens 6.9 and 12.0 us, 512 requests' 12.7 and 17.4 (one request's
+    // 512 tokens 8.8 and 8.2).
+    a.tokens <= 512 ? launch_tile<BF16, 4, true>(a, s) : launch_tile<BF16, 16, true>(a, s);
     return hipGetLastError();
   }
   launch_tile<BF16, 16, false>(a, s);

@@ -315,12 +315,12 @@ __device__ __forceinline__ int row_max(int x) {
   return max(x, row_ror<0x121>(x));
 }
 
-// Tokens of prompts.  A wavefront has as many neighbouring tokens as fill NT
-// tiles of 16 columns with their heads of a kv head (two tokens of 8 heads in a
-// tile), a workgroup four wavefronts.  Neighbours look at much the same blocks:
-// the workgroup walks the union of its tokens' blocks, each loaded once, and a
-// wavefront multiplies those that a token of its own takes; keys that a column's
-// token does not see get no weight.
+// Tokens of prompts.  A wavefront has as many neighbouring tokens as fill the 16
+// columns with their heads of a kv head (two of 8 heads), a workgroup four
+// wavefronts.  Neighbours look at much the same blocks: the workgroup walks the
+// union of its tokens' blocks, each loaded once, and a wavefront multiplies those
+// that a token of its own takes; keys that a column's token does not see get no
+// weight.
 //
 // What bounds it otherwise is loads: a wavefront's MFMA operands straight from
 // the cache are 16 bytes of 16 different rows to 16 neighbouring lanes, a row a
@@ -329,7 +329,10 @@ __device__ __forceinline__ int row_max(int x) {
 // 2.2 GB in 322 us, the same rate).  So tiles of keys and values go to LDS by
 // direct loads of neighbouring chunks, a tile ahead of the products, and the
 // operands come from there, in chunks that are swapped by row so that 8 lanes
-// read from 8 different sets of banks.
+// read from 8 different sets of banks: 250 us.  Of a tile of 64 keys that is now
+// 1.05 us for its products and weights (two wavefronts a SIMD, their chain of
+// scores, maxima, exponentials and sums not hidden by one another), 0.4 us for
+// issuing its copy, 0.5 us at its barrier.
 //
 // Lists in any order are right: one that does not ascend is sorted first, and a
 // block listed twice counts twice.
@@ -338,8 +341,6 @@ __device__ __forceinline__ int row_max(int x) {
 // token's keys are masked; one that only some of the tokens see would reach the
 // others' sums as NaN, so a workgroup whose sums are not finite does its tokens
 // over, one at a time.
-constexpr int kColumnTiles = 1;
-
 constexpr int kSharedWaves = 4;
 constexpr int kListInts = 3840;  // of all lists of a workgroup (two workgroups a CU)
 constexpr int kWindow = 2048;    // blocks whose union is made at a time
@@ -348,10 +349,10 @@ constexpr int kWindow = 2048;    // blocks whose union is made at a time
 struct Sharing {
   int tokens, tiles;
 };
-__host__ __device__ __forceinline__ Sharing sharing(int group, int columns, int n) {
-  if (group > columns) return {1, (group + columns - 1) / columns};
+__host__ __device__ __forceinline__ Sharing sharing(int group, int n) {
+  if (group > kColumns) return {1, (group + kColumns - 1) / kColumns};
   const int most = kListInts / kSharedWaves / (n + 1);
-  const int tokens = columns / group;
+  const int tokens = kColumns / group;
   return {tokens < most ? tokens : most, 1};
 }
 
@@ -370,7 +371,6 @@ struct AttendShared {
   using T = std::conditional_t<BF16, __bf16, _Float16>;
   using Tx8 = std::conditional_t<BF16, bf16x8, halfx8>;
   using Tx4 = std::conditional_t<BF16, bf16x4, halfx4>;
-  static constexpr int NT = kColumnTiles;
   static constexpr int kKeys = PK == 64 ? 64 : 32;  // of a tile
   static constexpr int kChunks = DP / 32, kTiles = DP / 16;
   // (room for a block that is listed 256 times)
@@ -400,12 +400,12 @@ struct AttendShared {
   const int lane, wave, col, grp, h;
   const int d, ps;  // values, keys of a page
   const float c;
-  Tx8 q[NT][kChunks];
-  floatx4 o[NT][kTiles];
-  float m[NT], l[NT];
-  int pos[NT];           // of the column's token
-  int at[NT], next[NT];  // its place in its list, and the block there
-  bool on[NT];
+  Tx8 q[kChunks];
+  floatx4 o[kTiles];
+  float m, l;
+  int pos;       // of the column's token
+  int at, next;  // its place in its list, and the block there
+  bool on;
   // what this lane copies, in bytes from a tile's start (bit 31: of the second page)
   uint32_t from_k[kCopiesK], from_v[kCopiesV];
   int at_k, at_v;  // where this lane's first operands are, in bytes
@@ -449,41 +449,34 @@ struct AttendShared {
 
   __device__ __forceinline__ void reset() {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int i = 0; i < kTiles; ++i) o[n][i] = floatx4{0, 0, 0, 0};
-      m[n] = -__builtin_inff();
-      l[n] = 0.0f;
-    }
+    for (int i = 0; i < kTiles; ++i) o[i] = floatx4{0, 0, 0, 0};
+    m = -__builtin_inff();
+    l = 0.0f;
   }
 
   // The block at the column's place of its list.
-  __device__ __forceinline__ int entry(int n) const {
-    if (!on[n]) return kNone;
-    if constexpr (LIST) return sh.lists[at[n]];
-    return at[n] <= min(pos[n] >> a.c.lps, a.q.cols - 1) ? at[n] : kNone;
+  __device__ __forceinline__ int entry() const {
+    if (!on) return kNone;
+    if constexpr (LIST) return sh.lists[at];
+    return at <= min(pos >> a.c.lps, a.q.cols - 1) ? at : kNone;
   }
 
   // How many keys of block b each column sees, and how often it has it listed.
   // Blocks before b that it has listed (their pages are absent) are passed by.
-  __device__ __forceinline__ void look(int b, int (&seen)[NT], int (&times)[NT]) {
-#pragma unroll
-    for (int n = 0; n < NT; ++n) times[n] = 0;
+  __device__ __forceinline__ void look(int b, int& seen, int& times) {
+    times = 0;
     bool some = true;
     while (some) {
       bool moved = false;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-        if (next[n] <= b) {
-          times[n] += next[n] == b;
-          ++at[n];
-          next[n] = entry(n);
-          moved = true;
-        }
+      if (next <= b) {
+        times += next == b;
+        ++at;
+        next = entry();
+        moved = true;
+      }
       some = __any(moved);
     }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) seen[n] = times[n] ? min(ps, pos[n] + 1 - (b << a.c.lps)) : 0;
+    seen = times ? min(ps, pos + 1 - (b << a.c.lps)) : 0;
   }
 
   // ---- the union of the workgroup's blocks, the same on every wavefront ----------
@@ -585,12 +578,10 @@ struct AttendShared {
     __syncthreads();
   }
 
-  // 32 keys of a buffer, from key `k0` of the tile on: of this lane's 8 keys
-  // column tile n sees the first n8[n].  `twice`: log2 of how often a block is
-  // listed.
-  __device__ __forceinline__ void step(Buffer from, int k0, const int (&n8)[NT], bool all,
-                                       const float (&twice)[NT]) {
-    floatx4 s[NT][2];
+  // 32 keys of a buffer, from key `k0` of the tile on: of this lane's 8 keys its
+  // column sees the first n8.  `twice`: log2 of how often a block is listed.
+  __device__ __forceinline__ void step(Buffer from, int k0, int n8, bool all, float twice) {
+    floatx4 s[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       uintx4 kf[kChunks];
@@ -600,32 +591,22 @@ struct AttendShared {
         kf[i] = *(const uintx4*)(from.k + 16 * kRow * (k0 + 4 * u) + (at_k ^ (64 * (i ^ u))));
         if (32 * i + 32 > sure_values(DP) && 32 * i + 8 * grp >= d) kf[i] = uintx4{};
       }
+      s[u] = floatx4{0, 0, 0, 0};
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        s[n][u] = floatx4{0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < kChunks; ++i)
-          s[n][u] = mfma(__builtin_bit_cast(Tx8, kf[i]), q[n][i], s[n][u]);
-      }
+      for (int i = 0; i < kChunks; ++i)
+        s[u] = mfma(__builtin_bit_cast(Tx8, kf[i]), q[i], s[u]);
     }
     uintx4 vf[kTiles];
     // (32 keys on, a chunk's place differs in one bit)
     const char* v = from.v + (at_v ^ (k0 ? 64 : 0));
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) vf[i] = *(const uintx4*)(v + i * 32 * kKeys);
-    Tx8 pr[NT];
+    if (!all) hide(s, n8);
+    Tx8 pr[1];
+    weights<1>(s, m, l, c, kBias + twice, o, pr);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      if (!all) hide(s[n], n8[n]);
-      Tx8 one[1];
-      weights<1>(s[n], m[n], l[n], c, kBias + twice[n], o[n], one);
-      pr[n] = one[0];
-    }
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < kTiles; ++i)
-        o[n][i] = mfma(__builtin_bit_cast(Tx8, vf[i]), pr[n], o[n][i]);
+    for (int i = 0; i < kTiles; ++i)
+      o[i] = mfma(__builtin_bit_cast(Tx8, vf[i]), pr[0], o[i]);
   }
 
   // A lane's 8 scores of which its column sees the first n.
@@ -642,47 +623,37 @@ struct AttendShared {
 
   // The steps of a tile in a buffer that this wavefront's tokens see; seen and
   // times are kept over the tiles of a block.
-  int seen[kBlocks][NT], times[kBlocks][NT];
+  int seen[kBlocks], times[kBlocks];
 
   __device__ __forceinline__ void use(const Tile& t, Buffer from) {
     if (t.off == 0) {
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i) {
         if (t.block[i] != kNone) look(t.block[i], seen[i], times[i]);
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-          if (t.page[i] < 0) seen[i][n] = 0;
+        if (t.page[i] < 0) seen[i] = 0;
       }
     }
-    int top = 0, n8[NT];
-    float twice[NT];
+    int top = 0, n8;
+    float twice;
     bool all = true;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int s0 = seen[0][n] - t.off;
-      if constexpr (PK == 16) {
-        const int s1 = seen[1][n];
-        top = max(top, s1 > 0 ? 16 + s1 : s0);
-        all &= s0 == 16 && s1 == 16;
-        n8[n] = (grp < 2 ? s0 : s1) - ((8 * grp) & 15);
-        twice[n] = __log2f((float)max(1, grp < 2 ? times[0][n] : times[1][n]));
-      } else {
-        top = max(top, s0);
-        all &= s0 >= kKeys;
-        n8[n] = s0 - 8 * grp;
-        twice[n] = __log2f((float)max(1, times[0][n]));
-      }
+    const int s0 = seen[0] - t.off;
+    if constexpr (PK == 16) {
+      const int s1 = seen[1];
+      top = max(top, s1 > 0 ? 16 + s1 : s0);
+      all &= s0 == 16 && s1 == 16;
+      n8 = (grp < 2 ? s0 : s1) - ((8 * grp) & 15);
+      twice = __log2f((float)max(1, grp < 2 ? times[0] : times[1]));
+    } else {
+      top = max(top, s0);
+      all &= s0 >= kKeys;
+      n8 = s0 - 8 * grp;
+      twice = __log2f((float)max(1, times[0]));
     }
     top = __builtin_amdgcn_readfirstlane(row_max(top));
     if (top <= 0) return;
     all = __all(all);
 #pragma unroll 1
-    for (int k0 = 0; k0 < min(top, kKeys); k0 += 32) {
-      int left[NT];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) left[n] = n8[n] - k0;
-      step(from, k0, left, all, twice);
-    }
+    for (int k0 = 0; k0 < min(top, kKeys); k0 += 32) step(from, k0, n8 - k0, all, twice);
   }
 
   uint64_t todo, with;  // tokens of this wavefront: to come, and of the request at hand
@@ -690,8 +661,7 @@ struct AttendShared {
 
   // Goes to the next request that some wavefront's tokens have; false: none.
   // Every wavefront of the workgroup comes here, and into window().
-  __device__ __forceinline__ bool request(int myreq, const int (&tok)[NT], const bool (&mine)[NT],
-                                          int stride) {
+  __device__ __forceinline__ bool request(int myreq, int tok, bool mine, int stride) {
     __syncthreads();
     if (threadIdx.x == 0) {
       sh.again = kNone;
@@ -709,13 +679,10 @@ struct AttendShared {
     todo &= ~with;
     table = a.q.table + (int64_t)r * a.q.table_stride;
     int far = -1;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      on[n] = mine[n] && (with >> tok[n] & 1);
-      at[n] = LIST ? (first_list + tok[n]) * stride : 0;
-      next[n] = entry(n);
-      if (on[n]) far = max(far, pos[n]);
-    }
+    on = mine && (with >> tok & 1);
+    at = LIST ? (first_list + tok) * stride : 0;
+    next = entry();
+    if (on) far = max(far, pos);
     far = row_max(far);
     if (lane == 0 && far >= 0) atomicMax(&sh.furthest, far);
     __syncthreads();
@@ -734,16 +701,14 @@ struct AttendShared {
     }
     // past the last window, whatever of it was absent: every window is a later one
     if (floor > 0) {
-      int seen[NT], times[NT];
+      int seen, times;
       look(floor - 1, seen, times);
     }
     __syncthreads();
     if (threadIdx.x < kWindow / 32) sh.window[threadIdx.x] = 0;
     if (threadIdx.x == 0) sh.lowest = kNone;
     __syncthreads();
-    int low = next[0];
-#pragma unroll
-    for (int n = 1; n < NT; ++n) low = min(low, next[n]);
+    int low = next;
     low = row_min(low);
     if (lane == 0 && low != kNone) atomicMin(&sh.lowest, low);
     __syncthreads();
@@ -765,8 +730,8 @@ struct AttendShared {
   }
 
   // All blocks of this wavefront's tokens `todo`.
-  __device__ __forceinline__ void run(int myreq, const int (&tok)[NT], const bool (&mine)[NT],
-                                      int stride, Buffer b0, Buffer b1) {
+  __device__ __forceinline__ void run(int myreq, int tok, bool mine, int stride, Buffer b0,
+                                      Buffer b1) {
     Tile now;
     bool more = false;
     open = false;
@@ -805,14 +770,14 @@ struct AttendShared {
 };
 
 template <int DP, bool BF16, bool LIST, int PK>
-__global__ __launch_bounds__(64 * kSharedWaves, DP <= 192 ? 2 : 1) void kv_attend_shared_kernel(KvAttendArgs a) {
+__global__ __launch_bounds__(64 * kSharedWaves, DP <= 192 ? 2 : 1)
+void kv_attend_shared_kernel(KvAttendArgs a) {
   using A = AttendShared<DP, BF16, LIST, PK>;
-  constexpr int NT = A::NT;
   __shared__ typename A::Shared sh;
   __shared__ __align__(16) char k0[A::kCopiesK * A::kPerCopy], k1[A::kCopiesK * A::kPerCopy],
       v0[A::kCopiesV * A::kPerCopy], v1[A::kCopiesV * A::kPerCopy];
   const int group = a.q.group;
-  const Sharing share = sharing(group, kColumns * NT, a.n);
+  const Sharing share = sharing(group, a.n);
   // wavefronts go through the head tiles of a set of tokens, then to the next
   const int h = (int)(blockIdx.x % a.c.heads);
   A w(a, sh, h);
@@ -866,24 +831,17 @@ __global__ __launch_bounds__(64 * kSharedWaves, DP <= 192 ? 2 : 1) void kv_atten
       }
     }
   }
-  int tok[NT], g[NT];
-  bool mine[NT];
+  const int x = mt * kColumns + w.col;  // column
+  const bool mine = x / group < tokens;
+  const int tok = mine ? x / group : 0, g = x % group;
+  w.pos = __shfl(mypos, tok);
+  const auto* src = (const typename A::T*)a.q.q + (t0 + tok) * a.q.q_token +
+                    (int64_t)(h * group + g) * a.q.q_head;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int x = mt * kColumns * NT + kColumns * n + w.col;  // column
-    tok[n] = x / group;
-    g[n] = x % group;
-    mine[n] = tok[n] < tokens;
-    if (!mine[n]) tok[n] = 0;
-    w.pos[n] = __shfl(mypos, tok[n]);
-    const auto* src = (const typename A::T*)a.q.q + (t0 + tok[n]) * a.q.q_token +
-                      (int64_t)(h * group + g[n]) * a.q.q_head;
-#pragma unroll
-    for (int i = 0; i < A::kChunks; ++i) {
-      uintx4 x4 = {};
-      if (mine[n] && 32 * i + 8 * w.grp < a.c.dim) x4 = *(const uintx4*)(src + 32 * i + 8 * w.grp);
-      w.q[n][i] = __builtin_bit_cast(typename A::Tx8, x4);
-    }
+  for (int i = 0; i < A::kChunks; ++i) {
+    uintx4 x4 = {};
+    if (mine && 32 * i + 8 * w.grp < a.c.dim) x4 = *(const uintx4*)(src + 32 * i + 8 * w.grp);
+    w.q[i] = __builtin_bit_cast(typename A::Tx8, x4);
   }
   // first all tokens together, a request after another; then, if that left
   // sums that are not finite, each token by itself
@@ -897,44 +855,40 @@ __global__ __launch_bounds__(64 * kSharedWaves, DP <= 192 ? 2 : 1) void kv_atten
     mfma_settle();
     bool good = true;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int i = 0; i < A::kTiles; ++i)
 #pragma unroll
-      for (int i = 0; i < A::kTiles; ++i)
+      for (int j = 0; j < 4; ++j)
+        good &= fabsf(w.o[i][j]) < __builtin_inff() || 16 * i + 4 * w.grp >= a.c.dim;
+    if (turn < 0 && __syncthreads_or(!good)) continue;
+    const float l = column_sum(w.l);
+    if (!mine || (turn >= 0 && tok != alone)) continue;
+    const float inv = 1.0f / l;
+    const int64_t at = ((t0 + tok) * a.c.heads + h) * group + g;
+#pragma unroll
+    for (int i = 0; i < A::kTiles; ++i) {
+      const int d = 16 * i + 4 * w.grp;
+      if (d < a.c.dim) {
+        typename A::Tx4 x;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          good &= fabsf(w.o[n][i][j]) < __builtin_inff() || 16 * i + 4 * w.grp >= a.c.dim;
-    if (turn < 0 && __syncthreads_or(!good)) continue;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const float l = column_sum(w.l[n]);
-      if (!mine[n] || (turn >= 0 && tok[n] != alone)) continue;
-      const float inv = 1.0f / l;
-      const int64_t at = ((t0 + tok[n]) * a.c.heads + h) * group + g[n];
-#pragma unroll
-      for (int i = 0; i < A::kTiles; ++i) {
-        const int d = 16 * i + 4 * w.grp;
-        if (d < a.c.dim) {
-          typename A::Tx4 x;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            x[j] = (typename A::T)(l == 0.0f ? 0.0f : w.o[n][i][j] * inv);
-          *(typename A::Tx4*)((typename A::T*)a.out + at * a.c.dim + d) = x;
-        }
+          x[j] = (typename A::T)(l == 0.0f ? 0.0f : w.o[i][j] * inv);
+        *(typename A::Tx4*)((typename A::T*)a.out + at * a.c.dim + d) = x;
       }
-      if (a.lse && w.grp == 0) a.lse[at] = lse_of(w.m[n], l, a.scale, A::kBias);
     }
+    if (a.lse && w.grp == 0) a.lse[at] = lse_of(w.m, l, a.scale, A::kBias);
     if (turn < 0) break;
   }
 }
 
-// A part of a row's keys for each workgroup, its steps dealt to the W wavefronts
-// in turn.
-template <int DP, bool BF16, bool LIST, bool P16, int W>
-__global__ __launch_bounds__(64 * W, 2) void kv_attend_parts_kernel(KvAttendArgs a) {
-  constexpr int H = 4;  // wavefronts whose sums meet in LDS at a time
+// A part of a row's keys for each workgroup, its steps dealt to 4 wavefronts in
+// turn.  (Eight spare 0.4 us of 12.8 on one token of 777 keys and cost 3 us of
+// 45.5 on 256 rows of 2,048.)
+template <int DP, bool BF16, bool LIST, bool P16>
+__global__ __launch_bounds__(256, 2) void kv_attend_parts_kernel(KvAttendArgs a) {
+  constexpr int W = 4;
   using A = Attend<DP, BF16, LIST, P16>;
-  __shared__ float so[H][kColumns][DP + 4];
-  __shared__ float sm[H][kColumns], sl[H][kColumns];
+  __shared__ float so[W][kColumns][DP + 4];
+  __shared__ float sm[W][kColumns], sl[W][kColumns];
   const int tiles = (a.q.group + kColumns - 1) / kColumns;
   // first parts first: a row's later ones may be empty, and workgroups go round
   // the 8 XCDs
@@ -965,46 +919,25 @@ __global__ __launch_bounds__(64 * W, 2) void kv_attend_parts_kernel(KvAttendArgs
   }
   w.l = column_sum(w.l);
   const float c = a.scale * kLog2e;
-  const auto put = [&](int x) {
-    if (w.grp == 0) {
-      sm[x][w.col] = w.m;
-      sl[x][w.col] = w.l;
-    }
-#pragma unroll
-    for (int i = 0; i < A::kTiles; ++i) *(floatx4*)&so[x][w.col][16 * i + 4 * w.grp] = w.o[i];
-  };
-  if constexpr (W > H) {
-    static_assert(W == 2 * H, "pairs of wavefronts");
-    if (wave >= H) put(wave - H);
-    __syncthreads();
-    if (wave < H) {
-      const float m = sm[wave][w.col], top = fmaxf(w.m, m);
-      const float safe = top == -__builtin_inff() ? 0.0f : top;
-      const float f0 = __builtin_amdgcn_exp2f((w.m - safe) * c);
-      const float f1 = __builtin_amdgcn_exp2f((m - safe) * c);
-      w.m = top;
-      w.l = w.l * f0 + sl[wave][w.col] * f1;
-#pragma unroll
-      for (int i = 0; i < A::kTiles; ++i)
-        w.o[i] = w.o[i] * f0 + *(const floatx4*)&so[wave][w.col][16 * i + 4 * w.grp] * f1;
-      put(wave);  // (in the places that this lane has read)
-    }
-  } else {
-    put(wave);
+  if (w.grp == 0) {
+    sm[wave][w.col] = w.m;
+    sl[wave][w.col] = w.l;
   }
+#pragma unroll
+  for (int i = 0; i < A::kTiles; ++i) *(floatx4*)&so[wave][w.col][16 * i + 4 * w.grp] = w.o[i];
   __syncthreads();
   const int groups = min(kColumns, a.q.group - mt * kColumns);
   const int quads = a.c.dim / 4;
-  for (int i = threadIdx.x; i < groups * quads; i += 64 * W) {
+  for (int i = threadIdx.x; i < groups * quads; i += 256) {
     const int g = i / quads, d = 4 * (i % quads);
     float top = sm[0][g];
 #pragma unroll
-    for (int x = 1; x < H; ++x) top = fmaxf(top, sm[x][g]);
+    for (int x = 1; x < W; ++x) top = fmaxf(top, sm[x][g]);
     const float safe = top == -__builtin_inff() ? 0.0f : top;
     float sum = 0.0f;
     floatx4 o = {0, 0, 0, 0};
 #pragma unroll
-    for (int x = 0; x < H; ++x) {
+    for (int x = 0; x < W; ++x) {
       const float f = __builtin_amdgcn_exp2f((sm[x][g] - safe) * c);
       sum = fmaf(sl[x][g], f, sum);
       o += *(const floatx4*)&so[x][g][d] * f;
@@ -1078,8 +1011,11 @@ __global__ __launch_bounds__(256) void kv_attend_join_kernel(KvAttendArgs a) {
   if (a.lse && tid == 0) a.lse[at] = lse_of(top, sum, a.scale, kBiasOf<T>);
 }
 
+// Keys of a tile (64 while two workgroups of such tiles fit a CU).
+int shared_tile(const KvAttendArgs& a) { return a.c.page <= 32 || a.c.dim > 128 ? 32 : 64; }
+
 int64_t shared_grid(const KvAttendArgs& a) {
-  const Sharing sh = sharing(a.q.group, kColumns * kColumnTiles, a.n);
+  const Sharing sh = sharing(a.q.group, a.n);
   const int64_t units = (a.q.tokens + sh.tokens - 1) / sh.tokens * sh.tiles;
   return (units + kSharedWaves - 1) / kSharedWaves * a.c.heads;
 }
@@ -1088,17 +1024,15 @@ template <int DP, bool BF16, bool LIST, bool P16>
 void launch_parts(const KvAttendArgs& a, hipStream_t s) {
   const int tiles = (a.q.group + kColumns - 1) / kColumns;
   const dim3 grid((unsigned)(a.q.tokens * a.c.heads * tiles * a.splits));
-  if (a.waves == 8) kv_attend_parts_kernel<DP, BF16, LIST, P16, 8><<<grid, 512, 0, s>>>(a);
-  else kv_attend_parts_kernel<DP, BF16, LIST, P16, 4><<<grid, 256, 0, s>>>(a);
+  kv_attend_parts_kernel<DP, BF16, LIST, P16><<<grid, 256, 0, s>>>(a);
 }
 
 template <int DP, bool BF16, bool LIST>
 void launch_listed(const KvAttendArgs& a, hipStream_t s) {
-  if (a.waves == 1) {
+  if (a.shared) {
     const dim3 grid((unsigned)shared_grid(a));
     constexpr int kThreads = 64 * kSharedWaves;
-    // (tiles of 64 keys while two workgroups of them fit a CU)
-    constexpr int kLarge = DP <= 128 ? 64 : 32;
+    constexpr int kLarge = DP <= 128 ? 64 : 32;  // (as in shared_tile)
     if (a.c.page == 16) kv_attend_shared_kernel<DP, BF16, LIST, 16><<<grid, kThreads, 0, s>>>(a);
     else if (a.c.page == 32) kv_attend_shared_kernel<DP, BF16, LIST, 32><<<grid, kThreads, 0, s>>>(a);
     else kv_attend_shared_kernel<DP, BF16, LIST, kLarge><<<grid, kThreads, 0, s>>>(a);
@@ -1122,6 +1056,29 @@ void launch_type(const KvAttendArgs& a, hipStream_t s) {
   else launch_dim<256, BF16>(a, s);
 }
 
+// Whether tokens of prompts share wavefronts.  A row by itself reads its keys,
+// 57 ns for 1,024 of them with the card full; a workgroup of shared wavefronts
+// walks its requests' keys or the union of their lists, 27 and 10 us for 1,024,
+// and 384 workgroups run at a time.  Measured (16 bits, 128 values, 8 kv heads),
+// a row by itself / shared: 4,096 keys, one request of 32 tokens 65 / 107 us, of
+// 64 121 / 107, of 512 872 / 109; 64 requests of 4 tokens 177 / 171 us (up to
+// 2,048 keys, 4 heads a kv head), 32 requests of 4 105 / 189; lists of 16 blocks
+// of 64, one request of 128 tokens 61 / 75 us, of 256 117 / 76; 64 requests of 4
+// tokens 128 / 223 (4 heads a kv head), 129 / 123 (8); 128 requests of 2 144 /
+// 193 (8).
+bool shares(const KvAttendArgs& a, int64_t rows) {
+  const int64_t each = a.q.tokens / std::max<int64_t>(1, a.q.requests);
+  if (each < 3) return false;
+  const Sharing sh = sharing(a.q.group, a.n);
+  const int64_t tokens = std::max(1, sh.tokens * kSharedWaves / sh.tiles);  // of a workgroup
+  int64_t walks = 1 + (tokens - 1) / each;  // requests, each its keys or some lists
+  if (a.n) walks *= std::max<int64_t>(1, std::min<int64_t>({tokens, each, a.q.cols / a.n}));
+  // (tiles of 32 keys take as long as ones of 64: 2,000 keys, 6 requests of 120
+  // tokens with 16 heads of one kv head 66 / 133 us in pages of 16)
+  if (shared_tile(a) == 32) walks *= 2;
+  return rows * 384 >= (a.n ? 180 : 480) * walks * std::max<int64_t>(384, shared_grid(a));
+}
+
 }  // namespace
 
 void kv_attend_plan(KvAttendArgs& a) {
@@ -1131,11 +1088,10 @@ void kv_attend_plan(KvAttendArgs& a) {
                                 : std::min<int64_t>(a.longest, (int64_t)a.q.cols << a.c.lps);
   a.splits = 1;
   a.chunk = 64;
-  a.waves = 4;
+  a.shared = false;
   if (rows == 0) return;
-  // tokens of prompts share wavefronts, if that leaves enough of them
-  if (a.q.tokens >= 4 * a.q.requests && shared_grid(a) >= 256) {
-    a.waves = 1;
+  if (shares(a, rows)) {
+    a.shared = true;
     return;
   }
   // As many parts as fill the card (2 workgroups a CU: chunks of 4,096 instead
@@ -1152,8 +1108,6 @@ void kv_attend_plan(KvAttendArgs& a) {
   chunk = std::max<int64_t>(512, std::min<int64_t>(chunk, 1 << 30));
   if (!whole) a.splits = (int)((most + chunk - 1) / chunk);
   a.chunk = whole ? 1 << 30 : (int)chunk;
-  // eight wavefronts share a part where there is no second workgroup for a CU
-  if (rows * a.splits <= 256) a.waves = 8;
 }
 
 int64_t kv_attend_workspace(const KvAttendArgs& a) {
@@ -1162,9 +1116,9 @@ int64_t kv_attend_workspace(const KvAttendArgs& a) {
 }
 
 int64_t kv_attend_grid(const KvAttendArgs& a) {
-  if (a.waves == 1) return shared_grid(a);
+  if (a.shared) return shared_grid(a);
   const int64_t rows = a.q.tokens * a.c.heads * ((a.q.group + kColumns - 1) / kColumns);
-  return std::max(a.q.tokens * a.c.heads * a.q.group, rows * a.splits * a.waves / 4);
+  return std::max(a.q.tokens * a.c.heads * a.q.group, rows * a.splits);
 }
 
 hipError_t launch_kv_attend(const KvAttendArgs& a, hipStream_t s) {

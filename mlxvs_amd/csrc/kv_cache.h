@@ -92,11 +92,11 @@ struct KvAttendArgs {
   // the split, from kv_attend_plan
   int splits;       // parts of a row's keys, joined by a second launch if more than one
   int chunk;        // keys of a part (a multiple of 64; the last part takes the rest)
-  int waves;        // wavefronts that share a part (1: a row each, no parts)
+  bool shared;      // neighbouring tokens share wavefronts (no parts)
   float* part_o;    // [tokens][heads][group][splits][dim]
   float* part_ml;   // [tokens][heads][group][splits][2]
 };
-void kv_attend_plan(KvAttendArgs& a);  // sets splits, chunk and waves
+void kv_attend_plan(KvAttendArgs& a);  // sets shared, splits and chunk
 int64_t kv_attend_workspace(const KvAttendArgs& a);
 int64_t kv_attend_grid(const KvAttendArgs& a);  // workgroups of its largest launch
 hipError_t launch_kv_attend(const KvAttendArgs& a, hipStream_t s);

@@ -124,9 +124,12 @@ __device__ __forceinline__ void pages(const KvPlanArgs& a, int64_t r, int32_t fi
 }
 
 // Up to kFew requests: one launch, every workgroup taking the running sums of
-// all requests for itself (reading 8 bytes a request from L2 costs less than a
-// second launch).  A thread sums a stretch of neighbouring requests.
-constexpr int kFew = 4096;
+// all requests for itself (8 bytes a request, from L2).  A thread sums a stretch
+// of neighbouring requests.  In one and two launches 1,024 requests take 8.7 and
+// 10.8 us with a token each, 11.9 and 11.8 with up to 63; 2,048 take 11.0 and
+// 11.9, 20.7 and 16.4.  Few bytes: what bounds both is the chain of dependent
+// accesses (lengths, cursor, free list, table).
+constexpr int kFew = 1024;
 
 __global__ __launch_bounds__(256) void kv_plan_kernel(KvPlanArgs a) {
   extern __shared__ int32_t places[];  // starts [requests + 1], first [requests]

@@ -564,18 +564,31 @@ __global__ __launch_bounds__(512) void kv_select_tile_kernel(KvSelectArgs a) {
     wave_take_best<NR>(ranks + i * S, cnt[i], a.n, a.blocks + ((t0 + i) * a.c.heads + h) * a.n);
 }
 
-// Ways to list: a row a workgroup, its ranks in LDS; over the workspace in two
-// launches where rows are long; 16 tokens a workgroup where requests have many.
-// A launch is a chain of five dependent accesses, about 10 us whatever its size:
-// one token of 8 heads takes 31.4 us by rows and 20.4 in two launches at 4,096
-// columns, 20.0 and 19.3 at 2,048, 11.3 and 13.5 at 512.
+// Ways to list (rows: tokens x kv heads; figures for 128 values, 4 heads a kv head):
+// - kTile, 16 tokens a workgroup, where requests have many: a block is read once
+//   for 16 tokens, but a launch is no shorter than a workgroup.  By row / by tile:
+//   1,024 rows of one request 10.4 / 10.4 us at 64 columns, 19.6 / 16.6 at 512,
+//   27.0 / 24.2 at 891, 29.5 / 38.1 at 1,024 (a workgroup has a CU to itself from
+//   897 on); 2,048 rows 17.9 / 10.6, 35.3 / 17.0, 48.4 / 23.9, 52.8 / 37.1, and
+//   91.7 / 45.7 at 2,048; 512 rows 14.2 / 16.9 at 512 columns.  32 requests of 8
+//   tokens 30.4 / 20.0, 16 requests of 8 16.0 / 19.0.
+// - kRow, a row a workgroup, its ranks in LDS.
+// - kParts, two launches over the workspace, for a few long rows (or ranks that no
+//   LDS holds): by row / in two launches, 128 rows 21.0 / 18.6 us at 2,048 columns,
+//   31.5 / 26.0 at 4,096; 8 rows 14.4 / 16.6 at 1,024; 256 rows 22.3 / 24.1 at
+//   2,048, 31.8 / 37.1 at 4,096.
+// What bounds small calls is a chain of five dependent accesses, about 10 us
+// whatever the size; large ones, the listing (32 counts of a row's ranks).
 enum class Way { kRow, kParts, kTile };
 
-constexpr int kTileCols = 64 * 14;  // ranks of 16 tokens in 58 KB of LDS
+constexpr int kTileCols = 64 * 32;  // ranks of 16 tokens in 128 KB of LDS
 
 Way way_of(const KvSelectArgs& a) {
-  if (a.q.cols <= kTileCols && a.q.tokens >= 8 * a.q.requests) return Way::kTile;
-  return a.q.cols <= 2048 ? Way::kRow : Way::kParts;
+  const int64_t rows = a.q.tokens * a.c.heads;
+  if (a.q.cols <= kTileCols && rows >= (a.q.cols <= 896 ? 1024 : 1536) &&
+      a.q.tokens >= 8 * a.q.requests)
+    return Way::kTile;
+  return a.q.cols > kLdsCols || (a.q.cols > 1024 && rows < 256) ? Way::kParts : Way::kRow;
 }
 
 template <bool BF16, int KD, bool A16, int NR>
@@ -591,10 +604,14 @@ void launch_select(const KvSelectArgs& a, hipStream_t s) {
     case Way::kTile:
       if (a.q.cols <= 256) launch_tile<BF16, KD, A16, 4>(a, s);
       else if (a.q.cols <= 512) launch_tile<BF16, KD, A16, 8>(a, s);
-      else launch_tile<BF16, KD, A16, 14>(a, s);
+      else if (a.q.cols <= 896) launch_tile<BF16, KD, A16, 14>(a, s);
+      else launch_tile<BF16, KD, A16, 32>(a, s);
       return;
     case Way::kRow:
-      if (rows < 512) kv_select_kernel<BF16, KD, A16, 1024><<<rows, 1024, a.q.cols * 4, s>>>(a);
+      // (1,024 / 256 threads: 256 rows 15.2 / 18.0 us at 1,024 columns, 10.4 / 10.1
+      // at 256; 384 rows 26.1 / 23.0 and 18.9 / 10.4)
+      if (rows <= 256 && a.q.cols > 512)
+        kv_select_kernel<BF16, KD, A16, 1024><<<rows, 1024, a.q.cols * 4, s>>>(a);
       else kv_select_kernel<BF16, KD, A16, 256><<<rows, 256, a.q.cols * 4, s>>>(a);
       return;
     case Way::kParts:

@@ -307,6 +307,26 @@ def test_select_for_prompts_among_many_blocks(engine, cols, heads, group, d):
         check_select(engine, q, codes, scales, table, who, positions, 16, n)
 
 
+@pytest.mark.parametrize("heads,tokens", [(64, 19), (24, 11)])
+@pytest.mark.parametrize("cols,d", [(256, 16), (512, 80), (600, 256), (897, 128), (2048, 64),
+                                    (2049, 16)])
+def test_select_of_many_rows(engine, cols, d, heads, tokens):
+    rng = np.random.default_rng(cols + heads)
+    codes, scales = summaries(rng, 300, heads, d)
+    scales[7, ::2] = np.inf
+    codes[100:140] = codes[100]  # ties
+    scales[100:140] = scales[100]
+    table = rng.integers(-3, 310, (2, cols)).astype(np.int32)
+    who = np.sort(rng.integers(0, 2, tokens))
+    who[-2] = 9
+    positions = rng.integers(0, 60 * 16, tokens)
+    positions[[0, 4]] = cols * 16 - 1, cols * 16 - 17
+    positions[7] = -1
+    q = dev(rng.standard_normal((tokens, heads * 2, d), np.float32)).bfloat16()
+    for n in (2, 48):
+        check_select(engine, q, codes, scales, table, who, positions, 16, n)
+
+
 @pytest.mark.parametrize("cols", [2048, 2049, 4096, 8192, 8193, 9000])
 def test_select_among_many_blocks(engine, cols):
     rng = np.random.default_rng(cols)
@@ -465,6 +485,23 @@ def test_attend_of_many_rows(engine, dtype, listed):
         q = dev(rng.standard_normal((tokens, heads * group, dim), np.float32)).to(DTYPES[dtype])
         blocks = rng.integers(-1, cols, (tokens, heads, 3)) if listed else None
         check_attend(cache, dtype, q, table, who, positions, blocks=blocks)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("tokens", [3, 16, 40])
+def test_attend_of_short_prompts(engine, tokens, dtype):
+    # few to many tokens for each of the requests, in either kernel
+    rng = np.random.default_rng(tokens)
+    heads, group, page, dim, requests = 8, 4, 32, 64, 4
+    cols = 20
+    cache = make_cache(engine, requests * cols, heads, page, dim, dtype, rng)
+    table = tables(rng, requests * cols, requests, cols)
+    who = np.repeat(np.arange(requests), tokens)
+    positions = np.tile(np.arange(tokens), requests) + np.repeat([0, 33, 300, 640 - tokens], tokens)
+    q = dev(rng.standard_normal((len(who), heads * group, dim), np.float32)).to(DTYPES[dtype])
+    check_attend(cache, dtype, q, table, who, positions)
+    blocks = cache.select(q, dev(table), dev(who, torch.int32), dev(positions, torch.int32), 6)
+    check_attend(cache, dtype, q, table, who, positions, blocks=blocks.cpu().numpy())
 
 
 SHARED = [(128, 2, 16, 64, 70), (64, 5, 32, 80, 60), (64, 16, 64, 128, 24), (40, 20, 128, 96, 33),
