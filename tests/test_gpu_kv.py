@@ -880,3 +880,17 @@ def test_refusals(engine):
         engine.kv_plan(who[:1], who[:1], table, who, plan.cursor, 16, 3, out=plan)
     with pytest.raises(ValueError, match="out.slots"):
         engine.kv_plan(who[:1], who[:1], table, who, who[:1], 16, 4, out=plan)
+
+
+def test_the_example(engine):
+    import importlib.util
+    from pathlib import Path
+    path = Path(__file__).resolve().parent.parent / "examples" / "paged_cache.py"
+    spec = importlib.util.spec_from_file_location("paged_cache", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    lengths, close, ms = example.run(requests=3, context=700, steps=5, blocks=16)
+    assert lengths == [238, 464, 691] and ms > 0
+    # (12 blocks at most: the lists hold everything, and the two answers are two
+    # roundings of one sum)
+    assert close > 0.999
