@@ -364,14 +364,17 @@ __device__ __forceinline__ void copy16_to_lds(const void* from, void* lds) {
 #endif
 }
 
-// PK: pages of 16 keys, two to a tile of 32, or tiles of 32 or 64 keys of larger
-// ones.
+// A tile's keys (64 while two workgroups of such tiles fit a CU).
+constexpr int tile_keys(int dim) { return dim <= 128 ? 64 : 32; }
+
+// PK: keys of a block in a tile: all of it for pages of 16 and 32, which share a
+// tile, else the tile's.
 template <int DP, bool BF16, bool LIST, int PK>
 struct AttendShared {
   using T = std::conditional_t<BF16, __bf16, _Float16>;
   using Tx8 = std::conditional_t<BF16, bf16x8, halfx8>;
   using Tx4 = std::conditional_t<BF16, bf16x4, halfx4>;
-  static constexpr int kKeys = PK == 64 ? 64 : 32;  // of a tile
+  static constexpr int kKeys = tile_keys(DP);
   static constexpr int kChunks = DP / 32, kTiles = DP / 16;
   // (room for a block that is listed 256 times)
   static constexpr float kBias = BF16 ? 0.0f : 7.0f;
@@ -382,7 +385,10 @@ struct AttendShared {
   static constexpr int kPerCopy = 1024 * kSharedWaves;
   static constexpr int kCopiesK = kKeys * kRow * 16 / kPerCopy;
   static constexpr int kCopiesV = (kKeys * DP * 2 + kPerCopy - 1) / kPerCopy;
-  static constexpr int kBlocks = PK == 16 ? 2 : 1;
+  static constexpr int kBlocks = kKeys / PK;
+
+  // Whole numbers of each of a tile's blocks, 16 bits a block.
+  using Counts = std::conditional_t<(kBlocks > 2), uint64_t, uint32_t>;
 
   // Two buffers with names of their own: loads into one are not taken to alias
   // reads of the other (which would wait for them).
@@ -406,15 +412,15 @@ struct AttendShared {
   int pos;       // of the column's token
   int at, next;  // its place in its list, and the block there
   bool on;
-  // what this lane copies, in bytes from a tile's start (bit 31: of the second page)
-  uint32_t from_k[kCopiesK], from_v[kCopiesV];
+  uint32_t from_k[kCopiesK], from_v[kCopiesV];  // what this lane copies, in bytes from a page's
+  int block_v;     // ... and whose values
   int at_k, at_v;  // where this lane's first operands are, in bytes
 
   // Chunks of a row are swapped so that the 8 lanes that read together, rows 0 to
   // 3 and 8 to 11 or neighbours, find 8 sets of banks.
   __device__ __forceinline__ static int swap_of_k(int row) {
-    row &= 31;  // (alike in both halves of a tile)
-    return (row ^ (row >> 3)) & (kRow - 1);
+    // (alike in both halves of a tile)
+    return ((row & 3) | ((row >> 2 ^ row >> 3) & 1) << 2 | (row >> 4 & 1) << 3) & (kRow - 1);
   }
   __device__ __forceinline__ static int swap_of_v(int row) {
     return kKeys == 64 ? row & 7 : (row ^ (row >> 2)) & 3;
@@ -423,24 +429,21 @@ struct AttendShared {
   __device__ __forceinline__ AttendShared(const KvAttendArgs& args, Shared& s, int head)
       : a(args), sh(s), lane(threadIdx.x & 63),
         wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), col(lane & 15), grp(lane >> 4),
-        h(head), d(args.c.dim), ps(PK == 16 ? 16 : args.c.page), c(args.scale * kLog2e) {
+        h(head), d(args.c.dim), ps(kBlocks > 1 ? PK : args.c.page), c(args.scale * kLog2e) {
     constexpr int nv = kKeys / 8;
     // (past the head's values: the tile's start, for chunks that nobody uses)
 #pragma unroll
     for (int i = 0; i < kCopiesK; ++i) {
       const int x = 64 * (wave + kSharedWaves * i) + lane;
       const int row = x / kRow, chunk = (x % kRow) ^ swap_of_k(row);
-      const bool second = PK == 16 && row >= 16;
-      from_k[i] = 8 * chunk < d ? 2 * ((second ? row - 16 : row) * d + 8 * chunk) : 0;
-      if (second) from_k[i] |= 1u << 31;
+      from_k[i] = 8 * chunk < d ? 2 * (row % PK * d + 8 * chunk) : 0;
     }
 #pragma unroll
     for (int i = 0; i < kCopiesV; ++i) {
       const int x = 64 * (wave + kSharedWaves * i) + lane;
       const int row = x / nv, chunk = (x % nv) ^ swap_of_v(row);
-      const bool second = PK == 16 && chunk >= 2;
-      from_v[i] = row < d ? 2 * (row * ps + 8 * (second ? chunk - 2 : chunk)) : 0;
-      if (second) from_v[i] |= 1u << 31;
+      from_v[i] = row < d ? 2 * (row * ps + 8 * chunk % PK) : 0;
+      block_v = 8 * chunk / PK;  // (the rows of its copies are swapped alike)
     }
     const int r = 8 * (col >> 2) + (col & 3);
     at_k = 16 * (r * kRow + (grp ^ swap_of_k(r)));
@@ -464,6 +467,10 @@ struct AttendShared {
   // How many keys of block b each column sees, and how often it has it listed.
   // Blocks before b that it has listed (their pages are absent) are passed by.
   __device__ __forceinline__ void look(int b, int& seen, int& times) {
+    if constexpr (!LIST) {
+      seen = on ? min(ps, pos + 1 - (b << a.c.lps)) : 0;
+      return;
+    }
     times = 0;
     bool some = true;
     while (some) {
@@ -505,7 +512,7 @@ struct AttendShared {
 
   // The next tile; false: no more.
   __device__ __forceinline__ bool next_tile(Tile& t) {
-    if constexpr (PK != 16) {
+    if constexpr (kBlocks == 1) {
       t.off += kKeys;
       if (t.off < ps && t.off < last + 1 - (t.block[0] << a.c.lps)) return true;
     }
@@ -541,38 +548,55 @@ struct AttendShared {
     const int64_t head = (int64_t)ps * d;
 #pragma unroll
     for (int i = 0; i < kBlocks; ++i) {
-      // (an absent page of a pair is read as page 0 and not seen)
+      // (an absent page among others is read as page 0 and not seen)
       const int64_t p = ((int64_t)max(0, t.page[i]) * a.c.heads + h) * head;
-      k[i] = (const char*)a.c.keys + 2 * (p + (PK == 16 ? 0 : t.off * d));
-      v[i] = (const char*)a.c.values + 2 * (p + (PK == 16 ? 0 : t.off));
+      k[i] = (const char*)a.c.keys + 2 * (p + t.off * d);
+      v[i] = (const char*)a.c.values + 2 * (p + t.off);
     }
-    const auto place = [](const char* const (&page)[kBlocks], uint32_t at) {
-      if constexpr (PK == 16) return (at >> 31 ? page[1] : page[0]) + (at & 0x7FFFFFFF);
-      else return page[0] + at;
-    };
+    // (1 KB of keys are rows of one block, often a round of copies is)
+    constexpr int kRows = 64 / kRow, kRound = kRows * kSharedWaves;
+    const int mine_k = kRound > PK ? kRows * wave / PK : 0;
 #pragma unroll
     for (int i = 0; i < kCopiesK; ++i)
-      copy16_to_lds(place(k, from_k[i]), to_.k + 1024 * (wave + kSharedWaves * i));
+      copy16_to_lds(of_block(k, i * kRound / PK + mine_k) + from_k[i],
+                    to_.k + 1024 * (wave + kSharedWaves * i));
+    const char* mine = of_block(v, block_v);
 #pragma unroll
     for (int i = 0; i < kCopiesV; ++i)
-      copy16_to_lds(place(v, from_v[i]), to_.v + 1024 * (wave + kSharedWaves * i));
+      copy16_to_lds(mine + from_v[i], to_.v + 1024 * (wave + kSharedWaves * i));
+  }
+
+  // (in registers: a choice among loads would keep the array in memory)
+  __device__ __forceinline__ static const char* of_block(const char* const (&x)[kBlocks], int b) {
+    const char* y = x[0];
+#pragma unroll
+    for (int i = 1; i < kBlocks; ++i) {
+      const char* z = x[i];
+#if defined(__HIP_DEVICE_COMPILE__)
+      asm("" : "+s"(z));
+#endif
+      y = b >= i ? z : y;
+    }
+    return y;
   }
 
   // Zeros in the place of values past the workgroup's furthest token, or of an
-  // absent page of a pair: a weight of 0 would not hide what is not finite.
+  // absent page among others: a weight of 0 would not hide what is not finite.
   __device__ __forceinline__ void clear(const Tile& t, Buffer in) {
-    constexpr int nv = kKeys / 8, kPer = PK == 16 ? 2 : nv;  // chunks of a row, of a page's
+    constexpr int nv = kKeys / 8, kPer = PK / 8;  // chunks of a row, of a block's
     bool some = false;
-    int shown[kBlocks];
+    Counts shown = 0;
 #pragma unroll
     for (int i = 0; i < kBlocks; ++i) {
-      shown[i] = t.block[i] == kNone || t.page[i] < 0 ? 0 : last + 1 - (t.block[i] << a.c.lps) - t.off;
-      some |= shown[i] < 8 * kPer;
+      const int n = t.block[i] == kNone || t.page[i] < 0
+                        ? 0 : last + 1 - (t.block[i] << a.c.lps) - t.off;
+      shown |= (Counts)min(max(0, n), PK) << 16 * i;
+      some |= n < PK;
     }
     if (!some) return;
     for (int x = threadIdx.x; x < d * nv; x += 64 * kSharedWaves) {
       const int row = x / nv, chunk = (x % nv) ^ swap_of_v(row);
-      const int left = shown[chunk / kPer] - 8 * (chunk % kPer);
+      const int left = (int)(shown >> 16 * (chunk / kPer) & 0xFFFF) - 8 * (chunk % kPer);
       if (left < 8) *(uintx4*)(in.v + 16 * x) = keep(*(const uintx4*)(in.v + 16 * x), left);
     }
     __syncthreads();
@@ -623,37 +647,28 @@ struct AttendShared {
 
   // The steps of a tile in a buffer that this wavefront's tokens see; seen and
   // times are kept over the tiles of a block.
-  int seen[kBlocks], times[kBlocks];
+  Counts seen, times;
 
   __device__ __forceinline__ void use(const Tile& t, Buffer from) {
     if (t.off == 0) {
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i) {
-        if (t.block[i] != kNone) look(t.block[i], seen[i], times[i]);
-        if (t.page[i] < 0) seen[i] = 0;
+        int n = 0, often = 0;
+        if (t.block[i] != kNone) look(t.block[i], n, often);
+        if (t.page[i] < 0) n = 0;
+        seen = (i ? seen : 0) | (Counts)max(0, n) << 16 * i;
+        times = (i ? times : 0) | (Counts)often << 16 * i;
       }
     }
-    int top = 0, n8;
-    float twice;
-    bool all = true;
-    const int s0 = seen[0] - t.off;
-    if constexpr (PK == 16) {
-      const int s1 = seen[1];
-      top = max(top, s1 > 0 ? 16 + s1 : s0);
-      all &= s0 == 16 && s1 == 16;
-      n8 = (grp < 2 ? s0 : s1) - ((8 * grp) & 15);
-      twice = __log2f((float)max(1, grp < 2 ? times[0] : times[1]));
-    } else {
-      top = max(top, s0);
-      all &= s0 >= kKeys;
-      n8 = s0 - 8 * grp;
-      twice = __log2f((float)max(1, times[0]));
-    }
-    top = __builtin_amdgcn_readfirstlane(row_max(top));
-    if (top <= 0) return;
-    all = __all(all);
 #pragma unroll 1
-    for (int k0 = 0; k0 < min(top, kKeys); k0 += 32) step(from, k0, n8 - k0, all, twice);
+    for (int k0 = 0; k0 < kKeys; k0 += 32) {
+      const int key = k0 + 8 * grp;  // this lane's first
+      const int place = 16 * (key / PK % kBlocks);
+      const int n8 = (int)(seen >> place & 0xFFFF) - t.off - (kBlocks > 1 ? key % PK : key);
+      if (!__any(n8 > 0)) continue;
+      const float twice = LIST ? __log2f((float)max(1, (int)(times >> place & 0xFFFF))) : 0.0f;
+      step(from, k0, n8, __all(n8 >= 8), twice);
+    }
   }
 
   uint64_t todo, with;  // tokens of this wavefront: to come, and of the request at hand
@@ -1011,9 +1026,6 @@ __global__ __launch_bounds__(256) void kv_attend_join_kernel(KvAttendArgs a) {
   if (a.lse && tid == 0) a.lse[at] = lse_of(top, sum, a.scale, kBiasOf<T>);
 }
 
-// Keys of a tile (64 while two workgroups of such tiles fit a CU).
-int shared_tile(const KvAttendArgs& a) { return a.c.page <= 32 || a.c.dim > 128 ? 32 : 64; }
-
 int64_t shared_grid(const KvAttendArgs& a) {
   const Sharing sh = sharing(a.q.group, a.n);
   const int64_t units = (a.q.tokens + sh.tokens - 1) / sh.tokens * sh.tiles;
@@ -1032,10 +1044,13 @@ void launch_listed(const KvAttendArgs& a, hipStream_t s) {
   if (a.shared) {
     const dim3 grid((unsigned)shared_grid(a));
     constexpr int kThreads = 64 * kSharedWaves;
-    constexpr int kLarge = DP <= 128 ? 64 : 32;  // (as in shared_tile)
-    if (a.c.page == 16) kv_attend_shared_kernel<DP, BF16, LIST, 16><<<grid, kThreads, 0, s>>>(a);
-    else if (a.c.page == 32) kv_attend_shared_kernel<DP, BF16, LIST, 32><<<grid, kThreads, 0, s>>>(a);
-    else kv_attend_shared_kernel<DP, BF16, LIST, kLarge><<<grid, kThreads, 0, s>>>(a);
+    constexpr int kKeys = tile_keys(DP);
+    if (a.c.page == 16)
+      kv_attend_shared_kernel<DP, BF16, LIST, 16><<<grid, kThreads, 0, s>>>(a);
+    else if (kKeys > 32 && a.c.page == 32)
+      kv_attend_shared_kernel<DP, BF16, LIST, 32><<<grid, kThreads, 0, s>>>(a);
+    else
+      kv_attend_shared_kernel<DP, BF16, LIST, kKeys><<<grid, kThreads, 0, s>>>(a);
     return;
   }
   if (a.c.page == 16) launch_parts<DP, BF16, LIST, true>(a, s);
@@ -1073,9 +1088,7 @@ bool shares(const KvAttendArgs& a, int64_t rows) {
   const int64_t tokens = std::max(1, sh.tokens * kSharedWaves / sh.tiles);  // of a workgroup
   int64_t walks = 1 + (tokens - 1) / each;  // requests, each its keys or some lists
   if (a.n) walks *= std::max<int64_t>(1, std::min<int64_t>({tokens, each, a.q.cols / a.n}));
-  // (tiles of 32 keys take as long as ones of 64: 2,000 keys, 6 requests of 120
-  // tokens with 16 heads of one kv head 66 / 133 us in pages of 16)
-  if (shared_tile(a) == 32) walks *= 2;
+  if (tile_keys(a.c.dim) == 32) walks *= 2;  // (they take as long as tiles of 64 do)
   return rows * 384 >= (a.n ? 180 : 480) * walks * std::max<int64_t>(384, shared_grid(a));
 }
 
