@@ -666,7 +666,8 @@ MLXVS_C_API int mlxvs_release_workspace(void);
 /**
  * Per-stage kernel timing: with enable != 0 every kernel launch of later
  * calls is bracketed by HIP events on its stream (stages: prep, fused_f32,
- * fused_f16, hamming, merge, scores, select, pack, fill, self_drop).
+ * fused_f16, hamming, merge, scores, select, pack, fill, self_drop, kv_plan,
+ * kv_append, kv_select, kv_attend).
  * Enabling or disabling clears the totals.
  */
 MLXVS_C_API int mlxvs_profile(int enable);

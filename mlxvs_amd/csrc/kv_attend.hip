@@ -18,6 +18,9 @@
 // precision; a sum of roundings that averages out), its sum is not; under f16
 // P is scaled up so that small terms of long sums stay normal numbers.
 // Scores, maxima, sums and the output are float32.
+//
+// Single tokens are bound by HBM: 64 ragged requests of up to 8,192 tokens (8 kv
+// heads of 4, 128 values) 247 us, 4.9 TB/s; one of 262,144 188 us, 5.7 TB/s.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -329,10 +332,15 @@ __device__ __forceinline__ int row_max(int x) {
 // 2.2 GB in 322 us, the same rate).  So tiles of keys and values go to LDS by
 // direct loads of neighbouring chunks, a tile ahead of the products, and the
 // operands come from there, in chunks that are swapped by row so that 8 lanes
-// read from 8 different sets of banks: 250 us.  Of a tile of 64 keys that is now
-// 1.05 us for its products and weights (two wavefronts a SIMD, their chain of
+// read from 8 different sets of banks: 246 us.  Of a tile of 64 keys that is now
+// about 1 us for its products and weights (two wavefronts a SIMD, their chain of
 // scores, maxima, exponentials and sums not hidden by one another), 0.4 us for
-// issuing its copy, 0.5 us at its barrier.
+// issuing its copy, 0.5 us at its barrier.  Without lists every wavefront uses
+// every tile: 4,096 tokens of 8,192 keys (8 kv heads of 4, 128 values) 684 us, 603
+// TFLOP/s; there LDS bounds it: every MFMA (16 cycles of a SIMD) takes an operand
+// of 1 KB, about 10 cycles of the reads that four SIMDs share.  (32 columns a
+// wavefront would halve that, but need more registers than two wavefronts a SIMD
+// have.)
 //
 // Lists in any order are right: one that does not ascend is sorted first, and a
 // block listed twice counts twice.
@@ -1073,23 +1081,29 @@ void launch_type(const KvAttendArgs& a, hipStream_t s) {
 
 // Whether tokens of prompts share wavefronts.  A row by itself reads its keys,
 // 57 ns for 1,024 of them with the card full; a workgroup of shared wavefronts
-// walks its requests' keys or the union of their lists, 27 and 10 us for 1,024,
-// and 384 workgroups run at a time.  Measured (16 bits, 128 values, 8 kv heads),
-// a row by itself / shared: 4,096 keys, one request of 32 tokens 65 / 107 us, of
-// 64 121 / 107, of 512 872 / 109; 64 requests of 4 tokens 177 / 171 us (up to
-// 2,048 keys, 4 heads a kv head), 32 requests of 4 105 / 189; lists of 16 blocks
-// of 64, one request of 128 tokens 61 / 75 us, of 256 117 / 76; 64 requests of 4
-// tokens 128 / 223 (4 heads a kv head), 129 / 123 (8); 128 requests of 2 144 /
-// 193 (8).
+// walks its requests' keys or the union of their lists, about 25 and 12 us for
+// 1,024, and 384 workgroups run at a time.  Measured (16 bits, 128 values, 8 kv
+// heads of 4), a row by itself / shared:
+//   4,096 keys: one request of 32 tokens 64 / 96 us, of 64 122 / 96, of 512 873 /
+//   100; up to 2,048 keys: 32 requests of 4 tokens 105 / 170, of 8 184 / 94;
+//   64 requests of 4 176 / 153;
+//   lists of 16 of 256 blocks of 64: one request of 128 tokens 62 / 73, of 256
+//   118 / 75, of 512 230 / 77; 64 requests of 4 130 / 218 (131 / 123 with 8 heads a
+//   kv head), 128 requests of 4 252 / 236; 128 of 2 149 / 189 (8 heads);
+//   lists of 64 of 1,024 blocks of 16: one request of 256 81 / 101;
+//   256 values, 4,096 keys: one request of 64 tokens 234 / 198, of 128 456 / 202.
 bool shares(const KvAttendArgs& a, int64_t rows) {
   const int64_t each = a.q.tokens / std::max<int64_t>(1, a.q.requests);
   if (each < 3) return false;
   const Sharing sh = sharing(a.q.group, a.n);
   const int64_t tokens = std::max(1, sh.tokens * kSharedWaves / sh.tiles);  // of a workgroup
-  int64_t walks = 1 + (tokens - 1) / each;  // requests, each its keys or some lists
-  if (a.n) walks *= std::max<int64_t>(1, std::min<int64_t>({tokens, each, a.q.cols / a.n}));
-  if (tile_keys(a.c.dim) == 32) walks *= 2;  // (they take as long as tiles of 64 do)
-  return rows * 384 >= (a.n ? 180 : 480) * walks * std::max<int64_t>(384, shared_grid(a));
+  int64_t walks = 1 + (tokens - 1) / each;  // requests, each its keys or the union of
+  if (a.n) {                                // some lists, which overlap
+    const int64_t lists = std::min(tokens, each), apart = std::max(1, a.q.cols / a.n);
+    walks *= std::max<int64_t>(1, lists * apart / (lists + apart));
+    if (a.c.page == 16) walks *= 2;
+  }
+  return rows * 384 >= (a.n ? 220 : 480) * walks * std::max<int64_t>(384, shared_grid(a));
 }
 
 }  // namespace
