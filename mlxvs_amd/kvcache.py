@@ -64,8 +64,10 @@ def _ints(x, name: str, op: str, device, dtype=torch.int32, size: Optional[int] 
 def _table(table, op: str, device):
     _need(isinstance(table, torch.Tensor) and table.dtype == torch.int32 and table.dim() == 2
           and table.device == device
-          and (table.shape[1] <= 1 or table.stride(1) == 1 or table.numel() == 0), op,
-          f"table must be an int32 [requests, columns] tensor on {device} with contiguous rows.")
+          and (table.shape[1] <= 1 or table.stride(1) == 1 or table.numel() == 0)
+          and (table.shape[0] <= 1 or table.stride(0) >= table.shape[1]), op,
+          f"table must be an int32 [requests, columns] tensor on {device} with contiguous rows "
+          "that do not overlap.")
     return table.data_ptr(), max(table.stride(0), table.shape[1])
 
 

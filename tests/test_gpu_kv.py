@@ -882,6 +882,23 @@ def test_refusals(engine):
         engine.kv_plan(who[:1], who[:1], table, who, who[:1], 16, 4, out=plan)
 
 
+def test_tables_whose_rows_overlap_are_refused(engine):
+    """A broadcast row, or rows that start within one another: neither is a
+    table of so many requests in memory."""
+    cache = engine.PagedKVCache.empty(4, 2, 16, 64)
+    q = torch.ones((3, 4, 64), dtype=torch.bfloat16, device="cuda")
+    who = torch.zeros(3, dtype=torch.int32, device="cuda")
+    row = torch.zeros(8, dtype=torch.int32, device="cuda")
+    for table in (row[:4].expand(3, 4), row.as_strided((3, 4), (2, 1))):
+        for call in (lambda: cache.attend(q, table, who, who),
+                     lambda: cache.select(q, table, who, who, 4),
+                     lambda: engine.kv_plan(who, who, table, row, row[:1], 16, 3)):
+            with pytest.raises(ValueError, match="do not overlap"):
+                call()
+    for table in (row[:4].expand(1, 4), row.as_strided((2, 1), (4, 7))):  # (one row, one column)
+        assert not cache.attend(q, table, who, who).any()
+
+
 def test_the_example(engine):
     import importlib.util
     from pathlib import Path
