@@ -262,7 +262,7 @@ class PagedKVCache:
 
     def _workspace(self, size, q, qs, *args):
         """(tensor, bytes) of scratch memory on the current stream."""
-        key = (size, q.shape, qs.columns, args)
+        key = (size, q.shape, qs.columns, qs.requests, args)
         need = self._sizes.get(key)
         if need is None:
             need = getattr(_L(), size)(self._ref, ctypes.byref(qs), *args)

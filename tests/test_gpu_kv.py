@@ -701,6 +701,26 @@ def test_a_cache_past_32_bits(engine):
                        small.attend(q, t_small, who, pos, blocks=b))
 
 
+def test_the_same_queries_over_tables_of_other_heights(engine):
+    """How work is split, and with it a call's workspace, goes by the requests
+    too: tokens of one request share wavefronts and tiles, those of many do not."""
+    rng = np.random.default_rng(77)
+    cols, tokens = 80, 128
+    cache = make_cache(engine, cols, 8, 64, 16, "bf16", rng)
+    q = dev(rng.standard_normal((tokens, 8, 16), np.float32), torch.bfloat16)
+    table = tables(rng, cols, 1, cols)
+    positions = rng.integers(4000, cols * 64, tokens)
+    wide = rng.integers(0, cols, (1, 800)).astype(np.int32)
+    lists = []
+    for height in (1, tokens, 1):
+        check_attend(cache, "bf16", q, np.repeat(table, height, 0), np.arange(tokens) % height,
+                     positions)
+        lists.append(cache.select(q, dev(np.repeat(wide, height, 0)),
+                                  dev(np.arange(tokens) % height, torch.int32),
+                                  dev(positions, torch.int32), 12))
+    assert torch.equal(lists[0], lists[1]) and torch.equal(lists[0], lists[2])
+
+
 def test_attend_none(engine):
     cache = engine.PagedKVCache.empty(2, 2, 16, 64)
     e = torch.empty((0, 4, 64), dtype=torch.bfloat16, device="cuda")
