@@ -815,7 +815,8 @@ void kv_attend_shared_kernel(KvAttendArgs a) {
     myreq = a.q.token_request[t0 + lane];
     mypos = a.q.positions[t0 + lane];
   }
-  const bool sees = myreq >= 0 && myreq < a.q.requests && mypos >= 0;
+  // (a table without columns has no entry to look up)
+  const bool sees = myreq >= 0 && myreq < a.q.requests && mypos >= 0 && a.q.cols > 0;
   const int stride = a.n + 1;
   w.first_list = w.wave * share.tokens;
   if constexpr (LIST) {

@@ -721,6 +721,17 @@ def test_the_same_queries_over_tables_of_other_heights(engine):
     assert torch.equal(lists[0], lists[1]) and torch.equal(lists[0], lists[2])
 
 
+@pytest.mark.parametrize("listed", [False, True])
+def test_prompts_over_a_table_without_columns(engine, listed):
+    cache = engine.PagedKVCache.empty(2, 8, 64, 64)
+    q = torch.ones((700, 8, 64), dtype=torch.bfloat16, device="cuda")
+    table = torch.zeros((1, 0), dtype=torch.int32, device="cuda")
+    zeros = torch.zeros(700, dtype=torch.int32, device="cuda")
+    blocks = torch.zeros((700, 8, 3), dtype=torch.int32, device="cuda") if listed else None
+    out, lse = cache.attend(q, table, zeros, zeros, blocks=blocks, lse=True)
+    assert not out.any() and lse.isneginf().all()
+
+
 def test_attend_none(engine):
     cache = engine.PagedKVCache.empty(2, 2, 16, 64)
     e = torch.empty((0, 4, 64), dtype=torch.bfloat16, device="cuda")
