@@ -885,21 +885,22 @@ void kv_attend_shared_kernel(KvAttendArgs a) {
         good &= fabsf(w.o[i][j]) < __builtin_inff() || 16 * i + 4 * w.grp >= a.c.dim;
     if (turn < 0 && __syncthreads_or(!good)) continue;
     const float l = column_sum(w.l);
-    if (!mine || (turn >= 0 && tok != alone)) continue;
-    const float inv = 1.0f / l;
-    const int64_t at = ((t0 + tok) * a.c.heads + h) * group + g;
+    if (mine && (turn < 0 || tok == alone)) {
+      const float inv = 1.0f / l;
+      const int64_t at = ((t0 + tok) * a.c.heads + h) * group + g;
 #pragma unroll
-    for (int i = 0; i < A::kTiles; ++i) {
-      const int d = 16 * i + 4 * w.grp;
-      if (d < a.c.dim) {
-        typename A::Tx4 x;
+      for (int i = 0; i < A::kTiles; ++i) {
+        const int d = 16 * i + 4 * w.grp;
+        if (d < a.c.dim) {
+          typename A::Tx4 x;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          x[j] = (typename A::T)(l == 0.0f ? 0.0f : w.o[i][j] * inv);
-        *(typename A::Tx4*)((typename A::T*)a.out + at * a.c.dim + d) = x;
+          for (int j = 0; j < 4; ++j)
+            x[j] = (typename A::T)(l == 0.0f ? 0.0f : w.o[i][j] * inv);
+          *(typename A::Tx4*)((typename A::T*)a.out + at * a.c.dim + d) = x;
+        }
       }
+      if (a.lse && w.grp == 0) a.lse[at] = lse_of(w.m, l, a.scale, A::kBias);
     }
-    if (a.lse && w.grp == 0) a.lse[at] = lse_of(w.m, l, a.scale, A::kBias);
     if (turn < 0) break;
   }
 }
