@@ -1133,7 +1133,18 @@ void kv_attend_plan(KvAttendArgs& a) {
   // keys: 51.5 us whole, 55.4 in two).
   const bool whole = most <= 1024 || (a.n && rows >= 256);
   int64_t chunk = (most * rows / 512 + 255) / 256 * 256;
-  if (a.q.tokens > 1 && !a.n) chunk = std::min<int64_t>(chunk, 1024);
+  if (a.q.tokens > 1 && !a.n) {
+    // nor more than 16,384 parts over all rows: a table may be far wider than its
+    // requests are long, and a part costs a workgroup and its place in the
+    // workspace.  Without a limit / with it (8 kv heads of 4, 128 values): 1,024
+    // requests of up to 8,192 tokens 3,359 / 3,073 us, and 4,118 / 2,954 in a table
+    // for 32,768; 256 of up to 2,048 in a table for 131,072 1,203 / 268; 4,096 of up
+    // to 1,500 in one for 4,096 2,889 / 2,219.  (65,536 parts: 3,370, 3,127, 447,
+    // 2,606; 8,192: 2,989, 2,889, 241, 2,216, but 300, not 266, for 64 of up to 8,192
+    // in a table for 131,072.)
+    const int64_t least = (most * rows / 16384 + 255) / 256 * 256;
+    chunk = std::max(least, std::min<int64_t>(chunk, 1024));
+  }
   chunk = std::max<int64_t>(512, std::min<int64_t>(chunk, 1 << 30));
   if (!whole) a.splits = (int)((most + chunk - 1) / chunk);
   a.chunk = whole ? 1 << 30 : (int)chunk;

@@ -721,6 +721,27 @@ def test_the_same_queries_over_tables_of_other_heights(engine):
     assert torch.equal(lists[0], lists[1]) and torch.equal(lists[0], lists[2])
 
 
+def test_many_requests_of_a_wide_table(engine):
+    """A place for a million tokens in each of 2,048 rows: the workspace and the
+    grid go by what the card can use, not by the table's width."""
+    rng = np.random.default_rng(78)
+    cache = make_cache(engine, 40, 8, 64, 64, "bf16", rng)
+    requests, wide = 2048, 16384
+    ids = rng.integers(0, 40, (requests, 25)).astype(np.int32)
+    table = torch.full((requests, wide), -1, dtype=torch.int32, device="cuda")
+    table[:, :25] = dev(ids)
+    positions = rng.integers(-1, 1600, requests)
+    q = dev(rng.standard_normal((requests, 8, 64), np.float32), torch.bfloat16)
+    who = torch.arange(requests, dtype=torch.int32, device="cuda")
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    got = cache.attend(q, table, who, dev(positions, torch.int32))
+    assert torch.cuda.max_memory_allocated() - before < 100 << 20
+    some = rng.choice(requests, 50, replace=False)
+    want = check_attend(cache, "bf16", q[dev(some)], ids, some, positions[some])
+    assert torch.allclose(got[dev(some)].float(), want.float(), rtol=2.0 ** -6, atol=2.0 ** -6)
+
+
 @pytest.mark.parametrize("listed", [False, True])
 def test_prompts_over_a_table_without_columns(engine, listed):
     cache = engine.PagedKVCache.empty(2, 8, 64, 64)
