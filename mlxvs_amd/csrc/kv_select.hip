@@ -268,39 +268,89 @@ __device__ void rank_row(const KvSelectArgs& a, int h, int own, const int32_t* t
   }
 }
 
-// The n largest of a wavefront's ranks (64 x + lane: k[x]), the lowest columns
-// among equal ones, ascending by column into out, -1 after.  The n-th largest
-// is found bit by bit, counting with ballots: no barrier.
+// Of a wavefront's N x 64 ranks: a `cut` that n of them reach (`upto` == n), or
+// the n-th largest, which more do; bit by bit, counting with ballots: no barrier.
+// Fewer than n candidates: 0.
+struct Cut {
+  uint32_t cut;
+  int upto;
+};
+
+template <int N>
+__device__ __forceinline__ Cut wave_cut(const uint32_t (&k)[N], int n) {
+  Cut r{0, 0};
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t c = r.cut | 1u << bit;
+    int m = 0;
+#pragma unroll
+    for (int x = 0; x < N; ++x) m += bits(__ballot(k[x] >= c));
+    if (m >= n) {
+      r = {c, m};
+      if (m == n) break;
+    }
+  }
+  return r;
+}
+
+template <int N>
+__device__ __forceinline__ int wave_above(const uint32_t (&k)[N], uint32_t cut) {
+  int m = 0;
+#pragma unroll
+  for (int x = 0; x < N; ++x) m += bits(__ballot(k[x] > cut));
+  return m;
+}
+
+// The n largest of a row's ranks in LDS by one wavefront (lane l: 64 x + l), the
+// lowest columns among equal ones, ascending by column into out, -1 after.  The
+// row is written over.
+//
+// A cut of the lanes' largest ranks is one that at least n of all reach, and few
+// more (64 ln(64 / (64 - n)) if they lie at random: 18 for 16, 44 for 32): those
+// are gathered, one a lane, and cut again, so that a count is one ballot and not
+// NR.  2,048 rows, n = 16, with NR ballots a count / so: 20.7 / 17.5 us at 512
+// columns, 29.3 / 21.6 at 891, 47.5 / 28.0 at 1,024, 53.3 / 33.8 at 2,048; n = 64,
+// of which more reach than there are lanes: 54.4 / 56.6 at 2,048.
+constexpr int kGather = 32;  // the longest lists made so
+
 template <int NR>
-__device__ void wave_take_best(const uint32_t (&k)[NR], int count, int n, int32_t* out) {
+__device__ void wave_take_best(uint32_t* ranks, int count, int n, int32_t* out) {
   const int lane = threadIdx.x & 63;
+  const uint64_t below = (uint64_t(1) << lane) - 1;
+  uint32_t k[NR], top[1] = {0};
+#pragma unroll
+  for (int x = 0; x < NR; ++x) {
+    k[x] = 64 * x + lane < count ? ranks[64 * x + lane] : 0;
+    top[0] = max(top[0], k[x]);
+  }
   // all ranks from `cut` on are taken, of those equal to it the first `ties`
   uint32_t cut = 1;
   int ties = 64 * NR;
   if (count > n) {
-    cut = 0;
-    int upto = 0;  // ranks at or above cut
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t c = cut | 1u << bit;
-      int m = 0;
+    Cut c = n <= kGather ? wave_cut(top, n) : Cut{0, 0};
+    const int reach = c.cut ? wave_above(k, c.cut - 1) : 0;
+    if (reach == n) {
+      cut = c.cut;
+    } else if (reach > n && reach <= 64) {
+      int at = 0;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-      for (int x = 0; x < NR; ++x) m += bits(__ballot(k[x] >= c));
-      if (m >= n) {
-        cut = c;
-        upto = m;
-        if (m == n) break;
+      for (int x = 0; x < NR; ++x) {
+        const uint64_t some = __ballot(k[x] >= c.cut);
+        if (k[x] >= c.cut) ranks[at + bits(some & below)] = k[x];
+        at += bits(some);
       }
-    }
-    if (cut == 0) {
-      cut = 1;  // (absent blocks: fewer candidates than n)
-    } else if (upto > n) {
-      int above = 0;
-#pragma unroll
-      for (int x = 0; x < NR; ++x) above += bits(__ballot(k[x] > cut));
-      ties = n - above;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      const uint32_t few[1] = {lane < reach ? ranks[lane] : 0};
+      c = wave_cut(few, n);
+      cut = c.cut;
+      if (c.upto > n) ties = n - wave_above(few, cut);
+    } else {
+      // longer lists, blocks that are absent from many lanes, or many equal ranks
+      c = wave_cut(k, n);
+      if (c.cut) cut = c.cut;  // (else fewer candidates than n: all)
+      if (c.upto > n) ties = n - wave_above(k, cut);
     }
   }
-  const uint64_t below = (uint64_t(1) << lane) - 1;
   int at = 0;
 #pragma unroll
   for (int x = 0; x < NR; ++x) {
@@ -312,15 +362,6 @@ __device__ void wave_take_best(const uint32_t (&k)[NR], int count, int n, int32_
     ties -= bits(tied);
   }
   for (int x = at + lane; x < n; x += 64) out[x] = -1;
-}
-
-template <int NR>
-__device__ void wave_take_best(const uint32_t* ranks, int count, int n, int32_t* out) {
-  const int lane = threadIdx.x & 63;
-  uint32_t k[NR];
-#pragma unroll
-  for (int x = 0; x < NR; ++x) k[x] = 64 * x + lane < count ? ranks[64 * x + lane] : 0;
-  wave_take_best(k, count, n, out);
 }
 
 template <int THREADS>

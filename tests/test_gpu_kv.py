@@ -348,6 +348,33 @@ def test_select_among_many_blocks_of_several_heads(engine, heads, group, d):
                  np.array([2100 * 16 - 1, 16 * 16, 2050 * 16]), 16, 11)
 
 
+@pytest.mark.parametrize("kind", ["a lane's", "equal", "few values", "neighbours", "few pages",
+                                  "a stretch"])
+def test_select_of_many_rows_wherever_the_best_lie(engine, kind):
+    """Tiles of tokens over 512 columns, a lane of a wavefront holding every 64th."""
+    rng = np.random.default_rng(12)
+    heads, d, cols, tokens = 64, 16, 512, 17
+    codes, scales = summaries(rng, cols, heads, d, spread=0.01)
+    table = np.arange(cols, dtype=np.int32)[None].copy()
+    if kind == "a lane's":         # 8 of 512 by far, then whatever comes
+        codes[5::64], scales[5::64] = 100, 1e6
+    elif kind == "equal":
+        codes[:], scales[:] = 1, 1.0
+    elif kind == "few values":     # more equal ones than a wavefront has lanes
+        codes[:], scales[:] = rng.integers(0, 3, (cols, heads, 1)), 1.0
+    elif kind == "neighbours":     # scores that differ in their last bits
+        codes[:] = 127
+        scales[:] = np.float32(1) + np.float32(2.0 ** -23) * rng.permutation(cols)[:, None]
+    elif kind == "few pages":
+        table[0, rng.permutation(cols)[:480]] = -1
+    else:                          # the best 100 side by side
+        codes[200:300], scales[200:300] = 120, 50.0
+    positions = cols * 16 - 1 - rng.integers(0, 700, tokens) * (np.arange(tokens) % 3)
+    q = dev(np.abs(rng.standard_normal((tokens, heads, d), np.float32))).bfloat16()
+    for n in (2, 16, 32, 33):
+        check_select(engine, q, codes, scales, table, np.zeros(tokens, int), positions, 16, n)
+
+
 def test_select_ties_go_to_the_lowest_block(engine):
     rng = np.random.default_rng(1)
     for kind in range(4):
