@@ -607,12 +607,14 @@ __global__ __launch_bounds__(512) void kv_select_tile_kernel(KvSelectArgs a) {
 
 // Ways to list (rows: tokens x kv heads; figures for 128 values, 4 heads a kv head):
 // - kTile, 16 tokens a workgroup, where requests have many: a block is read once
-//   for 16 tokens, but a launch is no shorter than a workgroup.  By row / by tile:
-//   1,024 rows of one request 10.4 / 10.4 us at 64 columns, 19.6 / 16.6 at 512,
-//   27.0 / 24.2 at 891, 29.5 / 38.1 at 1,024 (a workgroup has a CU to itself from
-//   897 on); 2,048 rows 17.9 / 10.6, 35.3 / 17.0, 48.4 / 23.9, 52.8 / 37.1, and
-//   91.7 / 45.7 at 2,048; 512 rows 14.2 / 16.9 at 512 columns.  32 requests of 8
-//   tokens 30.4 / 20.0, 16 requests of 8 16.0 / 19.0.
+//   for 16 tokens, but a launch is no shorter than a workgroup.  By row / by tile,
+//   16 blocks taken: 1,024 rows of one request 10.4 / 10.0 us at 64 columns, 20.4 /
+//   17.4 at 512, 28.0 / 21.6 at 891, 30.2 / 27.9 at 1,024 (a workgroup has a CU to
+//   itself from 897 on), 52.2 / 33.6 at 2,048; 2,048 rows 18.5 / 10.1, 35.8 / 17.1,
+//   48.8 / 21.9, 53.4 / 28.0, 92.9 / 33.7; 768 rows 9.7 / 11.7 at 64, 17.7 / 17.0 at
+//   512, 26.1 / 27.3 at 1,024.  32 requests of 8 tokens 35.8 / 20.6, 16 requests of 8
+//   20.2 / 20.4.  64 taken of 2,048 columns: 2,048 rows 55 by tile, as long as 1,024
+//   rows by row.
 // - kRow, a row a workgroup, its ranks in LDS.
 // - kParts, two launches over the workspace, for a few long rows (or ranks that no
 //   LDS holds): by row / in two launches, 128 rows 21.0 / 18.6 us at 2,048 columns,
@@ -626,9 +628,8 @@ constexpr int kTileCols = 64 * 32;  // ranks of 16 tokens in 128 KB of LDS
 
 Way way_of(const KvSelectArgs& a) {
   const int64_t rows = a.q.tokens * a.c.heads;
-  if (a.q.cols <= kTileCols && rows >= (a.q.cols <= 896 ? 1024 : 1536) &&
-      a.q.tokens >= 8 * a.q.requests)
-    return Way::kTile;
+  const int64_t many = a.q.cols <= 896 || a.n <= kGather ? 1024 : 1536;
+  if (a.q.cols <= kTileCols && rows >= many && a.q.tokens >= 8 * a.q.requests) return Way::kTile;
   return a.q.cols > kLdsCols || (a.q.cols > 1024 && rows < 256) ? Way::kParts : Way::kRow;
 }
 
