@@ -27,6 +27,7 @@
 #include <type_traits>
 
 #include "kv_cache.h"
+#include "kv_lists.h"
 #include "lds_stage.h"
 
 namespace mlxvs::kern {
@@ -351,7 +352,6 @@ __device__ __forceinline__ int row_max(int x) {
 // over, one at a time.
 constexpr int kSharedWaves = 4;
 constexpr int kListInts = 3840;  // of all lists of a workgroup (two workgroups a CU)
-constexpr int kWindow = 2048;    // blocks whose union is made at a time
 
 // Tokens that share a wavefront, and wavefronts that share a token's heads.
 struct Sharing {
@@ -386,7 +386,7 @@ struct AttendShared {
   static constexpr int kChunks = DP / 32, kTiles = DP / 16;
   // (room for a block that is listed 256 times)
   static constexpr float kBias = BF16 ? 0.0f : 7.0f;
-  static constexpr int kNone = 0x7FFFFFFF;
+  static constexpr int kNone = kNoBlock;
   // K rows lie at a power of two of 16-byte chunks in LDS, V^T rows densely; 1 KB
   // copies, dealt to the wavefronts
   static constexpr int kRow = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;
@@ -741,11 +741,8 @@ struct AttendShared {
     floor = base + kWindow;
     for (uint64_t left = with; left; left &= left - 1) {
       const int* list = sh.lists + (first_list + __builtin_ctzll(left)) * stride;
-      for (int e = lane; e < stride; e += 64) {
-        const int b = list[e];
-        if (b == kNone) break;
-        if (b >= base && b - base < kWindow) atomicOr(&sh.window[(b - base) >> 5], 1u << (b & 31));
-      }
+      blocks_in_window(list, stride, lane, base, a.q.cols,
+                       [&](int b) { atomicOr(&sh.window[b >> 5], 1u << (b & 31)); });
     }
     __syncthreads();
     bits = sh.window[lane];
@@ -829,7 +826,7 @@ void kv_attend_shared_kernel(KvAttendArgs a) {
       bool ascends = true;
       for (int e = lane; e - lane < a.n; e += 64) {
         const int b = e < a.n ? from[e] : -1;
-        const bool take = b >= 0 && b < a.q.cols && b <= own;
+        const bool take = block_shows(b, a.q.cols, own);
         const uint64_t taken = __ballot(take);
         const uint64_t mine = taken & ((uint64_t(1) << lane) - 1);
         if (take) list[at + (int)__popcll(mine)] = b;
@@ -838,7 +835,8 @@ void kv_attend_shared_kernel(KvAttendArgs a) {
         if (taken) before = __shfl(b, 63 - __builtin_clzll(taken));
         at += (int)__popcll(taken);
       }
-      if (lane == 0) list[at] = A::kNone;
+      end_list(list, at, stride, lane);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       if (!__all(ascends)) {
         // each entry's place is the number of those below it, or equal and before
         int b[kKvMaxBlocks / 64], to[kKvMaxBlocks / 64];

@@ -1,0 +1,44 @@
+"""The paged key-value cache's operators at their limits: lists that are partly
+empty beside other tables, extreme positions and values, moved tensors."""
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import kv_oracle  # noqa: E402
+from test_gpu_kv import (DTYPES, check_attend, check_select, dev, f32, make_cache,  # noqa: E402
+                         summaries, tables)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("n", [3, 40, 256])
+def test_ragged_lists_over_a_view_of_a_wider_table(engine, n, page):
+    """The view's spare columns, and the row after its last, name pages too
+    (of nothing but NaN): they are nobody's."""
+    rng = np.random.default_rng(n + page)
+    heads, group, dim, cols, tokens = 64, 8, 32, 9, 40
+    cache = make_cache(engine, 2 * cols + 1, heads, page, dim, "bf16", rng)
+    cache.keys[-1] = cache.values[-1] = float("nan")
+    wide = torch.full((3, 300), 2 * cols, dtype=torch.int32, device="cuda")
+    ids = tables(rng, 2 * cols, 2, cols)
+    wide[:2, :cols] = dev(ids)
+    view = wide[:2, :cols]
+    who = (np.arange(tokens) >= 25).astype(np.int32)
+    positions = rng.integers(0, cols * page, tokens)
+    q = dev(rng.standard_normal((tokens, heads * group, dim), np.float32)).bfloat16()
+    # another call's full lists first: what it leaves in LDS are blocks past this table
+    other = engine.PagedKVCache.empty(300, heads, page, dim)
+    full = dev(np.tile(np.arange(300 - n, 300), (tokens, heads, 1)), torch.int32)
+    other.attend(q, torch.arange(300, dtype=torch.int32, device="cuda")[None],
+                 torch.zeros(tokens, dtype=torch.int32, device="cuda"),
+                 torch.full((tokens,), 300 * page - 1, dtype=torch.int32, device="cuda"),
+                 blocks=full)
+    blocks = rng.integers(-2, cols + 3, (tokens, heads, n))
+    blocks[:, :, 2:] = np.where(rng.random((tokens, heads, max(0, n - 2))) < 0.9, -1, blocks[:, :, 2:])
+    blocks[::3] = -1
+    blocks[::3, :, 0] = 0
+    got = cache.attend(q, view, dev(who), dev(positions, torch.int32), blocks=dev(blocks, torch.int32))
+    assert torch.equal(got, check_attend(cache, "bf16", q, ids, who, positions, blocks=blocks))
