@@ -85,6 +85,12 @@ __device__ __forceinline__ int table_entry(const int32_t* table, int i) {
   return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)(table + i);
 }
 
+// A token's position, at most the table's last (-1 for a table without columns):
+// beyond it there is nothing to see, and position + 1 fits in 31 bits.
+__device__ __forceinline__ int position(const KvAttendArgs& a, int64_t t) {
+  return min(a.q.positions[t], (a.q.cols << a.c.lps) - 1);
+}
+
 // The first `n` of 8 values (n <= 0: none), zeros after.
 __device__ __forceinline__ uintx4 keep(uintx4 v, int n) {
 #pragma unroll
@@ -469,7 +475,7 @@ struct AttendShared {
   __device__ __forceinline__ int entry() const {
     if (!on) return kNone;
     if constexpr (LIST) return sh.lists[at];
-    return at <= min(pos >> a.c.lps, a.q.cols - 1) ? at : kNone;
+    return at <= pos >> a.c.lps ? at : kNone;
   }
 
   // How many keys of block b each column sees, and how often it has it listed.
@@ -502,7 +508,7 @@ struct AttendShared {
 
   __device__ __forceinline__ int next_block() {
     if constexpr (!LIST) {
-      return counter <= min(last >> a.c.lps, a.q.cols - 1) ? counter++ : kNone;
+      return counter <= last >> a.c.lps ? counter++ : kNone;
     } else {
       const uint64_t some = __ballot(bits != 0);
       if (!some) return kNone;
@@ -810,10 +816,9 @@ void kv_attend_shared_kernel(KvAttendArgs a) {
   int myreq = -1, mypos = -1;
   if (lane < tokens) {
     myreq = a.q.token_request[t0 + lane];
-    mypos = a.q.positions[t0 + lane];
+    mypos = position(a, t0 + lane);
   }
-  // (a table without columns has no entry to look up)
-  const bool sees = myreq >= 0 && myreq < a.q.requests && mypos >= 0 && a.q.cols > 0;
+  const bool sees = myreq >= 0 && myreq < a.q.requests && mypos >= 0;
   const int stride = a.n + 1;
   w.first_list = w.wave * share.tokens;
   if constexpr (LIST) {
@@ -923,11 +928,11 @@ __global__ __launch_bounds__(256, 2) void kv_attend_parts_kernel(KvAttendArgs a)
   const int part = (int)(b / a.q.tokens);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   A w(a, threadIdx.x & 63);
-  const int r = a.q.token_request[t], pos = a.q.positions[t];
+  const int r = a.q.token_request[t], pos = position(a, t);
   int64_t k0 = (int64_t)part * a.chunk, k1 = 0;
   int end = 0;
   if (r >= 0 && r < a.q.requests && pos >= 0) {
-    end = LIST ? a.n : min(pos >> a.c.lps, a.q.cols - 1) + 1;
+    end = LIST ? a.n : (pos >> a.c.lps) + 1;
     k1 = (int64_t)end << a.c.lps;
     if (!LIST) k1 = min(k1, (int64_t)pos + 1);
     if (part + 1 < a.splits) k1 = min(k1, k0 + a.chunk);

@@ -42,3 +42,26 @@ def test_ragged_lists_over_a_view_of_a_wider_table(engine, n, page):
     blocks[::3, :, 0] = 0
     got = cache.attend(q, view, dev(who), dev(positions, torch.int32), blocks=dev(blocks, torch.int32))
     assert torch.equal(got, check_attend(cache, "bf16", q, ids, who, positions, blocks=blocks))
+
+
+@pytest.mark.parametrize("listed", [False, True])
+@pytest.mark.parametrize("heads,group,page,dim,tokens",
+                         [(2, 4, 16, 64, 6), (1, 3, 64, 80, 1), (64, 8, 64, 64, 40), (64, 4, 16, 128, 40),
+                          (64, 16, 32, 40, 26)])
+def test_the_largest_position_sees_the_whole_table(engine, heads, group, page, dim, tokens, listed):
+    """Beside tokens that see less, whose values past it stay hidden and whose own stay."""
+    rng = np.random.default_rng(heads + page)
+    cols = 5
+    cache = make_cache(engine, 2 * cols, heads, page, dim, "bf16", rng)
+    table = tables(rng, 2 * cols, 2, cols)
+    who = (np.arange(tokens) % 7 == 3).astype(np.int32)
+    positions = rng.integers(0, cols * page, tokens)
+    positions[::3] = np.iinfo(np.int32).max - rng.integers(0, 3, len(positions[::3]))
+    positions[0] = np.iinfo(np.int32).max
+    q = dev(rng.standard_normal((tokens, heads * group, dim), np.float32)).bfloat16()
+    blocks = rng.integers(-1, cols + 1, (tokens, heads, 4)) if listed else None
+    if listed:
+        blocks[0] = [0, 4, 2, -1]
+    got = check_attend(cache, "bf16", q, table, who, positions, blocks=blocks)
+    edge = np.minimum(positions, cols * page - 1)
+    assert torch.equal(got, check_attend(cache, "bf16", q, table, who, edge, blocks=blocks))
