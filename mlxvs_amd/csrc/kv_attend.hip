@@ -354,8 +354,11 @@ __device__ __forceinline__ int row_max(int x) {
 //
 // A weight of 0 does not hide a value that is not finite.  Values past every
 // token's keys are masked; one that only some of the tokens see would reach the
-// others' sums as NaN, so a workgroup whose sums are not finite does its tokens
-// over, one at a time.
+// others' sums as NaN, so a workgroup with a token whose sums are not finite goes
+// over its tiles again, where tokens differ in what they see one token after
+// another.  An infinity that all see costs 512 tokens of 2,048 keys (64 heads of 64
+// values) 126 us, not 54; 4,096 tokens of 8,192 keys 1,839, not 797; over lists of 16
+// blocks 1.9 to 5 times as long (16 tokens a wavefront).
 constexpr int kSharedWaves = 4;
 constexpr int kListInts = 3840;  // of all lists of a workgroup (two workgroups a CU)
 
@@ -426,6 +429,7 @@ struct AttendShared {
   int pos;       // of the column's token
   int at, next;  // its place in its list, and the block there
   bool on;
+  int token, tokens;  // the column's of this wavefront's tokens (-1: none), and their number
   uint32_t from_k[kCopiesK], from_v[kCopiesV];  // what this lane copies, in bytes from a page's
   int block_v;     // ... and whose values
   int at_k, at_v;  // where this lane's first operands are, in bytes
@@ -618,6 +622,8 @@ struct AttendShared {
 
   // 32 keys of a buffer, from key `k0` of the tile on: of this lane's 8 keys its
   // column sees the first n8.  `twice`: log2 of how often a block is listed.
+  // EXACT: no value reaches a token that does not see it.
+  template <bool EXACT>
   __device__ __forceinline__ void step(Buffer from, int k0, int n8, bool all, float twice) {
     floatx4 s[2];
 #pragma unroll
@@ -634,17 +640,36 @@ struct AttendShared {
       for (int i = 0; i < kChunks; ++i)
         s[u] = mfma(__builtin_bit_cast(Tx8, kf[i]), q[i], s[u]);
     }
-    uintx4 vf[kTiles];
     // (32 keys on, a chunk's place differs in one bit)
     const char* v = from.v + (at_v ^ (k0 ? 64 : 0));
+    uintx4 vf[kTiles];
+    if constexpr (!EXACT) {
 #pragma unroll
-    for (int i = 0; i < kTiles; ++i) vf[i] = *(const uintx4*)(v + i * 32 * kKeys);
+      for (int i = 0; i < kTiles; ++i) vf[i] = *(const uintx4*)(v + i * 32 * kKeys);
+    }
     if (!all) hide(s, n8);
     Tx8 pr[1];
     weights<1>(s, m, l, c, kBias + twice, o, pr);
+    if constexpr (!EXACT) {
 #pragma unroll
-    for (int i = 0; i < kTiles; ++i)
-      o[i] = mfma(__builtin_bit_cast(Tx8, vf[i]), pr[0], o[i]);
+      for (int i = 0; i < kTiles; ++i)
+        o[i] = mfma(__builtin_bit_cast(Tx8, vf[i]), pr[0], o[i]);
+    } else {
+      // a token after another, unless all see everything: values that it does not
+      // see are zeros to it, and only its columns take the product
+#pragma unroll 1
+      for (int x = 0; x < tokens; ++x) {
+        const int n = all ? 8 : __shfl(n8, 16 * grp + x * a.q.group);
+        if (!__any(n > 0)) continue;
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+          const uintx4 vx = keep(*(const uintx4*)(v + i * 32 * kKeys), n);
+          const floatx4 y = mfma(__builtin_bit_cast(Tx8, vx), pr[0], o[i]);
+          o[i] = all || token == x ? y : o[i];
+        }
+        if (all) break;
+      }
+    }
   }
 
   // A lane's 8 scores of which its column sees the first n.
@@ -663,6 +688,7 @@ struct AttendShared {
   // times are kept over the tiles of a block.
   Counts seen, times;
 
+  template <bool EXACT>
   __device__ __forceinline__ void use(const Tile& t, Buffer from) {
     if (t.off == 0) {
 #pragma unroll
@@ -681,7 +707,7 @@ struct AttendShared {
       const int n8 = (int)(seen >> place & 0xFFFF) - t.off - (kBlocks > 1 ? key % PK : key);
       if (!__any(n8 > 0)) continue;
       const float twice = LIST ? __log2f((float)max(1, (int)(times >> place & 0xFFFF))) : 0.0f;
-      step(from, k0, n8, __all(n8 >= 8), twice);
+      step<EXACT>(from, k0, n8, __all(n8 >= 8 || (EXACT && token < 0)), twice);
     }
   }
 
@@ -690,7 +716,7 @@ struct AttendShared {
 
   // Goes to the next request that some wavefront's tokens have; false: none.
   // Every wavefront of the workgroup comes here, and into window().
-  __device__ __forceinline__ bool request(int myreq, int tok, bool mine, int stride) {
+  __device__ __forceinline__ bool request(int myreq, int stride) {
     __syncthreads();
     if (threadIdx.x == 0) {
       sh.again = kNone;
@@ -708,8 +734,8 @@ struct AttendShared {
     todo &= ~with;
     table = a.q.table + (int64_t)r * a.q.table_stride;
     int far = -1;
-    on = mine && (with >> tok & 1);
-    at = LIST ? (first_list + tok) * stride : 0;
+    on = token >= 0 && (with >> token & 1);
+    at = LIST ? (first_list + max(0, token)) * stride : 0;
     next = entry();
     if (on) far = max(far, pos);
     far = row_max(far);
@@ -756,8 +782,8 @@ struct AttendShared {
   }
 
   // All blocks of this wavefront's tokens `todo`.
-  __device__ __forceinline__ void run(int myreq, int tok, bool mine, int stride, Buffer b0,
-                                      Buffer b1) {
+  template <bool EXACT>
+  __device__ __forceinline__ void run(int myreq, int stride, Buffer b0, Buffer b1) {
     Tile now;
     bool more = false;
     open = false;
@@ -768,14 +794,14 @@ struct AttendShared {
       mfma_settle();
       if (more) copy(then, to);
       clear(now, from);
-      use(now, from);
+      use<EXACT>(now, from);
       now = then;
     };
     // (one loop around the sums, so that they stay in one set of registers)
     while (true) {
       if (!more) {
         while (true) {
-          if (!open && !request(myreq, tok, mine, stride)) return;
+          if (!open && !request(myreq, stride)) return;
           if (!window(stride)) continue;
           now.off = 1 << 30;  // (past any block)
           now.block[0] = 0;
@@ -870,41 +896,40 @@ void kv_attend_shared_kernel(KvAttendArgs a) {
     if (mine && 32 * i + 8 * w.grp < a.c.dim) x4 = *(const uintx4*)(src + 32 * i + 8 * w.grp);
     w.q[i] = __builtin_bit_cast(typename A::Tx8, x4);
   }
-  // first all tokens together, a request after another; then, if that left
-  // sums that are not finite, each token by itself
-  const int all_tokens = share.tokens * kSharedWaves;
-  for (int turn = -1; turn < all_tokens; ++turn) {
-    const int alone = turn < 0 ? -1 : turn - w.first_list;  // of this wavefront's
+  const uint64_t seeing = w.todo = __ballot(sees);
+  w.token = mine ? tok : -1;
+  w.tokens = share.tokens;
+  w.reset();
+  w.template run<false>(myreq, stride, {k0, v0}, {k1, v1});
+  mfma_settle();
+  bool good = true;
+#pragma unroll
+  for (int i = 0; i < A::kTiles; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      good &= fabsf(w.o[i][j]) < __builtin_inff() || 16 * i + 4 * w.grp >= a.c.dim;
+  if (__syncthreads_or(!good && mine && (seeing >> tok & 1))) {
+    w.todo = seeing;
     w.reset();
-    w.todo = __ballot(sees);
-    if (turn >= 0) w.todo &= alone >= 0 && alone < share.tokens ? uint64_t(1) << alone : 0;
-    w.run(myreq, tok, mine, stride, {k0, v0}, {k1, v1});
+    w.template run<true>(myreq, stride, {k0, v0}, {k1, v1});
     mfma_settle();
-    bool good = true;
+  }
+  const float l = column_sum(w.l);
+  if (mine) {
+    const float inv = 1.0f / l;
+    const int64_t at = ((t0 + tok) * a.c.heads + h) * group + g;
 #pragma unroll
-    for (int i = 0; i < A::kTiles; ++i)
+    for (int i = 0; i < A::kTiles; ++i) {
+      const int d = 16 * i + 4 * w.grp;
+      if (d < a.c.dim) {
+        typename A::Tx4 x;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        good &= fabsf(w.o[i][j]) < __builtin_inff() || 16 * i + 4 * w.grp >= a.c.dim;
-    if (turn < 0 && __syncthreads_or(!good)) continue;
-    const float l = column_sum(w.l);
-    if (mine && (turn < 0 || tok == alone)) {
-      const float inv = 1.0f / l;
-      const int64_t at = ((t0 + tok) * a.c.heads + h) * group + g;
-#pragma unroll
-      for (int i = 0; i < A::kTiles; ++i) {
-        const int d = 16 * i + 4 * w.grp;
-        if (d < a.c.dim) {
-          typename A::Tx4 x;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            x[j] = (typename A::T)(l == 0.0f ? 0.0f : w.o[i][j] * inv);
-          *(typename A::Tx4*)((typename A::T*)a.out + at * a.c.dim + d) = x;
-        }
+        for (int j = 0; j < 4; ++j)
+          x[j] = (typename A::T)(l == 0.0f ? 0.0f : w.o[i][j] * inv);
+        *(typename A::Tx4*)((typename A::T*)a.out + at * a.c.dim + d) = x;
       }
-      if (a.lse && w.grp == 0) a.lse[at] = lse_of(w.m, l, a.scale, A::kBias);
     }
-    if (turn < 0) break;
+    if (a.lse && w.grp == 0) a.lse[at] = lse_of(w.m, l, a.scale, A::kBias);
   }
 }
 

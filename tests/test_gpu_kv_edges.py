@@ -65,3 +65,63 @@ def test_the_largest_position_sees_the_whole_table(engine, heads, group, page, d
     got = check_attend(cache, "bf16", q, table, who, positions, blocks=blocks)
     edge = np.minimum(positions, cols * page - 1)
     assert torch.equal(got, check_attend(cache, "bf16", q, table, who, edge, blocks=blocks))
+
+
+@pytest.mark.parametrize("listed", [False, True])
+@pytest.mark.parametrize("heads,group,page,dim,tokens",
+                         [(64, 4, 64, 128, 45), (64, 5, 16, 80, 40), (128, 1, 32, 64, 70),
+                          (40, 33, 64, 64, 21), (64, 8, 128, 192, 33), (64, 16, 32, 256, 24),
+                          (96, 3, 256, 40, 50)])
+def test_values_that_are_not_finite_reach_who_sees_them(engine, heads, group, page, dim, tokens, listed):
+    """And nobody else: not the neighbours, another request's tokens or idle ones."""
+    rng = np.random.default_rng(heads + group)
+    cols = 6
+    cache = make_cache(engine, 2 * cols, heads, page, dim, "f16", rng)
+    table = np.arange(2 * cols, dtype=np.int32).reshape(2, cols)
+    who = (np.arange(tokens) % 9 == 4).astype(np.int32)
+    positions = np.sort(rng.integers(0, cols * page, tokens))
+    positions[5] = -1
+    q = dev(rng.standard_normal((tokens, heads * group, dim), np.float32)).half()
+    blocks = rng.integers(-1, cols, (tokens, heads, 3)) if listed else None
+    want = check_attend(cache, "f16", q, table, who, positions, blocks=blocks)
+    # of request 0, a key in the middle and one of its first block
+    bad = [(3 * page + 9, 2, float("inf")), (3 * page + 9, dim - 1, float("nan")),
+           (5, 7, float("-inf")), (3 * page + 9, 7, float("inf"))]
+    for key, d, x in bad:
+        cache.values[key // page, :, d, key % page] = x
+    got = cache.attend(q, dev(table), dev(who), dev(positions, torch.int32),
+                       blocks=None if blocks is None else dev(blocks, torch.int32))
+    got, want = f32(got), f32(want)
+    key_in = lambda k: (who == 0)[:, None] & (positions >= k)[:, None] & (  # noqa: E731
+        np.ones((tokens, heads), bool) if blocks is None else (blocks == k // page).any(2))
+    mid, low = (np.repeat(key_in(k), group, 1) for k in (3 * page + 9, 5))
+    want[..., 2][mid] = np.inf
+    want[..., dim - 1][mid] = np.nan
+    want[..., 7] = np.where(mid & low, np.nan, np.where(mid, np.inf, np.where(low, -np.inf, want[..., 7])))
+    assert np.array_equal(got, want, equal_nan=True)
+
+
+def test_what_one_infinite_value_costs(engine):
+    """A second round over a workgroup's tiles, not one for each of its tokens."""
+    rng = np.random.default_rng(4)
+    heads, page, dim, cols, tokens = 64, 64, 64, 32, 512
+    cache = make_cache(engine, cols, heads, page, dim, "bf16", rng)
+    q = dev(rng.standard_normal((tokens, heads, dim), np.float32)).bfloat16()
+    table, who = dev(np.arange(cols)[None], torch.int32), dev(np.zeros(tokens), torch.int32)
+    positions = dev(np.arange(tokens) + cols * page - tokens, torch.int32)
+
+    def spent():
+        times = []
+        for _ in range(4):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            cache.attend(q, table, who, positions)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    clean = spent()
+    cache.values[0, :, 3, 5] = float("inf")
+    # (measured: 2.4 times as long; with a round for each of 64 tokens 53 times)
+    assert spent() < 6 * clean
