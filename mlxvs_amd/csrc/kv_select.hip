@@ -40,7 +40,7 @@ __device__ __forceinline__ int bits(uint64_t x) { return (int)__popcll(x); }
 
 __device__ __forceinline__ uint32_t rank_of(int dot, float scale) {
   // a summary that is not finite ranks first (a broken block is not left out)
-  float x = scale < __builtin_inff() ? (float)dot * scale : FLT_MAX;
+  float x = fabsf(scale) < __builtin_inff() ? (float)dot * scale : FLT_MAX;
   x = fminf(fmaxf(x, -FLT_MAX), FLT_MAX) + 0.0f;  // (-0 and 0 are equal)
   const uint32_t u = __builtin_bit_cast(uint32_t, x);
   return u >> 31 ? ~u : u | 0x80000000u;

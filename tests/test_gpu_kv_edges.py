@@ -125,3 +125,19 @@ def test_what_one_infinite_value_costs(engine):
     cache.values[0, :, 3, 5] = float("inf")
     # (measured: 2.4 times as long; with a round for each of 64 tokens 53 times)
     assert spent() < 6 * clean
+
+
+@pytest.mark.parametrize("cols,tokens,heads", [(60, 5, 2), (300, 16, 64), (2300, 2, 2)])
+def test_scales_that_are_not_finite_rank_first(engine, cols, tokens, heads):
+    """Of either sign, by rows, by tiles and in parts."""
+    rng = np.random.default_rng(cols)
+    codes, scales = summaries(rng, 400, heads, 32)
+    for i, x in enumerate((-np.inf, np.inf, np.nan, -np.inf, -3e38, 3e38)):
+        scales[10 + 7 * i] = x
+    codes[31], scales[17] = 0, -np.inf
+    table = rng.permutation(400)[np.arange(2 * cols) % 400].reshape(2, cols).astype(np.int32)
+    who = np.zeros(tokens, int)
+    positions = cols * 16 - 1 - 3 * np.arange(tokens)
+    q = dev(rng.standard_normal((tokens, heads * 2, 32), np.float32)).bfloat16()
+    for n in (4, 9, 40):
+        check_select(engine, q, codes, scales, table, who, positions, 16, n)
