@@ -683,8 +683,14 @@ int64_t kv_select_workspace(const KvSelectArgs& a) {
 int64_t kv_select_grid(const KvSelectArgs& a) {
   // (in workgroups of 256)
   const int64_t rows = a.q.tokens * a.c.heads;
-  return way_of(a) == Way::kParts
-             ? 2 * rows * ((a.q.cols + kPartCols - 1) / kPartCols) : 4 * rows;
+  switch (way_of(a)) {
+    case Way::kTile: return 2 * ((a.q.tokens + kTile - 1) / kTile * a.c.heads);
+    case Way::kRow: return rows <= 256 ? 4 * rows : rows;
+    case Way::kParts: break;
+  }
+  const int64_t parts = (a.q.cols + kPartCols - 1) / kPartCols;
+  const int64_t sets = (a.c.heads + kPartHeads - 1) / kPartHeads;
+  return std::max(2 * a.q.tokens * sets * parts, 4 * rows);
 }
 
 hipError_t launch_kv_select(const KvSelectArgs& a, hipStream_t s) {

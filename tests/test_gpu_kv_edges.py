@@ -141,3 +141,21 @@ def test_scales_that_are_not_finite_rank_first(engine, cols, tokens, heads):
     q = dev(rng.standard_normal((tokens, heads * 2, 32), np.float32)).bfloat16()
     for n in (4, 9, 40):
         check_select(engine, q, codes, scales, table, who, positions, 16, n)
+
+
+def test_select_of_more_than_four_million_rows(engine):
+    rng = np.random.default_rng(13)
+    heads, d, cols, tokens = 8, 16, 6, 530_000
+    codes, scales = summaries(rng, 20, heads, d)
+    cache = engine.PagedKVCache(torch.empty((20, heads, 16, d), dtype=torch.bfloat16, device="cuda"),
+                                torch.empty((20, heads, d, 16), dtype=torch.bfloat16, device="cuda"),
+                                dev(codes), dev(scales))
+    table = tables(rng, 20, 2, cols)
+    q = torch.randn((tokens, heads, d), device="cuda", dtype=torch.bfloat16)
+    who = (np.arange(tokens) >= 300_000).astype(np.int32)
+    positions = rng.integers(0, cols * 16, tokens).astype(np.int32)
+    got = cache.select(q, dev(table), dev(who), dev(positions), 3)
+    some = np.r_[:20, 299_990:300_010, 524_280:524_300, tokens - 20:tokens]
+    want = kv_oracle.select(f32(q[dev(some)]), codes, scales, table, who[some], positions[some], 16,
+                            3, 1, 1)
+    assert np.array_equal(got[dev(some)].cpu().numpy(), want)
