@@ -189,6 +189,13 @@ __global__ __launch_bounds__(64) void kv_summaries_kernel(KvAppendArgs a, int sp
   }
 }
 
+// Whether one launch does it all, and how many tokens its workgroups take then.
+// Small tiles: a workgroup's summaries follow one another.  By 4 and 16: 64
+// requests' tokens 6.9 and 12.0 us, 512 requests' 12.7 and 17.4 (one request's
+// 512 tokens 8.8 and 8.2).
+bool few(const KvAppendArgs& a) { return a.tokens <= kFew && a.c.summaries; }
+int tile_of(const KvAppendArgs& a) { return few(a) && a.tokens <= 512 ? 4 : 16; }
+
 template <bool BF16, int TILE, bool FEW>
 void launch_tile(const KvAppendArgs& a, hipStream_t s) {
   const int64_t grid = (a.tokens + TILE - 1) / TILE * a.c.heads;
@@ -198,11 +205,8 @@ void launch_tile(const KvAppendArgs& a, hipStream_t s) {
 template <bool BF16>
 hipError_t launch_append(const KvAppendArgs& a, hipStream_t s) {
   constexpr int kSpan = 16;
-  if (a.tokens <= kFew && a.c.summaries) {
-    // Small tiles: a workgroup's summaries follow one another.  By 4 and 16: 64
-    // requests' tokens 6.9 and 12.0 us, 512 requests' 12.7 and 17.4 (one request's
-    // 512 tokens 8.8 and 8.2).
-    a.tokens <= 512 ? launch_tile<BF16, 4, true>(a, s) : launch_tile<BF16, 16, true>(a, s);
+  if (few(a)) {
+    tile_of(a) == 4 ? launch_tile<BF16, 4, true>(a, s) : launch_tile<BF16, 16, true>(a, s);
     return hipGetLastError();
   }
   launch_tile<BF16, 16, false>(a, s);
@@ -213,6 +217,10 @@ hipError_t launch_append(const KvAppendArgs& a, hipStream_t s) {
 }
 
 }  // namespace
+
+int64_t kv_append_grid(const KvAppendArgs& a) {
+  return (a.tokens + tile_of(a) - 1) / tile_of(a) * a.c.heads;
+}
 
 hipError_t launch_kv_append(const KvAppendArgs& a, hipStream_t s) {
   return a.c.bf16 ? launch_append<true>(a, s) : launch_append<false>(a, s);

@@ -1186,7 +1186,7 @@ int64_t kv_attend_workspace(const KvAttendArgs& a) {
 int64_t kv_attend_grid(const KvAttendArgs& a) {
   if (a.shared) return shared_grid(a);
   const int64_t rows = a.q.tokens * a.c.heads * ((a.q.group + kColumns - 1) / kColumns);
-  return std::max(a.q.tokens * a.c.heads * a.q.group, rows * a.splits);
+  return a.splits > 1 ? std::max(a.q.tokens * a.c.heads * a.q.group, rows * a.splits) : rows;
 }
 
 hipError_t launch_kv_attend(const KvAttendArgs& a, hipStream_t s) {

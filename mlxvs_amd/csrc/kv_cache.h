@@ -55,6 +55,7 @@ struct KvAppendArgs {
   const int64_t* slots;
   int64_t tokens;
 };
+int64_t kv_append_grid(const KvAppendArgs& a);  // workgroups of its largest launch
 hipError_t launch_kv_append(const KvAppendArgs& a, hipStream_t s);
 
 // Queries of tokens and where they stand.

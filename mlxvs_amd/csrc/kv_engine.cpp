@@ -143,7 +143,7 @@ void kv_append_device(const KvCache& cache, const void* k, int64_t k_token_strid
   check(aligned(k) && aligned(v) && k_token_stride % 8 == 0 && k_head_stride % 8 == 0 &&
             v_token_stride % 8 == 0 && v_head_stride % 8 == 0,
         "k and v must be 16-byte aligned, with strides that are multiples of 8.");
-  check_grid(tokens * a.c.heads, 64, check);
+  check_grid(kern::kv_append_grid(a), 256, check);
   if (tokens == 0) return;
   detail::need_device();
   detail::launch_stage<kern::KvAppendArgs, kern::launch_kv_append>((hipStream_t)stream,

@@ -1,9 +1,19 @@
 """How large a call of the paged key-value cache may be, without a GPU: what the
 launches have room for is not refused, and what they have not is."""
 
+import ctypes
+
 import pytest
 
-from test_kv_abi import INTERNAL, INVALID, cache, queries, select
+from test_kv_abi import INTERNAL, INVALID, attend, cache, queries, select
+
+
+@pytest.fixture(autouse=True)
+def no_gpu():
+    import mlxvs_amd._hip as hip
+
+    if hip.device_count() > 0:
+        pytest.skip("a GPU is present: the addresses are nobody's")
 
 
 @pytest.mark.parametrize("tokens,columns,requests,rc", [
@@ -14,10 +24,25 @@ from test_kv_abi import INTERNAL, INVALID, cache, queries, select
     (400_000, 9_000, 400_000, INVALID),    # 71 parts each
     (500_000, 1_025, 500_000, INTERNAL)])
 def test_selections_of_many_rows(engine, tokens, columns, requests, rc):
-    import mlxvs_amd._hip as hip
-
-    if hip.device_count() > 0:
-        pytest.skip("a GPU is present: the addresses are nobody's")
     lib = engine._L()
     q = queries(tokens=tokens, columns=columns, table_stride=columns, requests=requests)
     assert select(lib, cache(heads=8), q) == rc, lib.mlxvs_last_error()
+
+
+@pytest.mark.parametrize("tokens,rc", [(1, INTERNAL), (1024, INTERNAL), (10_000_000, INTERNAL),
+                                       (33_000_000, INTERNAL), (34_000_000, INVALID)])
+def test_appends_of_many_tokens(engine, tokens, rc):
+    # by 16 tokens and a head a workgroup: 16.8 million at most
+    lib = engine._L()
+    assert lib.mlxvs_kv_append_device(ctypes.byref(cache(heads=8)), 4096, 64, 64, 4096, 64, 64, 4096,
+                                      tokens, None) == rc, lib.mlxvs_last_error()
+
+
+@pytest.mark.parametrize("tokens,requests,rc", [
+    (600_000, 600_000, INTERNAL),       # single tokens of short requests: a row a workgroup
+    (2_200_000, 2_200_000, INVALID),    # 17.6 million
+    (2_200_000, 3, INTERNAL)])          # prompts share workgroups
+def test_attention_of_many_tokens(engine, tokens, requests, rc):
+    q = queries(tokens=tokens, requests=requests, q_heads=32, token_stride=2048)
+    lib = engine._L()
+    assert attend(lib, cache(heads=8), q) == rc, lib.mlxvs_last_error()
