@@ -52,9 +52,9 @@ def _need(ok: bool, op: str, what: str) -> None:
 
 def _ints(x, name: str, op: str, device, dtype=torch.int32, size: Optional[int] = None):
     """The pointer of a contiguous 1-D tensor of whole numbers."""
-    if not (isinstance(x, torch.Tensor) and x.dtype == dtype and x.dim() == 1
-            and x.is_contiguous() and x.device == device
-            and (size is None or x.shape[0] == size)):
+    if not (isinstance(x, torch.Tensor) and x.dtype == dtype
+            and (x.dim() == 1 if size is None else x.shape == (size,))
+            and x.is_contiguous() and x.device == device):
         of = "" if size is None else f" of {size}"
         raise ValueError(f"[mlxvs::{op}] {name} must be a contiguous 1-D {dtype} tensor{of} on "
                          f"{device}.")
@@ -171,7 +171,9 @@ class PagedKVCache:
 
     ``page_size`` is a power of two from 16 to 256, ``dim`` a multiple of 8 up
     to 256.  The tensors are used in place and must be contiguous;
-    ``PagedKVCache.empty`` makes them.
+    ``PagedKVCache.empty`` makes them.  They stay the cache's: one that is
+    resized or set to other memory is refused by the next call (a larger cache
+    is another PagedKVCache).
     """
 
     def __init__(self, keys, values, summaries=None, scales=None):
@@ -200,7 +202,11 @@ class PagedKVCache:
                   and scales.is_contiguous(), op,
                   f"scales must be a contiguous float32 [pages, kv_heads] tensor on "
                   f"{keys.device}.")
-        self.keys, self.values, self.summaries, self.scales = keys, values, summaries, scales
+        # (read-only from outside: what is checked here is what the kernels get)
+        self._keys, self._values, self._summaries, self._scales = keys, values, summaries, scales
+        self._held = [x for x in (keys, values, summaries, scales) if x is not None]
+        self._at = [x.data_ptr() for x in self._held]
+        self._dtype, self._device = keys.dtype, keys.device
         self.page_size, self.dim, self.kv_heads = page, dim, heads
         self._c = _Cache(keys.data_ptr(), values.data_ptr(),
                          None if summaries is None else summaries.data_ptr(),
@@ -208,6 +214,11 @@ class PagedKVCache:
                          _TYPES[keys.dtype])
         self._ref = ctypes.byref(self._c)
         self._sizes = {}  # workspace bytes of calls by their sizes
+
+    keys = property(lambda self: self._keys)
+    values = property(lambda self: self._values)
+    summaries = property(lambda self: self._summaries)
+    scales = property(lambda self: self._scales)
 
     @classmethod
     def empty(cls, pages, kv_heads, page_size, dim, *, dtype=torch.bfloat16, device="cuda",
@@ -220,45 +231,52 @@ class PagedKVCache:
                    make(pages, kv_heads, dim, kind=torch.int8) if summaries else None,
                    make(pages, kv_heads, kind=torch.float32) if summaries else None)
 
+    def _cache(self, op: str):
+        """The cache as the kernels take it, its memory being where it was."""
+        _need([x.data_ptr() for x in self._held] == self._at, op,
+              "the cache's tensors have moved: make another PagedKVCache of them.")
+        return self._ref
+
     def _rows(self, x, name: str, op: str, heads: Optional[int] = None):
-        """[tokens, heads, dim] rows as the kernels read them: any token and
-        head strides, 16-byte aligned (a copy where they are not)."""
-        keys = self.keys
-        if not (isinstance(x, torch.Tensor) and x.dim() == 3 and x.dtype == keys.dtype
-                and x.device == keys.device and x.shape[2] == self.dim
+        """[tokens, heads, dim] rows as the kernels read them, with their address
+        and strides: any token and head strides, 16-byte aligned (a copy where
+        they are not)."""
+        if not (isinstance(x, torch.Tensor) and x.dim() == 3 and x.dtype == self._dtype
+                and x.device == self._device and x.shape[2] == self.dim
                 and (heads is None or x.shape[1] == heads)):
-            raise ValueError(f"[mlxvs::{op}] {name} must be a {keys.dtype} [tokens, heads, "
-                             f"{self.dim}] tensor on {keys.device}.")
-        st = x.stride()
-        if st[2] != 1 or st[0] & 7 or st[1] & 7 or x.data_ptr() & 15:
+            raise ValueError(f"[mlxvs::{op}] {name} must be a {self._dtype} [tokens, heads, "
+                             f"{self.dim}] tensor on {self._device}.")
+        at, st = x.data_ptr(), x.stride()
+        if st[2] != 1 or st[0] & 7 or st[1] & 7 or at & 15:
             x = x.clone(memory_format=torch.contiguous_format)
-        return x
+            at, st = x.data_ptr(), x.stride()
+        return x, at, st
 
     def append(self, k, v, slots) -> None:
         """Write the tokens' keys and values [tokens, kv_heads, dim] into their
         ``slots`` (int64 [tokens]; -1 or outside the cache: skipped), and the
         summaries of the pages that this completes."""
         op = "kv_append"
-        k = self._rows(k, "k", op, self.kv_heads)
-        v = self._rows(v, "v", op, self.kv_heads)
+        cache = self._cache(op)
+        k, pk, ks = self._rows(k, "k", op, self.kv_heads)
+        v, pv, vs = self._rows(v, "v", op, self.kv_heads)
         tokens = k.shape[0]
         _need(v.shape[0] == tokens, op, "k and v must have the same tokens.")
-        ps = _ints(slots, "slots", op, k.device, torch.int64, tokens)
-        ks, vs = k.stride(), v.stride()
-        with _On(k.device) as stream:
-            _check(_L().mlxvs_kv_append_device(self._ref, k.data_ptr(), ks[0], ks[1], v.data_ptr(),
-                                               vs[0], vs[1], ps, tokens, stream))
+        ps = _ints(slots, "slots", op, self._device, torch.int64, tokens)
+        with _On(self._device) as stream:
+            _check(_L().mlxvs_kv_append_device(cache, pk, ks[0], ks[1], pv, vs[0], vs[1], ps,
+                                               tokens, stream))
 
     def _queries(self, q, table, requests, positions, op: str):
-        q = self._rows(q, "q", op)
-        tokens, heads = q.shape[:2]
-        _need(heads >= self.kv_heads and heads % self.kv_heads == 0, op,
-              f"q must have a multiple of {self.kv_heads} heads.")
-        pt, stride = _table(table, op, q.device)
-        st = q.stride()
-        return q, _Queries(q.data_ptr(), st[0], st[1], tokens, heads, table.shape[1], pt, stride,
-                           table.shape[0], _ints(requests, "requests", op, q.device, size=tokens),
-                           _ints(positions, "positions", op, q.device, size=tokens))
+        q, pq, st = self._rows(q, "q", op)
+        tokens, heads, _ = q.shape
+        if heads < self.kv_heads or heads % self.kv_heads:
+            raise ValueError(f"[mlxvs::{op}] q must have a multiple of {self.kv_heads} heads.")
+        pt, stride = _table(table, op, self._device)
+        rows, columns = table.shape
+        return q, _Queries(pq, st[0], st[1], tokens, heads, columns, pt, stride, rows,
+                           _ints(requests, "requests", op, self._device, size=tokens),
+                           _ints(positions, "positions", op, self._device, size=tokens))
 
     def _workspace(self, size, q, qs, *args):
         """(tensor, bytes) of scratch memory on the current stream."""
@@ -286,13 +304,14 @@ class PagedKVCache:
         is the same from every implementation."""
         op = "kv_select"
         n = int(n)
-        _need(self.summaries is not None, op, "the cache keeps no summaries.")
+        cache = self._cache(op)
+        _need(self._summaries is not None, op, "the cache keeps no summaries.")
         q, qs = self._queries(q, table, requests, positions, op)
-        with _On(q.device) as stream:
+        with _On(self._device) as stream:
             work, size = self._workspace("mlxvs_kv_select_workspace", q, qs, n)
             out = q.new_empty((q.shape[0], self.kv_heads, n), dtype=torch.int32)
             _check(_L().mlxvs_kv_select_device(
-                self._ref, ctypes.byref(qs), n, int(first), int(last), out.data_ptr(),
+                cache, ctypes.byref(qs), n, int(first), int(last), out.data_ptr(),
                 None if work is None else work.data_ptr(), size, stream))
         return out
 
@@ -308,6 +327,7 @@ class PagedKVCache:
         what is computed).  With ``lse`` returns (out, float32 [tokens,
         q_heads] logarithms of the sums of exponentials)."""
         op = "kv_attend"
+        cache = self._cache(op)
         q, qs = self._queries(q, table, requests, positions, op)
         tokens, heads, dim = q.shape
         n, pb = 0, None
@@ -322,7 +342,7 @@ class PagedKVCache:
         if scale is None:
             scale = 1.0 / math.sqrt(dim)
         longest = int(longest)
-        with _On(q.device) as stream:
+        with _On(self._device) as stream:
             work, size = self._workspace("mlxvs_kv_attend_workspace", q, qs, n, longest)
             if out is None:
                 out = q.new_empty((tokens, heads, dim))
@@ -335,7 +355,7 @@ class PagedKVCache:
             sums = q.new_empty((tokens, heads), dtype=torch.float32) if lse else None
             if tokens:
                 _check(_L().mlxvs_kv_attend_device(
-                    self._ref, ctypes.byref(qs), pb, n, float(scale), longest, out.data_ptr(),
+                    cache, ctypes.byref(qs), pb, n, float(scale), longest, out.data_ptr(),
                     None if sums is None else sums.data_ptr(),
                     None if work is None else work.data_ptr(), size, stream))
         return (out, sums) if lse else out

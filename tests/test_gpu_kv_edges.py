@@ -159,3 +159,30 @@ def test_select_of_more_than_four_million_rows(engine):
     want = kv_oracle.select(f32(q[dev(some)]), codes, scales, table, who[some], positions[some], 16,
                             3, 1, 1)
     assert np.array_equal(got[dev(some)].cpu().numpy(), want)
+
+
+def test_a_cache_keeps_its_tensors(engine):
+    """Other ones are another cache's; memory that has moved is not used."""
+    def make():
+        return engine.PagedKVCache.empty(4, 2, 16, 64)
+
+    kv = torch.ones((3, 2, 64), dtype=torch.bfloat16, device="cuda")
+    slots = torch.arange(3, device="cuda")
+    who = torch.zeros(3, dtype=torch.int32, device="cuda")
+    table = torch.arange(4, dtype=torch.int32, device="cuda")[None]
+    cache = make()
+    for name in ("keys", "values", "summaries", "scales"):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, getattr(cache, name).clone())
+    cache.append(kv, kv, slots)
+    for name, move in (("keys", lambda x: x.resize_(40, 2, 16, 64)),
+                       ("values", lambda x: x.set_(torch.empty_like(x))),
+                       ("summaries", lambda x: x.untyped_storage().resize_(0)),
+                       ("scales", lambda x: x.set_(torch.zeros(1, device="cuda")))):
+        cache = make()
+        cache.append(kv, kv, slots)
+        move(getattr(cache, name))
+        for call in (lambda: cache.append(kv, kv, slots), lambda: cache.select(kv, table, who, who, 2),
+                     lambda: cache.attend(kv, table, who, who)):
+            with pytest.raises(ValueError, match="have moved"):
+                call()
