@@ -111,7 +111,8 @@ class _KvPlan(NamedTuple):
 class KvPlan(_KvPlan):
     """A step's bookkeeping (kv_plan): int32 tensors but ``slots`` (int64)."""
 
-    # (what kv_plan made itself it need not check when it is passed back)
+    # (what kv_plan made itself it need not check when it is passed back, as long
+    # as its memory is where it was)
     made = None
 
 
@@ -145,15 +146,15 @@ def kv_plan(past, new, table, free_pages, cursor, page_size, tokens, *, out=None
             i = past.new_empty
             out = KvPlan(past.new_empty(tokens, dtype=torch.int64), i(tokens), i(tokens),
                          i(requests + 1), i(requests), i(requests), i(1))
-            out.made = (device, requests, tokens, [x.data_ptr() for x in out])
-        elif not isinstance(out, KvPlan):
-            raise ValueError(f"[mlxvs::{op}] out must be a KvPlan.")
-        if out.made is not None and out.made[:3] == (device, requests, tokens):
-            ptrs = out.made[3]
+            ptrs = [x.data_ptr() for x in out]
+            out.made = (device, requests, tokens, ptrs)
         else:
-            sizes = (tokens, tokens, tokens, requests + 1, requests, requests, 1)
-            ptrs = [_ints(x, f"out.{name}", op, device, torch.int32 if i else torch.int64, size)
-                    for i, (x, name, size) in enumerate(zip(out, out._fields, sizes))]
+            _need(isinstance(out, KvPlan), op, "out must be a KvPlan.")
+            ptrs = out.made and [x.data_ptr() for x in out]
+            if ptrs is None or out.made != (device, requests, tokens, ptrs):
+                sizes = (tokens, tokens, tokens, requests + 1, requests, requests, 1)
+                ptrs = [_ints(x, f"out.{name}", op, device, torch.int32 if i else torch.int64, size)
+                        for i, (x, name, size) in enumerate(zip(out, out._fields, sizes))]
         _check(_L().mlxvs_kv_plan_device(pp, pn, requests, pt, stride, table.shape[1], pf,
                                          free_pages.numel(), pc, int(page_size), tokens, *ptrs,
                                          stream))

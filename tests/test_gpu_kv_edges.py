@@ -186,3 +186,30 @@ def test_a_cache_keeps_its_tensors(engine):
                      lambda: cache.attend(kv, table, who, who)):
             with pytest.raises(ValueError, match="have moved"):
                 call()
+
+
+def test_a_plan_whose_tensors_have_moved(engine):
+    one = torch.ones(2, dtype=torch.int32, device="cuda")
+    table = torch.zeros((2, 4), dtype=torch.int32, device="cuda")
+    free, cursor = torch.arange(9, dtype=torch.int32, device="cuda"), torch.zeros_like(one[:1])
+
+    def plan(out=None):
+        return engine.kv_plan(0 * one, one, table, free, cursor, 16, 5, out=out)
+
+    out = plan()
+    assert plan(out) is out and out.slots.tolist() == [0, 16, -1, -1, -1]
+    out.slots.resize_(5000)
+    with pytest.raises(ValueError, match="out.slots"):
+        plan(out)
+    out = plan()
+    out.first.set_(torch.zeros(1, dtype=torch.int32, device="cuda"))
+    with pytest.raises(ValueError, match="out.first"):
+        plan(out)
+    out = plan()
+    other = torch.full((2,), 7, dtype=torch.int32, device="cuda")
+    out.first.set_(other)  # (other memory of the right size is as good)
+    assert plan(out).first.tolist() == [0, 1] and other.tolist() == [0, 1]
+    with pytest.raises(ValueError, match="KvPlan"):
+        plan(tuple(out))
+    with pytest.raises(ValueError, match="out.slots"):
+        plan(engine.KvPlan(*[None] * 7))
