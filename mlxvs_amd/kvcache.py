@@ -11,9 +11,10 @@ a serving loop:
 
 (or ``attend`` without ``blocks``: over everything).  Tensors are on one GPU;
 every call runs on torch's current stream there, returns as soon as its work is
-enqueued and can be captured into a graph.  The work is done by libmlxvs_c.so
-(``mlxvs_kv_*`` in include/mlxvs/mlxvs_c.h); without it the calls raise
-ImportError.  Extensions: the reference has no counterpart.
+enqueued and can be captured into a graph.  The cache serves: no call has a
+gradient.  The work is done by libmlxvs_c.so (``mlxvs_kv_*`` in
+include/mlxvs/mlxvs_c.h); without it the calls raise ImportError.  Extensions:
+the reference has no counterpart.
 """
 
 from __future__ import annotations
@@ -96,6 +97,20 @@ class _On:
     def __exit__(self, *a):
         if self.guard is not None:
             self.guard.__exit__(*a)
+
+
+class _NoGradient(torch.autograd.Function):
+    """Marks results as depending on inputs that want a gradient: asking for it is
+    an error then, not a gradient that is silently missing."""
+
+    @staticmethod
+    def forward(ctx, op, results, *inputs):
+        ctx.op = op
+        return results
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"[mlxvs::{ctx.op}] has no gradient.")
 
 
 class _KvPlan(NamedTuple):
@@ -256,7 +271,8 @@ class PagedKVCache:
     def append(self, k, v, slots) -> None:
         """Write the tokens' keys and values [tokens, kv_heads, dim] into their
         ``slots`` (int64 [tokens]; -1 or outside the cache: skipped), and the
-        summaries of the pages that this completes."""
+        summaries of the pages that this completes.  What is written are values:
+        no gradient goes back to ``k`` and ``v``."""
         op = "kv_append"
         cache = self._cache(op)
         k, pk, ks = self._rows(k, "k", op, self.kv_heads)
@@ -326,10 +342,16 @@ class PagedKVCache:
         scores, 1 / sqrt(dim) by default.  ``longest``: tokens of the longest
         request, if the caller knows it (it guides how work is split, never
         what is computed).  With ``lse`` returns (out, float32 [tokens,
-        q_heads] logarithms of the sums of exponentials)."""
+        q_heads] logarithms of the sums of exponentials).
+
+        It has no gradient: the result of inputs that want one can be used, but
+        not differentiated, and not written into ``out``."""
         op = "kv_attend"
         cache = self._cache(op)
         q, qs = self._queries(q, table, requests, positions, op)
+        keys, values = self._keys, self._values
+        wanted = (q.requires_grad or keys.requires_grad or values.requires_grad) \
+            and torch.is_grad_enabled()
         tokens, heads, dim = q.shape
         n, pb = 0, None
         if blocks is not None:
@@ -348,6 +370,7 @@ class PagedKVCache:
             if out is None:
                 out = q.new_empty((tokens, heads, dim))
             else:
+                _need(not wanted, op, "out takes no result that wants a gradient.")
                 _need(isinstance(out, torch.Tensor) and out.shape == q.shape
                       and out.dtype == q.dtype and out.device == q.device
                       and out.is_contiguous(), op,
@@ -359,4 +382,7 @@ class PagedKVCache:
                     cache, ctypes.byref(qs), pb, n, float(scale), longest, out.data_ptr(),
                     None if sums is None else sums.data_ptr(),
                     None if work is None else work.data_ptr(), size, stream))
+        if wanted:
+            results = _NoGradient.apply(op, (out, sums) if lse else (out,), q, keys, values)
+            return results if lse else results[0]
         return (out, sums) if lse else out

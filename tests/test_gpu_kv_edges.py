@@ -213,3 +213,31 @@ def test_a_plan_whose_tensors_have_moved(engine):
         plan(tuple(out))
     with pytest.raises(ValueError, match="out.slots"):
         plan(engine.KvPlan(*[None] * 7))
+
+
+def test_a_gradient_that_is_asked_for_is_an_error(engine):
+    cache = engine.PagedKVCache.empty(2, 2, 16, 64)
+    cache.keys.normal_()
+    cache.values.normal_()
+    wide = torch.randn((3, 4, 65), device="cuda").bfloat16()
+    table = torch.zeros((1, 2), dtype=torch.int32, device="cuda")
+    who, positions = torch.zeros(3, dtype=torch.int32, device="cuda"), dev([3, 0, -1], torch.int32)
+    for q in (wide[..., :64].contiguous(), wide[..., 1:]):  # (the second is copied by the call)
+        want, sums = cache.attend(q, table, who, positions, lse=True)
+        assert not want.requires_grad and not sums.requires_grad
+        leaf = q.detach().requires_grad_()
+        got, lse = cache.attend(leaf, table, who, positions, lse=True)
+        assert torch.equal(got, want) and torch.equal(lse, sums)
+        for loss in (got.float().sum(), lse[0].sum(), cache.attend(leaf, table, who, positions)[0, 0, 0]):
+            with pytest.raises(RuntimeError, match="kv_attend. has no gradient"):
+                loss.backward()
+        assert leaf.grad is None
+        with pytest.raises(ValueError, match="wants a gradient"):
+            cache.attend(leaf, table, who, positions, out=torch.empty_like(want))
+        with torch.no_grad():
+            out = torch.empty_like(want)
+            assert cache.attend(leaf, table, who, positions, out=out) is out
+            assert not out.requires_grad and torch.equal(out, want)
+        assert not cache.select(leaf, table, who, positions, 2).requires_grad
+    cache.append(wide[:, :2, :64].float().bfloat16().requires_grad_(), wide[:, :2, :64], who.long())
+    assert not cache.keys.requires_grad
