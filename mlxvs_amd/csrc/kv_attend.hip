@@ -1172,6 +1172,13 @@ void kv_attend_plan(KvAttendArgs& a) {
     // in a table for 131,072.)
     const int64_t least = (most * rows / 16384 + 255) / 256 * 256;
     chunk = std::max(least, std::min<int64_t>(chunk, 1024));
+  } else if (!a.n && a.longest == INT32_MAX) {
+    // A single token whose history nobody tells: most of the table may be empty, so
+    // parts of 2,048 keys, unless that makes more than 2,048 parts.  Without / with
+    // it (8 kv heads of 4, 128 values), in a table for 1,048,576 tokens: 777 keys
+    // 20.7 / 24.5 us, 16,000 224 / 67, 131,072 256 / 96, all 627 / 644; for 262,144:
+    // 777 keys 20.9 / 22.0, 16,000 64.5 / 38.1, 131,072 98.6 / 104, all 189 / 191.
+    chunk = std::min(chunk, std::max<int64_t>(2048, most * rows / 2048));
   }
   chunk = std::max<int64_t>(512, std::min<int64_t>(chunk, 1 << 30));
   if (!whole) a.splits = (int)((most + chunk - 1) / chunk);

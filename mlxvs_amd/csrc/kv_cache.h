@@ -89,7 +89,7 @@ struct KvAttendArgs {
   float scale;
   void* out;   // [tokens][heads * group][dim]
   float* lse;  // [tokens][heads * group] or null
-  int64_t longest;  // tokens the longest request is expected to hold
+  int64_t longest;  // tokens the longest request is expected to hold, INT32_MAX: unknown
   // the split, from kv_attend_plan
   int splits;       // parts of a row's keys, joined by a second launch if more than one
   int chunk;        // keys of a part (a multiple of 64; the last part takes the rest)

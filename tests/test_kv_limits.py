@@ -46,3 +46,17 @@ def test_attention_of_many_tokens(engine, tokens, requests, rc):
     q = queries(tokens=tokens, requests=requests, q_heads=32, token_stride=2048)
     lib = engine._L()
     assert attend(lib, cache(heads=8), q) == rc, lib.mlxvs_last_error()
+
+
+@pytest.mark.parametrize("tokens_held,longest,keys", [
+    (1 << 20, 0, 4096),        # a million places: 256 parts of 8 kv heads
+    (1 << 18, 0, 2048),
+    (1 << 20, 1 << 20, 16384),  # the caller says that they are taken
+    (1 << 20, 16_000, 512)])
+def test_parts_of_a_single_token_in_a_wide_table(engine, tokens_held, longest, keys):
+    lib = engine._L()
+    c = cache(heads=8, page_size=64, dim=128)
+    q = queries(tokens=1, q_heads=32, columns=tokens_held // 64, table_stride=tokens_held // 64)
+    size = lib.mlxvs_kv_attend_workspace(ctypes.byref(c), ctypes.byref(q), 0, longest)
+    parts = -(-(min(tokens_held, longest) if longest else tokens_held) // keys)
+    assert size == 32 * parts * (128 + 2) * 4
