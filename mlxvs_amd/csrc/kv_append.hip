@@ -13,15 +13,13 @@
 // in 127ths of the largest sum: int8 codes, with the scale that makes code x
 // scale the mean key.  Sums of whole numbers are the same in every order, so
 // codes do not depend on how a page was filled or on how a kernel adds.
-#include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
 #include "kv_cache.h"
+#include "kv_values.h"
 
 namespace mlxvs::kern {
 namespace {
-
-typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 
 // Valid slots name a page of the cache; others are skipped.
 __device__ __forceinline__ bool in_cache(const KvCache& c, int64_t slot) {
@@ -29,29 +27,6 @@ __device__ __forceinline__ bool in_cache(const KvCache& c, int64_t slot) {
 }
 __device__ __forceinline__ bool completes(const KvCache& c, int64_t slot) {
   return in_cache(c, slot) && (slot & (c.page - 1)) == c.page - 1;
-}
-
-template <bool BF16>
-__device__ __forceinline__ float value(uint16_t x) {
-  if constexpr (BF16) return __builtin_bit_cast(float, (uint32_t)x << 16);
-  else return (float)__builtin_bit_cast(_Float16, x);
-}
-template <bool BF16>
-__device__ __forceinline__ float value(const uintx4& v, int j) {
-  return value<BF16>((uint16_t)(v[j / 2] >> (16 * (j & 1))));
-}
-
-template <int THREADS>
-__device__ __forceinline__ float block_max(float x, float* shared) {
-#pragma unroll
-  for (int i = 32; i >= 1; i >>= 1) x = fmaxf(x, __shfl_xor(x, i));
-  if constexpr (THREADS == 64) return x;
-  if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = x;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < THREADS / 64; ++i) x = fmaxf(x, shared[i]);
-  __syncthreads();
-  return x;
 }
 
 struct Sums {

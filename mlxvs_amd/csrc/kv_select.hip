@@ -12,28 +12,21 @@
 //
 // Ranks are 32-bit keys in the scores' order: 0 for no candidate, all ones for
 // a block that is always taken.
-#include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <cfloat>
 
 #include "kv_cache.h"
+#include "kv_values.h"
 
 namespace mlxvs::kern {
 namespace {
 
-typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
 
 constexpr uint32_t kAlways = 0xFFFFFFFFu;
 constexpr int kLdsCols = 8192;  // ranks of a row that stay in LDS (32 KB)
-
-template <bool BF16>
-__device__ __forceinline__ float value(uint16_t x) {
-  if constexpr (BF16) return __builtin_bit_cast(float, (uint32_t)x << 16);
-  else return (float)__builtin_bit_cast(_Float16, x);
-}
 
 // Bits set, signed: counts are subtracted and compared.
 __device__ __forceinline__ int bits(uint64_t x) { return (int)__popcll(x); }
@@ -54,19 +47,6 @@ __device__ __forceinline__ float finite_abs(float x) {
 // The factor that takes values of at most `top` to codes, 0 where there is none.
 __device__ __forceinline__ float to_codes(float top) {
   return top > 1e-30f && top < __builtin_inff() ? 127.0f / top : 0.0f;
-}
-
-template <int THREADS>
-__device__ __forceinline__ float block_max(float x, float* shared) {
-#pragma unroll
-  for (int i = 32; i >= 1; i >>= 1) x = fmaxf(x, __shfl_xor(x, i));
-  if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = x;
-  __syncthreads();
-  float y = shared[0];
-#pragma unroll
-  for (int i = 1; i < THREADS / 64; ++i) y = fmaxf(y, shared[i]);
-  __syncthreads();
-  return y;
 }
 
 // The codes of a (token, head)'s query, zeros past dim.  A query that holds
@@ -103,12 +83,6 @@ __device__ __forceinline__ intx4 mfma_i8(uintx4 x, uintx4 y, intx4 c) {
 #else
   return c;
 #endif
-}
-
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int i = 32; i >= 1; i >>= 1) x = fmaxf(x, __shfl_xor(x, i));
-  return x;
 }
 
 // query_codes of a wavefront's tokens t0, t0 + step, ..: two neighbouring values
