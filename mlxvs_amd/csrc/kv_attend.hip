@@ -373,6 +373,24 @@ __host__ __device__ __forceinline__ Sharing sharing(int group, int n) {
   return {tokens < most ? tokens : most, 1};
 }
 
+// Calls of both kernels (KvAttendArgs::mixed): a span of neighbouring tokens, as many
+// as a workgroup of shared wavefronts takes, is a prompt's if one request has its
+// first and its last; if the call has at least `least` such spans, their tokens share
+// wavefronts and the others do not.  Whether token t (the same for the workgroup's
+// 256 threads) is one of them; every kernel of the call finds the same.
+__device__ __forceinline__ bool in_prompt(const KvAttendArgs& a, int64_t t) {
+  const int64_t spans = a.q.tokens / a.span, mine = t / a.span;
+  const auto of_one = [&](int64_t s) {
+    const int32_t* r = a.q.token_request + s * a.span;
+    return r[0] >= 0 && r[0] == r[a.span - 1];
+  };
+  if (mine >= spans || !of_one(mine)) return false;
+  int64_t found = 0;
+  for (int64_t s = 0; s < spans && found < a.least; s += 256)
+    found += __syncthreads_count(s + threadIdx.x < spans && of_one(s + threadIdx.x));
+  return found >= a.least;
+}
+
 // 16 bytes a lane from `from` to lds + 16 lane.
 __device__ __forceinline__ void copy16_to_lds(const void* from, void* lds) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -832,6 +850,7 @@ void kv_attend_shared_kernel(KvAttendArgs a) {
   const Sharing share = sharing(group, a.n);
   // wavefronts go through the head tiles of a set of tokens, then to the next
   const int h = (int)(blockIdx.x % a.c.heads);
+  if (a.mixed && !in_prompt(a, (int64_t)(blockIdx.x / a.c.heads) * a.span)) return;
   A w(a, sh, h);
   const int lane = w.lane;
   const int64_t unit = (int64_t)(blockIdx.x / a.c.heads) * kSharedWaves + w.wave;
@@ -951,6 +970,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_parts_kernel(KvAttendArgs a)
   b /= a.c.heads;
   const int64_t t = b % a.q.tokens;
   const int part = (int)(b / a.q.tokens);
+  if (a.mixed && in_prompt(a, t)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   A w(a, threadIdx.x & 63);
   const int r = a.q.token_request[t], pos = position(a, t);
@@ -1024,6 +1044,7 @@ __global__ __launch_bounds__(256) void kv_attend_join_kernel(KvAttendArgs a) {
   __shared__ float ss[256], sm[4];
   const int tid = threadIdx.x;
   const int64_t at = blockIdx.x;  // (token, query head)
+  if (a.mixed && in_prompt(a, at / (a.c.heads * a.q.group))) return;
   const float c = a.scale * kLog2e;
   const float* ml = a.part_ml + 2 * at * a.splits;
   float top = -__builtin_inff();
@@ -1079,20 +1100,20 @@ void launch_parts(const KvAttendArgs& a, hipStream_t s) {
 
 template <int DP, bool BF16, bool LIST>
 void launch_listed(const KvAttendArgs& a, hipStream_t s) {
-  if (a.shared) {
-    const dim3 grid((unsigned)shared_grid(a));
-    constexpr int kThreads = 64 * kSharedWaves;
-    constexpr int kKeys = tile_keys(DP);
-    if (a.c.page == 16)
-      kv_attend_shared_kernel<DP, BF16, LIST, 16><<<grid, kThreads, 0, s>>>(a);
-    else if (kKeys > 32 && a.c.page == 32)
-      kv_attend_shared_kernel<DP, BF16, LIST, 32><<<grid, kThreads, 0, s>>>(a);
-    else
-      kv_attend_shared_kernel<DP, BF16, LIST, kKeys><<<grid, kThreads, 0, s>>>(a);
-    return;
+  if (!a.shared) {
+    if (a.c.page == 16) launch_parts<DP, BF16, LIST, true>(a, s);
+    else launch_parts<DP, BF16, LIST, false>(a, s);
   }
-  if (a.c.page == 16) launch_parts<DP, BF16, LIST, true>(a, s);
-  else launch_parts<DP, BF16, LIST, false>(a, s);
+  if (!a.shared && !a.mixed) return;
+  const dim3 grid((unsigned)shared_grid(a));
+  constexpr int kThreads = 64 * kSharedWaves;
+  constexpr int kKeys = tile_keys(DP);
+  if (a.c.page == 16)
+    kv_attend_shared_kernel<DP, BF16, LIST, 16><<<grid, kThreads, 0, s>>>(a);
+  else if (kKeys > 32 && a.c.page == 32)
+    kv_attend_shared_kernel<DP, BF16, LIST, 32><<<grid, kThreads, 0, s>>>(a);
+  else
+    kv_attend_shared_kernel<DP, BF16, LIST, kKeys><<<grid, kThreads, 0, s>>>(a);
 }
 
 template <int DP, bool BF16>
@@ -1122,18 +1143,43 @@ void launch_type(const KvAttendArgs& a, hipStream_t s) {
 //   kv head), 128 requests of 4 252 / 236; 128 of 2 149 / 189 (8 heads);
 //   lists of 64 of 1,024 blocks of 16: one request of 256 81 / 101;
 //   256 values, 4,096 keys: one request of 64 tokens 234 / 198, of 128 456 / 202.
-bool shares(const KvAttendArgs& a, int64_t rows) {
-  const int64_t each = a.q.tokens / std::max<int64_t>(1, a.q.requests);
-  if (each < 3) return false;
-  const Sharing sh = sharing(a.q.group, a.n);
-  const int64_t tokens = std::max(1, sh.tokens * kSharedWaves / sh.tiles);  // of a workgroup
+//
+// The cost of a workgroup's walk for `tokens` tokens, `each` to a request, in those
+// figures' measure.
+int64_t cost_of_walk(const KvAttendArgs& a, int64_t tokens, int64_t each) {
   int64_t walks = 1 + (tokens - 1) / each;  // requests, each its keys or the union of
   if (a.n) {                                // some lists, which overlap
     const int64_t lists = std::min(tokens, each), apart = std::max(1, a.q.cols / a.n);
     walks *= std::max<int64_t>(1, lists * apart / (lists + apart));
     if (a.c.page == 16) walks *= 2;
   }
-  return rows * 384 >= (a.n ? 220 : 480) * walks * std::max<int64_t>(384, shared_grid(a));
+  return (a.n ? 220 : 480) * walks;
+}
+
+bool shares(const KvAttendArgs& a, int64_t rows) {
+  const int64_t each = a.q.tokens / std::max<int64_t>(1, a.q.requests);
+  if (each < 3) return false;
+  const Sharing sh = sharing(a.q.group, a.n);
+  const int64_t tokens = std::max(1, sh.tokens * kSharedWaves / sh.tiles);  // of a workgroup
+  return rows * 384 >= cost_of_walk(a, tokens, each) * std::max<int64_t>(384, shared_grid(a));
+}
+
+// Whether both kernels run: a call of fewer than three tokens a row of the table may
+// still hold a prompt, the other rows being idle or having a token each, which the
+// device finds (in_prompt).  One kernel / both, 4,096 keys, 256 rows (8 kv heads of 4,
+// 128 values): one row with 512 tokens, the others idle 874 / 162 us (3,523 / 425 over
+// 16,384 keys), with a token each 1,551 / 856, 128 tokens so 913 / 825, 16 706 / 713;
+// no prompt 690 / 697 and 330 / 331 for 128 rows, which is what the second launch and
+// the workgroups that find nothing cost.  So it is made where rows by themselves
+// take 0.45 ms; lists: 512 tokens and 500 single ones of 32 blocks 1,118 / 802, none
+// and 1,024 of 16 695 / 696.
+void mix(KvAttendArgs& a, int64_t rows, int64_t most) {
+  const Sharing sh = sharing(a.q.group, a.n);
+  if (sh.tiles > 1 || rows * most < 8 << 20) return;
+  a.span = sh.tokens * kSharedWaves;
+  const int64_t cost = cost_of_walk(a, a.span, a.span), per = (int64_t)a.span * a.c.heads;
+  a.least = (int)((cost + per - 1) / per);
+  a.mixed = a.span * 384 >= cost && a.q.tokens / a.span >= a.least;
 }
 
 }  // namespace
@@ -1145,7 +1191,7 @@ void kv_attend_plan(KvAttendArgs& a) {
                                 : std::min<int64_t>(a.longest, (int64_t)a.q.cols << a.c.lps);
   a.splits = 1;
   a.chunk = 64;
-  a.shared = false;
+  a.shared = a.mixed = false;
   if (rows == 0) return;
   if (shares(a, rows)) {
     a.shared = true;
@@ -1183,6 +1229,7 @@ void kv_attend_plan(KvAttendArgs& a) {
   chunk = std::max<int64_t>(512, std::min<int64_t>(chunk, 1 << 30));
   if (!whole) a.splits = (int)((most + chunk - 1) / chunk);
   a.chunk = whole ? 1 << 30 : (int)chunk;
+  mix(a, rows, most);
 }
 
 int64_t kv_attend_workspace(const KvAttendArgs& a) {
@@ -1193,7 +1240,8 @@ int64_t kv_attend_workspace(const KvAttendArgs& a) {
 int64_t kv_attend_grid(const KvAttendArgs& a) {
   if (a.shared) return shared_grid(a);
   const int64_t rows = a.q.tokens * a.c.heads * ((a.q.group + kColumns - 1) / kColumns);
-  return a.splits > 1 ? std::max(a.q.tokens * a.c.heads * a.q.group, rows * a.splits) : rows;
+  const int64_t join = a.splits > 1 ? a.q.tokens * a.c.heads * a.q.group : 0;
+  return std::max({rows * a.splits, join, a.mixed ? shared_grid(a) : 0});
 }
 
 hipError_t launch_kv_attend(const KvAttendArgs& a, hipStream_t s) {

@@ -94,10 +94,12 @@ struct KvAttendArgs {
   int splits;       // parts of a row's keys, joined by a second launch if more than one
   int chunk;        // keys of a part (a multiple of 64; the last part takes the rest)
   bool shared;      // neighbouring tokens share wavefronts (no parts)
+  bool mixed;       // those of prompts do, the others have parts: as the device finds them,
+  int span, least;  // by spans of so many tokens, if at least so many are a prompt's
   float* part_o;    // [tokens][heads][group][splits][dim]
   float* part_ml;   // [tokens][heads][group][splits][2]
 };
-void kv_attend_plan(KvAttendArgs& a);  // sets shared, splits and chunk
+void kv_attend_plan(KvAttendArgs& a);  // sets the split
 int64_t kv_attend_workspace(const KvAttendArgs& a);
 int64_t kv_attend_grid(const KvAttendArgs& a);  // workgroups of its largest launch
 hipError_t launch_kv_attend(const KvAttendArgs& a, hipStream_t s);

@@ -101,6 +101,18 @@ def test_values_that_are_not_finite_reach_who_sees_them(engine, heads, group, pa
     assert np.array_equal(got, want, equal_nan=True)
 
 
+def best_time(call, n=4):
+    times = []
+    for _ in range(n):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        call()
+        b.record()
+        b.synchronize()
+        times.append(a.elapsed_time(b))
+    return min(times)
+
+
 def test_what_one_infinite_value_costs(engine):
     """A second round over a workgroup's tiles, not one for each of its tokens."""
     rng = np.random.default_rng(4)
@@ -111,15 +123,7 @@ def test_what_one_infinite_value_costs(engine):
     positions = dev(np.arange(tokens) + cols * page - tokens, torch.int32)
 
     def spent():
-        times = []
-        for _ in range(4):
-            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
-            a.record()
-            cache.attend(q, table, who, positions)
-            b.record()
-            b.synchronize()
-            times.append(a.elapsed_time(b))
-        return min(times)
+        return best_time(lambda: cache.attend(q, table, who, positions))
 
     clean = spent()
     cache.values[0, :, 3, 5] = float("inf")
@@ -241,3 +245,47 @@ def test_a_gradient_that_is_asked_for_is_an_error(engine):
         assert not cache.select(leaf, table, who, positions, 2).requires_grad
     cache.append(wide[:, :2, :64].float().bfloat16().requires_grad_(), wide[:, :2, :64], who.long())
     assert not cache.keys.requires_grad
+
+
+@pytest.mark.parametrize("listed", [False, True])
+@pytest.mark.parametrize("heads,group,page,dim", [(8, 4, 64, 64), (16, 5, 16, 40), (8, 16, 32, 128),
+                                                  (16, 1, 256, 24)])
+def test_prompts_among_single_tokens(engine, heads, group, page, dim, listed):
+    """Tokens of a few prompts and of many requests with one, in a table with idle
+    rows: the prompts start and end within spans of tokens that share a workgroup."""
+    rng = np.random.default_rng(heads * group + page)
+    requests, cols = 300, -(-4096 // page)
+    cache = make_cache(engine, 80, heads, page, dim, "bf16", rng)
+    table = rng.integers(0, 80, (requests, cols)).astype(np.int32)
+    new = np.ones(requests, int)
+    new[150:] = 0
+    new[[7, 60, 149]] = 121, 203, 70
+    held = rng.integers(1, 330, requests)
+    held[[7, 60, 149]] += 200
+    who = np.repeat(np.arange(requests), new)
+    positions = np.concatenate([np.arange(h - n, h) for h, n in zip(held, new)])
+    who, positions = np.r_[who, -1, -1, 5], np.r_[positions, -1, -1, 9]
+    tokens = len(who)
+    q = dev(rng.standard_normal((tokens, heads * group, dim), np.float32)).bfloat16()
+    blocks = rng.integers(-1, 330 // page + 2, (tokens, heads, 4)) if listed else None
+    check_attend(cache, "bf16", q, table, who, positions, blocks=blocks)
+
+
+@pytest.mark.parametrize("rows", [256, 512])
+def test_a_prompt_in_a_table_with_idle_rows(engine, rows):
+    """Takes not much longer than alone, its tokens sharing wavefronts there too."""
+    rng = np.random.default_rng(5)
+    cache = make_cache(engine, 64, 8, 64, 128, "bf16", rng)
+    tokens = 512
+    q = dev(rng.standard_normal((tokens, 32, 128), np.float32)).bfloat16()
+    table = dev(rng.permutation(64)[None], torch.int32)
+    tall = torch.full((rows, 64), -1, dtype=torch.int32, device="cuda")
+    tall[rows // 2] = table
+    who = torch.zeros(tokens, dtype=torch.int32, device="cuda")
+    positions = dev(np.arange(tokens) + 4096 - tokens, torch.int32)
+    alone = cache.attend(q, table, who, positions)
+    assert torch.equal(cache.attend(q, tall, who + rows // 2, positions), alone)
+    there = who + rows // 2
+    # (measured: 162 and 100 us; every token by itself 874)
+    assert best_time(lambda: cache.attend(q, tall, there, positions)) \
+        < 3 * best_time(lambda: cache.attend(q, table, who, positions))
