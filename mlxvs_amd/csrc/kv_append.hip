@@ -5,8 +5,9 @@
 // within a page, through LDS: neighbouring lanes store neighbouring tokens, so
 // that a prompt's stores cover whole sectors (16-byte stores of 8 tokens' values
 // are slower: 22.7 us, not 20.7, for 4,001 tokens of 5 requests, 4 kv heads of 80
-// values).  It moves bytes: 277,688 tokens of 8 x 128 values take 0.6 ms and 0.33
-// for the summaries, 3.7 and 1.7 TB/s; small calls are one launch, 6.8 us.
+// values).  It moves bytes: 277,688 tokens of 8 x 128 values take 0.59 ms and 0.33
+// for the summaries, 3.9 and 1.7 TB/s (the keys are read for their largest, and again
+// for the sums); small calls are one launch, 6.8 us.
 //
 // A page's summary (a page and head): each key value over the largest of the
 // page in 127ths, rounded to a whole number; their sums over the page; the sums

@@ -7,7 +7,8 @@
 // sum.  The G query heads of a kv head are the 16 columns of the products:
 // S^T = K Q^T and O^T = V^T P^T, both on the 16x16x32 MFMA (bf16 / f16 in,
 // float32 out).  With values transposed within a page, K rows and V^T rows are
-// 16-byte loads in the A operand's own layout, so nothing goes through LDS; and
+// 16-byte loads in the A operand's own layout: a single token's go from the cache
+// straight into registers (those of prompts, which share them, through LDS); and
 // S^T comes out with its keys along the registers.  The keys of a 32-key pair
 // of S tiles are dealt to the tiles' rows so that a lane ends up with 8
 // consecutive keys (row m of tile t is key 8 (m / 4) + 4 t + m % 4): exactly
@@ -15,12 +16,15 @@
 // registers too, and the V^T loads stay 16 bytes wide.
 //
 // P is rounded to the cache's type for the second product (the values' own
-// precision; a sum of roundings that averages out), its sum is not; under f16
-// P is scaled up so that small terms of long sums stay normal numbers.
+// precision; a sum of roundings that averages out: error against 64 bits 2.0e-3 of
+// an output's norm in bf16 and 2.5e-4 in f16, where the output's own rounding makes
+// 1.7e-3 and 2.1e-4), its sum is not; under f16 P is scaled up, by 2^14 or, for
+// prompts, 2^7, so that small terms of long sums stay normal numbers.
 // Scores, maxima, sums and the output are float32.
 //
 // Single tokens are bound by HBM: 64 ragged requests of up to 8,192 tokens (8 kv
-// heads of 4, 128 values) 247 us, 4.9 TB/s; one of 262,144 188 us, 5.7 TB/s.
+// heads of 4, 128 values) 247 us, 4.9 TB/s; one of 262,144 188 us, 5.7 TB/s (a large
+// read alone: 6.3 TB/s with plain loads).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -339,15 +343,20 @@ __device__ __forceinline__ int row_max(int x) {
 // 2.2 GB in 322 us, the same rate).  So tiles of keys and values go to LDS by
 // direct loads of neighbouring chunks, a tile ahead of the products, and the
 // operands come from there, in chunks that are swapped by row so that 8 lanes
-// read from 8 different sets of banks: 246 us.  Of a tile of 64 keys that is now
-// about 1 us for its products and weights (two wavefronts a SIMD, their chain of
-// scores, maxima, exponentials and sums not hidden by one another), 0.4 us for
-// issuing its copy, 0.5 us at its barrier.  Without lists every wavefront uses
-// every tile: 4,096 tokens of 8,192 keys (8 kv heads of 4, 128 values) 684 us, 603
-// TFLOP/s; there LDS bounds it: every MFMA (16 cycles of a SIMD) takes an operand
-// of 1 KB, about 10 cycles of the reads that four SIMDs share.  (32 columns a
-// wavefront would halve that, but need more registers than two wavefronts a SIMD
-// have.)
+// read from 8 different sets of banks: 246 us.  What bounds it now is the number of
+// tiles and the time of each: a workgroup of 8 tokens walks 30 blocks, the union of
+// their lists of 16, of which a wavefront uses two thirds; that makes 88 tiles of 64
+// keys one after another for each of the 512 workgroups that run at a time, 2.8 us a
+// tile, of which products and weights are about 1 us (two wavefronts a SIMD, their
+// chain of scores, maxima, exponentials and sums not hidden by one another), the
+// rest is waiting for the copy, with one tile ahead, and the barrier.
+//
+// Without lists every wavefront uses every tile: 4,096 tokens of 8,192 keys (8 kv
+// heads of 4, 128 values) 690 us, 600 TFLOP/s.  Operands from LDS, 1 KB and about 10
+// cycles each of what four SIMDs share, for an MFMA of 16 cycles, would allow 1,000;
+// 6.7 vector instructions an MFMA, in that chain, make the rest.  (32 columns a
+// wavefront need more registers than two wavefronts a SIMD have; 192 values over
+// lists spill 6 to 10 as it is.)
 //
 // Lists in any order are right: one that does not ascend is sorted first, and a
 // block listed twice counts twice.

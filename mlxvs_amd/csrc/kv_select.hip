@@ -594,6 +594,10 @@ __global__ __launch_bounds__(512) void kv_select_tile_kernel(KvSelectArgs a) {
 //   LDS holds): by row / in two launches, 128 rows 21.0 / 18.6 us at 2,048 columns,
 //   31.5 / 26.0 at 4,096; 8 rows 14.4 / 16.6 at 1,024; 256 rows 22.3 / 24.1 at
 //   2,048, 31.8 / 37.1 at 4,096.
+// Beyond kTileCols columns prompts go by rows too, each reading its summaries again:
+// 1,500 tokens of 8 heads 99 us at 2,048 columns, 490 at 2,049, 1,725 at 8,192.  "Many"
+// tokens go by the table's height, idle rows included: 512 tokens of 8 heads over 512
+// columns 17 us, 64 in a table of 256 rows.
 // What bounds small calls is a chain of five dependent accesses, about 10 us
 // whatever the size; large ones, the listing (32 counts of a row's ranks).
 enum class Way { kRow, kParts, kTile };

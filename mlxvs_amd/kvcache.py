@@ -344,6 +344,10 @@ class PagedKVCache:
         what is computed).  With ``lse`` returns (out, float32 [tokens,
         q_heads] logarithms of the sums of exponentials).
 
+        Neighbouring tokens of one request (kv_plan's order) are done together.
+        A single token with a very long history is best given in a call of its
+        own (slices of the same tensors) when the others are prompts.
+
         It has no gradient: the result of inputs that want one can be used, but
         not differentiated, and not written into ``out``."""
         op = "kv_attend"
