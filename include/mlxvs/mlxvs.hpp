@@ -309,6 +309,81 @@ MLXVS_API void kv_attend_device(const KvCache& cache, const KvQueries& queries,
 MLXVS_API int64_t kv_attend_workspace(const KvCache& cache, const KvQueries& queries, int n,
                                       int64_t longest);
 
+/** How the frequencies of positions are scaled, as mlxvs_kv_rotary_scaling. */
+enum class KvScaling { None = 0, Linear = 1, Base = 2, Ramp = 3 };
+/** Which values of a head are turned together, as mlxvs_kv_rotary_layout. */
+enum class KvRotaryLayout { Halves = 0, Pairs = 1 };
+/** Type of a norm's weights, as mlxvs_kv_norm. */
+enum class KvNorm { Own = 0, Float32 = 1 };
+
+/** Positions as rotations, as mlxvs_kv_rotary. */
+struct KvRotary {
+  const uint64_t* turns = nullptr;
+  int32_t dim = 0;
+  int32_t rotated = 0;
+  KvRotaryLayout layout = KvRotaryLayout::Halves;
+  float magnitude = 1.0f;
+  KvType type = KvType::Float16;
+};
+
+/** Heads of tokens to be rotated, as mlxvs_kv_heads. */
+struct KvHeads {
+  const void* x = nullptr;
+  int64_t token_stride = 0;
+  int64_t head_stride = 0;
+  int32_t heads = 0;
+  const void* norm = nullptr;
+  KvNorm norm_type = KvNorm::Own;
+  void* out = nullptr;
+  int64_t out_token_stride = 0;
+  int64_t out_head_stride = 0;
+};
+
+/** What kv_compact_device reads and writes, as mlxvs_kv_compact_device's
+ * arguments. */
+struct KvCompact {
+  const int32_t* table = nullptr;
+  int64_t table_stride = 0;
+  int32_t columns = 0;
+  int64_t requests = 0;
+  const int32_t* lengths = nullptr;
+  const int32_t* kept = nullptr;
+  int32_t n = 0;
+  int32_t* free_pages = nullptr;
+  int64_t free_count = 0;
+  const int32_t* cursor = nullptr;
+  float* mass = nullptr;
+  int64_t slots = 0;
+  int32_t* lengths_out = nullptr;
+  int32_t* cursor_out = nullptr;
+};
+
+/** Radians a position of each pair (mlxvs_kv_rotary_frequencies); on the host. */
+MLXVS_API void kv_rotary_frequencies(int32_t rotated, double base, KvScaling scaling,
+                                     double factor, double context, double* frequencies,
+                                     float* magnitude);
+/** Radians a position as KvRotary::turns (mlxvs_kv_rotary_turns); on the host. */
+MLXVS_API void kv_rotary_turns(const double* frequencies, int32_t n, uint64_t* turns);
+/** Queries and keys normed and rotated (mlxvs_kv_rotate_device); enqueues only. */
+MLXVS_API void kv_rotate_device(const KvRotary& rotary, const KvHeads& q, const KvHeads& k,
+                                int64_t tokens, const int32_t* positions,
+                                const int32_t* token_request, const int32_t* evicted,
+                                int64_t requests, float eps, void* stream = nullptr);
+/** The attention that each cached key gets (mlxvs_kv_weigh_device); enqueues
+ * only. */
+MLXVS_API void kv_weigh_device(const KvCache& cache, const KvQueries& queries,
+                               const int32_t* starts, const float* lse, float scale, float decay,
+                               int64_t longest, float* mass, int64_t slots,
+                               void* stream = nullptr);
+/** The tokens that a budget leaves (mlxvs_kv_keep_device); enqueues only. */
+MLXVS_API void kv_keep_device(const float* mass, int64_t requests, int32_t heads, int64_t slots,
+                              const int32_t* lengths, int32_t n, int32_t first, int32_t recent,
+                              int32_t above, int32_t* kept, void* stream = nullptr);
+/** Requests cut to those tokens (mlxvs_kv_compact_device); enqueues only. */
+MLXVS_API void kv_compact_device(const KvCache& cache, const KvCompact& compact, void* workspace,
+                                 int64_t workspace_bytes, void* stream = nullptr);
+MLXVS_API int64_t kv_compact_workspace(const KvCache& cache, const KvCompact& compact);
+
 /** Frees the per-device workspace kept between calls. */
 MLXVS_API void release_workspace();
 

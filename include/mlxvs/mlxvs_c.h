@@ -480,8 +480,11 @@ MLXVS_C_API int mlxvs_pairwise_knn(
  * lengths (mlxvs_kv_plan_device), the write of its tokens
  * (mlxvs_kv_append_device), the blocks that a cheap score selects for each of
  * them (mlxvs_kv_select_device) and their attention, over every block or the
- * selected ones (mlxvs_kv_attend_device).  All arrays are device memory; the
- * calls enqueue their work on `stream`, allocate nothing, keep nothing and can
+ * selected ones (mlxvs_kv_attend_device).  Queries and keys get their positions
+ * from mlxvs_kv_rotate_device; a budget is kept by the attention that each key got
+ * (mlxvs_kv_weigh_device), the tokens that have most of it
+ * (mlxvs_kv_keep_device), and a cut to those (mlxvs_kv_compact_device).  All
+ * arrays are device memory; the calls enqueue their work on `stream`, allocate nothing, keep nothing and can
  * be captured into graphs.  Calls that depend on one another go to one stream
  * or are ordered by the caller; a workspace serves one call at a time.
  */
@@ -656,6 +659,154 @@ MLXVS_C_API int64_t mlxvs_kv_attend_workspace(const mlxvs_kv_cache* cache,
                                               const mlxvs_kv_queries* queries, int32_t n,
                                               int64_t longest);
 
+/** Which values of a head are turned together: the first half of the rotated
+ * ones with the second, or neighbours. */
+typedef enum {
+  MLXVS_KV_HALVES = 0, /* (x[i], x[i + rotated / 2]) */
+  MLXVS_KV_PAIRS = 1,  /* (x[2 i], x[2 i + 1]) */
+} mlxvs_kv_rotary_layout;
+
+/** How the frequencies of positions are scaled for texts `factor` times as long as
+ * those (of `context` tokens) that a model learnt on. */
+typedef enum {
+  MLXVS_KV_SCALING_NONE = 0,   /* f_i = base^(-2 i / rotated) */
+  MLXVS_KV_SCALING_LINEAR = 1, /* f_i / factor */
+  MLXVS_KV_SCALING_BASE = 2,   /* base x factor^(rotated / (rotated - 2)) for base */
+  /* f_i where it makes 32 turns or more over the context, f_i / factor where it
+   * makes one or less, between them a straight line in the turns; rotated values by
+   * 0.1 ln(factor) + 1 (Peng et al. 2023, YaRN) */
+  MLXVS_KV_SCALING_RAMP = 3,
+} mlxvs_kv_rotary_scaling;
+
+/**
+ * Radians a position of each pair of rotated values, frequencies [rotated / 2], and
+ * the factor of the rotated values, magnitude[0].  On the host, no GPU needed.
+ */
+MLXVS_C_API int mlxvs_kv_rotary_frequencies(int32_t rotated, double base,
+                                            mlxvs_kv_rotary_scaling scaling, double factor,
+                                            double context, double* frequencies,
+                                            float* magnitude);
+
+/** n radians a position as turns a position in 2^-64 of a turn (whole turns
+ * left out), for mlxvs_kv_rotary.  On the host, no GPU needed. */
+MLXVS_C_API int mlxvs_kv_rotary_turns(const double* frequencies, int32_t n, uint64_t* turns);
+
+/**
+ * Positions as rotations of heads of `dim` values (a multiple of 8, at most 256):
+ * their first `rotated` ones (even, at most dim) are turned, the others pass.
+ * turns [rotated / 2] in device memory, from mlxvs_kv_rotary_turns.
+ */
+typedef struct {
+  const uint64_t* turns;
+  int32_t dim;
+  int32_t rotated;
+  mlxvs_kv_rotary_layout layout;
+  float magnitude;
+  mlxvs_kv_type type; /* of the heads */
+} mlxvs_kv_rotary;
+
+/** Type of a norm's weights. */
+typedef enum {
+  MLXVS_KV_NORM_OWN = 0, /* the heads' own */
+  MLXVS_KV_NORM_F32 = 1,
+} mlxvs_kv_norm;
+
+/**
+ * Heads of tokens: x [tokens][heads][dim] and the place of their results, strides
+ * in values (multiples of 8; 16-byte aligned).  `out` may be x, with its strides;
+ * else the results may overlap nothing that the call reads.  norm [dim]: weights of
+ * a norm before the rotation, x rsqrt(mean(x^2) + eps) norm over the whole head;
+ * null: none.  heads 0: nothing.
+ */
+typedef struct {
+  const void* x;
+  int64_t token_stride;
+  int64_t head_stride;
+  int32_t heads;
+  const void* norm;
+  mlxvs_kv_norm norm_type;
+  void* out;
+  int64_t out_token_stride;
+  int64_t out_head_stride;
+} mlxvs_kv_heads;
+
+/**
+ * Queries and keys (either may be null) normed and rotated by positions int32
+ * [tokens].  With evicted int32 [requests], a token's position in its text is
+ * positions[t] + evicted[token_request[t]]: what its request's cache has lost
+ * (mlxvs_kv_compact_device) still counts (a request out of range: nothing).  A
+ * token with a negative position is not turned.  Computed in float32 and rounded
+ * once; angles are exact to 2^-32 of a turn at every position.
+ */
+MLXVS_C_API int mlxvs_kv_rotate_device(const mlxvs_kv_rotary* rotary, const mlxvs_kv_heads* q,
+                                       const mlxvs_kv_heads* k, int64_t tokens,
+                                       const int32_t* positions, const int32_t* token_request,
+                                       const int32_t* evicted, int64_t requests, float eps,
+                                       void* stream);
+
+/**
+ * The attention that each key gets from the step's tokens, added to what it got
+ * before: mass float32 [requests][heads][slots], slots >= columns x page_size.  The
+ * tokens of request r (a row of queries->table) are starts[r] .. starts[r + 1] - 1
+ * (int32 [requests + 1], as mlxvs_kv_plan_device makes them), their positions
+ * ascending; queries->token_request is not read and may be null.  lse float32
+ * [tokens][q_heads]: what mlxvs_kv_attend_device over every block returned for
+ * the same queries and scale.  For the positions p up to the last token's
+ *   mass[p] = (p < first ? decay x mass[p] : 0) + the sum over the tokens that see p
+ *             and the head's query heads of exp(scale x q.k_p - lse),
+ * first being the first token's position: the step's own keys start from zero.  The
+ * others, and requests without tokens (or with position -1), stay as they are; a
+ * key of an absent page gets nothing.  decay in [0, 1]; with 0 masses are not read.
+ * A page that several rows share has a mass in each.  longest guides how work is
+ * split, as in mlxvs_kv_attend_device.  The same bits every time.
+ */
+MLXVS_C_API int mlxvs_kv_weigh_device(const mlxvs_kv_cache* cache,
+                                      const mlxvs_kv_queries* queries, const int32_t* starts,
+                                      const float* lse, float scale, float decay,
+                                      int64_t longest, float* mass, int64_t slots, void* stream);
+
+/**
+ * The tokens that a budget of n leaves: kept int32 [requests][heads][n], ascending.
+ * Request r holds lengths[r] tokens (at most slots count).  Of more than `above`
+ * (>= n) its first `first` and last `recent` (first + recent <= n) are kept, and of
+ * the others those of the largest mass, the lowest among equal ones; NaN counts
+ * as less than any other.  A request of at most `above` keeps all: its list is -1
+ * throughout.
+ */
+MLXVS_C_API int mlxvs_kv_keep_device(const float* mass, int64_t requests, int32_t heads,
+                                     int64_t slots, const int32_t* lengths, int32_t n,
+                                     int32_t first, int32_t recent, int32_t above, int32_t* kept,
+                                     void* stream);
+
+/**
+ * Cuts requests to the tokens of their lists, kept int32 [requests][heads][n]
+ * (mlxvs_kv_keep_device's, or others: n ascending positions below the request's
+ * length for each head, the same requests in all heads).  Key, value and mass (mass
+ * float32 [requests][heads][slots], or null) of position kept[j] move to position
+ * j, in place; what lies past position n stays in its places.  Complete pages of
+ * which a token changed get new summaries, if the cache keeps any.  The table stays
+ * as it is: the request's pages past the new end, columns ceil(n / page_size) ..
+ * ceil(length / page_size) - 1, are written into free_pages before entry cursor[0],
+ * in the requests' order from there down, so that entries from cursor_out[0] on are
+ * free.  Not cut, and given back nothing: a request whose list starts with -1, one
+ * of at most n tokens or of more than the table holds, and, from the first one on
+ * whose pages find no room in free_pages, each that would give pages back.
+ * lengths_out [requests], cursor_out [1]: the lengths and the cursor after it.  The
+ * pages of a request that is cut have to be its own: in place of shared ones the
+ * requests' tokens would be mixed up.  workspace: mlxvs_kv_compact_workspace bytes.
+ */
+MLXVS_C_API int mlxvs_kv_compact_device(const mlxvs_kv_cache* cache, const int32_t* table,
+                                        int64_t table_stride, int32_t columns, int64_t requests,
+                                        const int32_t* lengths, const int32_t* kept, int32_t n,
+                                        int32_t* free_pages, int64_t free_count,
+                                        const int32_t* cursor, float* mass, int64_t slots,
+                                        int32_t* lengths_out, int32_t* cursor_out,
+                                        void* workspace, int64_t workspace_bytes, void* stream);
+
+/** Bytes of workspace of a call with these sizes, -1 if they are invalid. */
+MLXVS_C_API int64_t mlxvs_kv_compact_workspace(const mlxvs_kv_cache* cache, int32_t columns,
+                                               int64_t requests, int32_t n);
+
 /**
  * Releases the workspace the library keeps on the current device between
  * calls (it is grown on demand and reused).  Safe to call at any time when
@@ -667,7 +818,7 @@ MLXVS_C_API int mlxvs_release_workspace(void);
  * Per-stage kernel timing: with enable != 0 every kernel launch of later
  * calls is bracketed by HIP events on its stream (stages: prep, fused_f32,
  * fused_f16, hamming, merge, scores, select, pack, fill, self_drop, kv_plan,
- * kv_append, kv_select, kv_attend).
+ * kv_append, kv_select, kv_attend, kv_rotate, kv_weigh, kv_keep, kv_compact).
  * Enabling or disabling clears the totals.
  */
 MLXVS_C_API int mlxvs_profile(int enable);

@@ -26,10 +26,12 @@ import numpy as np
 
 __all__ = [
     "IvfFlatIndex",
+    "KvCompact",
     "KvPlan",
     "Metric",
     "NearestNeighbors",
     "PagedKVCache",
+    "Rotary",
     "all_neighbors",
     "brute_force_knn",
     "brute_force_knn_filtered",
@@ -97,6 +99,15 @@ def _load():
         "mlxvs_kv_append_device": [vp, vp, i64, i64, vp, i64, i64, vp, i64, vp],
         "mlxvs_kv_select_device": [vp, vp, i32, i32, i32, vp, vp, i64, vp],
         "mlxvs_kv_attend_device": [vp, vp, vp, i32, ctypes.c_float, i64, vp, vp, vp, i64, vp],
+        "mlxvs_kv_rotary_frequencies": [i32, ctypes.c_double, ctypes.c_int, ctypes.c_double,
+                                        ctypes.c_double, vp, vp],
+        "mlxvs_kv_rotary_turns": [vp, i32, vp],
+        "mlxvs_kv_rotate_device": [vp, vp, vp, i64, vp, vp, vp, i64, ctypes.c_float, vp],
+        "mlxvs_kv_weigh_device": [vp, vp, vp, vp, ctypes.c_float, ctypes.c_float, i64, vp, i64,
+                                  vp],
+        "mlxvs_kv_keep_device": [vp, i64, i32, i64, vp, i32, i32, i32, i32, vp, vp],
+        "mlxvs_kv_compact_device": [vp, vp, i64, i32, i64, vp, vp, i32, vp, i64, vp, vp, i64, vp,
+                                    vp, vp, i64, vp],
         "mlxvs_release_workspace": [],
         "mlxvs_profile": [ctypes.c_int],
         "mlxvs_profile_report": [ctypes.c_char_p, i64],
@@ -106,7 +117,8 @@ def _load():
         fn.argtypes = args
         fn.restype = ctypes.c_int
     for name, args in (("mlxvs_kv_select_workspace", [vp, vp, i32]),
-                       ("mlxvs_kv_attend_workspace", [vp, vp, i32, i64])):
+                       ("mlxvs_kv_attend_workspace", [vp, vp, i32, i64]),
+                       ("mlxvs_kv_compact_workspace", [vp, i32, i64, i32])):
         fn = getattr(lib, name)
         fn.argtypes = args
         fn.restype = i64
@@ -571,7 +583,7 @@ def ivf_flat_search_device(centers_ptr, lists, data_ptr, n, indices_ptr, offsets
 def __getattr__(name):
     # the paged key-value cache works on torch tensors: torch is imported only
     # where it is used
-    if name in ("KvPlan", "PagedKVCache", "kv_plan"):
+    if name in ("KvCompact", "KvPlan", "PagedKVCache", "Rotary", "kv_plan"):
         from mlxvs_amd import kvcache
 
         return getattr(kvcache, name)

@@ -67,6 +67,14 @@ mlxvs::KvQueries kv_queries(const mlxvs_kv_queries* q) {
           q->table, q->table_stride, q->requests,    q->token_request, q->positions};
 }
 
+mlxvs::KvHeads kv_heads(const mlxvs_kv_heads* x) {
+  if (x == nullptr) return {};
+  require(x->norm_type == MLXVS_KV_NORM_OWN || x->norm_type == MLXVS_KV_NORM_F32,
+          "unknown type of a norm's weights.");
+  return {x->x,   x->token_stride,     x->head_stride,     x->heads, x->norm, (mlxvs::KvNorm)x->norm_type,
+          x->out, x->out_token_stride, x->out_head_stride};
+}
+
 void copy_out(const mlxvs::Neighbors& r, int32_t* ids, float* distances) {
   const size_t count = (size_t)r.nq * (size_t)r.k;
   for (size_t i = 0; i < count; ++i) ids[i] = r.ids[i];
@@ -386,6 +394,85 @@ int64_t mlxvs_kv_attend_workspace(const mlxvs_kv_cache* cache, const mlxvs_kv_qu
   int64_t bytes = -1;
   guarded([&] {
     bytes = mlxvs::kv_attend_workspace(kv_cache(cache), kv_queries(queries), n, longest);
+  });
+  return bytes;
+}
+
+int mlxvs_kv_rotary_frequencies(int32_t rotated, double base, mlxvs_kv_rotary_scaling scaling,
+                                double factor, double context, double* frequencies,
+                                float* magnitude) {
+  return guarded([&] {
+    require(scaling >= MLXVS_KV_SCALING_NONE && scaling <= MLXVS_KV_SCALING_RAMP,
+            "unknown scaling of positions.");
+    mlxvs::kv_rotary_frequencies(rotated, base, (mlxvs::KvScaling)scaling, factor, context,
+                                 frequencies, magnitude);
+  });
+}
+
+int mlxvs_kv_rotary_turns(const double* frequencies, int32_t n, uint64_t* turns) {
+  return guarded([&] { mlxvs::kv_rotary_turns(frequencies, n, turns); });
+}
+
+int mlxvs_kv_rotate_device(const mlxvs_kv_rotary* rotary, const mlxvs_kv_heads* q,
+                           const mlxvs_kv_heads* k, int64_t tokens, const int32_t* positions,
+                           const int32_t* token_request, const int32_t* evicted, int64_t requests,
+                           float eps, void* stream) {
+  return guarded([&] {
+    require(rotary != nullptr, "rotary must not be NULL.");
+    require(rotary->type == MLXVS_KV_F16 || rotary->type == MLXVS_KV_BF16,
+            "unknown type of heads.");
+    require(rotary->layout == MLXVS_KV_HALVES || rotary->layout == MLXVS_KV_PAIRS,
+            "unknown layout of rotated values.");
+    mlxvs::kv_rotate_device({rotary->turns, rotary->dim, rotary->rotated,
+                             (mlxvs::KvRotaryLayout)rotary->layout, rotary->magnitude,
+                             (mlxvs::KvType)rotary->type},
+                            kv_heads(q), kv_heads(k), tokens, positions, token_request, evicted,
+                            requests, eps, stream);
+  });
+}
+
+int mlxvs_kv_weigh_device(const mlxvs_kv_cache* cache, const mlxvs_kv_queries* queries,
+                          const int32_t* starts, const float* lse, float scale, float decay,
+                          int64_t longest, float* mass, int64_t slots, void* stream) {
+  return guarded([&] {
+    mlxvs::kv_weigh_device(kv_cache(cache), kv_queries(queries), starts, lse, scale, decay,
+                           longest, mass, slots, stream);
+  });
+}
+
+int mlxvs_kv_keep_device(const float* mass, int64_t requests, int32_t heads, int64_t slots,
+                         const int32_t* lengths, int32_t n, int32_t first, int32_t recent,
+                         int32_t above, int32_t* kept, void* stream) {
+  return guarded([&] {
+    mlxvs::kv_keep_device(mass, requests, heads, slots, lengths, n, first, recent, above, kept,
+                          stream);
+  });
+}
+
+int mlxvs_kv_compact_device(const mlxvs_kv_cache* cache, const int32_t* table,
+                            int64_t table_stride, int32_t columns, int64_t requests,
+                            const int32_t* lengths, const int32_t* kept, int32_t n,
+                            int32_t* free_pages, int64_t free_count, const int32_t* cursor,
+                            float* mass, int64_t slots, int32_t* lengths_out, int32_t* cursor_out,
+                            void* workspace, int64_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    mlxvs::kv_compact_device(kv_cache(cache),
+                             {table, table_stride, columns, requests, lengths, kept, n, free_pages,
+                              free_count, cursor, mass, slots, lengths_out, cursor_out},
+                             workspace, workspace_bytes, stream);
+  });
+}
+
+int64_t mlxvs_kv_compact_workspace(const mlxvs_kv_cache* cache, int32_t columns, int64_t requests,
+                                   int32_t n) {
+  int64_t bytes = -1;
+  guarded([&] {
+    mlxvs::KvCompact c;
+    c.columns = columns;
+    c.table_stride = columns;
+    c.requests = requests;
+    c.n = n;
+    bytes = mlxvs::kv_compact_workspace(kv_cache(cache), c);
   });
   return bytes;
 }

@@ -32,37 +32,18 @@
 
 #include "kv_cache.h"
 #include "kv_lists.h"
+#include "kv_mfma.h"
 #include "lds_stage.h"
 
 namespace mlxvs::kern {
 namespace {
 
 typedef float floatx2 __attribute__((ext_vector_type(2)));
-typedef float floatx4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
 typedef _Float16 halfx4 __attribute__((ext_vector_type(4)));
-typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 
 constexpr int kColumns = 16;  // query heads of one product
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-
-__device__ __forceinline__ floatx4 mfma(bf16x8 a, bf16x8 b, floatx4 c) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-#else
-  return c;
-#endif
-}
-__device__ __forceinline__ floatx4 mfma(halfx8 a, halfx8 b, floatx4 c) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-#else
-  return c;
-#endif
-}
 
 // The maximum over the lanes of one column (l, l ^ 16, l ^ 32, l ^ 48).  The lane
 // swaps are VALU instructions: a shuffle would wait for LDS.  (Written out: the
@@ -103,16 +84,6 @@ __device__ __forceinline__ uintx4 keep(uintx4 v, int n) {
     v[i] &= m >= 2 ? 0xFFFFFFFFu : (m == 1 ? 0xFFFFu : 0u);
   }
   return v;
-}
-
-// Head sizes are rounded up to one of these; a kernel for DP has more values than
-// the next smaller one holds, so that only the last of them need a check.
-constexpr int kSizes[] = {64, 96, 128, 192, 256};
-constexpr int sure_values(int dp) {
-  int below = 0;
-  for (int s : kSizes)
-    if (s < dp) below = s;
-  return below;
 }
 
 // log2 of what weights are scaled by: under f16 small terms of long sums stay

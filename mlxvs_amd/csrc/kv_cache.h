@@ -1,6 +1,7 @@
 // Launch interface between the host side (kv_engine.cpp) and the gfx950
-// kernels of the paged key-value cache (kv_plan.hip, kv_append.hip,
-// kv_select.hip, kv_attend.hip).
+// kernels of the paged key-value cache (kv_plan.hip, kv_rotate.hip,
+// kv_append.hip, kv_select.hip, kv_attend.hip, kv_weigh.hip, kv_keep.hip,
+// kv_compact.hip).
 //
 // Layout, for pages of `page` = 2^lps tokens (16 to 256), `heads` kv heads and
 // `dim` values a head (a multiple of 8, at most 256), binary16 or bfloat16:
@@ -103,5 +104,73 @@ void kv_attend_plan(KvAttendArgs& a);  // sets the split
 int64_t kv_attend_workspace(const KvAttendArgs& a);
 int64_t kv_attend_grid(const KvAttendArgs& a);  // workgroups of its largest launch
 hipError_t launch_kv_attend(const KvAttendArgs& a, hipStream_t s);
+
+// Heads of tokens as they are read and written: [tokens][heads][dim].
+struct KvRows {
+  const void* x;
+  int64_t token, head;  // strides in values
+  int heads;
+  const void* norm;  // [dim] weights, or null: no norm
+  bool norm_f32;     // float32, else of the rows' type
+  void* out;
+  int64_t out_token, out_head;
+};
+
+struct KvRotateArgs {
+  KvRows q, k;             // (k.heads 0: queries only)
+  const uint64_t* turns;   // [rotated / 2] turns a position, in 2^-64 of a turn
+  int dim, rotated;
+  bool pairs, bf16;
+  float magnitude, eps;
+  int64_t tokens, requests;
+  const int32_t* positions;
+  const int32_t* token_request;  // with evicted
+  const int32_t* evicted;        // [requests] added to positions, or null
+};
+int64_t kv_rotate_grid(const KvRotateArgs& a);  // workgroups of its launch
+hipError_t launch_kv_rotate(const KvRotateArgs& a, hipStream_t s);
+
+struct KvWeighArgs {
+  KvCache c;
+  KvQueries q;            // (token_request is not read)
+  const int32_t* starts;  // [requests + 1]
+  const float* lse;       // [tokens][heads * group]
+  float scale, decay;
+  int64_t longest;  // tokens the longest request is expected to hold, INT32_MAX: unknown
+  float* mass;      // [requests][heads][slots]
+  int64_t slots;
+};
+int64_t kv_weigh_grid(const KvWeighArgs& a);  // workgroups of its largest launch
+hipError_t launch_kv_weigh(const KvWeighArgs& a, hipStream_t s);
+
+struct KvKeepArgs {
+  const float* mass;  // [requests][heads][slots]
+  int64_t slots, requests;
+  int heads;
+  const int32_t* lengths;  // [requests]
+  int n, first, recent, above;
+  int32_t* kept;  // [requests][heads][n]
+};
+int64_t kv_keep_grid(const KvKeepArgs& a);
+hipError_t launch_kv_keep(const KvKeepArgs& a, hipStream_t s);
+
+struct KvCompactArgs {
+  KvCache c;
+  const int32_t* table;
+  int64_t table_stride, requests, free_count;
+  int cols, n;
+  const int32_t* lengths;
+  const int32_t* kept;  // [requests][heads][n]
+  int32_t* free_pages;
+  const int32_t* cursor;
+  float* mass;  // [requests][heads][slots] or null
+  int64_t slots;
+  int32_t* lengths_out;
+  int32_t* cursor_out;
+  int32_t* cut;  // workspace, [requests]: whether a request is cut
+};
+int64_t kv_compact_workspace(const KvCompactArgs& a);
+int64_t kv_compact_grid(const KvCompactArgs& a);
+hipError_t launch_kv_compact(const KvCompactArgs& a, hipStream_t s);
 
 }  // namespace mlxvs::kern

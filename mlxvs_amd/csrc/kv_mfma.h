@@ -1,0 +1,41 @@
+// The matrix products of attention's kernels: 16-bit values in, float32 out.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace mlxvs::kern {
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ floatx4 mfma(bf16x8 a, bf16x8 b, floatx4 c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+#else
+  return c;
+#endif
+}
+__device__ __forceinline__ floatx4 mfma(halfx8 a, halfx8 b, floatx4 c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+#else
+  return c;
+#endif
+}
+
+// Head sizes are rounded up to one of these; a kernel for DP has more values than
+// the next smaller one holds, so that only the last of them need a check.
+constexpr int kSizes[] = {64, 96, 128, 192, 256};
+constexpr int sure_values(int dp) {
+  int below = 0;
+  for (int s : kSizes)
+    if (s < dp) below = s;
+  return below;
+}
+
+}  // namespace mlxvs::kern

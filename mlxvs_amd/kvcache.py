@@ -9,10 +9,23 @@ a serving loop:
     blocks = cache.select(q, table, plan.requests, plan.positions, 32)
     out = cache.attend(q, table, plan.requests, plan.positions, blocks=blocks)
 
-(or ``attend`` without ``blocks``: over everything).  Tensors are on one GPU;
-every call runs on torch's current stream there, returns as soon as its work is
-enqueued and can be captured into a graph.  The cache serves: no call has a
-gradient.  The work is done by libmlxvs_c.so (``mlxvs_kv_*`` in
+(or ``attend`` without ``blocks``: over everything).  Queries and keys get their
+positions, and a norm of each head if the model has one, before that:
+
+    q, k = rotary.rotate(q, k, plan.positions, requests=plan.requests, evicted=evicted)
+
+and a cache that may hold only so much is cut now and then to the tokens that got
+most attention, the pages of the others going back into the free list:
+
+    out, lse = cache.attend(q, table, plan.requests, plan.positions, lse=True)
+    cache.weigh(q, table, plan.starts, plan.positions, lse, mass)
+    kept = cache.keep(mass, plan.lengths, budget, first=4, recent=128)
+    lengths, cursor = cache.compact(table, plan.lengths, kept, free_pages, plan.cursor, mass=mass)
+    evicted += plan.lengths - lengths
+
+Tensors are on one GPU; every call runs on torch's current stream there, returns as
+soon as its work is enqueued and can be captured into a graph.  The cache serves:
+no call has a gradient.  The work is done by libmlxvs_c.so (``mlxvs_kv_*`` in
 include/mlxvs/mlxvs_c.h); without it the calls raise ImportError.  Extensions:
 the reference has no counterpart.
 """
@@ -44,6 +57,18 @@ class _Queries(ctypes.Structure):
                 ("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
                 ("requests", ctypes.c_int64), ("token_request", ctypes.c_void_p),
                 ("positions", ctypes.c_void_p)]
+
+
+class _Rotary(ctypes.Structure):
+    _fields_ = [("turns", ctypes.c_void_p), ("dim", ctypes.c_int32), ("rotated", ctypes.c_int32),
+                ("layout", ctypes.c_int), ("magnitude", ctypes.c_float), ("type", ctypes.c_int)]
+
+
+class _Heads(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("token_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64), ("heads", ctypes.c_int32),
+                ("norm", ctypes.c_void_p), ("norm_type", ctypes.c_int), ("out", ctypes.c_void_p),
+                ("out_token_stride", ctypes.c_int64), ("out_head_stride", ctypes.c_int64)]
 
 
 def _need(ok: bool, op: str, what: str) -> None:
@@ -176,6 +201,156 @@ def kv_plan(past, new, table, free_pages, cursor, page_size, tokens, *, out=None
     return out
 
 
+def _aligned(x) -> bool:
+    """Whether the kernels read [tokens, heads, dim] rows as they are."""
+    st = x.stride()
+    return st[2] == 1 and not (st[0] & 7 or st[1] & 7 or x.data_ptr() & 15)
+
+
+class Rotary:
+    """Positions as rotations of queries and keys, with a norm of each head before
+    it where the model has one.
+
+    Args:
+        dim: values a head, a multiple of 8 up to 256.
+        rotated: how many of them are turned, the first ones (even; all of them
+            by default); the others pass.
+        layout: "halves": value i is turned with value i + rotated / 2; "pairs":
+            value 2 i with value 2 i + 1.
+        base: pair i turns by base^(-2 i / rotated) radians a position.
+        scaling: None, or how that is changed for texts ``factor`` times as long
+            as those of ``context`` tokens that the model learnt on: "linear" (all
+            of them divided by factor), "base" (a larger base), "ramp" (those that
+            make less than one turn over the context divided by factor, those that
+            make 32 or more kept, a straight line between them; rotated values
+            times 0.1 ln(factor) + 1).
+        frequencies, magnitude: radians a position of each pair and the factor
+            of rotated values, instead of all that.
+
+    An angle is the exact product of the position and a 64-bit frequency, at
+    every position.  ``frequencies`` and ``magnitude`` can be read back.
+    """
+
+    _LAYOUTS = {"halves": 0, "pairs": 1}
+    _SCALINGS = {None: 0, "linear": 1, "base": 2, "ramp": 3}
+
+    def __init__(self, dim, *, rotated=None, layout="halves", base=10000.0, scaling=None,
+                 factor=1.0, context=1, frequencies=None, magnitude=None, device="cuda"):
+        op = "Rotary"
+        dim = int(dim)
+        rotated = dim if rotated is None else int(rotated)
+        _need(8 <= dim <= 256 and dim % 8 == 0, op, "dim must be a multiple of 8 in [8, 256].")
+        _need(0 <= rotated <= dim and rotated % 2 == 0, op, "rotated must be even, in [0, dim].")
+        _need(layout in self._LAYOUTS, op, "layout must be 'halves' or 'pairs'.")
+        _need(scaling in self._SCALINGS, op,
+              "scaling must be None, 'linear', 'base' or 'ramp'.")
+        pairs = rotated // 2
+        radians, gain = (ctypes.c_double * pairs)(), ctypes.c_float(1.0)
+        if frequencies is None:
+            _check(_L().mlxvs_kv_rotary_frequencies(rotated, float(base), self._SCALINGS[scaling],
+                                                    float(factor), float(context), radians,
+                                                    ctypes.byref(gain)))
+        else:
+            _need(scaling is None, op, "frequencies are not scaled.")
+            given = [float(f) for f in frequencies]
+            _need(len(given) == pairs, op, f"frequencies must be {pairs} numbers.")
+            radians[:] = given
+        gain = gain.value if magnitude is None else float(magnitude)
+        _need(math.isfinite(gain), op, "magnitude must be finite.")
+        turns = (ctypes.c_uint64 * pairs)()
+        _check(_L().mlxvs_kv_rotary_turns(radians, pairs, turns))
+        self.dim, self.rotated, self.layout = dim, rotated, layout
+        self.frequencies, self.magnitude = list(radians), gain
+        device = torch.device(device)
+        _need(device.type == "cuda", op, "device must be a GPU.")
+        signed = [x - (1 << 64) if x >> 63 else x for x in turns]
+        self._turns = torch.tensor(signed or [0], dtype=torch.int64, device=device)
+        self._c = {dtype: _Rotary(self._turns.data_ptr(), dim, rotated, self._LAYOUTS[layout],
+                                  gain, kind) for dtype, kind in _TYPES.items()}
+
+    def _heads(self, x, name, norm, out, like):
+        """(rows, where their results go, both as the kernels take them)"""
+        op = "kv_rotate"
+        device = self._turns.device
+        if not (isinstance(x, torch.Tensor) and x.dim() == 3 and x.dtype in _TYPES
+                and x.device == device and x.shape[2] == self.dim
+                and (like is None or (x.shape[0] == like.shape[0] and x.dtype == like.dtype))):
+            raise ValueError(f"[mlxvs::{op}] {name} must be a float16 or bfloat16 [tokens, heads, "
+                             f"{self.dim}] tensor on {device}, as many tokens and of one type.")
+        if norm is not None:
+            _need(isinstance(norm, torch.Tensor) and norm.shape == (self.dim,)
+                  and norm.dtype in (x.dtype, torch.float32) and norm.device == device
+                  and norm.is_contiguous(), op,
+                  f"{name}_norm must be a contiguous {x.dtype} or float32 [{self.dim}] tensor on "
+                  f"{device}.")
+        if out is None:
+            out = x.new_empty(x.shape)
+        else:
+            _need(isinstance(out, torch.Tensor) and out.shape == x.shape and out.dtype == x.dtype
+                  and out.device == device and _aligned(out), op,
+                  f"out of {name} must be a {x.dtype} {list(x.shape)} tensor on {device}, 16-byte "
+                  "aligned with contiguous heads.")
+        if not _aligned(x):
+            x = x.clone(memory_format=torch.contiguous_format)
+        st, so = x.stride(), out.stride()
+        return x, out, _Heads(x.data_ptr(), st[0], st[1], x.shape[1],
+                              None if norm is None else norm.data_ptr(),
+                              norm is not None and norm.dtype == torch.float32, out.data_ptr(),
+                              so[0], so[1])
+
+    def rotate(self, q, k, positions, *, q_norm=None, k_norm=None, eps=1e-6, requests=None,
+               evicted=None, out=None):
+        """Queries [tokens, q_heads, dim] and keys [tokens, kv_heads, dim] (any
+        token and head strides; k may be None), normed and turned.
+
+        ``positions`` int32 [tokens] (KvPlan's); a token without one (-1) is not
+        turned.  ``evicted`` int32 [requests]: how many tokens a request's cache has
+        lost, added to its tokens' positions; ``requests`` int32 [tokens] (KvPlan's)
+        says whose they are.  ``q_norm`` / ``k_norm`` [dim]: weights of a norm of
+        each head before that, x / sqrt(mean(x^2) + eps) x weight, over the whole
+        head.  ``out``: (q, k) tensors to write into, which may be q and k
+        themselves.  Returns (q, k).
+
+        It has no gradient: the result of inputs that want one can be used, but not
+        differentiated, and not written into ``out``."""
+        op = "kv_rotate"
+        wanted = torch.is_grad_enabled() and any(
+            x is not None and x.requires_grad for x in (q, k, q_norm, k_norm))
+        _need(out is None or not wanted, op, "out takes no result that wants a gradient.")
+        _need(out is None or (isinstance(out, (tuple, list)) and len(out) == 2), op,
+              "out must be (q, k).")
+        _need(k is not None or k_norm is None, op, "k_norm needs k.")
+        to_q, to_k = (None, None) if out is None else out
+        inputs = [x for x in (q, k, q_norm, k_norm) if x is not None]
+        q, q_out, hq = self._heads(q, "q", q_norm, to_q, None)
+        k_out, hk = None, None
+        if k is not None:
+            k, k_out, hk = self._heads(k, "k", k_norm, to_k, q)
+        device, tokens = q.device, q.shape[0]
+        pp = _ints(positions, "positions", op, device, size=tokens)
+        pr = pe = None
+        if evicted is not None:
+            _need(requests is not None, op, "evicted needs requests.")
+            pe = _ints(evicted, "evicted", op, device)
+            pr = _ints(requests, "requests", op, device, size=tokens)
+        with _On(device) as stream:
+            _check(_L().mlxvs_kv_rotate_device(
+                ctypes.byref(self._c[q.dtype]), ctypes.byref(hq), hk and ctypes.byref(hk), tokens,
+                pp, pr, pe, 0 if evicted is None else evicted.numel(), float(eps), stream))
+        if wanted:
+            some = (q_out,) if k is None else (q_out, k_out)
+            some = _NoGradient.apply(op, some, *inputs)
+            return some[0], (None if k is None else some[1])
+        return q_out, k_out
+
+
+class KvCompact(NamedTuple):
+    """What PagedKVCache.compact leaves: int32 tensors."""
+
+    lengths: torch.Tensor  # [requests] tokens held now
+    cursor: torch.Tensor   # [1] the first unused entry of free_pages
+
+
 class PagedKVCache:
     """Attention keys and values in pages, and retrieval over them.
 
@@ -292,7 +467,8 @@ class PagedKVCache:
         pt, stride = _table(table, op, self._device)
         rows, columns = table.shape
         return q, _Queries(pq, st[0], st[1], tokens, heads, columns, pt, stride, rows,
-                           _ints(requests, "requests", op, self._device, size=tokens),
+                           None if requests is None
+                           else _ints(requests, "requests", op, self._device, size=tokens),
                            _ints(positions, "positions", op, self._device, size=tokens))
 
     def _workspace(self, size, q, qs, *args):
@@ -390,3 +566,124 @@ class PagedKVCache:
             results = _NoGradient.apply(op, (out, sums) if lse else (out,), q, keys, values)
             return results if lse else results[0]
         return (out, sums) if lse else out
+
+    def _mass(self, mass, op: str, requests: int, slots: int):
+        if not (isinstance(mass, torch.Tensor) and mass.dim() == 3 and mass.dtype == torch.float32
+                and mass.device == self._device and mass.is_contiguous()
+                and mass.shape[0] == requests and mass.shape[1] == self.kv_heads
+                and mass.shape[2] >= slots):
+            raise ValueError(f"[mlxvs::{op}] mass must be a contiguous float32 [{requests}, "
+                             f"{self.kv_heads}, slots] tensor on {self._device}, with at least "
+                             f"{slots} slots.")
+        return mass.data_ptr()
+
+    def weigh(self, q, table, starts, positions, lse, mass, *, scale=None, decay=1.0,
+              longest=0) -> None:
+        """Add the attention that each key gets from the step's tokens to ``mass``
+        (float32 [requests, kv_heads, slots], a slot for each token that the table
+        can hold).
+
+        ``q`` and ``lse`` are those of ``attend(..., lse=True)`` over everything,
+        with its ``scale``; ``starts`` and ``positions`` KvPlan's.  A key's mass is
+        the sum of its probabilities over the tokens that see it and the query heads
+        of its kv head.  The step's own keys start from zero, so a row of ``mass``
+        needs no clearing before a new request gets it; what the others had is
+        multiplied by ``decay`` (0: not read).  Masses past a request's last token,
+        and of requests without tokens, stay as they are.  The same bits every time.
+        """
+        op = "kv_weigh"
+        cache = self._cache(op)
+        q, qs = self._queries(q, table, None, positions, op)
+        tokens, heads, dim = q.shape
+        ps = _ints(starts, "starts", op, self._device, size=qs.requests + 1)
+        _need(isinstance(lse, torch.Tensor) and lse.shape == (tokens, heads)
+              and lse.dtype == torch.float32 and lse.device == self._device
+              and lse.is_contiguous(), op,
+              f"lse must be a contiguous float32 [tokens, q_heads] tensor on {self._device}.")
+        pm = self._mass(mass, op, qs.requests, qs.columns * self.page_size)
+        if scale is None:
+            scale = 1.0 / math.sqrt(dim)
+        with _On(self._device) as stream:
+            _check(_L().mlxvs_kv_weigh_device(cache, ctypes.byref(qs), ps, lse.data_ptr(),
+                                              float(scale), float(decay), int(longest), pm,
+                                              mass.shape[2], stream))
+
+    def keep(self, mass, lengths, n, *, first=1, recent=1, above=None):
+        """The ``n`` tokens of each request and kv head that a budget leaves: int32
+        [requests, kv_heads, n], ascending.
+
+        Of a request of more than ``above`` tokens (n by default) the ``first``
+        first and the ``recent`` last ones are kept, and of the others those of the
+        largest ``mass``, the lowest among equal ones (NaN counts as less than any
+        other).  A request of at most ``above`` keeps all: its list is -1
+        throughout.  ``lengths`` int32 [requests]."""
+        op = "kv_keep"
+        n = int(n)
+        device = self._device
+        pl = _ints(lengths, "lengths", op, device)
+        requests = lengths.numel()
+        pm = self._mass(mass, op, requests, 0)
+        with _On(device) as stream:
+            _need(n >= 1, op, "n must be at least 1.")
+            kept = mass.new_empty((requests, self.kv_heads, n), dtype=torch.int32)
+            _check(_L().mlxvs_kv_keep_device(pm, requests, self.kv_heads, mass.shape[2], pl, n,
+                                             int(first), int(recent),
+                                             n if above is None else int(above), kept.data_ptr(),
+                                             stream))
+        return kept
+
+    def compact(self, table, lengths, kept, free_pages, cursor, *, mass=None,
+                out=None) -> KvCompact:
+        """Cut requests to the tokens of their lists, in place.
+
+        ``kept`` int32 [requests, kv_heads, n]: ``keep``'s, or other ascending
+        positions below a request's length, as many for every head.  Key, value and
+        (with ``mass``) mass of position ``kept[r, h, j]`` move to position j;
+        pages of which a token changed get new summaries.  The table stays as it is;
+        the pages past a request's new end are written into ``free_pages`` before
+        entry ``cursor[0]``, from where ``kv_plan`` takes them again.  A request
+        whose list starts with -1 stays as it is, and so does one whose pages
+        find no room in ``free_pages``.  Keys were rotated by their tokens'
+        positions before they were written, so what they say stays true; new tokens
+        are to be rotated by ``evicted`` more than their positions (``Rotary``).
+
+        The pages of a request that is cut must be its own, not shared with another
+        row.  ``lengths`` int32 [requests], ``cursor`` int32 [1].  ``out``: an
+        earlier result of as many requests to write into (not the tensors that this
+        call reads).  Returns KvCompact(lengths, cursor) after it."""
+        op = "kv_compact"
+        cache = self._cache(op)
+        device = self._device
+        pt, stride = _table(table, op, device)
+        requests, columns = table.shape
+        pl = _ints(lengths, "lengths", op, device, size=requests)
+        if not (isinstance(kept, torch.Tensor) and kept.dim() == 3 and kept.dtype == torch.int32
+                and kept.is_contiguous() and kept.device == device
+                and kept.shape[:2] == (requests, self.kv_heads) and kept.shape[2] >= 1):
+            raise ValueError(f"[mlxvs::{op}] kept must be a contiguous int32 [requests, kv_heads, "
+                             f"n] tensor on {device}.")
+        pf = _ints(free_pages, "free_pages", op, device)
+        pc = _ints(cursor, "cursor", op, device, size=1)
+        slots = columns * self.page_size if mass is None else mass.shape[-1]
+        pm = None if mass is None else self._mass(mass, op, requests, columns * self.page_size)
+        n = kept.shape[2]
+        with _On(device) as stream:
+            if out is None:
+                out = KvCompact(lengths.new_empty(requests), lengths.new_empty(1))
+            else:
+                _need(isinstance(out, KvCompact), op, "out must be a KvCompact.")
+            po = _ints(out.lengths, "out.lengths", op, device, size=requests)
+            pn = _ints(out.cursor, "out.cursor", op, device, size=1)
+            key = ("compact", requests, columns, n)
+            need = self._sizes.get(key)
+            if need is None:
+                need = _L().mlxvs_kv_compact_workspace(cache, columns, requests, n)
+                if need < 0:
+                    raise ValueError(_L().mlxvs_last_error().decode())
+                self._sizes[key] = need
+            work = lengths.new_empty(need, dtype=torch.uint8) if need else None
+            _check(_L().mlxvs_kv_compact_device(
+                cache, pt, stride, columns, requests, pl, kept.data_ptr(), n, pf,
+                free_pages.numel(), pc, pm, slots, po, pn,
+                None if work is None else work.data_ptr(), need, stream))
+        return out
