@@ -167,7 +167,7 @@ struct KvCompactArgs {
   int64_t slots;
   int32_t* lengths_out;
   int32_t* cursor_out;
-  int32_t* cut;  // workspace, [requests]: whether a request is cut
+  int32_t* work;  // kv_compact_workspace bytes
 };
 int64_t kv_compact_workspace(const KvCompactArgs& a);
 int64_t kv_compact_grid(const KvCompactArgs& a);

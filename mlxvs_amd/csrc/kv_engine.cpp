@@ -410,7 +410,7 @@ void kv_compact_device(const KvCache& cache, const KvCompact& p, void* workspace
   check(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace)),
         "the workspace is too small, or not 16-byte aligned.");
   detail::need_device();
-  a.cut = (int32_t*)workspace;
+  a.work = (int32_t*)workspace;
   detail::launch_stage<kern::KvCompactArgs, kern::launch_kv_compact>((hipStream_t)stream,
                                                                      "kv_compact", a);
 }
