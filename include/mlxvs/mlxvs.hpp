@@ -373,8 +373,10 @@ MLXVS_API void kv_rotate_device(const KvRotary& rotary, const KvHeads& q, const 
  * only. */
 MLXVS_API void kv_weigh_device(const KvCache& cache, const KvQueries& queries,
                                const int32_t* starts, const float* lse, float scale, float decay,
-                               int64_t longest, float* mass, int64_t slots,
-                               void* stream = nullptr);
+                               int64_t longest, float* mass, int64_t slots, void* workspace,
+                               int64_t workspace_bytes, void* stream = nullptr);
+MLXVS_API int64_t kv_weigh_workspace(const KvCache& cache, const KvQueries& queries,
+                                     int64_t longest);
 /** The tokens that a budget leaves (mlxvs_kv_keep_device); enqueues only. */
 MLXVS_API void kv_keep_device(const float* mass, int64_t requests, int32_t heads, int64_t slots,
                               const int32_t* lengths, int32_t n, int32_t first, int32_t recent,

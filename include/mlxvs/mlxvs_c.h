@@ -758,12 +758,18 @@ MLXVS_C_API int mlxvs_kv_rotate_device(const mlxvs_kv_rotary* rotary, const mlxv
  * others, and requests without tokens (or with position -1), stay as they are; a
  * key of an absent page gets nothing.  decay in [0, 1]; with 0 masses are not read.
  * A page that several rows share has a mass in each.  longest guides how work is
- * split, as in mlxvs_kv_attend_device.  The same bits every time.
+ * split, as in mlxvs_kv_attend_device.  The same bits every time.  workspace:
+ * mlxvs_kv_weigh_workspace bytes (may be 0).
  */
 MLXVS_C_API int mlxvs_kv_weigh_device(const mlxvs_kv_cache* cache,
                                       const mlxvs_kv_queries* queries, const int32_t* starts,
                                       const float* lse, float scale, float decay,
-                                      int64_t longest, float* mass, int64_t slots, void* stream);
+                                      int64_t longest, float* mass, int64_t slots,
+                                      void* workspace, int64_t workspace_bytes, void* stream);
+
+/** Bytes of workspace of a call with these arguments, -1 if they are invalid. */
+MLXVS_C_API int64_t mlxvs_kv_weigh_workspace(const mlxvs_kv_cache* cache,
+                                             const mlxvs_kv_queries* queries, int64_t longest);
 
 /**
  * The tokens that a budget of n leaves: kept int32 [requests][heads][n], ascending.

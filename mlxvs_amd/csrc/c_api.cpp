@@ -433,11 +433,21 @@ int mlxvs_kv_rotate_device(const mlxvs_kv_rotary* rotary, const mlxvs_kv_heads* 
 
 int mlxvs_kv_weigh_device(const mlxvs_kv_cache* cache, const mlxvs_kv_queries* queries,
                           const int32_t* starts, const float* lse, float scale, float decay,
-                          int64_t longest, float* mass, int64_t slots, void* stream) {
+                          int64_t longest, float* mass, int64_t slots, void* workspace,
+                          int64_t workspace_bytes, void* stream) {
   return guarded([&] {
     mlxvs::kv_weigh_device(kv_cache(cache), kv_queries(queries), starts, lse, scale, decay,
-                           longest, mass, slots, stream);
+                           longest, mass, slots, workspace, workspace_bytes, stream);
   });
+}
+
+int64_t mlxvs_kv_weigh_workspace(const mlxvs_kv_cache* cache, const mlxvs_kv_queries* queries,
+                                 int64_t longest) {
+  int64_t bytes = -1;
+  guarded([&] {
+    bytes = mlxvs::kv_weigh_workspace(kv_cache(cache), kv_queries(queries), longest);
+  });
+  return bytes;
 }
 
 int mlxvs_kv_keep_device(const float* mass, int64_t requests, int32_t heads, int64_t slots,

@@ -371,14 +371,6 @@ __device__ __forceinline__ bool in_prompt(const KvAttendArgs& a, int64_t t) {
   return found >= a.least;
 }
 
-// 16 bytes a lane from `from` to lds + 16 lane.
-__device__ __forceinline__ void copy16_to_lds(const void* from, void* lds) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                   (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
-#endif
-}
-
 // A tile's keys (64 while two workgroups of such tiles fit a CU).
 constexpr int tile_keys(int dim) { return dim <= 128 ? 64 : 32; }
 

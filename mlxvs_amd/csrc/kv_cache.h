@@ -139,7 +139,11 @@ struct KvWeighArgs {
   int64_t longest;  // tokens the longest request is expected to hold, INT32_MAX: unknown
   float* mass;      // [requests][heads][slots]
   int64_t slots;
+  int64_t piece;  // rows (tokens x group) of a piece, 0: requests are whole (kv_weigh_plan)
+  int32_t* work;  // kv_weigh_workspace bytes
 };
+void kv_weigh_plan(KvWeighArgs& a);  // sets the pieces
+int64_t kv_weigh_workspace(const KvWeighArgs& a);
 int64_t kv_weigh_grid(const KvWeighArgs& a);  // workgroups of its largest launch
 hipError_t launch_kv_weigh(const KvWeighArgs& a, hipStream_t s);
 

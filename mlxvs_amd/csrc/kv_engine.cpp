@@ -103,6 +103,18 @@ kern::KvAttendArgs attend_args(const KvCache& cache, const KvQueries& queries, b
   return a;
 }
 
+kern::KvWeighArgs weigh_args(const KvCache& cache, const KvQueries& queries, int64_t longest,
+                             const Check& check) {
+  kern::KvWeighArgs a{};
+  a.c = cache_of(cache, check);
+  a.q = queries_of(queries, a.c, check, false);
+  check(longest >= 0, "longest must not be negative.");
+  a.longest = longest ? longest : kIntMax;
+  kern::kv_weigh_plan(a);
+  check_grid(kern::kv_weigh_grid(a), 256, check);
+  return a;
+}
+
 // Whether [tokens][heads][dim] places with these strides, in values, are apart.
 bool apart(int64_t tokens, int64_t token, int64_t heads, int64_t head, int64_t dim) {
   if (tokens <= 1 && heads <= 1) return true;
@@ -341,30 +353,34 @@ void kv_attend_device(const KvCache& cache, const KvQueries& queries, const int3
                                                                    "kv_attend", a);
 }
 
+int64_t kv_weigh_workspace(const KvCache& cache, const KvQueries& queries, int64_t longest) {
+  const Check check{"mlxvs::kv_weigh"};
+  return kern::kv_weigh_workspace(weigh_args(cache, queries, longest, check));
+}
+
 void kv_weigh_device(const KvCache& cache, const KvQueries& queries, const int32_t* starts,
                      const float* lse, float scale, float decay, int64_t longest, float* mass,
-                     int64_t slots, void* stream) {
+                     int64_t slots, void* workspace, int64_t workspace_bytes, void* stream) {
   const Check check{"mlxvs::kv_weigh"};
-  kern::KvWeighArgs a{};
-  a.c = cache_of(cache, check);
-  a.q = queries_of(queries, a.c, check, false);
-  check(longest >= 0, "longest must not be negative.");
+  kern::KvWeighArgs a = weigh_args(cache, queries, longest, check);
   check(scale > 0.0f && std::isfinite(scale), "scale must be positive and finite.");
   check(decay >= 0.0f && decay <= 1.0f, "decay must be in [0, 1].");
   check(slots >= (int64_t)a.q.cols << a.c.lps,
         "mass must have a slot for each token of the table.");
   check(a.q.tokens == 0 || a.q.requests == 0 || (starts && lse && mass),
         "starts, lse and mass must not be NULL.");
+  const int64_t need = kern::kv_weigh_workspace(a);
+  check(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace)),
+        "the workspace is too small, or not 16-byte aligned.");
+  if (a.q.tokens == 0 || a.q.requests == 0 || a.q.cols == 0) return;
+  detail::need_device();
   a.starts = starts;
   a.lse = lse;
   a.scale = scale;
   a.decay = decay;
-  a.longest = longest ? longest : kIntMax;
   a.mass = mass;
   a.slots = slots;
-  check_grid(kern::kv_weigh_grid(a), 256, check);
-  if (a.q.tokens == 0 || a.q.requests == 0 || a.q.cols == 0) return;
-  detail::need_device();
+  a.work = (int32_t*)workspace;
   detail::launch_stage<kern::KvWeighArgs, kern::launch_kv_weigh>((hipStream_t)stream, "kv_weigh",
                                                                  a);
 }

@@ -28,6 +28,23 @@ __device__ __forceinline__ floatx4 mfma(halfx8 a, halfx8 b, floatx4 c) {
 #endif
 }
 
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ floatx16 mfma(bf16x8 a, bf16x8 b, floatx16 c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+#else
+  return c;
+#endif
+}
+__device__ __forceinline__ floatx16 mfma(halfx8 a, halfx8 b, floatx16 c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+#else
+  return c;
+#endif
+}
+
 // Head sizes are rounded up to one of these; a kernel for DP has more values than
 // the next smaller one holds, so that only the last of them need a check.
 constexpr int kSizes[] = {64, 96, 128, 192, 256};

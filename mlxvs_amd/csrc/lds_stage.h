@@ -27,6 +27,14 @@ __device__ __forceinline__ void load4_to_lds(__amdgpu_buffer_rsrc_t r, void* lds
 #endif
 }
 
+// 16 bytes a lane from `from` to lds + 16 lane.
+__device__ __forceinline__ void copy16_to_lds(const void* from, void* lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                   (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+#endif
+}
+
 // A workgroup barrier after this wavefront's outstanding vector-memory
 // operations -- its LDS-direct loads among them -- have completed: an LDS
 // buffer that every wavefront fills with LDS-direct loads is whole once all

@@ -603,10 +603,12 @@ class PagedKVCache:
         pm = self._mass(mass, op, qs.requests, qs.columns * self.page_size)
         if scale is None:
             scale = 1.0 / math.sqrt(dim)
+        longest = int(longest)
         with _On(self._device) as stream:
-            _check(_L().mlxvs_kv_weigh_device(cache, ctypes.byref(qs), ps, lse.data_ptr(),
-                                              float(scale), float(decay), int(longest), pm,
-                                              mass.shape[2], stream))
+            work, size = self._workspace("mlxvs_kv_weigh_workspace", q, qs, longest)
+            _check(_L().mlxvs_kv_weigh_device(
+                cache, ctypes.byref(qs), ps, lse.data_ptr(), float(scale), float(decay), longest,
+                pm, mass.shape[2], None if work is None else work.data_ptr(), size, stream))
 
     def keep(self, mass, lengths, n, *, first=1, recent=1, above=None):
         """The ``n`` tokens of each request and kv head that a budget leaves: int32

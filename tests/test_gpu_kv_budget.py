@@ -289,6 +289,15 @@ def test_weights_of_prompts_of_any_length(engine, tokens):
     assert abs(total - 2 * tokens) <= 2 * tokens * 2.0 ** -10
 
 
+@pytest.mark.parametrize("lengths,counts,heads,group,dim", [
+    ([900, 40, 5], [900, 1, 5], 1, 4, 64), ([1000, 700, 0, 600], [500, 700, 0, 2], 1, 3, 16),
+    ([300], [300], 2, 16, 128), ([300], [299], 1, 24, 256), ([700], [650], 1, 2, 192)])
+def test_weights_of_prompts_in_pieces(engine, lengths, counts, heads, group, dim):
+    # more rows than one workgroup goes through
+    Step(engine, lengths, counts, page=64, heads=heads, group=group, dim=dim,
+         seed=len(lengths)).attend().check(decay=0.5)
+
+
 def test_weights_decay_and_begin_anew(engine):
     for decay in (0.0, 0.5, 1.0):
         s = Step(engine, [50, 90, 7], [3, 1, 7], seed=3)

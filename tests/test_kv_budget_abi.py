@@ -41,9 +41,10 @@ def rotate(lib, rot=None, q=None, k=None, tokens=3, positions=P, who=None, evict
                                       requests, eps, None)
 
 
-def weigh(lib, c=None, q=None, starts=P, lse=P, scale=0.125, decay=1.0, longest=0, mass=P, slots=80):
+def weigh(lib, c=None, q=None, starts=P, lse=P, scale=0.125, decay=1.0, longest=0, mass=P, slots=80,
+          work=P, size=1 << 30):
     return lib.mlxvs_kv_weigh_device(ctypes.byref(c or cache()), ctypes.byref(q or queries()), starts,
-                                     lse, scale, decay, longest, mass, slots, None)
+                                     lse, scale, decay, longest, mass, slots, work, size, None)
 
 
 def keep(lib, **k):
@@ -155,6 +156,15 @@ def test_weights_that_are_refused(engine):
               dict(q=queries(table_stride=4)), dict(q=queries(q=P + 8))):
         assert weigh(lib, **k) == INVALID, k
         assert b"[mlxvs::kv_weigh]" in lib.mlxvs_last_error()
+    # a prompt's workspace
+    q = queries(tokens=5000, columns=320, table_stride=320)
+    need = lib.mlxvs_kv_weigh_workspace(ctypes.byref(cache()), ctypes.byref(q), 0)
+    assert need > 0
+    for k in (dict(work=None), dict(size=need - 1), dict(work=P + 4)):
+        assert weigh(lib, q=q, slots=5120, **k) == INVALID
+        assert b"workspace" in lib.mlxvs_last_error()
+    assert lib.mlxvs_kv_weigh_workspace(ctypes.byref(cache()), ctypes.byref(queries()), 0) == 0
+    assert lib.mlxvs_kv_weigh_workspace(ctypes.byref(cache()), ctypes.byref(q), -1) == -1
 
 
 @pytest.mark.parametrize("bad", [
