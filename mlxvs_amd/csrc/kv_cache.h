@@ -139,7 +139,7 @@ struct KvWeighArgs {
   int64_t longest;  // tokens the longest request is expected to hold, INT32_MAX: unknown
   float* mass;      // [requests][heads][slots]
   int64_t slots;
-  int64_t piece;  // rows (tokens x group) of a piece, 0: requests are whole (kv_weigh_plan)
+  int64_t piece;  // tokens of a piece, 0: requests are whole (kv_weigh_plan)
   int32_t* work;  // kv_weigh_workspace bytes
 };
 void kv_weigh_plan(KvWeighArgs& a);  // sets the pieces

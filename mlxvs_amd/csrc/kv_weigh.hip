@@ -10,8 +10,8 @@
 //
 // S = K Q^T on the 32x32x16 MFMA with the keys as rows.  A wavefront keeps 64 keys
 // in registers, the operand of every product; the rows of Q (a token's query
-// head each) come through LDS by direct loads, 64 at a time, one tile ahead, for
-// all four wavefronts.  A lane adds up its column's weights of each of its 32 keys
+// head each) come through LDS by direct loads, whole tokens of up to 64 rows at a
+// time, three tiles ahead, for all four wavefronts.  A lane adds up its column's weights of each of its 32 keys
 // over all rows, and the 32 columns meet once at the end.
 #include <hip/hip_runtime.h>
 
@@ -69,7 +69,7 @@ __device__ __forceinline__ Span span_of(const KvWeighArgs& a, int64_t r) {
 }
 
 __device__ __forceinline__ int64_t pieces_of(const KvWeighArgs& a, int tokens) {
-  return max((int64_t)1, ((int64_t)tokens * a.q.group + a.piece - 1) / a.piece);
+  return max((int64_t)1, (tokens + a.piece - 1) / a.piece);
 }
 
 constexpr int kPlanThreads = 1024;
@@ -141,7 +141,17 @@ __device__ __forceinline__ void put(const KvWeighArgs& a, float* mass, int p, in
   mass[p] = before + got;
 }
 
-__device__ const uintx4 kZeros = {};  // what rows have past the head
+// What rows of a tile have past the head.  Rows that no token fills are zeros with a
+// logarithm that leaves no weight, and see all keys, so that a tile of them takes
+// the short way; rows that are not the piece's see none.
+__device__ const uintx4 kZeros = {};
+__device__ const float kNoLse = __builtin_inff();
+__device__ const int kNoRowsPosition = INT32_MAX, kNoPosition = -1;
+
+// x, which is the same in all lanes.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+constexpr int kStages = 4;  // tiles in LDS: one in use, the others on their way
 
 // DP: head size rounded up.
 template <int DP, bool BF16>
@@ -154,78 +164,86 @@ struct Weigh {
   static constexpr int kRow = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;
   static constexpr int kTileBytes = kRows * kRow * 16;
   static constexpr int kCopies = kRow / 4;  // of 1 KB a wavefront and tile
+  static constexpr int kLoads = kCopies + 1;  // ... and one of 256 bytes
   __device__ __forceinline__ static int swap(int row) {
     return kRow == 8 ? row >> 1 & 7 : row & 15;
   }
 
-  struct Info {
-    float lse;  // times log2(e); infinity for a row that is not there
-    int pos;
+  // (aligned so that a chunk's place in its row is some bits of its address)
+  struct __align__(512) Tile {
+    char q[kTileBytes];
+    float lse[kRows];  // infinity for a row that is not there
+    int pos[kRows];
+    int none[kRows];
   };
 
   const KvWeighArgs& a;
   const int lane, wave, h, group;
-  // the row of the next tile that this thread (of the first wavefront) prepares
-  uint32_t x, end;       // which row of the request's, of how many
-  int token, head, begin;  // its token and head there; the request's first token
-  // the chunk that this lane copies of its rows: they are 16 apart, or 8, whose
-  // chunks' places differ
-  static constexpr int kFrom = kRow == 32 ? 2 : 1;
-  int from[kFrom];
+  const int heads_tile, tokens_tile;  // a tile: heads of a token, or all of some tokens
+  int64_t rows[kCopies];  // this lane's pieces of a tile, from its first row on
+  int token_told, head_told;  // the row whose logarithm or position it brings; -1: none
+  int token, end, head;   // the next tile's first, one past the last of all, its head
   uintx4 kf[2][kSteps];
   float sum[32];
 
   __device__ __forceinline__ Weigh(const KvWeighArgs& args, int hd)
-      : a(args), lane(threadIdx.x & 63), wave(threadIdx.x >> 6), h(hd), group(args.q.group) {
-#pragma unroll
-    for (int i = 0; i < kFrom; ++i) {
-      const int slot = (wave + 4 * i) * 64 + lane, chunk = (slot % kRow) ^ swap(slot / kRow);
-      from[i] = 8 * chunk < a.c.dim ? 8 * chunk : -1;
-    }
-  }
-
-  // Rows x0 .. x1 - 1 of a request.
-  __device__ __forceinline__ void start(int first_token, int64_t x0, int64_t x1) {
-    begin = first_token;
-    end = (uint32_t)x1;
-    x = (uint32_t)x0 + lane;
-    token = (int)(x / group);
-    head = (int)(x % group);
-  }
-
-  // The first wavefront: where the next tile's rows begin (those past the last are
-  // the last one).
-  __device__ __forceinline__ void address(int64_t* to) {
-    const uint32_t last = end - 1;
-    const bool there = x < end;
-    const int t = there ? token : (int)(last / group), g = there ? head : (int)(last % group);
-    to[lane] = (int64_t)(begin + t) * a.q.q_token + (int64_t)(h * group + g) * a.q.q_head;
-  }
-  // ... and what the columns need of them, before it goes on by a tile.
-  __device__ __forceinline__ Info info() {
-    Info n{__builtin_inff(), -1};
-    if (x < end) {
-      const int64_t t = begin + token;
-      n.lse = a.lse[t * a.c.heads * group + h * group + head];
-      n.pos = max(-1, a.q.positions[t]);
-    }
-    x += kRows;
-    token += kRows / group;
-    head += kRows % group;
-    if (head >= group) {
-      head -= group;
-      ++token;
-    }
-    return n;
-  }
-
-  // Copies a tile into LDS.
-  __device__ __forceinline__ void copy(const int64_t* rows, char* to) const {
+      : a(args), lane(threadIdx.x & 63), wave(uniform(threadIdx.x >> 6)), h(hd), group(args.q.group),
+        heads_tile(min(args.q.group, kRows)), tokens_tile(max(1, kRows / args.q.group)) {
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) {
-      const int f = from[i % kFrom];
-      const T* src = (const T*)a.q.q + rows[((wave + 4 * i) * 64 + lane) / kRow] + f;
-      copy16_to_lds(f >= 0 ? (const void*)src : &kZeros, to + 1024 * (wave + 4 * i));
+      const int slot = (wave + 4 * i) * 64 + lane, j = slot / kRow, chunk = (slot % kRow) ^ swap(j);
+      // (tokens past the batch's: another one)
+      const int t = min(j / heads_tile, (int)a.q.tokens - 1);
+      rows[i] = t * a.q.q_token + j % heads_tile * a.q.q_head + 8 * chunk;
+      if (8 * chunk >= a.c.dim || j / heads_tile >= tokens_tile) rows[i] = kNoRow;
+    }
+    token_told = lane / heads_tile < tokens_tile ? lane / heads_tile : -1;
+    head_told = lane % heads_tile;
+  }
+  static constexpr int64_t kNoRow = INT64_MIN;
+
+  // Tokens t0 .. t1 - 1 of the batch.
+  __device__ __forceinline__ void start(int t0, int t1) {
+    token = t0;
+    end = t1;
+    head = 0;
+  }
+  __device__ __forceinline__ int tiles() const {
+    return (end - token + tokens_tile - 1) / tokens_tile * ((group + kRows - 1) / kRows);
+  }
+
+  // Copies the next tile into LDS (past the last: anything), kLoads loads.  A tile
+  // that would reach past the batch, or the group, begins before its first row:
+  // rows that are not its own are copied and not seen.
+  __device__ __forceinline__ void copy(Tile& to) {
+    const int t = max(0, min(token, (int)a.q.tokens - tokens_tile)), g = min(head, group - heads_tile);
+    const T* q = (const T*)a.q.q + t * a.q.q_token + (int64_t)(h * group + g) * a.q.q_head;
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const void* src = q + rows[i];
+      if (rows[i] == kNoRow) src = &kZeros;
+      stream16_to_lds(src, to.q + 1024 * (wave + 4 * i));
+    }
+    // two wavefronts bring what the columns need, the others as much of nothing, so
+    // that all have as many loads on their way
+    const void* src = &kZeros;
+    void* dst = to.none;
+    if (wave < 2) {
+      const int x = t + token_told;
+      const bool own = token_told >= 0 && x >= token && x < end && g + head_told >= head;
+      if (wave == 0) {
+        src = own ? (const void*)(a.lse + ((int64_t)x * a.c.heads + h) * group + g + head_told) : &kNoLse;
+        dst = to.lse;
+      } else {
+        src = own ? a.q.positions + x : token_told < 0 ? &kNoRowsPosition : &kNoPosition;
+        dst = to.pos;
+      }
+    }
+    stream4_to_lds(src, dst);
+    head += kRows;
+    if (head >= group) {
+      head = 0;
+      token = min(token + tokens_tile, end);
     }
   }
 
@@ -251,14 +269,14 @@ struct Weigh {
 
   // The products of 32 rows of a tile; between(i) is done beside step i's.
   template <typename Between>
-  __device__ __forceinline__ void products(const char* tile, int ct, floatx16 (&s)[2],
+  __device__ __forceinline__ void products(const Tile& tile, int ct, floatx16 (&s)[2],
                                            Between between) const {
     const int col = lane & 31, half = lane >> 5;
-    const char* at = tile + (32 * ct + col) * kRow * 16;
-    const int sw = half ^ swap(32 * ct + col);
+    const uint32_t at = lds_address(tile.q) + (32 * ct + col) * kRow * 16 +
+                        16 * (half ^ swap(32 * ct + col));
     uintx4 q[kSteps];
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) q[i] = *(const uintx4*)(at + 16 * (sw ^ (2 * i)));
+    for (int i = 0; i < kSteps; ++i) q[i] = lds_read16(at ^ (32 * i));
 #pragma unroll
     for (int u = 0; u < 2; ++u) s[u] = floatx16{};
 #pragma unroll
@@ -279,22 +297,23 @@ struct Weigh {
   }
 
   // A tile's rows against this wavefront's keys.
-  __device__ __forceinline__ void use(const char* tile, const Info* info, int k0, float c) {
+  __device__ __forceinline__ void use(const Tile& tile, int k0, float c) {
     const int col = lane & 31, half = lane >> 5;
-    const Info n0 = info[col], n1 = info[32 + col];
+    const float l0 = tile.lse[col] * kLog2e, l1 = tile.lse[32 + col] * kLog2e;
+    const int p0 = tile.pos[col], p1 = tile.pos[32 + col];
     floatx16 s0[2], s1[2];
-    if (__all(min(n0.pos, n1.pos) >= k0 + kWaveKeys - 1)) {
+    if (__all(min(p0, p1) >= k0 + kWaveKeys - 1)) {
       products(tile, 0, s0, [](int) {});
       products(tile, 1, s1, [&](int i) {
-        add(s0, i * 32 / kSteps, (i + 1) * 32 / kSteps, c, n0.lse);
+        add(s0, i * 32 / kSteps, (i + 1) * 32 / kSteps, c, l0);
       });
-      add(s1, 0, 32, c, n1.lse);
+      add(s1, 0, 32, c, l1);
       return;
     }
 #pragma unroll 1
     for (int ct = 0; ct < 2; ++ct) {
-      const float lse = ct ? n1.lse : n0.lse;
-      const int pos = ct ? n1.pos : n0.pos, seen = pos - k0 - 4 * half;
+      const float lse = ct ? l1 : l0;
+      const int pos = max(-1, ct ? p1 : p0), seen = pos - k0 - 4 * half;
       if (!__any(pos >= k0)) continue;
       products(tile, ct, s0, [](int) {});
 #pragma unroll
@@ -328,70 +347,53 @@ template <int DP, bool BF16>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1)
 void kv_weigh_kernel(KvWeighArgs a, int chunks) {
   using W = Weigh<DP, BF16>;
-  using Info = typename W::Info;
-  __shared__ __align__(16) char t0[W::kTileBytes], t1[W::kTileBytes];
-  __shared__ Info i0[kRows], i1[kRows];
-  __shared__ int64_t r0[kRows], r1[kRows];
+  using Tile = typename W::Tile;
+  __shared__ Tile tiles[kStages];
   const int h = (int)(blockIdx.x % a.c.heads);
   const int64_t rest = blockIdx.x / a.c.heads;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t r = rest / chunks, base = -1;
-  int piece = 0;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  int64_t piece = 0;
+  int r = (int)(rest / chunks), base = -1;
   if (a.piece) {
     const Work work = work_of(a);
-    const int p = (int)r, requests = (int)a.q.requests;
+    const int p = r, requests = (int)a.q.requests;
     if (p >= work.first[requests]) return;
-    r = below(requests, lane, [&](int i) { return work.first[i]; }, p + 1) - 1;
-    piece = p - work.first[r];
-    base = work.base[r];
+    r = uniform(below(requests, lane, [&](int i) { return work.first[i]; }, p + 1)) - 1;
+    piece = p - uniform(work.first[r]);
+    base = uniform(work.base[r]);
   }
-  const Span sp = span_of(a, r);
+  Span sp = span_of(a, r);
+  sp = {uniform(sp.begin), uniform(sp.tokens), uniform(sp.first), uniform(sp.last)};
   const int32_t* table = a.q.table + r * a.q.table_stride;
-  float* mass = a.mass + (r * a.c.heads + h) * a.slots;
-  const int64_t rows = (int64_t)sp.tokens * a.q.group;
+  float* mass = a.mass + ((int64_t)r * a.c.heads + h) * a.slots;
   const float c = a.scale * kLog2e;
   W w(a, h);
   for (int64_t chunk = rest % chunks; chunk * kChunk <= sp.last; chunk += chunks) {
-    // the rows that see the chunk, of the piece's
-    const int from = (int)(chunk * kChunk), k0 = from + wave * kWaveKeys;
-    const int blind = below(sp.tokens, lane, [&](int i) { return a.q.positions[sp.begin + i]; }, from);
-    const int64_t x0 = max((int64_t)blind * a.q.group, base < 0 ? 0 : piece * a.piece);
-    const int64_t x1 = base < 0 ? rows : min(rows, (piece + 1) * a.piece);
-    w.keys(table, k0, sp.last);
+    // the tokens that see the chunk, of the piece's
+    const int first = (int)(chunk * kChunk), k0 = first + wave * kWaveKeys;
+    const int blind = uniform(
+        below(sp.tokens, lane, [&](int i) { return a.q.positions[sp.begin + i]; }, first));
+    const int x0 = base < 0 ? blind : (int)max((int64_t)blind, piece * a.piece);
+    const int x1 = base < 0 ? sp.tokens : (int)min((int64_t)sp.tokens, (piece + 1) * a.piece);
 #pragma unroll
     for (int e = 0; e < 32; ++e) w.sum[e] = 0.0f;
     if (x0 < x1) {
-      w.start(sp.begin, x0, x1);
-      const bool tells = wave == 0;
-      const auto tell = [&](Info* to, Info n) { to[lane] = {n.lse * kLog2e, n.pos}; };
-      int todo = (int)((x1 - x0 + kRows - 1) / kRows);
-      const auto turn = [&](char* tile, Info* info, int64_t* rows, char* other, Info* then,
-                            int64_t* next) {
-        dma_barrier();  // this tile is there, and the other buffer is free
-        Info n{};
-        const bool more = --todo > 0;
-        if (more) {
-          w.copy(next, other);
-          if (tells) {
-            n = w.info();
-            w.address(rows);
-          }
-        }
-        if (k0 <= sp.last) w.use(tile, info, k0, c);
-        if (more && tells) tell(then, n);
-      };
-      __syncthreads();  // (the last chunk's buffers are free)
-      if (tells) {
-        w.address(r0);
-        tell(i0, w.info());
-        w.address(r1);
+      w.start(sp.begin + x0, sp.begin + x1);
+      const int todo = w.tiles();
+#pragma unroll
+      for (int n = 0; n < kStages - 1; ++n) w.copy(tiles[n]);
+      w.keys(table, k0, sp.last);
+      // (known to the compiler, which else waits for the keys, and with them for all
+      // that was loaded since, in every turn)
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+#pragma unroll 1
+      for (int n = 0; n < todo; ++n) {
+        staged_barrier<(kStages - 2) * W::kLoads>();
+        w.copy(tiles[(n + kStages - 1) % kStages]);  // (the place of the one before)
+        if (k0 <= sp.last) w.use(tiles[n % kStages], k0, c);
       }
-      __syncthreads();
-      w.copy(r0, t0);
-      while (todo > 0) {
-        turn(t0, i0, r0, t1, i1, r1);
-        if (todo > 0) turn(t1, i1, r1, t0, i0, r0);
-      }
+      dma_barrier();  // (nothing is on its way into the tiles any more)
+      mfma_settle();
     }
     const float got = w.meet();
     const int p = k0 + W::key_of(lane);
@@ -438,7 +440,7 @@ struct Most {
 };
 Most most_of(const KvWeighArgs& a) {
   if (!a.piece) return {a.q.requests, 0, 0};
-  const int64_t full = a.q.tokens * a.q.group / a.piece;
+  const int64_t full = a.q.tokens / a.piece;
   return {a.q.requests + full, 2 * full, std::min(a.q.requests, full)};
 }
 
@@ -463,10 +465,11 @@ constexpr int64_t kLeast = 1024;  // rows of a piece
 }  // namespace
 
 void kv_weigh_plan(KvWeighArgs& a) {
-  const int64_t rows = a.q.tokens * a.q.group, units = chunks_of(a) * a.c.heads;
-  const int64_t pieces = std::max<int64_t>(1, kUnits / units);
-  const int64_t piece = std::max(kLeast, ((rows + pieces - 1) / pieces + kRows - 1) / kRows * kRows);
-  a.piece = piece < rows ? piece : 0;
+  const int64_t pieces = std::max<int64_t>(1, kUnits / (chunks_of(a) * a.c.heads));
+  const int64_t each = std::max<int64_t>(1, kRows / a.q.group);  // tokens of a tile
+  const int64_t piece = std::max((a.q.tokens + pieces - 1) / pieces, kLeast / a.q.group);
+  a.piece = (piece + each - 1) / each * each;
+  if (a.piece >= a.q.tokens) a.piece = 0;
 }
 
 int64_t kv_weigh_workspace(const KvWeighArgs& a) {

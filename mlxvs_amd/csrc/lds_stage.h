@@ -35,6 +35,54 @@ __device__ __forceinline__ void copy16_to_lds(const void* from, void* lds) {
 #endif
 }
 
+// A place in LDS as the instructions take it, and 16 bytes from one.
+__device__ __forceinline__ uint32_t lds_address(const void* lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds;
+#else
+  return 0;
+#endif
+}
+__device__ __forceinline__ auto lds_read16(uint32_t at) {
+  typedef uint32_t uintx4_t __attribute__((ext_vector_type(4)));
+#if defined(__HIP_DEVICE_COMPILE__)
+  return *(const __attribute__((address_space(3))) uintx4_t*)(uintptr_t)at;
+#else
+  return uintx4_t{};
+#endif
+}
+
+// Direct loads of 16 or 4 bytes a lane for tiles that are several loads ahead.  The
+// compiler waits for all loads like those above before it reads any LDS that one of
+// them may have written, and takes every buffer for such; of these it knows
+// nothing: whoever reads what they bring waits for them (staged_barrier).  They
+// return nothing to registers.  The place in LDS is the wavefront's.
+__device__ __forceinline__ void stream16_to_lds(const void* from, void* lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const int to = __builtin_amdgcn_readfirstlane((int)lds_address(lds));
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+               ::"v"(from), "s"(to) : "memory", "m0");
+#endif
+}
+__device__ __forceinline__ void stream4_to_lds(const void* from, void* lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const int to = __builtin_amdgcn_readfirstlane((int)lds_address(lds));
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
+               ::"v"(from), "s"(to) : "memory", "m0");
+#endif
+}
+
+// A workgroup barrier once all but the latest LEFT of this wavefront's loads are
+// done, for buffers that stream*_to_lds fill.
+template <int LEFT>
+__device__ __forceinline__ void staged_barrier() {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+  __builtin_amdgcn_sched_barrier(0);
+#endif
+}
+
 // A workgroup barrier after this wavefront's outstanding vector-memory
 // operations -- its LDS-direct loads among them -- have completed: an LDS
 // buffer that every wavefront fills with LDS-direct loads is whole once all
