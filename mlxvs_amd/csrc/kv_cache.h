@@ -139,7 +139,8 @@ struct KvWeighArgs {
   int64_t longest;  // tokens the longest request is expected to hold, INT32_MAX: unknown
   float* mass;      // [requests][heads][slots]
   int64_t slots;
-  int64_t piece;  // tokens of a piece, 0: requests are whole (kv_weigh_plan)
+  int64_t piece;  // tokens of a workgroup's share, 0: single tokens (kv_weigh_plan)
+  int64_t most_units, most_several, most_slots;  // shares and partial sums at most
   int32_t* work;  // kv_weigh_workspace bytes
 };
 void kv_weigh_plan(KvWeighArgs& a);  // sets the pieces

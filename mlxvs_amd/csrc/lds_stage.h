@@ -52,21 +52,31 @@ __device__ __forceinline__ auto lds_read16(uint32_t at) {
 #endif
 }
 
+template <typename T>
+__device__ __forceinline__ T lds_read4(uint32_t at) {
+  static_assert(sizeof(T) == 4);
+#if defined(__HIP_DEVICE_COMPILE__)
+  return *(const __attribute__((address_space(3))) T*)(uintptr_t)at;
+#else
+  return T{};
+#endif
+}
+
 // Direct loads of 16 or 4 bytes a lane for tiles that are several loads ahead.  The
 // compiler waits for all loads like those above before it reads any LDS that one of
 // them may have written, and takes every buffer for such; of these it knows
 // nothing: whoever reads what they bring waits for them (staged_barrier).  They
 // return nothing to registers.  The place in LDS is the wavefront's.
-__device__ __forceinline__ void stream16_to_lds(const void* from, void* lds) {
+__device__ __forceinline__ void stream16_to_lds(const void* from, uint32_t lds) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  const int to = __builtin_amdgcn_readfirstlane((int)lds_address(lds));
+  const int to = __builtin_amdgcn_readfirstlane((int)lds);
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
                ::"v"(from), "s"(to) : "memory", "m0");
 #endif
 }
-__device__ __forceinline__ void stream4_to_lds(const void* from, void* lds) {
+__device__ __forceinline__ void stream4_to_lds(const void* from, uint32_t lds) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  const int to = __builtin_amdgcn_readfirstlane((int)lds_address(lds));
+  const int to = __builtin_amdgcn_readfirstlane((int)lds);
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
                ::"v"(from), "s"(to) : "memory", "m0");
 #endif

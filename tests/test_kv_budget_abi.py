@@ -163,7 +163,7 @@ def test_weights_that_are_refused(engine):
     for k in (dict(work=None), dict(size=need - 1), dict(work=P + 4)):
         assert weigh(lib, q=q, slots=5120, **k) == INVALID
         assert b"workspace" in lib.mlxvs_last_error()
-    assert lib.mlxvs_kv_weigh_workspace(ctypes.byref(cache()), ctypes.byref(queries()), 0) == 0
+    assert lib.mlxvs_kv_weigh_workspace(ctypes.byref(cache()), ctypes.byref(queries(requests=3)), 0) == 0
     assert lib.mlxvs_kv_weigh_workspace(ctypes.byref(cache()), ctypes.byref(q), -1) == -1
 
 
