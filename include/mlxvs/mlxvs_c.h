@@ -715,8 +715,8 @@ typedef enum {
  * Heads of tokens: x [tokens][heads][dim] and the place of their results, strides
  * in values (multiples of 8; 16-byte aligned).  `out` may be x, with its strides;
  * else the results may overlap nothing that the call reads.  norm [dim]: weights of
- * a norm before the rotation, x rsqrt(mean(x^2) + eps) norm over the whole head;
- * null: none.  heads 0: nothing.
+ * a norm before the rotation, x rsqrt(mean(x^2) + eps) norm over the whole head,
+ * 16-byte aligned; null: none.  heads 0: nothing.
  */
 typedef struct {
   const void* x;

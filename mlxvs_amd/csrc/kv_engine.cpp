@@ -129,8 +129,8 @@ kern::KvRows rows_of(const KvHeads& x, int64_t tokens, int dim, const Check& che
   if (x.heads == 0 || tokens == 0) return {};
   check(x.x && x.out, "rows and their outputs must not be NULL.");
   check(aligned(x.x) && x.token_stride % 8 == 0 && x.head_stride % 8 == 0 && aligned(x.out) &&
-            x.out_token_stride % 8 == 0 && x.out_head_stride % 8 == 0,
-        "rows must be 16-byte aligned, with strides that are multiples of 8.");
+            x.out_token_stride % 8 == 0 && x.out_head_stride % 8 == 0 && aligned(x.norm),
+        "rows and norms must be 16-byte aligned, with strides that are multiples of 8.");
   check(apart(tokens, x.out_token_stride, x.heads, x.out_head_stride, dim),
         "outputs must not overlap one another.");
   check(x.x != x.out || ((tokens <= 1 || x.token_stride == x.out_token_stride) &&

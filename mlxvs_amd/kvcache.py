@@ -283,8 +283,10 @@ class Rotary:
                   and norm.is_contiguous(), op,
                   f"{name}_norm must be a contiguous {x.dtype} or float32 [{self.dim}] tensor on "
                   f"{device}.")
+            if norm.data_ptr() & 15:
+                norm = norm.clone()
         if out is None:
-            out = x.new_empty(x.shape)
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
         else:
             _need(isinstance(out, torch.Tensor) and out.shape == x.shape and out.dtype == x.dtype
                   and out.device == device and _aligned(out), op,
@@ -293,10 +295,10 @@ class Rotary:
         if not _aligned(x):
             x = x.clone(memory_format=torch.contiguous_format)
         st, so = x.stride(), out.stride()
-        return x, out, _Heads(x.data_ptr(), st[0], st[1], x.shape[1],
-                              None if norm is None else norm.data_ptr(),
-                              norm is not None and norm.dtype == torch.float32, out.data_ptr(),
-                              so[0], so[1])
+        return x, norm, out, _Heads(x.data_ptr(), st[0], st[1], x.shape[1],
+                                    None if norm is None else norm.data_ptr(),
+                                    norm is not None and norm.dtype == torch.float32,
+                                    out.data_ptr(), so[0], so[1])
 
     def rotate(self, q, k, positions, *, q_norm=None, k_norm=None, eps=1e-6, requests=None,
                evicted=None, out=None):
@@ -314,18 +316,20 @@ class Rotary:
         It has no gradient: the result of inputs that want one can be used, but not
         differentiated, and not written into ``out``."""
         op = "kv_rotate"
-        wanted = torch.is_grad_enabled() and any(
-            x is not None and x.requires_grad for x in (q, k, q_norm, k_norm))
+        wanted = (q.requires_grad or (k is not None and k.requires_grad)
+                  or (q_norm is not None and q_norm.requires_grad)
+                  or (k_norm is not None and k_norm.requires_grad)) and torch.is_grad_enabled()
         _need(out is None or not wanted, op, "out takes no result that wants a gradient.")
         _need(out is None or (isinstance(out, (tuple, list)) and len(out) == 2), op,
               "out must be (q, k).")
         _need(k is not None or k_norm is None, op, "k_norm needs k.")
         to_q, to_k = (None, None) if out is None else out
-        inputs = [x for x in (q, k, q_norm, k_norm) if x is not None]
-        q, q_out, hq = self._heads(q, "q", q_norm, to_q, None)
+        given = (q, k, q_norm, k_norm)
+        # (what is copied for the kernel has to live until the call is made)
+        q, q_norm, q_out, hq = self._heads(q, "q", q_norm, to_q, None)
         k_out, hk = None, None
         if k is not None:
-            k, k_out, hk = self._heads(k, "k", k_norm, to_k, q)
+            k, k_norm, k_out, hk = self._heads(k, "k", k_norm, to_k, q)
         device, tokens = q.device, q.shape[0]
         pp = _ints(positions, "positions", op, device, size=tokens)
         pr = pe = None
@@ -339,7 +343,7 @@ class Rotary:
                 pp, pr, pe, 0 if evicted is None else evicted.numel(), float(eps), stream))
         if wanted:
             some = (q_out,) if k is None else (q_out, k_out)
-            some = _NoGradient.apply(op, some, *inputs)
+            some = _NoGradient.apply(op, some, *(x for x in given if x is not None))
             return some[0], (None if k is None else some[1])
         return q_out, k_out
 

@@ -71,7 +71,7 @@ def test_rotations_that_are_refused(engine, bad):
 
 
 @pytest.mark.parametrize("bad", [
-    dict(x=None), dict(out=None), dict(x=P + 8), dict(out=P + 2), dict(token_stride=12),
+    dict(x=None), dict(out=None), dict(x=P + 8), dict(norm=P + 8), dict(out=P + 2), dict(token_stride=12),
     dict(head_stride=4), dict(out_token_stride=20), dict(heads=-1), dict(norm_type=2),
     dict(out=P * 2, out_head_stride=0), dict(out=P * 2, out_token_stride=64),
     dict(out_token_stride=1024), dict(token_stride=1024)])
