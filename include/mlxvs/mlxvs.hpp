@@ -380,7 +380,9 @@ MLXVS_API int64_t kv_weigh_workspace(const KvCache& cache, const KvQueries& quer
 /** The tokens that a budget leaves (mlxvs_kv_keep_device); enqueues only. */
 MLXVS_API void kv_keep_device(const float* mass, int64_t requests, int32_t heads, int64_t slots,
                               const int32_t* lengths, int32_t n, int32_t first, int32_t recent,
-                              int32_t above, int32_t* kept, void* stream = nullptr);
+                              int32_t above, int32_t* kept, void* workspace,
+                              int64_t workspace_bytes, void* stream = nullptr);
+MLXVS_API int64_t kv_keep_workspace(int64_t requests, int32_t heads, int64_t slots);
 /** Requests cut to those tokens (mlxvs_kv_compact_device); enqueues only. */
 MLXVS_API void kv_compact_device(const KvCache& cache, const KvCompact& compact, void* workspace,
                                  int64_t workspace_bytes, void* stream = nullptr);

@@ -777,12 +777,15 @@ MLXVS_C_API int64_t mlxvs_kv_weigh_workspace(const mlxvs_kv_cache* cache,
  * (>= n) its first `first` and last `recent` (first + recent <= n) are kept, and of
  * the others those of the largest mass, the lowest among equal ones; NaN counts
  * as less than any other.  A request of at most `above` keeps all: its list is -1
- * throughout.
+ * throughout.  workspace: mlxvs_kv_keep_workspace bytes (may be 0).
  */
 MLXVS_C_API int mlxvs_kv_keep_device(const float* mass, int64_t requests, int32_t heads,
                                      int64_t slots, const int32_t* lengths, int32_t n,
                                      int32_t first, int32_t recent, int32_t above, int32_t* kept,
-                                     void* stream);
+                                     void* workspace, int64_t workspace_bytes, void* stream);
+
+/** Bytes of workspace of a call with these sizes, -1 if they are invalid. */
+MLXVS_C_API int64_t mlxvs_kv_keep_workspace(int64_t requests, int32_t heads, int64_t slots);
 
 /**
  * Cuts requests to the tokens of their lists, kept int32 [requests][heads][n]

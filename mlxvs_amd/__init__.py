@@ -105,7 +105,7 @@ def _load():
         "mlxvs_kv_rotate_device": [vp, vp, vp, i64, vp, vp, vp, i64, ctypes.c_float, vp],
         "mlxvs_kv_weigh_device": [vp, vp, vp, vp, ctypes.c_float, ctypes.c_float, i64, vp, i64,
                                   vp, i64, vp],
-        "mlxvs_kv_keep_device": [vp, i64, i32, i64, vp, i32, i32, i32, i32, vp, vp],
+        "mlxvs_kv_keep_device": [vp, i64, i32, i64, vp, i32, i32, i32, i32, vp, vp, i64, vp],
         "mlxvs_kv_compact_device": [vp, vp, i64, i32, i64, vp, vp, i32, vp, i64, vp, vp, i64, vp,
                                     vp, vp, i64, vp],
         "mlxvs_release_workspace": [],
@@ -119,6 +119,7 @@ def _load():
     for name, args in (("mlxvs_kv_select_workspace", [vp, vp, i32]),
                        ("mlxvs_kv_attend_workspace", [vp, vp, i32, i64]),
                        ("mlxvs_kv_weigh_workspace", [vp, vp, i64]),
+                       ("mlxvs_kv_keep_workspace", [i64, i32, i64]),
                        ("mlxvs_kv_compact_workspace", [vp, i32, i64, i32])):
         fn = getattr(lib, name)
         fn.argtypes = args

@@ -452,11 +452,18 @@ int64_t mlxvs_kv_weigh_workspace(const mlxvs_kv_cache* cache, const mlxvs_kv_que
 
 int mlxvs_kv_keep_device(const float* mass, int64_t requests, int32_t heads, int64_t slots,
                          const int32_t* lengths, int32_t n, int32_t first, int32_t recent,
-                         int32_t above, int32_t* kept, void* stream) {
+                         int32_t above, int32_t* kept, void* workspace, int64_t workspace_bytes,
+                         void* stream) {
   return guarded([&] {
     mlxvs::kv_keep_device(mass, requests, heads, slots, lengths, n, first, recent, above, kept,
-                          stream);
+                          workspace, workspace_bytes, stream);
   });
+}
+
+int64_t mlxvs_kv_keep_workspace(int64_t requests, int32_t heads, int64_t slots) {
+  int64_t bytes = -1;
+  guarded([&] { bytes = mlxvs::kv_keep_workspace(requests, heads, slots); });
+  return bytes;
 }
 
 int mlxvs_kv_compact_device(const mlxvs_kv_cache* cache, const int32_t* table,

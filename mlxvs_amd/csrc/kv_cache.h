@@ -155,7 +155,9 @@ struct KvKeepArgs {
   const int32_t* lengths;  // [requests]
   int n, first, recent, above;
   int32_t* kept;  // [requests][heads][n]
+  void* work;     // kv_keep_workspace bytes
 };
+int64_t kv_keep_workspace(const KvKeepArgs& a);
 int64_t kv_keep_grid(const KvKeepArgs& a);
 hipError_t launch_kv_keep(const KvKeepArgs& a, hipStream_t s);
 

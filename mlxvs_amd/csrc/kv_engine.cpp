@@ -140,6 +140,18 @@ kern::KvRows rows_of(const KvHeads& x, int64_t tokens, int dim, const Check& che
           x.norm, x.norm_type == KvNorm::Float32, x.out, x.out_token_stride, x.out_head_stride};
 }
 
+kern::KvKeepArgs keep_args(int64_t requests, int32_t heads, int64_t slots, const Check& check) {
+  check(requests >= 0 && requests <= kIntMax && heads >= 1 && heads <= 1 << 16 && slots >= 0 &&
+            slots <= kIntMax,
+        "requests and slots must be in [0, 2^31), heads in [1, 65536].");
+  kern::KvKeepArgs a{};
+  a.requests = requests;
+  a.heads = heads;
+  a.slots = slots;
+  check_grid(kern::kv_keep_grid(a), 1024, check);
+  return a;
+}
+
 kern::KvCompactArgs compact_args(const KvCache& cache, const KvCompact& p, const Check& check) {
   kern::KvCompactArgs a{};
   a.c = cache_of(cache, check);
@@ -385,23 +397,36 @@ void kv_weigh_device(const KvCache& cache, const KvQueries& queries, const int32
                                                                  a);
 }
 
+int64_t kv_keep_workspace(int64_t requests, int32_t heads, int64_t slots) {
+  const Check check{"mlxvs::kv_keep"};
+  return kern::kv_keep_workspace(keep_args(requests, heads, slots, check));
+}
+
 void kv_keep_device(const float* mass, int64_t requests, int32_t heads, int64_t slots,
                     const int32_t* lengths, int32_t n, int32_t first, int32_t recent,
-                    int32_t above, int32_t* kept, void* stream) {
+                    int32_t above, int32_t* kept, void* workspace, int64_t workspace_bytes,
+                    void* stream) {
   const Check check{"mlxvs::kv_keep"};
-  check(requests >= 0 && requests <= kIntMax && heads >= 1 && heads <= 1 << 16 && slots >= 0 &&
-            slots <= kIntMax,
-        "requests and slots must be in [0, 2^31), heads in [1, 65536].");
+  kern::KvKeepArgs a = keep_args(requests, heads, slots, check);
   check(n >= 1, "n must be at least 1.");
   check(first >= 0 && recent >= 0 && first <= n && recent <= n - first,
         "first >= 0, recent >= 0 and first + recent <= n are needed.");
   check(above >= n, "above must be at least n.");
   check(requests == 0 || (lengths && kept && (mass || slots == 0)),
         "mass, lengths and kept must not be NULL.");
-  const kern::KvKeepArgs a{mass, slots, requests, heads, lengths, n, first, recent, above, kept};
-  check_grid(kern::kv_keep_grid(a), 1024, check);
+  const int64_t need = kern::kv_keep_workspace(a);
+  check(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace)),
+        "the workspace is too small, or not 16-byte aligned.");
   if (requests == 0) return;
   detail::need_device();
+  a.mass = mass;
+  a.lengths = lengths;
+  a.n = n;
+  a.first = first;
+  a.recent = recent;
+  a.above = above;
+  a.kept = kept;
+  a.work = workspace;
   detail::launch_stage<kern::KvKeepArgs, kern::launch_kv_keep>((hipStream_t)stream, "kv_keep", a);
 }
 

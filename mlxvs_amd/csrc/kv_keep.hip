@@ -4,8 +4,14 @@
 // list is empty.
 //
 // Masses are compared as 32-bit ranks in their order (NaN last), so the list is a
-// matter of definition.  A row is a workgroup's: the n-th largest rank 8 bits at a
-// time, then the ones above it and the first of those that equal it.
+// matter of definition.  The n-th largest rank is found by 11, 11 and 10 of its
+// bits, a histogram of 2,048 bins in LDS each; then the tokens above it are taken,
+// and the first of those that equal it.
+//
+// A row of up to 65,536 slots is a workgroup's and read once: its ranks stay in
+// registers.  A longer one is split into parts of 16,384, a workgroup each, with a
+// launch for every histogram and one for the list: the parts' histograms are summed
+// by whoever needs them, so that nothing is counted by atomics in memory.
 #include <hip/hip_runtime.h>
 
 #include "kv_cache.h"
@@ -15,6 +21,14 @@ namespace {
 
 constexpr uint32_t kAlways = 0xFFFFFFFFu;
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kBins = 2048, kDigits = 3;
+constexpr int kPart = 16384;       // slots of a part
+constexpr int kRowSlots = 65536;   // the longest row of one workgroup
+
+__device__ __forceinline__ int shift_of(int digit) { return digit == 0 ? 21 : digit == 1 ? 10 : 0; }
+__device__ __forceinline__ uint32_t digit_of(uint32_t rank, int digit) {
+  return digit == 2 ? rank & 1023 : rank >> shift_of(digit) & 2047;
+}
 
 __device__ __forceinline__ int bits(uint64_t x) { return (int)__popcll(x); }
 
@@ -26,83 +40,288 @@ __device__ __forceinline__ uint32_t rank_of(float x) {
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-__global__ __launch_bounds__(kThreads) void kv_keep_kernel(KvKeepArgs a) {
-  __shared__ uint32_t hist[256];
-  __shared__ int gt[kWaves], eq[kWaves];
-  __shared__ uint32_t found;
-  __shared__ int rest;
+// Ranks of 64 R tokens from `from` on for each wavefront, 64 neighbours at a time.
+template <int R>
+struct Ranks {
+  uint32_t k[R];
+  int from;  // this lane's first token
+
+  __device__ __forceinline__ Ranks(const KvKeepArgs& a, const float* mass, int start, int length) {
+    from = start + (threadIdx.x >> 6) * 64 * R + (threadIdx.x & 63);
+    float x[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) x[i] = from + 64 * i < length ? mass[from + 64 * i] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int t = from + 64 * i;
+      k[i] = t >= length                                 ? 0
+             : t < a.first || t >= length - a.recent ? kAlways
+                                                         : rank_of(x[i]);
+    }
+  }
+
+  // Counts those whose higher digits are prefix's in hist.
+  __device__ __forceinline__ void count(uint32_t* hist, int digit, uint32_t prefix) const {
+    const int lane = threadIdx.x & 63;
+    const uint32_t known = digit == 0 ? 0 : ~0u << shift_of(digit - 1);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const bool mine = k[i] != 0 && (k[i] & known) == prefix;
+      const uint32_t b = digit_of(k[i], digit);
+      // (equal masses are common: one of the lanes counts for all)
+      const uint64_t some = __ballot(mine);
+      if (!some) continue;
+      const uint32_t first = __shfl(b, __builtin_ctzll(some));
+      if (__all(!mine || b == first)) {
+        if (lane == 0) atomicAdd(&hist[first], (uint32_t)bits(some));
+      } else if (mine) {
+        atomicAdd(&hist[b], 1u);
+      }
+    }
+  }
+
+  // The tokens above `cut`, and of those that equal it the first `ties` of the
+  // workgroup, into out in their order.
+  __device__ __forceinline__ void take(uint32_t cut, int ties, int32_t* out, int (*waves)[2]) const {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int gt = 0, eq = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      gt += bits(__ballot(k[i] > cut));
+      eq += bits(__ballot(k[i] == cut));
+    }
+    if (lane == 0) {
+      waves[wave][0] = gt;
+      waves[wave][1] = eq;
+    }
+    __syncthreads();
+    int at = 0, before = 0;
+    for (int w = 0; w < wave; ++w) {
+      at += waves[w][0] + min(waves[w][1], max(0, ties - before));
+      before += waves[w][1];
+    }
+    const uint64_t below = (uint64_t(1) << lane) - 1;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const uint64_t tied = __ballot(k[i] == cut);
+      const bool taken = k[i] > cut || (k[i] == cut && before + bits(tied & below) < ties);
+      const uint64_t all = __ballot(taken);
+      if (taken) out[at + bits(all & below)] = from + 64 * i;
+      at += bits(all);
+      before += bits(tied);
+    }
+  }
+};
+
+struct Pick {
+  int waves[kWaves];
+  uint32_t bin;
+  int left;
+};
+
+// The bin in which the left-th largest lies, and the how manieth it is there, from
+// this thread's two bins (counted from the largest: thread i has 2047 - 2 i and the
+// one below).
+__device__ __forceinline__ void pick(int hi, int lo, int left, Pick& s) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t r = blockIdx.x / a.heads;
-  const int length = (int)min<int64_t>(a.lengths[r], a.slots);
-  const float* mass = a.mass + (int64_t)blockIdx.x * a.slots;
-  int32_t* out = a.kept + (int64_t)blockIdx.x * a.n;
-  if (length <= a.above) {
-    for (int i = threadIdx.x; i < a.n; i += kThreads) out[i] = -1;
-    return;
+  int upto = hi + lo;
+#pragma unroll
+  for (int by = 1; by < 64; by <<= 1) {
+    const int y = __shfl_up(upto, by);
+    if (lane >= by) upto += y;
   }
-  const auto rank = [&](int i) {
-    return i < a.first || i >= length - a.recent ? kAlways : rank_of(mass[i]);
-  };
-  uint32_t cut = 0;
-  int left = a.n;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (threadIdx.x < 256) hist[threadIdx.x] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < length; i += kThreads) {
-      const uint32_t k = rank(i);
-      if (shift == 24 || (k >> (shift + 8)) == (cut >> (shift + 8)))
-        atomicAdd(&hist[(k >> shift) & 255], 1u);
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      int n = 0, b = 255;
-      while (b > 0 && n + (int)hist[b] < left) n += (int)hist[b--];
-      found = cut | (uint32_t)b << shift;
-      rest = left - n;
-    }
-    __syncthreads();
-    cut = found;
-    left = rest;
-  }
-  // each wavefront a stretch of the tokens
-  const int per = (length + kThreads - 1) / kThreads * 64;
-  const int from = min(length, wave * per), to = min(length, from + per);
-  int above = 0, same = 0;
-  for (int i = from + lane; i - lane < to; i += 64) {
-    const uint32_t k = i < to ? rank(i) : 0;
-    above += bits(__ballot(k > cut));
-    same += bits(__ballot(k == cut && i < to));
-  }
-  if (lane == 0) {
-    gt[wave] = above;
-    eq[wave] = same;
+  if (lane == 63) s.waves[wave] = upto;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) upto += s.waves[w];
+  const int before = upto - hi - lo;
+  if (before < left && left <= upto) {
+    const bool upper = left <= before + hi;
+    s.bin = kBins - 1 - 2 * threadIdx.x - (upper ? 0 : 1);
+    s.left = left - before - (upper ? 0 : hi);
   }
   __syncthreads();
-  int at = 0, ties = 0;
-  for (int w = 0; w < wave; ++w) {
-    at += gt[w] + min(eq[w], max(0, left - ties));
-    ties += eq[w];
+}
+
+__device__ __forceinline__ int length_of(const KvKeepArgs& a, int64_t row) {
+  return (int)min<int64_t>(a.lengths[row / a.heads], a.slots);
+}
+
+__device__ __forceinline__ void none(const KvKeepArgs& a, int32_t* out) {
+  for (int i = threadIdx.x; i < a.n; i += kThreads) out[i] = -1;
+}
+
+// A row a workgroup, of up to 1,024 R slots.
+template <int R>
+__global__ __launch_bounds__(kThreads) void kv_keep_kernel(KvKeepArgs a) {
+  __shared__ uint32_t hist[kBins];
+  __shared__ Pick s;
+  __shared__ int waves[kWaves][2];
+  const int64_t row = blockIdx.x;
+  const int length = length_of(a, row), tid = threadIdx.x;
+  int32_t* out = a.kept + row * a.n;
+  if (length <= a.above) return none(a, out);
+  const Ranks<R> ranks(a, a.mass + row * a.slots, 0, length);
+  uint32_t cut = 0;
+  int left = a.n;
+#pragma unroll 1
+  for (int digit = 0; digit < kDigits; ++digit) {
+    hist[tid] = hist[tid + kThreads] = 0;
+    __syncthreads();
+    ranks.count(hist, digit, cut);
+    __syncthreads();
+    pick((int)hist[kBins - 1 - 2 * tid], (int)hist[kBins - 2 - 2 * tid], left, s);
+    cut |= s.bin << shift_of(digit);
+    left = s.left;
+    if (left == (int)hist[s.bin] && cut != 0 && digit + 1 < kDigits) {
+      // all of the bin are taken: those above the rank below it
+      cut -= 1;
+      left = 0;
+      break;
+    }
+    __syncthreads();
   }
-  const uint64_t below = (uint64_t(1) << lane) - 1;
-  for (int i = from + lane; i - lane < to; i += 64) {
-    const uint32_t k = i < to ? rank(i) : 0;
-    const bool tie = k == cut && i < to;
-    const uint64_t tied = __ballot(tie);
-    const bool take = k > cut || (tie && ties + bits(tied & below) < left);
-    const uint64_t taken = __ballot(take);
-    if (take) out[at + bits(taken & below)] = i;
-    at += bits(taken);
-    ties += bits(tied);
+  ranks.take(cut, left, out, waves);
+}
+
+// ---- rows in parts ----------------------------------------------------------------
+
+// The workspace, for each row and part: a histogram for each digit, how many of it
+// are above the digits known; for each row: those digits and how many are left.
+struct Work {
+  uint32_t* hist;  // [rows][parts][3][2048]
+  int* above;      // [rows][parts][2]: by the first digit, by the second
+  uint32_t* known; // [rows][2][2]: after the first and second digit: prefix, left
+};
+__host__ __device__ __forceinline__ int64_t parts_of(const KvKeepArgs& a) {
+  return (a.slots + kPart - 1) / kPart;
+}
+__device__ __forceinline__ Work work_of(const KvKeepArgs& a) {
+  const int64_t rows = a.requests * a.heads, units = rows * parts_of(a);
+  uint32_t* w = (uint32_t*)a.work;
+  return {w, (int*)(w + units * kDigits * kBins), w + units * (kDigits * kBins + 2)};
+}
+
+// STEP 0, 1, 2: the part's histogram of that digit, the one before it being found
+// first.  STEP 3: the list.
+template <int STEP>
+__global__ __launch_bounds__(kThreads) void kv_keep_part_kernel(KvKeepArgs a) {
+  __shared__ uint32_t hist[kBins];
+  __shared__ Pick s;
+  __shared__ int waves[kWaves][2];
+  __shared__ int sums[kWaves];
+  const int parts = (int)parts_of(a), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t row = blockIdx.x / parts;
+  const int part = (int)(blockIdx.x % parts), length = length_of(a, row);
+  int32_t* out = a.kept + row * a.n;
+  if (length <= a.above) {
+    if (STEP == 3 && part == 0) none(a, out);
+    return;
   }
+  const int some = (length + kPart - 1) / kPart;  // parts that hold tokens
+  if (part >= some) return;
+  const Work work = work_of(a);
+  const Ranks<kPart / kThreads> ranks(a, a.mass + row * a.slots, part * kPart, length);
+  const auto hist_of = [&](int p, int digit) {
+    return work.hist + ((row * parts + p) * kDigits + digit) * kBins;
+  };
+  uint32_t prefix = 0;
+  int left = a.n;
+  const int b0 = kBins - 2 - 2 * tid;  // this thread's bins: b0 + 1, b0
+  if constexpr (STEP > 0) {
+    constexpr int kDigit = STEP - 1;
+    if constexpr (STEP > 1) {
+      prefix = work.known[row * 4 + (STEP - 2) * 2];
+      left = (int)work.known[row * 4 + (STEP - 2) * 2 + 1];
+    }
+    int hi = 0, lo = 0;
+#pragma unroll 8
+    for (int p = 0; p < some; ++p) {
+      const uint2 x = *(const uint2*)(hist_of(p, kDigit) + b0);
+      lo += (int)x.x;
+      hi += (int)x.y;
+    }
+    pick(hi, lo, left, s);
+    const uint32_t bin = s.bin;
+    prefix |= bin << shift_of(kDigit);
+    left = s.left;
+    // how many of a part are above the bin
+    const auto over = [&](int p) {
+      const uint2 x = *(const uint2*)(hist_of(p, kDigit) + b0);
+      return (b0 + 1 > (int)bin ? (int)x.y : 0) + (b0 > (int)bin ? (int)x.x : 0);
+    };
+    const auto total = [&](int x) {
+#pragma unroll
+      for (int i = 32; i >= 1; i >>= 1) x += __shfl_xor(x, i);
+      if (lane == 0) sums[wave] = x;
+      __syncthreads();
+      x = 0;
+      for (int w = 0; w < kWaves; ++w) x += sums[w];
+      return x;
+    };
+    if constexpr (STEP < 3) {
+      const int mine = total(over(part));
+      if (tid == 0) {
+        work.above[(row * parts + part) * 2 + kDigit] = mine;
+        if (part == 0) {
+          work.known[row * 4 + kDigit * 2] = prefix;
+          work.known[row * 4 + kDigit * 2 + 1] = (uint32_t)left;
+        }
+      }
+    } else {
+      // where this part's tokens go: after those of the parts before it
+      int gt = 0, eq = 0;
+      for (int p = 0; p < part; ++p) gt += over(p);
+      for (int p = tid; p < part; p += kThreads) {
+        gt += work.above[(row * parts + p) * 2] + work.above[(row * parts + p) * 2 + 1];
+        eq += (int)hist_of(p, kDigit)[bin];
+      }
+      gt = total(gt);
+      __syncthreads();
+      eq = total(eq);
+      ranks.take(prefix, max(0, left - eq), out + gt + min(eq, left), waves);
+      return;
+    }
+  }
+  hist[tid] = hist[tid + kThreads] = 0;
+  __syncthreads();
+  ranks.count(hist, STEP, prefix);
+  __syncthreads();
+  uint2* to = (uint2*)hist_of(part, STEP);
+  to[tid] = *(const uint2*)(hist + 2 * tid);
+}
+
+template <int STEP>
+hipError_t launch_step(const KvKeepArgs& a, hipStream_t s) {
+  kv_keep_part_kernel<STEP><<<dim3((unsigned)kv_keep_grid(a)), kThreads, 0, s>>>(a);
+  return hipGetLastError();
 }
 
 }  // namespace
 
-int64_t kv_keep_grid(const KvKeepArgs& a) { return a.requests * a.heads; }
+int64_t kv_keep_workspace(const KvKeepArgs& a) {
+  if (a.slots <= kRowSlots) return 0;
+  const int64_t rows = a.requests * a.heads;
+  return 4 * (rows * parts_of(a) * (kDigits * kBins + 2) + 4 * rows);
+}
+
+int64_t kv_keep_grid(const KvKeepArgs& a) {
+  return a.requests * a.heads * (a.slots <= kRowSlots ? 1 : parts_of(a));
+}
 
 hipError_t launch_kv_keep(const KvKeepArgs& a, hipStream_t s) {
-  kv_keep_kernel<<<dim3((unsigned)kv_keep_grid(a)), kThreads, 0, s>>>(a);
-  return hipGetLastError();
+  if (a.slots <= kRowSlots) {
+    const dim3 grid((unsigned)kv_keep_grid(a));
+    if (a.slots <= 4096) kv_keep_kernel<4><<<grid, kThreads, 0, s>>>(a);
+    else if (a.slots <= 16384) kv_keep_kernel<16><<<grid, kThreads, 0, s>>>(a);
+    else if (a.slots <= 32768) kv_keep_kernel<32><<<grid, kThreads, 0, s>>>(a);
+    else kv_keep_kernel<64><<<grid, kThreads, 0, s>>>(a);
+    return hipGetLastError();
+  }
+  hipError_t e = launch_step<0>(a, s);
+  if (e == hipSuccess) e = launch_step<1>(a, s);
+  if (e == hipSuccess) e = launch_step<2>(a, s);
+  if (e == hipSuccess) e = launch_step<3>(a, s);
+  return e;
 }
 
 }  // namespace mlxvs::kern

@@ -477,16 +477,23 @@ class PagedKVCache:
 
     def _workspace(self, size, q, qs, *args):
         """(tensor, bytes) of scratch memory on the current stream."""
-        key = (size, q.shape, qs.columns, qs.requests, args)
+        return self._memory((size, q.shape, qs.columns, qs.requests, args), q, size, self._ref,
+                            ctypes.byref(qs), *args)
+
+    def _scratch(self, size, like, *args):
+        """The same for calls whose sizes are the numbers among args."""
+        return self._memory((size, args), like, size, *args)
+
+    def _memory(self, key, like, size, *args):
         need = self._sizes.get(key)
         if need is None:
-            need = getattr(_L(), size)(self._ref, ctypes.byref(qs), *args)
+            need = getattr(_L(), size)(*args)
             if need < 0:
                 raise ValueError(_L().mlxvs_last_error().decode())
             if len(self._sizes) >= 1024:
                 self._sizes.clear()
             self._sizes[key] = need
-        return (q.new_empty(need, dtype=torch.uint8) if need else None), need
+        return (like.new_empty(need, dtype=torch.uint8) if need else None), need
 
     def select(self, q, table, requests, positions, n, *, first=1, last=1):
         """The ``n`` best blocks of each token and kv head: int32 [tokens,
@@ -632,9 +639,12 @@ class PagedKVCache:
         with _On(device) as stream:
             _need(n >= 1, op, "n must be at least 1.")
             kept = mass.new_empty((requests, self.kv_heads, n), dtype=torch.int32)
+            work, size = self._scratch("mlxvs_kv_keep_workspace", mass, requests, self.kv_heads,
+                                       mass.shape[2])
             _check(_L().mlxvs_kv_keep_device(pm, requests, self.kv_heads, mass.shape[2], pl, n,
                                              int(first), int(recent),
                                              n if above is None else int(above), kept.data_ptr(),
+                                             None if work is None else work.data_ptr(), size,
                                              stream))
         return kept
 
@@ -680,14 +690,8 @@ class PagedKVCache:
                 _need(isinstance(out, KvCompact), op, "out must be a KvCompact.")
             po = _ints(out.lengths, "out.lengths", op, device, size=requests)
             pn = _ints(out.cursor, "out.cursor", op, device, size=1)
-            key = ("compact", requests, columns, n)
-            need = self._sizes.get(key)
-            if need is None:
-                need = _L().mlxvs_kv_compact_workspace(cache, columns, requests, n)
-                if need < 0:
-                    raise ValueError(_L().mlxvs_last_error().decode())
-                self._sizes[key] = need
-            work = lengths.new_empty(need, dtype=torch.uint8) if need else None
+            work, need = self._scratch("mlxvs_kv_compact_workspace", lengths, cache, columns,
+                                       requests, n)
             _check(_L().mlxvs_kv_compact_device(
                 cache, pt, stride, columns, requests, pl, kept.data_ptr(), n, pf,
                 free_pages.numel(), pc, pm, slots, po, pn,

@@ -49,7 +49,7 @@ def weigh(lib, c=None, q=None, starts=P, lse=P, scale=0.125, decay=1.0, longest=
 
 def keep(lib, **k):
     f = dict(mass=P, requests=2, heads=2, slots=80, lengths=P, n=16, first=1, recent=1, above=16,
-             kept=P)
+             kept=P, work=P, size=1 << 40)
     f.update(k)
     return lib.mlxvs_kv_keep_device(*f.values(), None)
 
@@ -175,6 +175,17 @@ def test_budgets_that_are_refused(engine, bad):
     lib = lib_of(engine)
     assert keep(lib, **bad) == INVALID
     assert b"[mlxvs::kv_keep]" in lib.mlxvs_last_error()
+
+
+def test_budgets_of_long_rows_need_a_workspace(engine):
+    lib = lib_of(engine)
+    assert lib.mlxvs_kv_keep_workspace(2, 2, 60_000) == 0
+    assert lib.mlxvs_kv_keep_workspace(2, 2, -1) == -1
+    need = lib.mlxvs_kv_keep_workspace(2, 2, 100_000)
+    assert need > 0
+    for k in (dict(work=None), dict(size=need - 1), dict(work=P + 8)):
+        assert keep(lib, slots=100_000, **k) == INVALID
+        assert b"workspace" in lib.mlxvs_last_error()
 
 
 @pytest.mark.parametrize("bad", [
