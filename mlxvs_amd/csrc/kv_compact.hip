@@ -377,7 +377,9 @@ hipError_t launch_kv_compact(const KvCompactArgs& a, hipStream_t s) {
   kv_compact_plan_kernel<<<1 + clear, kPlanThreads, 0, s>>>(a);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || a.requests == 0) return e;
   if (a.c.dim <= 64) launch_move<64>(a, s);
+  else if (a.c.dim <= 96) launch_move<96>(a, s);
   else if (a.c.dim <= 128) launch_move<128>(a, s);
+  else if (a.c.dim <= 192) launch_move<192>(a, s);
   else launch_move<256>(a, s);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   const int pages = a.n >> a.c.lps;
