@@ -423,7 +423,7 @@ def test_budgets_of_rows_of_any_length(engine, slots):
         check_keep(engine, mass, lengths, n, first, recent)
 
 
-@pytest.mark.parametrize("slots,n", [(20_000, 5_000), (33_000, 9), (65_536, 65_000), (70_000, 300), (70_000, 69_999),
+@pytest.mark.parametrize("slots,n", [(20_000, 5_000), (33_000, 150), (65_536, 65_000), (70_000, 300), (70_000, 69_999),
                                      (140_001, 40_000)])
 def test_budgets_of_long_rows(engine, slots, n):
     rng = np.random.default_rng(slots)

@@ -179,7 +179,7 @@ def test_budgets_that_are_refused(engine, bad):
 
 def test_budgets_of_long_rows_need_a_workspace(engine):
     lib = lib_of(engine)
-    assert lib.mlxvs_kv_keep_workspace(2, 2, 60_000) == 0
+    assert lib.mlxvs_kv_keep_workspace(2, 2, 30_000) == 0
     assert lib.mlxvs_kv_keep_workspace(2, 2, -1) == -1
     need = lib.mlxvs_kv_keep_workspace(2, 2, 100_000)
     assert need > 0
