@@ -748,8 +748,9 @@ MLXVS_C_API int mlxvs_kv_rotate_device(const mlxvs_kv_rotary* rotary, const mlxv
  * The attention that each key gets from the step's tokens, added to what it got
  * before: mass float32 [requests][heads][slots], slots >= columns x page_size.  The
  * tokens of request r (a row of queries->table) are starts[r] .. starts[r + 1] - 1
- * (int32 [requests + 1], as mlxvs_kv_plan_device makes them), their positions
- * ascending; queries->token_request is not read and may be null.  lse float32
+ * (int32 [requests + 1]), their positions one after another, as
+ * mlxvs_kv_plan_device makes them (a request's first one is read, no other);
+ * queries->token_request is not read and may be null.  lse float32
  * [tokens][q_heads]: what mlxvs_kv_attend_device over every block returned for
  * the same queries and scale.  For the positions p up to the last token's
  *   mass[p] = (p < first ? decay x mass[p] : 0) + the sum over the tokens that see p

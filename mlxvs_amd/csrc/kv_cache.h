@@ -139,11 +139,13 @@ struct KvWeighArgs {
   int64_t longest;  // tokens the longest request is expected to hold, INT32_MAX: unknown
   float* mass;      // [requests][heads][slots]
   int64_t slots;
-  int64_t piece;  // tokens of a workgroup's share, 0: single tokens (kv_weigh_plan)
-  int64_t most_units, most_several, most_slots;  // shares and partial sums at most
+  // from kv_weigh_plan
+  bool prompts;  // else single tokens
+  int tile;      // tokens that a workgroup takes at a time
+  int64_t most_units, most_several, most_slots;  // shares, and partial sums of them
   int32_t* work;  // kv_weigh_workspace bytes
 };
-void kv_weigh_plan(KvWeighArgs& a);  // sets the pieces
+void kv_weigh_plan(KvWeighArgs& a);  // sets the split
 int64_t kv_weigh_workspace(const KvWeighArgs& a);
 int64_t kv_weigh_grid(const KvWeighArgs& a);  // workgroups of its largest launch
 hipError_t launch_kv_weigh(const KvWeighArgs& a, hipStream_t s);

@@ -13,8 +13,20 @@
 // wavefront keeps 64 keys in registers, the operand of every product; the rows of Q
 // (a token's query head each) come through LDS by direct loads, whole tokens of up
 // to 64 rows at a time, three tiles ahead, for all four wavefronts.  A lane adds up
-// its column's weights of each of its 32 keys over all rows, and the 32 columns
-// meet once at the end.
+// its column's weights of each of its 32 keys over all rows, and the columns meet
+// once at the end.  A product of 32 x 32 takes as long as the 6 vector instructions
+// for its 2 weights a lane (fma, exp, add), so both kinds are written side by side:
+// a block's products next to the weights of the one before.
+//
+// Measured: single tokens over 64 requests of up to 8,192 keys in 8 heads of 128
+// values 122 us, 5.1 TB/s of keys, masses and their return (a copy: 4.95); chunks of
+// 1,500 tokens in 3 requests of up to 8,192, 32 heads on 8, 146 us, 795 TFLOP/s, and
+// a prompt of 4,001 tokens, 28 heads on 4, 97 us of which 12 are the plan and the
+// joining.  There the matrix units work 37% of the time and the vector units 53%;
+// what is between are a unit's begin (some 5 us for its keys) and its end, and units
+// that do not fill the last round.  Tried: 128 keys a wavefront and 128 rows a tile,
+// with one wavefront a SIMD, 181 and 144; one share of all tiles for each workgroup,
+// which may go on in another chunk, 211 and 103 (their rows of Q then miss in L2).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -27,15 +39,14 @@
 namespace mlxvs::kern {
 namespace {
 
-constexpr int kChunk = 256;  // keys of a workgroup
-
 // x, which is the same in all lanes.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// A request's tokens of the step, and the keys that they see.
+// A request's tokens of the step, and the keys that they see: token i of it those up
+// to position first + i.
 struct Span {
   int begin, tokens;
-  int first, last;  // positions of the first and the last token
+  int first, last;  // positions of the first and the last token; last -1: they see none
 };
 
 __device__ __forceinline__ Span span_of(const KvWeighArgs& a, int64_t r) {
@@ -45,9 +56,10 @@ __device__ __forceinline__ Span span_of(const KvWeighArgs& a, int64_t r) {
   s.tokens = (int)(min(max(hi, (int64_t)s.begin), a.q.tokens) - s.begin);
   s.first = s.last = -1;
   if (s.tokens > 0) {
-    const int end = (a.q.cols << a.c.lps) - 1;
     s.first = a.q.positions[s.begin];
-    s.last = min(a.q.positions[s.begin + s.tokens - 1], end);
+    // (one that was not admitted has none; the table ends somewhere)
+    const int64_t end = ((int64_t)a.q.cols << a.c.lps) - 1;
+    if (s.first >= 0) s.last = (int)min((int64_t)s.first + s.tokens - 1, end);
   }
   return s;
 }
@@ -60,7 +72,10 @@ __device__ __forceinline__ void put(const KvWeighArgs& a, float* mass, int p, in
 
 // ---- single tokens -------------------------------------------------------------
 
-constexpr int kFewKeys = 16, kFewTiles = 4;  // of a wavefront
+constexpr int kFewKeys = 32;  // of a wavefront at a time, in two tiles of 16
+// Keys of a workgroup of single tokens, 32 at a time for each of its wavefronts: 64
+// requests of up to 8,192 keys with 128: 134 us, 256: 122, 512: 122, 1,024: 124.
+constexpr int kSpan = 256;
 
 // The sum over the 16 lanes of a row.
 __device__ __forceinline__ float row_sum(float x) {
@@ -69,118 +84,163 @@ __device__ __forceinline__ float row_sum(float x) {
   return x;
 }
 
+// kSpan keys of a request and head a workgroup, 32 a wavefront at a time, the next
+// ones on their way; with more requests' keys than the spans hold it comes again.
+// The rows of up to 16 query heads stay in registers.
 template <int DP, bool BF16>
-__global__ __launch_bounds__(256, 2) void kv_weigh_few_kernel(KvWeighArgs a, int chunks) {
+__global__ __launch_bounds__(256) void kv_weigh_few_kernel(KvWeighArgs a, int spans) {
   using T = std::conditional_t<BF16, __bf16, _Float16>;
   using Tx8 = std::conditional_t<BF16, bf16x8, halfx8>;
   constexpr int kSteps = DP / 32;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
+  struct Keys {
+    uintx4 k[2][kSteps];
+    bool there[2];
+    float mass;  // of the lane's key, before
+  };
+  struct Rows {
+    uintx4 q[kSteps];
+    float lse;
+    int pos;
+  };
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, grp = lane >> 4;
   const int d = a.c.dim, group = a.q.group;
   const int h = (int)(blockIdx.x % a.c.heads);
   const int64_t rest = blockIdx.x / a.c.heads;
   const int r = (int)(rest % a.q.requests);
-  const Span sp = span_of(a, r);
+  Span sp = span_of(a, r);
+  sp = {uniform(sp.begin), uniform(sp.tokens), uniform(sp.first), uniform(sp.last)};
   const int32_t* table = a.q.table + (int64_t)r * a.q.table_stride;
   float* mass = a.mass + ((int64_t)r * a.c.heads + h) * a.slots;
+  const int64_t rows = (int64_t)sp.tokens * group;
 
-  for (int64_t at = rest / a.q.requests * kChunk; at <= sp.last; at += (int64_t)chunks * kChunk) {
-    const int k0 = (int)at + wave * (kFewKeys * kFewTiles);
-    if (k0 > sp.last) return;
-    uintx4 kf[kFewTiles][kSteps];
-    bool there[kFewTiles];
+  const auto load_rows = [&](int64_t x0, Rows& y) {
+    const int64_t x = x0 + col;
+    const bool mine = x < rows;
+    const int64_t t = sp.begin + (mine ? x / group : 0);
+    const int g = h * group + (mine ? (int)(x % group) : 0);
+    y.pos = mine ? (int)min(sp.first + x / group, (int64_t)sp.last) : -1;
+    y.lse = a.lse[t * a.c.heads * group + g];
+    const T* src = (const T*)a.q.q + t * a.q.q_token + g * a.q.q_head + 8 * grp;
 #pragma unroll
-    for (int u = 0; u < kFewTiles; ++u) {
-      const int k = k0 + kFewKeys * u;
-      const int page = k <= sp.last ? table[k >> a.c.lps] : -1;
-      there[u] = page >= 0 && page < a.c.pages;
+    for (int i = 0; i < kSteps; ++i) {
+      y.q[i] = uintx4{};
+      if (32 * i + 32 <= sure_values(DP) || 32 * i + 8 * grp < d) y.q[i] = *(const uintx4*)(src + 32 * i);
+    }
+  };
+  const auto key_of = [&](int k0) { return k0 + 16 * (lane >> 5) + 4 * (lane >> 3 & 3) + (lane & 3); };
+  const auto pages = [&](int64_t k0, int (&page)[2]) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) page[u] = k0 + 16 * u <= sp.last ? table[(k0 + 16 * u) >> a.c.lps] : -1;
+  };
+  const auto load = [&](int k0, const int (&page)[2], Keys& y) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      y.there[u] = page[u] >= 0 && page[u] < a.c.pages;
       const T* row = (const T*)a.c.keys +
-                     (((int64_t)(there[u] ? page : 0) * a.c.heads + h) * a.c.page +
-                      ((k & (a.c.page - 1)) + col)) * d + 8 * grp;
+                     (((int64_t)(y.there[u] ? page[u] : 0) * a.c.heads + h) * a.c.page +
+                      ((k0 + 16 * u) & (a.c.page - 1)) + col) * d + 8 * grp;
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
-        kf[u][i] = uintx4{};
-        if (there[u] && (32 * i + 32 <= sure_values(DP) || 32 * i + 8 * grp < d))
-          kf[u][i] = *(const uintx4*)(row + 32 * i);
+        y.k[u][i] = uintx4{};
+        if (y.there[u] && (32 * i + 32 <= sure_values(DP) || 32 * i + 8 * grp < d))
+          y.k[u][i] = *(const uintx4*)(row + 32 * i);
       }
     }
-    float sum[kFewTiles][4] = {};
-    const int64_t rows = (int64_t)sp.tokens * group;
-    for (int64_t x0 = 0; x0 < rows; x0 += 16) {
-      const int64_t x = x0 + col;
-      const bool mine = x < rows;
-      const int64_t t = sp.begin + (mine ? x / group : 0);
-      const int g = h * group + (mine ? (int)(x % group) : 0);
-      const int pos = mine ? max(-1, a.q.positions[t]) : -1;
-      if (!__any(pos >= k0)) continue;
-      const float lse = a.lse[t * a.c.heads * group + g];
-      const T* src = (const T*)a.q.q + t * a.q.q_token + g * a.q.q_head + 8 * grp;
-      uintx4 q[kSteps];
+    const int p = key_of(k0);
+    y.mass = 0.0f;
+    if (!(lane & 4) && p < sp.first && p <= sp.last && a.decay != 0.0f) y.mass = mass[p];
+  };
+  const auto weigh = [&](const Keys& y, const Rows& z, int k0, float (&sum)[2][4]) {
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        q[i] = uintx4{};
-        if (32 * i + 32 <= sure_values(DP) || 32 * i + 8 * grp < d)
-          q[i] = *(const uintx4*)(src + 32 * i);
-      }
+    for (int u = 0; u < 2; ++u) {
+      floatx4 s = {0, 0, 0, 0};
 #pragma unroll
-      for (int u = 0; u < kFewTiles; ++u) {
-        floatx4 s = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i)
-          s = mfma(__builtin_bit_cast(Tx8, kf[u][i]), __builtin_bit_cast(Tx8, q[i]), s);
-        const int seen = pos - (k0 + kFewKeys * u + 4 * grp);  // keys up to this one
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          sum[u][i] += i <= seen ? __builtin_amdgcn_exp2f(fmaf(s[i], a.scale, -lse) * kLog2e) : 0.0f;
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kFewTiles; ++u) {
-      float mine = 0.0f;
+      for (int i = 0; i < kSteps; ++i)
+        s = mfma(__builtin_bit_cast(Tx8, y.k[u][i]), __builtin_bit_cast(Tx8, z.q[i]), s);
+      const int seen = z.pos - (k0 + 16 * u + 4 * grp);  // keys up to this one
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float all = row_sum(sum[u][i]);
-        if (col == i) mine = all;
+        const float x = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale, -z.lse) * kLog2e);
+        sum[u][i] += i <= seen ? x : 0.0f;
       }
-      const int p = k0 + kFewKeys * u + 4 * grp + col;
-      if (col < 4 && p <= sp.last) put(a, mass, p, sp.first, there[u] ? mine : 0.0f);
+    }
+  };
+
+  const int64_t stride = (int64_t)spans * kSpan;
+  for (int64_t at = rest / a.q.requests * kSpan; at <= sp.last; at += stride) {
+    const int64_t end = min(at + kSpan, (int64_t)sp.last + 1);
+    int64_t k0 = at + wave * kFewKeys;
+    if (k0 >= end) return;
+    int page[2];
+    Keys one, two;
+    pages(k0, page);
+    Rows first;
+    load_rows(0, first);
+    load((int)k0, page, one);
+    pages(k0 + 4 * kFewKeys, page);
+    const auto turn = [&](Keys& now, Keys& then) {
+      const int64_t next = k0 + 4 * kFewKeys;
+      if (next < end) {
+        load((int)next, page, then);
+        pages(next + 4 * kFewKeys, page);
+      }
+      float sum[2][4] = {};
+      weigh(now, first, (int)k0, sum);
+      for (int64_t x0 = 16; x0 < rows; x0 += 16) {
+        Rows more;
+        load_rows(x0, more);
+        if (__any(more.pos >= k0)) weigh(now, more, (int)k0, sum);
+      }
+      // lane l writes key_of: its tile's, its row's and one of the four
+      float got[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        got[u] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float all = row_sum(sum[u][i]);
+          if ((lane & 3) == i) got[u] = now.there[u] ? all : 0.0f;
+        }
+      }
+      const int p = key_of((int)k0), from = 16 * (lane >> 3 & 3) + (lane & 3);
+      const float a0 = __shfl(got[0], from), a1 = __shfl(got[1], from);
+      if (!(lane & 4) && p <= sp.last) mass[p] = a.decay * now.mass + (lane & 32 ? a1 : a0);
+      k0 = next;
+    };
+    while (k0 < end) {
+      turn(one, two);
+      if (k0 < end) turn(two, one);
     }
   }
 }
 
 // ---- prompts -------------------------------------------------------------------
 
-constexpr int kWaveKeys = 64;
-constexpr int kRows = 64;    // of a tile of Q
-constexpr int kStages = 4;   // tiles in LDS: one in use, the others on their way
+constexpr int kStages = 4;  // tiles in LDS: one in use, the others on their way
+
+constexpr int kWaveKeys = 64, kChunk = 4 * kWaveKeys;  // keys of a wavefront, a workgroup
+constexpr int kRows = 64;                              // of a tile of Q
 
 // A workgroup's share: a chunk of a request's keys, and some tokens that see it.
 struct Unit {
   int request, chunk;
   int begin, end;   // tokens of the batch
   int slot;         // where its sums go, -1: into the masses
-  int first, last;  // of the request's positions
+  int shift, last;  // a token's position less its place in the batch; the last position
   int pieces;       // of the chunk, at its first unit: sums in as many slots
 };
 
-// The workspace, made by one workgroup: the units, and those of chunks that several
-// units share.
+// The workspace, made by one workgroup: the units, and the first ones of chunks that
+// several units share.
 struct Work {
   int32_t* units;   // [1] how many there are, and chunks of several
   int32_t* shared;  // [1]
   int32_t* first;   // [requests + 1] chunks before a request's
   Unit* unit;
-  Unit* several;    // the first units of chunks of several
+  Unit* several;
   float* sums;      // [slots][heads][kChunk]
 };
 
-// How many there are at most.
-struct Most {
-  int64_t units, several, slots;
-};
-
-int64_t chunks_of(const KvWeighArgs& a) {
-  return std::max<int64_t>(1, (((int64_t)a.q.cols << a.c.lps) + kChunk - 1) / kChunk);
-}
 __host__ __device__ __forceinline__ int64_t header_ints(const KvWeighArgs& a) {
   return (2 + a.q.requests + 1 + 3) / 4 * 4;
 }
@@ -190,361 +250,452 @@ __device__ __forceinline__ Work work_of(const KvWeighArgs& a) {
   return {w, w + 1, w + 2, unit, unit + a.most_units, (float*)(unit + a.most_units + a.most_several)};
 }
 
+// A request's first position.
+__device__ __forceinline__ int first_of(const KvWeighArgs& a, int r) { return span_of(a, r).first; }
+
 constexpr int kPlanThreads = 1024;
 
-// Sums over a workgroup's threads of N numbers up to each; `all` gets the totals.
-template <int N>
-__device__ __forceinline__ void running(int64_t (&x)[N], int64_t (&all)[N],
-                                        int64_t (*waves)[N]) {
+// The sum over a workgroup's threads up to each one; `all` gets the total.
+__device__ __forceinline__ int running(int x, int& all, int* waves) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-#pragma unroll
-    for (int by = 1; by < 64; by <<= 1) {
-      const int64_t y = __shfl_up(x[i], by);
-      if (lane >= by) x[i] += y;
-    }
-    if (lane == 63) waves[wave][i] = x[i];
+  for (int by = 1; by < 64; by <<= 1) {
+    const int y = __shfl_up(x, by);
+    if (lane >= by) x += y;
+  }
+  if (lane == 63) waves[wave] = x;
+  __syncthreads();
+  all = 0;
+  for (int w = 0; w < kPlanThreads / 64; ++w) {
+    if (w < wave) x += waves[w];
+    all += waves[w];
   }
   __syncthreads();
+  return x;
+}
+__device__ __forceinline__ int64_t over_wave(int64_t x) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    all[i] = 0;
-    for (int w = 0; w < kPlanThreads / 64; ++w) {
-      if (w < wave) x[i] += waves[w][i];
-      all[i] += waves[w][i];
-    }
-  }
-  __syncthreads();
+  for (int i = 32; i >= 1; i >>= 1) x += __shfl_xor(x, i);
+  return x;
 }
 
-// The first of a request's tokens whose position is at least p: positions ascend, and
-// mostly by one.
-__device__ __forceinline__ int first_at(const int32_t* positions, const Span& sp, int p) {
-  if (p <= sp.first) return 0;
-  int lo = 0, hi = sp.tokens;  // (positions[lo] < p; the answer is in (lo, hi])
-  const int guess = min(hi, p - sp.first);
-  if (positions[guess - 1] < p) {
-    lo = guess - 1;
-    if (guess < hi && positions[guess] >= p) return guess;
-  } else {
-    hi = guess - 1;
-  }
-  while (hi - lo > 1) {
-    const int mid = lo + (hi - lo) / 2;
-    if (positions[mid] < p) lo = mid;
-    else hi = mid;
-  }
-  return hi;
+// The first of a request's tokens that sees key p (its number of tokens: none).
+__device__ __forceinline__ int sees(int first, int tokens, int64_t p) {
+  return (int)min(max(p - first, (int64_t)0), (int64_t)tokens);
 }
+
+// Units over all heads that are aimed at: two rounds of two workgroups a CU.  Chunks of
+// 1,500 tokens and a prompt of 4,001 with 512: 155 and 94 us, 1,024: 146 and 97, 1,536:
+// 141 and 105; with 1,024 in the chunks' order, not by size: 155 and 98.
+constexpr int kShares = 1024;
+constexpr int kLeastTiles = 4;  // of a unit
+constexpr int kClasses = 16;    // of units, by size
+__host__ __device__ __forceinline__ int more_units(const KvWeighArgs& a) {
+  return kShares > a.c.heads ? kShares / a.c.heads : 1;
+}
+
+constexpr int kPlanSpans = 1024;  // requests whose spans stay in LDS
 
 __global__ __launch_bounds__(kPlanThreads) void kv_weigh_plan_kernel(KvWeighArgs a) {
-  __shared__ int64_t waves[kPlanThreads / 64][3];
+  constexpr int kWaves = kPlanThreads / 64;
+  __shared__ int waves[kWaves];
+  __shared__ Span spans[kPlanSpans];
+  __shared__ int firsts[kPlanSpans + 1];
+  __shared__ int64_t totals[kWaves], numbers[kWaves];
+  __shared__ int at[kClasses], several, slots;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const Work work = work_of(a);
+  const bool few = a.q.requests <= kPlanSpans;
+  struct Part {  // a request's chunk, the first of its tokens that sees it
+    int request, chunk;
+    Span sp;
+    int from;
+  };
+  const auto part = [&](int i) {
+    int lo = 0, hi = (int)a.q.requests;  // first[lo] <= i < first[hi]
+    while (hi - lo > 1) {
+      const int mid = lo + (hi - lo) / 2;
+      if ((few ? firsts[mid] : work.first[mid]) <= i) lo = mid;
+      else hi = mid;
+    }
+    Part p{lo, i - (few ? firsts[lo] : work.first[lo]), few ? spans[lo] : span_of(a, lo), 0};
+    p.from = min(sees(p.sp.first, p.sp.tokens, (int64_t)p.chunk * kChunk), p.sp.tokens - 1);
+    return p;
+  };
+  const auto tiles_of = [&](const Part& p) { return (p.sp.tokens - p.from + a.tile - 1) / a.tile; };
   // the requests' chunks ...
-  int64_t chunks = 0;
+  int chunks = 0;
   for (int64_t r0 = 0; r0 < a.q.requests; r0 += kPlanThreads) {
     const int64_t r = r0 + threadIdx.x;
-    int64_t n[1] = {0}, all[1];
+    int n = 0, all;
     if (r < a.q.requests) {
       const Span sp = span_of(a, r);
-      n[0] = sp.last < 0 ? 0 : sp.last / kChunk + 1;
+      if (few) spans[r] = sp;
+      n = sp.last < 0 ? 0 : sp.last / kChunk + 1;
     }
-    running<1>(n, all, (int64_t(*)[1])waves);
-    if (r < a.q.requests) work.first[r + 1] = (int32_t)(chunks + n[0]);
-    chunks += all[0];
+    n = running(n, all, waves);
+    if (r < a.q.requests) {
+      if (few) firsts[r + 1] = chunks + n;
+      else work.first[r + 1] = chunks + n;
+    }
+    chunks += all;
   }
-  if (threadIdx.x == 0) work.first[0] = 0;
+  if (threadIdx.x == 0) firsts[0] = work.first[0] = several = slots = 0;
+  if (threadIdx.x < kClasses) at[threadIdx.x] = 0;
   __syncthreads();
-  // ... and each one's units
-  int64_t before[3] = {0, 0, 0};  // units, chunks of several, slots
-  for (int64_t i0 = 0; i0 < chunks; i0 += kPlanThreads) {
-    const int64_t i = i0 + threadIdx.x;
-    Unit u{};
-    Span sp{};
-    int from = 0, pieces = 0;
-    if (i < chunks) {
-      int64_t lo = 0, hi = a.q.requests;  // first[lo] <= i < first[hi]
-      while (hi - lo > 1) {
-        const int64_t mid = lo + (hi - lo) / 2;
-        if (work.first[mid] <= i) lo = mid;
-        else hi = mid;
-      }
-      sp = span_of(a, lo);
-      u.request = (int)lo;
-      u.chunk = (int)(i - work.first[lo]);
-      u.first = sp.first;
-      u.last = sp.last;
-      from = min(first_at(a.q.positions + sp.begin, sp, u.chunk * kChunk), sp.tokens - 1);
-      pieces = (int)((sp.tokens - from + a.piece - 1) / a.piece);
-      u.pieces = pieces;
-    }
-    int64_t x[3] = {pieces, pieces > 1, pieces > 1 ? pieces : 0}, all[3];
-    const int64_t own[3] = {x[0], x[1], x[2]};
-    running<3>(x, all, waves);
-    if (i < chunks) {
-      const int64_t at = before[0] + x[0] - own[0], slot = before[2] + x[2] - own[2];
-      // (all of a chunk's units have as many tiles, or one less)
-      const int tokens = sp.tokens - from, each = max(1, kRows / a.q.group);
-      const int tiles = (tokens + each - 1) / each;
-      for (int p = 0; p < pieces; ++p) {
-        u.begin = sp.begin + from + (int)((int64_t)tiles * p / pieces) * each;
-        u.end = sp.begin + min(sp.tokens, from + (int)((int64_t)tiles * (p + 1) / pieces) * each);
-        u.slot = pieces > 1 ? (int)(slot + p) : -1;
-        work.unit[at + p] = u;
-        if (p == 0 && pieces > 1) work.several[before[1] + x[1] - 1] = u;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 3; ++j) before[j] += all[j];
+  // ... how many tiles they have, of which a unit gets so many that the units are no
+  // more than the chunks and as many as aimed at ...
+  int64_t total = 0;
+  for (int i = threadIdx.x; i < chunks; i += kPlanThreads) total += tiles_of(part(i));
+  total = over_wave(total);
+  if (lane == 0) totals[wave] = total;
+  __syncthreads();
+  total = 0;
+  for (int w = 0; w < kWaves; ++w) total += totals[w];
+  const int extra = more_units(a);
+  const auto piece_of = [&](int w) {
+    return (int)min(max((int64_t)kLeastTiles, (total + extra - 1) / extra) * (kWaves + w) / kWaves,
+                    (int64_t)INT32_MAX);
+  };
+  int piece = piece_of(0);
+  // ... if the chunks are few, no more than that altogether: each wavefront tries a number
+  if (2 * chunks <= extra) {
+    int64_t n = 0;
+    const int mine = piece_of(wave);
+    for (int i = lane; i < chunks; i += 64) n += (tiles_of(part(i)) + mine - 1) / mine;
+    n = over_wave(n);
+    if (lane == 0) numbers[wave] = n;
+    __syncthreads();
+    int w = 0;
+    while (w < kWaves - 1 && numbers[w] > extra) ++w;
+    piece = piece_of(w);
   }
+  // ... and the units, the large ones first.  (Which of the same class comes first only
+  // changes where its sums are.)
+  const auto pieces_of = [&](int tiles) { return (tiles + piece - 1) / piece; };
+  const auto class_of = [&](int tiles) {
+    const int n = pieces_of(tiles);
+    return (int)((int64_t)(piece - (tiles + n - 1) / n) * kClasses / piece);
+  };
+  for (int i = threadIdx.x; i < chunks; i += kPlanThreads) {
+    const int tiles = tiles_of(part(i));
+    atomicAdd(&at[class_of(tiles)], pieces_of(tiles));
+  }
+  __syncthreads();
   if (threadIdx.x == 0) {
-    work.units[0] = (int32_t)before[0];
-    work.shared[0] = (int32_t)before[1];
+    int n = 0;
+    for (int i = 0; i < kClasses; ++i) {
+      const int x = at[i];
+      at[i] = n;
+      n += x;
+    }
+    work.units[0] = n;
   }
+  __syncthreads();
+  for (int i = threadIdx.x; i < chunks; i += kPlanThreads) {
+    const Part p = part(i);
+    const int tiles = tiles_of(p), pieces = pieces_of(tiles);
+    const int to = atomicAdd(&at[class_of(tiles)], pieces);
+    const int slot = pieces > 1 ? atomicAdd(&slots, pieces) : 0;
+    Unit u{p.request, p.chunk, 0, 0, -1, p.sp.first - p.sp.begin, p.sp.last, pieces};
+    // (all of a chunk's units have as many tiles, or one less)
+    for (int j = 0; j < pieces; ++j) {
+      u.begin = p.sp.begin + p.from + (int)((int64_t)tiles * j / pieces) * a.tile;
+      u.end = p.sp.begin +
+              min(p.sp.tokens, p.from + (int)((int64_t)tiles * (j + 1) / pieces) * a.tile);
+      u.slot = pieces > 1 ? slot + j : -1;
+      work.unit[to + j] = u;
+      if (j == 0 && pieces > 1) work.several[atomicAdd(&several, 1)] = u;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) work.shared[0] = several;
 }
 
-// What rows of a tile have past the head.  Rows that no token fills are zeros with a
-// logarithm that leaves no weight, and see all keys, so that a tile of them takes
-// the short way; rows that are not the unit's see none.
+// What rows of a tile have past the head, and rows that are not the unit's: zeros, with
+// a logarithm that leaves no weight.
 __device__ const uintx4 kZeros = {};
 __device__ const float kNoLse = __builtin_inff();
-__device__ const int kNoRowsPosition = INT32_MAX, kNoPosition = -1;
 
 // DP: head size rounded up.
 template <int DP, bool BF16>
 struct Weigh {
   using T = std::conditional_t<BF16, __bf16, _Float16>;
-  using Tx8 = std::conditional_t<BF16, bf16x8, halfx8>;
   static constexpr int kSteps = DP / 16;
-  // A tile in LDS: rows of 16-byte chunks, their logarithms and positions, and
-  // 256 bytes that are not read.  A chunk's place in its row is swapped so that 16
-  // rows' same chunk lies in all banks; tiles are aligned so that it is some bits of
-  // its address.
+  // A tile in LDS: rows of 16-byte chunks, their logarithms, and 256 bytes that are not
+  // read.  A chunk's place in its row is swapped so that 16 rows' same chunk lies in all
+  // banks; tiles are aligned so that it is some bits of its address.
   static constexpr int kRow = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;
-  static constexpr int kLse = kRows * kRow * 16, kPos = kLse + 4 * kRows, kNone = kPos + 4 * kRows;
-  static constexpr int kTileBytes = (kNone + 4 * kRows + 511) / 512 * 512;
-  static constexpr int kCopies = kRow / 4;  // of 1 KB a wavefront and tile
+  static constexpr int kLse = kRows * kRow * 16, kNone = kLse + 4 * kRows;
+  static constexpr int kTileBytes = (kNone + 256 + 511) / 512 * 512;
+  static constexpr int kCopies = kRow / 4;    // of 1 KB a wavefront and tile
   static constexpr int kLoads = kCopies + 1;  // ... and one of 256 bytes
   __device__ __forceinline__ static int swap(int row) {
     return kRow == 8 ? row >> 1 & 7 : row & 15;
   }
 
   const KvWeighArgs& a;
-  const int lane, wave, h, group;
-  const int heads_tile, tokens_tile;  // a tile: heads of a token, or all of some tokens
-  const bool gaps;        // it has chunks or rows that are zeros
-  int64_t rows[kCopies];  // this lane's pieces of a tile, from its first row on
-  static constexpr int64_t kNoRow = INT64_MIN;
-  int token_told, head_told;  // the row whose logarithm or position it brings; -1: none
-  int told;                   // ... from the tile's first row on
-  int token, end, head;   // the next tile's first, one past the last of all, its head
+  const int lane, wave, h, group, tokens_tile;  // (a tile: all of some tokens' heads)
+  int64_t rows[kCopies];       // this lane's pieces of a tile, in bytes from its first row on
+  uint64_t tokens;             // which of the tile's tokens they are of, a byte each
+  static constexpr int kNoToken = 255;  // none: zeros
+  int told, told_token;        // the row whose logarithm it brings
+  int of[2];                   // the tokens of this lane's columns
+  int token, end;              // the next tile's first token, one past the last of all
   uintx4 kf[2][kSteps];
   float sum[32];
 
-  __device__ __forceinline__ Weigh(const KvWeighArgs& args, int hd)
-      : a(args), lane(threadIdx.x & 63), wave(uniform(threadIdx.x >> 6)), h(hd), group(args.q.group),
-        heads_tile(min(args.q.group, kRows)), tokens_tile(max(1, kRows / args.q.group)),
-        gaps(args.c.dim != 8 * kRow || heads_tile * tokens_tile != kRows) {
+  __device__ __forceinline__ Weigh(const KvWeighArgs& args, int head)
+      : a(args), lane(threadIdx.x & 63), wave(uniform(threadIdx.x >> 6)), h(head),
+        group(args.q.group), tokens_tile(args.tile) {
+    tokens = 0;
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) {
       const int slot = (wave + 4 * i) * 64 + lane, j = slot / kRow, chunk = (slot % kRow) ^ swap(j);
-      // (tokens past the batch's: another one)
-      const int t = min(j / heads_tile, (int)a.q.tokens - 1);
-      rows[i] = t * a.q.q_token + j % heads_tile * a.q.q_head + 8 * chunk;
-      if (8 * chunk >= a.c.dim || j / heads_tile >= tokens_tile) rows[i] = kNoRow;
+      rows[i] = 2 * (j / group * a.q.q_token + j % group * a.q.q_head + 8 * chunk);
+      const bool none = 8 * chunk >= a.c.dim || j / group >= tokens_tile;
+      tokens |= (uint64_t)(none ? kNoToken : j / group) << 8 * i;
     }
-    token_told = lane / heads_tile < tokens_tile ? lane / heads_tile : -1;
-    head_told = lane % heads_tile;
-    told = wave == 0 ? token_told * a.c.heads * group + head_told : token_told;
+    told_token = lane / group < tokens_tile ? lane / group : kNoToken;
+    told = lane / group * a.c.heads * group + lane % group;
+    of[0] = (lane & 31) / group;
+    of[1] = (32 + (lane & 31)) / group;
   }
 
   // Tokens t0 .. t1 - 1 of the batch; returns their tiles.
   __device__ __forceinline__ int start(int t0, int t1) {
     token = t0;
     end = t1;
-    head = 0;
-#pragma unroll
-    for (int e = 0; e < 32; ++e) sum[e] = 0.0f;
-    return (t1 - t0 + tokens_tile - 1) / tokens_tile * ((group + kRows - 1) / kRows);
+    return (t1 - t0 + tokens_tile - 1) / tokens_tile;
   }
 
-  // Copies the next tile into LDS (past the last: anything), kLoads loads.  A tile
-  // that would reach past the batch, or the group, begins before its first row:
-  // rows that are not its own are copied and not seen.
-  __device__ __forceinline__ void copy(uint32_t tile) {
-    const int t = max(0, min(token, (int)a.q.tokens - tokens_tile)), g = min(head, group - heads_tile);
-    const T* q = (const T*)a.q.q + t * a.q.q_token + (int64_t)(h * group + g) * a.q.q_head;
+  // The next tile's copy into LDS (past the last: zeros), kLoads loads, one by one.
+  struct Copy {
+    const char* q;
+    int left;  // tokens
+    uint32_t to;
+  };
+  __device__ __forceinline__ Copy next(uint32_t tile) const {
+    return {(const char*)a.q.q + 2 * (token * a.q.q_token + (int64_t)h * group * a.q.q_head),
+            end - token, tile};
+  }
+  __device__ __forceinline__ void copy(const Copy& n, int i) {
+    if (i < kCopies) {
+      const bool there = (int)(tokens >> 8 * i & 255) < min(n.left, kNoToken);
+      stream16_to_lds(there ? (const void*)(n.q + rows[i]) : &kZeros, n.to + 1024 * (wave + 4 * i));
+      return;
+    }
+    // one wavefront brings the rows' logarithms, the others as much of nothing, so that
+    // all have as many loads on their way
+    const float* lse = a.lse + ((int64_t)token * a.c.heads + h) * group + told;
+    stream4_to_lds(told_token < min(n.left, kNoToken) ? lse : &kNoLse,
+                   n.to + (wave == 0 ? kLse : kNone));
+    token = min(token + tokens_tile, end);
+  }
+  __device__ __forceinline__ void copy_all(uint32_t tile) {
+    const Copy n = next(tile);
 #pragma unroll
-    for (int i = 0; i < kCopies; ++i) {
-      const void* src = q + rows[i];
-      if (gaps && rows[i] == kNoRow) src = &kZeros;
-      stream16_to_lds(src, tile + 1024 * (wave + 4 * i));
-    }
-    // two wavefronts bring what the columns need, the others as much of nothing, so
-    // that all have as many loads on their way
-    const void* src = &kZeros;
-    if (wave < 2) {
-      const int x = t + token_told;
-      const bool own = token_told >= 0 && x >= token && x < end && g + head_told >= head;
-      if (wave == 0) {
-        const float* lse = a.lse + ((int64_t)t * a.c.heads + h) * group + g;
-        src = own ? lse + told : &kNoLse;
-      } else {
-        src = own ? a.q.positions + t + told : token_told < 0 ? &kNoRowsPosition : &kNoPosition;
-      }
-    }
-    stream4_to_lds(src, tile + (wave == 0 ? kLse : wave == 1 ? kPos : kNone));
-    head += kRows;
-    if (head >= group) {
-      head = 0;
-      token = min(token + tokens_tile, end);
-    }
+    for (int i = 0; i < kLoads; ++i) copy(n, i);
   }
 
-  // The keys k0 .. k0 + 63 of a table's row, zeros where none is.
+  // The keys from k0 on of a table's row.  (Where there is none some key of the cache
+  // is read, whose sum is left out.)
   __device__ __forceinline__ void keys(const int32_t* table, int k0, int upto) {
     const int d = a.c.dim, col = lane & 31, half = lane >> 5;
     int page[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int k = k0 + 32 * u + col;
-      page[u] = k <= upto ? table[k >> a.c.lps] : -1;
-    }
+    for (int u = 0; u < 2; ++u) page[u] = table[min(k0 + 32 * u + col, upto) >> a.c.lps];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int k = k0 + 32 * u + col;
-      const bool there = page[u] >= 0 && page[u] < a.c.pages;
-      const T* src = (const T*)a.c.keys +
-                     (((int64_t)(there ? page[u] : 0) * a.c.heads + h) * a.c.page +
-                      (k & (a.c.page - 1))) * d;
+      const int64_t p = page[u] >= 0 && page[u] < a.c.pages ? page[u] : 0;
+      const T* src = (const T*)a.c.keys + ((p * a.c.heads + h) * a.c.page + (k & (a.c.page - 1))) * d;
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
         const int at = 16 * i + 8 * half;
-        kf[u][i] = uintx4{};
-        if (there && (16 * i + 16 <= sure_values(DP) || at < d)) kf[u][i] = *(const uintx4*)(src + at);
-      }
-    }
-  }
-
-  // The products of 32 rows of a tile.  beside(i) is done while step i's products are
-  // made.
-  template <bool MIX, typename Beside>
-  __device__ __forceinline__ void products(uint32_t tile, int ct, floatx16 (&s)[2], Beside beside) {
-    constexpr int kAhead = 4;  // reads of Q
-    const int col = lane & 31, half = lane >> 5;
-    const uint32_t at = tile + (32 * ct + col) * kRow * 16 + 16 * (half ^ swap(32 * ct + col));
-    uintx4 q[kSteps];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) q[i] = lds_read16(at ^ (32 * i));
-    s[0] = s[1] = floatx16{};
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      if (i + kAhead < kSteps) q[i + kAhead] = lds_read16(at ^ (32 * (i + kAhead)));
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        s[u] = mfma(__builtin_bit_cast(Tx8, kf[u][i]), __builtin_bit_cast(Tx8, q[i]), s[u]);
-      beside(i);
-      if constexpr (MIX) __builtin_amdgcn_sched_barrier(0);
-    }
-  }
-
-  // Adds the weights of the keys of a column that belong to step i, all of which it
-  // sees.  (The sums are tied to their place: they would be moved behind all
-  // products, which then have nothing beside them.)
-  __device__ __forceinline__ void add(const floatx16 (&s)[2], int i, float c, float lse) {
-    constexpr int kPer = (32 + kSteps - 1) / kSteps;
-#pragma unroll
-    for (int e = i * kPer; e < (i + 1) * kPer; ++e) {
-      if (e >= 32) continue;
-      sum[e] += __builtin_amdgcn_exp2f(fmaf(s[e / 16][e % 16], c, -lse));
-#if defined(__HIP_DEVICE_COMPILE__)
-      asm volatile("" : "+v"(sum[e]));
-#endif
-    }
-  }
-
-  // What a tile's columns are: rows 0 .. 31 and 32 .. 63.
-  struct Columns {
-    float lse[2];  // times log2(e)
-    int pos[2];
-  };
-  __device__ __forceinline__ Columns columns(uint32_t tile) const {
-    const int col = 4 * (lane & 31);
-    Columns n;
-#pragma unroll
-    for (int ct = 0; ct < 2; ++ct) {
-      n.lse[ct] = lds_read4<float>(tile + kLse + 128 * ct + col) * kLog2e;
-      n.pos[ct] = lds_read4<int>(tile + kPos + 128 * ct + col);
-    }
-    return n;
-  }
-  // Whether all of them see all of this wavefront's keys, from k0 on.
-  __device__ __forceinline__ bool full(const Columns& n, int k0) const {
-    return __all(min(n.pos[0], n.pos[1]) >= k0 + kWaveKeys - 1);
-  }
-
-  // A tile of which some see some.
-  __device__ __forceinline__ void use_some(uint32_t tile, const Columns& n, int k0, float c) {
-#pragma unroll 1
-    for (int ct = 0; ct < 2; ++ct) {
-      const float lse = ct ? n.lse[1] : n.lse[0];
-      const int pos = max(-1, ct ? n.pos[1] : n.pos[0]), seen = pos - k0 - 4 * (lane >> 5);
-      if (!__any(pos >= k0)) continue;
-      floatx16 s[2];
-      products<false>(tile, ct, s, [](int) {});
-#pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        const float x = __builtin_amdgcn_exp2f(fmaf(s[e / 16][e % 16], c, -lse));
-        sum[e] += 32 * (e / 16) + 8 * (e % 16 / 4) + e % 4 <= seen ? x : 0.0f;
-      }
-    }
-  }
-
-  // All `todo` tiles against the keys from k0 on; tile(n) is the n-th's place,
-  // enter(n) waits for it.
-  template <typename Tile, typename Enter>
-  __device__ __forceinline__ void run(int todo, int k0, float c, Tile tile, Enter enter) {
-    int n = 0;
-    while (n < todo) {
-      enter(n);
-      Columns x = columns(tile(n));
-      if (full(x, k0)) {
-        // the weights of a half tile are taken while the next one's products are made
-        floatx16 open[2] = {};
-        float lse = __builtin_inff();
-#pragma unroll 1
-        while (true) {
-          floatx16 s[2];
-          products<true>(tile(n), 0, s, [&](int i) { add(open, i, c, lse); });
-          products<true>(tile(n), 1, open, [&](int i) { add(s, i, c, x.lse[0]); });
-          lse = x.lse[1];
-          if (++n == todo) break;
-          enter(n);
-          x = columns(tile(n));
-          if (!full(x, k0)) break;
+        if (16 * i + 16 <= sure_values(DP)) {
+          kf[u][i] = *(const uintx4*)(src + at);
+        } else {
+          kf[u][i] = uintx4{};
+          if (at < d) kf[u][i] = *(const uintx4*)(src + at);
         }
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) add(open, i, c, lse);
-        if (n == todo) return;
       }
-      use_some(tile(n), x, k0, c);
-      ++n;
     }
+  }
+
+  // Once they are there: keys of more than 128 values stay in accumulation registers,
+  // which products read and vector instructions do not.  (With two wavefronts on a
+  // SIMD it is better not to use any: the compiler then has all 256 registers for the
+  // rest, and with some only half of them.)
+  static constexpr bool kHeld = DP > 128;
+  __device__ __forceinline__ void hold() {
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        if constexpr (kHeld) asm volatile("" : "+a"(kf[u][i]));
+        else asm volatile("" : "+v"(kf[u][i]));
+      }
+#endif
+  }
+
+  // Where the lane's column (row 32 ct + lane % 32 of the tile) begins.
+  __device__ __forceinline__ uint32_t column(uint32_t tile, int ct) const {
+    const int row = 32 * ct + (lane & 31);
+    return tile + row * kRow * 16 + 16 * ((lane >> 5) ^ swap(row));
+  }
+
+  // s (+)= keys x rows.  (Written out: left to itself the compiler has the sums in
+  // accumulation registers, from where every value is moved before it is used.)
+  template <bool FIRST>
+  __device__ __forceinline__ static void product(floatx16& s, const uintx4& k, const uintx4& q) {
+#if defined(__HIP_DEVICE_COMPILE__)
+#define MLXVS_PRODUCT(TYPE, K)                                                              \
+  if constexpr (FIRST)                                                                      \
+    asm volatile("v_mfma_f32_32x32x16_" TYPE " %0, %1, %2, 0" : "=&v"(s) : K(k), "v"(q));   \
+  else asm volatile("v_mfma_f32_32x32x16_" TYPE " %0, %1, %2, %0" : "+v"(s) : K(k), "v"(q))
+    if constexpr (kHeld && BF16) { MLXVS_PRODUCT("bf16", "a"); }
+    else if constexpr (kHeld) { MLXVS_PRODUCT("f16", "a"); }
+    else if constexpr (BF16) { MLXVS_PRODUCT("bf16", "v"); }
+    else { MLXVS_PRODUCT("f16", "v"); }
+#undef MLXVS_PRODUCT
+#endif
+  }
+  // Wait states before the sums are read, which the compiler does not count (12 of
+  // them after a product of 8 passes).
+  __device__ __forceinline__ static void settle() {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15");
+    __builtin_amdgcn_sched_barrier(0);
+#endif
+  }
+
+  // A block of products, 32 rows by 64 keys, whose weights are to be taken.
+  struct Block {
+    floatx16 s[2];
+    float lse;  // times log2(e)
+    int seen;   // the last of the keys that the lane's column sees, less 4 (lane / 32)
+  };
+
+  // The weights of a block, some for each of the next one's products; each is added a
+  // step after it is made.  (The sums are tied to their place: they would be moved
+  // behind all products, which then have nothing beside them.)
+  static constexpr int kPer = (32 + 2 * kSteps - 1) / (2 * kSteps);
+  static constexpr int kTurns = (32 + kPer - 1) / kPer;  // ... and one to add the last
+  template <bool MASK>
+  __device__ __forceinline__ void weigh(const Block& b, int i, float c, float (&x)[kPer]) {
+    if (i > 0) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int e = (i - 1) * kPer + j;
+        if (e >= 32) continue;
+        sum[e] += x[j];
+#if defined(__HIP_DEVICE_COMPILE__)
+        asm volatile("" : "+v"(sum[e]));
+#endif
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int e = i * kPer + j;
+      if (e >= 32) continue;
+      x[j] = __builtin_amdgcn_exp2f(fmaf(b.s[e / 16][e % 16], c, -b.lse));
+      if (MASK) x[j] = 32 * (e / 16) + 8 * (e % 16 / 4) + e % 4 <= b.seen ? x[j] : 0.0f;
+    }
+  }
+
+  // The products of 32 rows with the keys, and beside them the weights of the block
+  // before: one product and 6 vector instructions take as long.  Block B of a tile; its
+  // rows' next values are read while the last ones are used, and also(i) does something
+  // else beside the i-th product.
+  static constexpr int kAhead = 4;
+  template <int B, bool MASK, typename Also>
+  __device__ __forceinline__ void products(uint32_t t, uintx4 (&q)[kAhead], Block& now,
+                                           const Block& before, float c, Also also) {
+    float x[kPer];
+#pragma unroll
+    for (int i = 0; i < 2 * kSteps; ++i) {
+      constexpr int at = B * kSteps;
+      uintx4& rows = q[(at + i / 2) % kAhead];
+      if (i < 2) product<true>(now.s[i], kf[i][0], rows);
+      else product<false>(now.s[i % 2], kf[i % 2][i / 2], rows);
+      __builtin_amdgcn_sched_barrier(0);
+      if (i <= kTurns) weigh<MASK>(before, i, c, x);
+      if (const int n = at + i / 2 + kAhead; i % 2 && n < 2 * kSteps)
+        rows = lds_read16(column(t, n / kSteps) ^ (32 * (n % kSteps)));
+      also(i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (2 * kSteps <= kTurns) weigh<MASK>(before, kTurns, c, x);
+    // (the next block's first weights read sums whose last product has another one and
+    // two products' vector instructions behind it: wait states enough, if there are some)
+    if constexpr (6 * kPer + 2 < 14 || kTurns < 2 * kSteps) settle();
+  }
+
+  // Tiles from `from` to `to`, of which token t is `seen` + t - token.  Without MASK every
+  // row sees every key (or is none).
+  template <bool MASK, typename Tile, typename Wait>
+  __device__ __forceinline__ void use(int from, int to, int k0, int shift, float c, Tile tile,
+                                      Wait wait) {
+    if (from >= to) return;
+    constexpr int kEach = (kLoads + 1) / 2;  // copies beside a block
+    constexpr int kApart = 2 * kSteps / kEach;
+    Block open;
+    open.s[0] = open.s[1] = floatx16{};
+    open.lse = __builtin_inff();
+    open.seen = 0;
+#pragma unroll 1
+    for (int n = from; n < to; ++n) {
+      wait();
+      const Copy then = next(tile(n + kStages - 1));  // (the place of the one before)
+      const uint32_t t = tile(n);
+      uintx4 q[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) q[i] = lds_read16(column(t, 0) ^ (32 * i));
+      const float l0 = lds_read4<float>(t + kLse + 4 * (lane & 31)),
+                  l1 = lds_read4<float>(t + kLse + 128 + 4 * (lane & 31));
+      // (the tile's first token's position, less the keys that are not this lane's)
+      const int pos = shift + n * tokens_tile - k0 - 4 * (lane >> 5);
+      const auto also = [&](int block, int i) {
+        if (i % kApart == kApart - 1 && i / kApart < kEach && block * kEach + i / kApart < kLoads)
+          copy(then, block * kEach + i / kApart);
+      };
+      Block now;
+      now.lse = l0 * kLog2e;
+      now.seen = pos + of[0];
+      products<0, MASK>(t, q, now, open, c, [&](int i) { also(0, i); });
+      products<1, MASK>(t, q, open, now, c, [&](int i) { also(1, i); });
+      open.lse = l1 * kLog2e;
+      open.seen = pos + of[1];
+    }
+    settle();
+    float x[kPer];
+#pragma unroll
+    for (int i = 0; i <= kTurns; ++i) weigh<MASK>(open, i, c, x);
   }
 
   // The sums over the columns: lane l's key is key_of(l).
-  __device__ __forceinline__ float meet() {
+  template <int B>
+  __device__ __forceinline__ void halve(float (&x)[32]) const {
+    const bool up = lane & B;
 #pragma unroll
-    for (int b = 16; b >= 1; b >>= 1)
+    for (int j = 0; j < B; ++j) {
+      const float mine = up ? x[j + B] : x[j], other = up ? x[j] : x[j + B];
+      x[j] = mine + __shfl_xor(other, B);
+    }
+  }
+  __device__ __forceinline__ float meet() const {
+    float x[32];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        if (j >= b) continue;
-        const bool up = lane & b;
-        const float mine = up ? sum[j + b] : sum[j], other = up ? sum[j] : sum[j + b];
-        sum[j] = mine + __shfl_xor(other, b);
-      }
-    return sum[0];
+    for (int e = 0; e < 32; ++e) x[e] = sum[e];
+    halve<16>(x);
+    halve<8>(x);
+    halve<4>(x);
+    halve<2>(x);
+    halve<1>(x);
+    return x[0];
   }
   __device__ __forceinline__ static int key_of(int lane) {
     const int e = lane & 31;
@@ -560,32 +711,42 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_weigh_kernel(KvWeig
   const Work work = work_of(a);
   const int h = (int)(blockIdx.x % a.c.heads), lane = threadIdx.x & 63;
   const int units = uniform(work.units[0]);
-  const float c = a.scale * kLog2e;
+  const float c = __builtin_bit_cast(float, uniform(__builtin_bit_cast(int, a.scale * kLog2e)));
+  const auto tile = [&](int n) { return at + n % kStages * W::kTileBytes; };
+  const auto wait = [] {
+    staged_barrier<(kStages - 2) * W::kLoads>();
+    mfma_settle();
+  };
   W w(a, h);
   for (int x = (int)(blockIdx.x / a.c.heads); x < units; x += (int)(gridDim.x / a.c.heads)) {
     const Unit u = work.unit[x];
     const int r = uniform(u.request), last = uniform(u.last), slot = uniform(u.slot);
+    const int begin = uniform(u.begin), end = uniform(u.end), shift = uniform(u.shift);
     const int k0 = uniform(u.chunk) * kChunk + w.wave * kWaveKeys;
     const int32_t* table = a.q.table + r * a.q.table_stride;
-    const int todo = w.start(uniform(u.begin), uniform(u.end));
 #pragma unroll
-    for (int n = 0; n < kStages - 1; ++n) w.copy(at + n * W::kTileBytes);
+    for (int e = 0; e < 32; ++e) w.sum[e] = 0.0f;
+    const int todo = w.start(begin, end);
     w.keys(table, k0, last);
+#pragma unroll
+    for (int n = 0; n < kStages - 1; ++n) w.copy_all(tile(n));
     // (known to the compiler, which else waits for the keys, and with them for all
     // that was loaded since, in every turn)
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-    const auto tile = [&](int n) { return at + n % kStages * W::kTileBytes; };
-    const auto enter = [&](int n) {
-      staged_barrier<(kStages - 2) * W::kLoads>();
-      mfma_settle();
-      w.copy(tile(n + kStages - 1));  // (the place of the one before)
-    };
-    if (k0 <= last) {
-      w.run(todo, k0, c, tile, enter);
-    } else {
+    w.hold();
+    // the tiles of which some rows see some of this wavefront's keys, and those of which
+    // all rows see all
+    const int position = shift + begin;  // of the first token
+    const int some = k0 > last ? todo : min(todo, sees(position, end - begin, k0) / w.tokens_tile);
+    const int all = max(some, min(todo, (sees(position, end - begin, (int64_t)k0 + kWaveKeys - 1) +
+                                         w.tokens_tile - 1) / w.tokens_tile));
 #pragma unroll 1
-      for (int n = 0; n < todo; ++n) enter(n);
+    for (int n = 0; n < some; ++n) {
+      wait();
+      w.copy_all(tile(n + kStages - 1));
     }
+    w.template use<true>(some, all, k0, position, c, tile, wait);
+    w.template use<false>(all, todo, k0, position, c, tile, wait);
     dma_barrier();  // (nothing is on its way into the tiles any more)
     mfma_settle();
     const float got = w.meet();
@@ -595,7 +756,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_weigh_kernel(KvWeig
       work.sums[((int64_t)slot * a.c.heads + h) * kChunk + w.wave * kWaveKeys + key] = got;
     } else {
       const int page = table[p >> a.c.lps];
-      put(a, a.mass + ((int64_t)r * a.c.heads + h) * a.slots, p, u.first,
+      put(a, a.mass + ((int64_t)r * a.c.heads + h) * a.slots, p, first_of(a, r),
           page >= 0 && page < a.c.pages ? got : 0.0f);
     }
   }
@@ -614,28 +775,26 @@ __global__ __launch_bounds__(kChunk) void kv_weigh_join_kernel(KvWeighArgs a) {
 #pragma unroll 4
     for (int i = 0; i < u.pieces; ++i) got += sums[(int64_t)i * a.c.heads * kChunk];
     const int page = a.q.table[u.request * a.q.table_stride + (p >> a.c.lps)];
-    put(a, a.mass + ((int64_t)u.request * a.c.heads + h) * a.slots, p, u.first,
+    put(a, a.mass + ((int64_t)u.request * a.c.heads + h) * a.slots, p, first_of(a, u.request),
         page >= 0 && page < a.c.pages ? got : 0.0f);
   }
 }
 
 // ---- which one ------------------------------------------------------------------
 
-// Workgroups that single tokens' chunks are dealt to, for each request.
-int64_t few_chunks(const KvWeighArgs& a) {
-  const int64_t most = std::min<int64_t>(a.longest, (int64_t)a.q.cols << a.c.lps);
-  return std::max<int64_t>(1, (most + kChunk - 1) / kChunk);
+// Chunks of so many keys that requests are expected to have.
+int64_t chunks_of(const KvWeighArgs& a, int64_t chunk, int64_t most) {
+  most = std::min<int64_t>(most, (int64_t)a.q.cols << a.c.lps);
+  return std::max<int64_t>(1, (most + chunk - 1) / chunk);
 }
 
 constexpr int64_t kGrid = 2048;  // workgroups at most
-constexpr int64_t kUnits = 2048;
-constexpr int64_t kLeast = 1024;  // rows of a unit
 
 template <int DP, bool BF16>
 void launch_dim(const KvWeighArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)kv_weigh_grid(a));
-  if (a.piece) kv_weigh_kernel<DP, BF16><<<grid, 256, 0, s>>>(a);
-  else kv_weigh_few_kernel<DP, BF16><<<grid, 256, 0, s>>>(a, (int)few_chunks(a));
+  if (a.prompts) kv_weigh_kernel<DP, BF16><<<grid, 256, 0, s>>>(a);
+  else kv_weigh_few_kernel<DP, BF16><<<grid, 256, 0, s>>>(a, (int)chunks_of(a, kSpan, a.longest));
 }
 
 template <bool BF16>
@@ -650,32 +809,30 @@ void launch_type(const KvWeighArgs& a, hipStream_t s) {
 }  // namespace
 
 void kv_weigh_plan(KvWeighArgs& a) {
-  a.piece = a.most_units = a.most_several = a.most_slots = 0;
-  if (a.q.tokens <= a.q.requests || a.q.cols == 0) return;
-  const int64_t chunks = few_chunks(a), pieces = std::max<int64_t>(1, kUnits / (chunks * a.c.heads));
-  const int64_t each = std::max<int64_t>(1, kRows / a.q.group);  // tokens of a tile
-  const int64_t piece = std::max((a.q.tokens + pieces - 1) / pieces, kLeast / a.q.group);
-  a.piece = (piece + each - 1) / each * each;
-  // a chunk of a request of t tokens has at most 1 + t / piece units
-  const int64_t all = chunks_of(a), full = a.q.tokens / a.piece;
-  a.most_units = all * (a.q.requests + full);
-  a.most_several = all * std::min(a.q.requests, full);
-  a.most_slots = 2 * all * full;
+  a.prompts = a.q.tokens > a.q.requests && a.q.cols > 0 && a.q.group <= kRows;
+  a.most_units = a.most_several = a.most_slots = 0;
+  if (!a.prompts) return;
+  a.tile = kRows / a.q.group;
+  // a chunk of several units has two for each one more than the first, at most
+  const int64_t extra = more_units(a);
+  a.most_units = chunks_of(a, kChunk, INT32_MAX) * a.q.requests + extra;
+  a.most_several = extra;
+  a.most_slots = 2 * extra;
 }
 
 int64_t kv_weigh_workspace(const KvWeighArgs& a) {
-  if (!a.piece) return 0;
+  if (!a.prompts) return 0;
   return 4 * header_ints(a) + (a.most_units + a.most_several) * (int64_t)sizeof(Unit) +
          a.most_slots * a.c.heads * kChunk * 4;
 }
 
 int64_t kv_weigh_grid(const KvWeighArgs& a) {
-  if (!a.piece) return a.q.requests * a.c.heads * few_chunks(a);
+  if (!a.prompts) return a.q.requests * a.c.heads * chunks_of(a, kSpan, a.longest);
   return std::min(a.most_units, std::max<int64_t>(1, kGrid / a.c.heads)) * a.c.heads;
 }
 
 hipError_t launch_kv_weigh(const KvWeighArgs& a, hipStream_t s) {
-  if (a.piece) {
+  if (a.prompts) {
     kv_weigh_plan_kernel<<<1, kPlanThreads, 0, s>>>(a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
