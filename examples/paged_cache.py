@@ -3,10 +3,12 @@
 Several requests with prompts of different lengths share one cache.  Their
 prompts are written and attended to in one step; then each step adds a token to
 every request, which attends to the blocks of its context that score best for
-it (and, for comparison, to all of them).  One attention layer with random
-weights stands for the model.
+it (and, for comparison, to all of them).  With a budget every request is cut to
+the tokens that got most attention, after its prompt and whenever it has grown by a
+page since.  One attention layer with random weights stands for the model.
 
     python examples/paged_cache.py [--requests 8] [--context 16384] [--steps 32]
+                                   [--budget 4096]
 """
 
 from __future__ import annotations
@@ -42,9 +44,10 @@ class Layer:
             v.unflatten(1, (KV_HEADS, DIM))
 
 
-def run(requests=8, context=16384, steps=32, blocks=32, seed=0):
+def run(requests=8, context=16384, steps=32, blocks=32, seed=0, budget=0):
     """Returns the lengths at the end, the mean cosine of the two answers' outputs
-    and the mean time of a decoding step in milliseconds."""
+    and the mean time of a decoding step in milliseconds.  budget: tokens of a
+    request that are kept, 0 for all."""
     g = torch.Generator(device="cuda").manual_seed(seed)
     ints = dict(dtype=torch.int32, device="cuda")
     prompts = [max(1, context * (i + 1) // requests - 7 * i) for i in range(requests)]
@@ -57,17 +60,34 @@ def run(requests=8, context=16384, steps=32, blocks=32, seed=0):
     free = torch.randperm(pages, generator=g, device="cuda").int()
     cursor = torch.zeros(1, **ints)  # how much of the free list is taken
     lengths = torch.zeros(requests, **ints)
+    rotary = mlxvs.Rotary(DIM)
+    evicted = torch.zeros(requests, **ints)  # tokens of a request that the cache has lost
+    mass = torch.zeros(requests, KV_HEADS, columns * PAGE, device="cuda") if budget else None
+
+    def cut(q, plan, lse):
+        """The step's attention counted, and the requests cut that hold a page too many."""
+        nonlocal lengths, cursor, evicted
+        cache.weigh(q, table, plan.starts, plan.positions, lse, mass,
+                    longest=max(prompts) + steps)
+        kept = cache.keep(mass, plan.lengths, budget, first=min(4, budget // 2),
+                          recent=min(2 * PAGE, budget // 2), above=budget + PAGE - 1)
+        lengths, cursor = cache.compact(table, plan.lengths, kept, free, plan.cursor, mass=mass)
+        evicted = evicted + plan.lengths - lengths
 
     # the prompts, all tokens in one step
     total = sum(prompts)
     plan = mlxvs.kv_plan(lengths, torch.tensor(prompts, **ints), table, free, cursor, PAGE, total)
     x = torch.randn(total, WIDTH, generator=g, device="cuda").bfloat16()
     q, k, v = layer.project(x)
+    q, k = rotary.rotate(q, k, plan.positions)
     cache.append(k, v, plan.slots)
-    out = cache.attend(q, table, plan.requests, plan.positions, longest=max(prompts))
+    out, lse = cache.attend(q, table, plan.requests, plan.positions, longest=max(prompts),
+                            lse=True)
     last = torch.tensor(prompts, device="cuda").cumsum(0) - 1  # the prompts' last tokens
     x = torch.tanh(out[last].flatten(1) @ layer.out)
     lengths, cursor = plan.lengths, plan.cursor
+    if budget:
+        cut(q, plan, lse)
 
     one = torch.ones(requests, **ints)
     close, spent = 0.0, 0.0
@@ -76,6 +96,7 @@ def run(requests=8, context=16384, steps=32, blocks=32, seed=0):
         start = time.perf_counter()
         plan = mlxvs.kv_plan(lengths, one, table, free, cursor, PAGE, requests)
         q, k, v = layer.project(x)
+        q, k = rotary.rotate(q, k, plan.positions, requests=plan.requests, evicted=evicted)
         cache.append(k, v, plan.slots)
         best = cache.select(q, table, plan.requests, plan.positions, blocks, last=2)
         out = cache.attend(q, table, plan.requests, plan.positions, blocks=best)
@@ -83,8 +104,10 @@ def run(requests=8, context=16384, steps=32, blocks=32, seed=0):
         lengths, cursor = plan.lengths, plan.cursor
         torch.cuda.synchronize()
         spent += time.perf_counter() - start if i else 0.0  # (the first one warms up)
-        full = cache.attend(q, table, plan.requests, plan.positions,
-                            longest=max(prompts) + steps)
+        full, lse = cache.attend(q, table, plan.requests, plan.positions,
+                                 longest=max(prompts) + steps, lse=True)
+        if budget:
+            cut(q, plan, lse)
         close += torch.cosine_similarity(out.float().flatten(1), full.float().flatten(1)).mean() \
             .item()
     return lengths.tolist(), close / max(1, steps), 1e3 * spent / max(1, steps - 1)
@@ -96,8 +119,9 @@ def main():
     p.add_argument("--context", type=int, default=16384, help="tokens of the longest prompt")
     p.add_argument("--steps", type=int, default=32, help="tokens to answer with")
     p.add_argument("--blocks", type=int, default=32, help="blocks of 64 tokens to attend to")
+    p.add_argument("--budget", type=int, default=0, help="tokens of a request to keep (0: all)")
     a = p.parse_args()
-    lengths, close, ms = run(a.requests, a.context, a.steps, a.blocks)
+    lengths, close, ms = run(a.requests, a.context, a.steps, a.blocks, budget=a.budget)
     print(f"{a.requests} requests of {min(lengths)} to {max(lengths)} tokens, {a.steps} steps of "
           f"{ms:.3f} ms; {a.blocks} selected blocks against all: cosine {close:.4f}")
 

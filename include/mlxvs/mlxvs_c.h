@@ -736,7 +736,8 @@ typedef struct {
  * positions[t] + evicted[token_request[t]]: what its request's cache has lost
  * (mlxvs_kv_compact_device) still counts (a request out of range: nothing).  A
  * token with a negative position is not turned.  Computed in float32 and rounded
- * once; angles are exact to 2^-32 of a turn at every position.
+ * once; angles are exact to 2^-32 of a turn at every position.  out may be x with its
+ * strides; otherwise what is written may not overlap what is read.
  */
 MLXVS_C_API int mlxvs_kv_rotate_device(const mlxvs_kv_rotary* rotary, const mlxvs_kv_heads* q,
                                        const mlxvs_kv_heads* k, int64_t tokens,
@@ -757,7 +758,8 @@ MLXVS_C_API int mlxvs_kv_rotate_device(const mlxvs_kv_rotary* rotary, const mlxv
  *             and the head's query heads of exp(scale x q.k_p - lse),
  * first being the first token's position: the step's own keys start from zero.  The
  * others, and requests without tokens (or with position -1), stay as they are; a
- * key of an absent page gets nothing.  decay in [0, 1]; with 0 masses are not read.
+ * key of an absent page gets nothing, and one with values that are not finite may
+ * get NaN.  decay in [0, 1]; with 0 masses are not read.
  * A page that several rows share has a mass in each.  longest guides how work is
  * split, as in mlxvs_kv_attend_device.  The same bits every time.  workspace:
  * mlxvs_kv_weigh_workspace bytes (may be 0).
@@ -798,7 +800,7 @@ MLXVS_C_API int64_t mlxvs_kv_keep_workspace(int64_t requests, int32_t heads, int
  * as it is: the request's pages past the new end, columns ceil(n / page_size) ..
  * ceil(length / page_size) - 1, are written into free_pages before entry cursor[0],
  * in the requests' order from there down, so that entries from cursor_out[0] on are
- * free.  Not cut, and given back nothing: a request whose list starts with -1, one
+ * free (a column of an absent block gives its entry, whatever it is).  Not cut, and given back nothing: a request whose list starts with -1, one
  * of at most n tokens or of more than the table holds, and, from the first one on
  * whose pages find no room in free_pages, each that would give pages back.
  * lengths_out [requests], cursor_out [1]: the lengths and the cursor after it.  The

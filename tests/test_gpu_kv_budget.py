@@ -299,6 +299,82 @@ def test_weights_of_prompts_in_pieces(engine, lengths, counts, heads, group, dim
          seed=len(lengths)).attend().check(decay=0.5)
 
 
+@pytest.mark.parametrize("group", [32, 33, 63, 64, 65, 130])
+def test_weights_of_many_query_heads_of_a_key(engine, group):
+    Step(engine, [150, 20, 90], [40, 1, 90], heads=1, group=group, dim=32, seed=group).attend().check()
+
+
+def test_weights_of_a_batch_that_is_one_request_s(engine):
+    # no more tokens than requests, all of them one request's
+    counts = [0, 0, 21] + [0] * 20
+    Step(engine, [30, 0, 300] + [5] * 20, counts, heads=1, group=2, dim=16, seed=5).attend().check()
+    Step(engine, [30, 0, 300], [0, 0, 3], heads=2, group=24, dim=96, seed=6).attend().check()
+
+
+@pytest.mark.parametrize("most", [1, 3])
+def test_weights_of_many_requests(engine, most):
+    rng = np.random.default_rng(most)
+    lengths = rng.integers(0, 40, 1_100)
+    lengths[[7, 1_099]] = 300, 290
+    counts = np.minimum(lengths, rng.integers(0, most + 1, 1_100))
+    counts[1_099] = 200 if most > 1 else 1
+    Step(engine, lengths, counts, heads=1, group=2, dim=16, seed=most).attend().check()
+
+
+@pytest.mark.parametrize("longest", [0, 1, 1_000])
+def test_weights_of_prompts_of_other_sizes_together(engine, longest):
+    # units of many sizes, keys that few of the tokens see, masked tiles in between
+    Step(engine, [1_290, 700, 256, 5, 999], [290, 513, 256, 1, 130], page=32, heads=2, group=3, dim=64,
+         spare=2, seed=longest).attend().check(longest=longest, decay=0.25)
+
+
+def test_weights_on_two_streams_at_once(engine):
+    steps = [Step(engine, [900, 400], [600, 1], page=64, heads=2, group=4, dim=128, seed=i).attend()
+             for i in range(2)]
+    want = []
+    for s in steps:
+        want.append(s.mass.clone())
+        s.cache.weigh(s.q, s.table, s.starts, s.positions, s.lse, want[-1])
+    streams = [torch.cuda.Stream() for _ in steps]
+    masses = [[s.mass.clone() for _ in range(10)] for s in steps]
+    torch.cuda.synchronize()
+    for i in range(10):
+        for s, stream, m in zip(steps, streams, masses):
+            with torch.cuda.stream(stream):
+                s.cache.weigh(s.q, s.table, s.starts, s.positions, s.lse, m[i])
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, w) for m, w in zip(masses, want) for x in m)
+
+
+def test_weights_in_a_captured_graph(engine):
+    # other tokens, lengths and keys at every replay: units of other sizes and numbers
+    s = Step(engine, [800, 500, 300], [300, 1, 20], page=64, heads=2, group=3, dim=64, seed=1).attend()
+    start, mass = s.mass.clone(), s.mass.clone()
+    s.cache.weigh(s.q, s.table, s.starts, s.positions, s.lse, mass.clone())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        s.cache.weigh(s.q, s.table, s.starts, s.positions, s.lse, mass)
+    tokens = len(s.q)
+    for counts in ([300, 1, 20], [0, 0, 300], [1, 320, 0], [107, 107, 107], [0, 0, 0]):
+        starts = np.concatenate([[0], np.cumsum(counts)])
+        where = np.concatenate([np.arange(n - m, n) for n, m in zip([800, 500, 300], counts)]
+                               + [[-1] * (tokens - sum(counts))])
+        s.starts.copy_(dev(starts, torch.int32))
+        s.positions.copy_(dev(where, torch.int32))
+        s.requests.copy_(dev(list(np.repeat([0, 1, 2], counts)) + [-1] * (tokens - sum(counts)),
+                             torch.int32))
+        lse = s.cache.attend(s.q, s.table, s.requests, s.positions, lse=True)[1]
+        s.lse.copy_(lse)
+        mass.copy_(start)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = start.clone()
+        s.cache.weigh(s.q, s.table, s.starts, s.positions, s.lse, want)
+        assert torch.equal(mass, want), counts
+        s.mass.copy_(start)
+        s.check()
+
+
 def test_weights_decay_and_begin_anew(engine):
     for decay in (0.0, 0.5, 1.0):
         s = Step(engine, [50, 90, 7], [3, 1, 7], seed=3)
@@ -793,3 +869,17 @@ def test_calls_run_on_the_current_stream(engine):
         kept2 = s.cache.keep(mass, lengths, 100)
     stream.synchronize()
     assert torch.equal(mass, want) and torch.equal(again, turned) and torch.equal(kept, kept2)
+
+
+def test_the_example_within_a_budget(engine):
+    import importlib.util
+    from pathlib import Path
+
+    path = Path(__file__).resolve().parent.parent / "examples" / "paged_cache.py"
+    spec = importlib.util.spec_from_file_location("paged_cache", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    lengths, close, ms = example.run(requests=3, context=900, steps=70, blocks=4, budget=256)
+    # (prompts of 593 and 886 tokens cut to 256, and again after 64; one of 300 after 20)
+    assert lengths == [256 + 50, 256 + 6, 256 + 6] and math.isfinite(close) and ms > 0
+    assert example.run(requests=2, context=100, steps=3, blocks=4, budget=1)[0] == [53, 4]
