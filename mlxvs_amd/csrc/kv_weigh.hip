@@ -20,13 +20,14 @@
 //
 // Measured: single tokens over 64 requests of up to 8,192 keys in 8 heads of 128
 // values 122 us, 5.1 TB/s of keys, masses and their return (a copy: 4.95); chunks of
-// 1,500 tokens in 3 requests of up to 8,192, 32 heads on 8, 146 us, 795 TFLOP/s, and
-// a prompt of 4,001 tokens, 28 heads on 4, 97 us of which 12 are the plan and the
-// joining.  There the matrix units work 37% of the time and the vector units 53%;
-// what is between are a unit's begin (some 5 us for its keys) and its end, and units
-// that do not fill the last round.  Tried: 128 keys a wavefront and 128 rows a tile,
-// with one wavefront a SIMD, 181 and 144; one share of all tiles for each workgroup,
-// which may go on in another chunk, 211 and 103 (their rows of Q then miss in L2).
+// 1,500 tokens in 3 requests of up to 8,192, 32 heads on 8, 145 us, 798 TFLOP/s, and
+// a prompt of 4,001 tokens, 28 heads on 4, 87 us, 659.  Two workgroups on a CU take
+// 28 ns a product and SIMD, as a large library product does (27, the card's power); the
+// rest are some 4 us at a unit's begin, until its keys and first rows are there, the
+// end, where CUs run dry, masked tiles, and 12 us of plan and joining.  Tried: 128
+// keys a wavefront and 128 rows a tile, with one wavefront a SIMD, 181 and 144; one
+// share of all tiles for each workgroup, which may go on in another chunk, 211 and 103
+// (the rows of Q then miss in L2); a fifth of the tiles in small units, the same.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -273,23 +274,19 @@ __device__ __forceinline__ int running(int x, int& all, int* waves) {
   __syncthreads();
   return x;
 }
-__device__ __forceinline__ int64_t over_wave(int64_t x) {
-#pragma unroll
-  for (int i = 32; i >= 1; i >>= 1) x += __shfl_xor(x, i);
-  return x;
-}
-
 // The first of a request's tokens that sees key p (its number of tokens: none).
 __device__ __forceinline__ int sees(int first, int tokens, int64_t p) {
   return (int)min(max(p - first, (int64_t)0), (int64_t)tokens);
 }
 
-// Units over all heads that are aimed at: two rounds of two workgroups a CU.  Chunks of
-// 1,500 tokens and a prompt of 4,001 with 512: 155 and 94 us, 1,024: 146 and 97, 1,536:
-// 141 and 105; with 1,024 in the chunks' order, not by size: 155 and 98.
+// Units over all heads, besides one for each chunk: two rounds of two workgroups a CU.
+// The costly ones come first, as workgroups are not equally fast (of two on a CU the
+// older one takes 1.5 us a tile, the other 2.15).  Chunks of 1,500 tokens and a prompt
+// of 4,001 with 512: 161 and 99 us, 768: 148 and 93, 1,024: 145 and 87, 1,536: 152 and
+// 89; with 1,024 in the chunks' order 151 and 93.
 constexpr int kShares = 1024;
 constexpr int kLeastTiles = 4;  // of a unit
-constexpr int kClasses = 16;    // of units, by size
+constexpr int kClasses = 64;    // of units, by cost
 __host__ __device__ __forceinline__ int more_units(const KvWeighArgs& a) {
   return kShares > a.c.heads ? kShares / a.c.heads : 1;
 }
@@ -301,7 +298,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_weigh_plan_kernel(KvWeighArgs
   __shared__ int waves[kWaves];
   __shared__ Span spans[kPlanSpans];
   __shared__ int firsts[kPlanSpans + 1];
-  __shared__ int64_t totals[kWaves], numbers[kWaves];
+  __shared__ int64_t totals[kWaves];
   __shared__ int at[kClasses], several, slots;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const Work work = work_of(a);
@@ -343,69 +340,76 @@ __global__ __launch_bounds__(kPlanThreads) void kv_weigh_plan_kernel(KvWeighArgs
   if (threadIdx.x == 0) firsts[0] = work.first[0] = several = slots = 0;
   if (threadIdx.x < kClasses) at[threadIdx.x] = 0;
   __syncthreads();
-  // ... how many tiles they have, of which a unit gets so many that the units are no
-  // more than the chunks and as many as aimed at ...
+  // ... how many tiles they have altogether ...
   int64_t total = 0;
   for (int i = threadIdx.x; i < chunks; i += kPlanThreads) total += tiles_of(part(i));
-  total = over_wave(total);
+#pragma unroll
+  for (int i = 32; i >= 1; i >>= 1) total += __shfl_xor(total, i);
   if (lane == 0) totals[wave] = total;
   __syncthreads();
   total = 0;
   for (int w = 0; w < kWaves; ++w) total += totals[w];
   const int extra = more_units(a);
-  const auto piece_of = [&](int w) {
-    return (int)min(max((int64_t)kLeastTiles, (total + extra - 1) / extra) * (kWaves + w) / kWaves,
-                    (int64_t)INT32_MAX);
+  const int piece = (int)max((int64_t)kLeastTiles, (total + extra - 1) / extra);
+  // ... and their units, of as many tiles or one less, the costly ones first
+  struct Cut {
+    int tiles, units, masked;  // (masked: tiles of which a row does not see all keys)
   };
-  int piece = piece_of(0);
-  // ... if the chunks are few, no more than that altogether: each wavefront tries a number
-  if (2 * chunks <= extra) {
-    int64_t n = 0;
-    const int mine = piece_of(wave);
-    for (int i = lane; i < chunks; i += 64) n += (tiles_of(part(i)) + mine - 1) / mine;
-    n = over_wave(n);
-    if (lane == 0) numbers[wave] = n;
-    __syncthreads();
-    int w = 0;
-    while (w < kWaves - 1 && numbers[w] > extra) ++w;
-    piece = piece_of(w);
-  }
-  // ... and the units, the large ones first.  (Which of the same class comes first only
-  // changes where its sums are.)
-  const auto pieces_of = [&](int tiles) { return (tiles + piece - 1) / piece; };
-  const auto class_of = [&](int tiles) {
-    const int n = pieces_of(tiles);
-    return (int)((int64_t)(piece - (tiles + n - 1) / n) * kClasses / piece);
+  const auto cut = [&](const Part& p) {
+    const int tiles = tiles_of(p);
+    Cut c{tiles, (tiles + piece - 1) / piece, 0};
+    const int all = sees(p.sp.first, p.sp.tokens, (int64_t)(p.chunk + 1) * kChunk - 1) - p.from;
+    c.masked = min(c.tiles, (max(all, 0) + a.tile - 1) / a.tile);
+    return c;
   };
-  for (int i = threadIdx.x; i < chunks; i += kPlanThreads) {
-    const int tiles = tiles_of(part(i));
-    atomicAdd(&at[class_of(tiles)], pieces_of(tiles));
+  const auto edge = [&](const Cut& c, int j) {  // where unit j begins
+    return c.tiles / c.units * j + min(j, c.tiles % c.units);
+  };
+  const auto class_of = [&](const Cut& c, int from, int to) {
+    const float cost = (float)(to - from) + 0.3f * (float)min(max(c.masked - from, 0), to - from);
+    return (int)((float)(kClasses - 1) * max(0.0f, 1.0f - cost / (1.3f * (float)piece)));
+  };
+  // (a wavefront a chunk, a lane a unit, but for many chunks)
+  const int lanes = chunks <= kPlanThreads ? 64 : 1;
+  const int first = threadIdx.x / lanes, step = kPlanThreads / lanes, mine = threadIdx.x % lanes;
+  for (int i = first; i < chunks; i += step) {
+    const Cut c = cut(part(i));
+    for (int j = mine; j < c.units; j += lanes)
+      atomicAdd(&at[class_of(c, edge(c, j), edge(c, j + 1))], 1);
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    int n = 0;
-    for (int i = 0; i < kClasses; ++i) {
-      const int x = at[i];
-      at[i] = n;
-      n += x;
+  if (wave == 0) {
+    int n = lane < kClasses ? at[lane] : 0;
+    const int own = n;
+#pragma unroll
+    for (int by = 1; by < 64; by <<= 1) {
+      const int y = __shfl_up(n, by);
+      if (lane >= by) n += y;
     }
-    work.units[0] = n;
+    if (lane < kClasses) at[lane] = n - own;
+    if (lane == 63) work.units[0] = n;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < chunks; i += kPlanThreads) {
+  // (which of a class comes first only changes where its sums are)
+  for (int i = first; i < chunks; i += step) {
     const Part p = part(i);
-    const int tiles = tiles_of(p), pieces = pieces_of(tiles);
-    const int to = atomicAdd(&at[class_of(tiles)], pieces);
-    const int slot = pieces > 1 ? atomicAdd(&slots, pieces) : 0;
-    Unit u{p.request, p.chunk, 0, 0, -1, p.sp.first - p.sp.begin, p.sp.last, pieces};
-    // (all of a chunk's units have as many tiles, or one less)
-    for (int j = 0; j < pieces; ++j) {
-      u.begin = p.sp.begin + p.from + (int)((int64_t)tiles * j / pieces) * a.tile;
-      u.end = p.sp.begin +
-              min(p.sp.tokens, p.from + (int)((int64_t)tiles * (j + 1) / pieces) * a.tile);
-      u.slot = pieces > 1 ? slot + j : -1;
-      work.unit[to + j] = u;
-      if (j == 0 && pieces > 1) work.several[atomicAdd(&several, 1)] = u;
+    const Cut c = cut(p);
+    Unit u{p.request, p.chunk, 0, 0, -1, p.sp.first - p.sp.begin, p.sp.last, c.units};
+    int slot = 0, place = 0;
+    if (c.units > 1) {
+      if (mine == 0) {
+        slot = atomicAdd(&slots, c.units);
+        place = atomicAdd(&several, 1);
+      }
+      if (lanes > 1) slot = uniform(slot);
+    }
+    for (int j = mine; j < c.units; j += lanes) {
+      const int from = edge(c, j), to = edge(c, j + 1);
+      u.begin = p.sp.begin + p.from + from * a.tile;
+      u.end = p.sp.begin + min(p.sp.tokens, p.from + to * a.tile);
+      u.slot = c.units > 1 ? slot + j : -1;
+      work.unit[atomicAdd(&at[class_of(c, from, to)], 1)] = u;
+      if (j == 0 && c.units > 1) work.several[place] = u;
     }
   }
   __syncthreads();

@@ -66,7 +66,10 @@ __device__ __forceinline__ T lds_read4(uint32_t at) {
 // compiler waits for all loads like those above before it reads any LDS that one of
 // them may have written, and takes every buffer for such; of these it knows
 // nothing: whoever reads what they bring waits for them (staged_barrier).  They
-// return nothing to registers.  The place in LDS is the wavefront's.
+// return nothing to registers.  The place in LDS is the wavefront's.  (m0 is named as
+// written, of which the compiler warns, since it has uses for it itself.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void stream16_to_lds(const void* from, uint32_t lds) {
 #if defined(__HIP_DEVICE_COMPILE__)
   const int to = __builtin_amdgcn_readfirstlane((int)lds);
@@ -81,6 +84,7 @@ __device__ __forceinline__ void stream4_to_lds(const void* from, uint32_t lds) {
                ::"v"(from), "s"(to) : "memory", "m0");
 #endif
 }
+#pragma clang diagnostic pop
 
 // A workgroup barrier once all but the latest LEFT of this wavefront's loads are
 // done, for buffers that stream*_to_lds fill.
