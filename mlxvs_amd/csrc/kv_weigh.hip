@@ -20,8 +20,8 @@
 //
 // Measured: single tokens over 64 requests of up to 8,192 keys in 8 heads of 128
 // values 122 us, 5.1 TB/s of keys, masses and their return (a copy: 4.95); chunks of
-// 1,500 tokens in 3 requests of up to 8,192, 32 heads on 8, 145 us, 798 TFLOP/s, and
-// a prompt of 4,001 tokens, 28 heads on 4, 87 us, 659.  Two workgroups on a CU take
+// 1,500 tokens in 3 requests of up to 8,192, 32 heads on 8, 138 us, 836 TFLOP/s, and
+// a prompt of 4,001 tokens, 28 heads on 4, 86 us, 667 (16 long prompts together 877).  Two workgroups on a CU take
 // 28 ns a product and SIMD, as a large library product does (27, the card's power); the
 // rest are some 4 us at a unit's begin, until its keys and first rows are there, the
 // end, where CUs run dry, masked tiles, and 12 us of plan and joining.  Tried: 128
@@ -282,8 +282,8 @@ __device__ __forceinline__ int sees(int first, int tokens, int64_t p) {
 // Units over all heads, besides one for each chunk: two rounds of two workgroups a CU.
 // The costly ones come first, as workgroups are not equally fast (of two on a CU the
 // older one takes 1.5 us a tile, the other 2.15).  Chunks of 1,500 tokens and a prompt
-// of 4,001 with 512: 161 and 99 us, 768: 148 and 93, 1,024: 145 and 87, 1,536: 152 and
-// 89; with 1,024 in the chunks' order 151 and 93.
+// of 4,001 with 512: 155 and 99 us, 768: 141 and 93, 1,024: 138 and 86, 1,536: 145 and
+// 93; with 1,024 in the chunks' order 150 and 94.
 constexpr int kShares = 1024;
 constexpr int kLeastTiles = 4;  // of a unit
 constexpr int kClasses = 64;    // of units, by cost
@@ -300,6 +300,11 @@ __global__ __launch_bounds__(kPlanThreads) void kv_weigh_plan_kernel(KvWeighArgs
   __shared__ int firsts[kPlanSpans + 1];
   __shared__ int64_t totals[kWaves];
   __shared__ int at[kClasses], several, slots;
+  struct Cut {  // a chunk; masked: tiles of which a row does not see all keys
+    int request, chunk, from, tiles, masked, units, slot;
+  };
+  __shared__ Cut cuts[kPlanThreads];
+  __shared__ int ends[kPlanThreads];  // units up to a chunk's last
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const Work work = work_of(a);
   const bool few = a.q.requests <= kPlanSpans;
@@ -352,15 +357,34 @@ __global__ __launch_bounds__(kPlanThreads) void kv_weigh_plan_kernel(KvWeighArgs
   const int extra = more_units(a);
   const int piece = (int)max((int64_t)kLeastTiles, (total + extra - 1) / extra);
   // ... and their units, of as many tiles or one less, the costly ones first
-  struct Cut {
-    int tiles, units, masked;  // (masked: tiles of which a row does not see all keys)
+  const auto fill = [&](int i0, bool placing) {  // kPlanThreads chunks; their number of units
+    const int i = i0 + threadIdx.x;
+    Cut c{};
+    if (i < chunks) {
+      const Part p = part(i);
+      const int tiles = tiles_of(p);
+      const int all = sees(p.sp.first, p.sp.tokens, (int64_t)(p.chunk + 1) * kChunk - 1) - p.from;
+      c = {p.request, p.chunk, p.from, tiles, min(tiles, (max(all, 0) + a.tile - 1) / a.tile),
+           (tiles + piece - 1) / piece, -1};
+      if (placing && c.units > 1) c.slot = atomicAdd(&slots, c.units);
+    }
+    int all;
+    ends[threadIdx.x] = running(c.units, all, waves);
+    cuts[threadIdx.x] = c;
+    __syncthreads();
+    return all;
   };
-  const auto cut = [&](const Part& p) {
-    const int tiles = tiles_of(p);
-    Cut c{tiles, (tiles + piece - 1) / piece, 0};
-    const int all = sees(p.sp.first, p.sp.tokens, (int64_t)(p.chunk + 1) * kChunk - 1) - p.from;
-    c.masked = min(c.tiles, (max(all, 0) + a.tile - 1) / a.tile);
-    return c;
+  const auto each = [&](int units, auto use) {  // (chunk, its how many-th unit)
+    for (int u = threadIdx.x; u < units; u += kPlanThreads) {
+      int lo = 0, hi = kPlanThreads - 1;  // the first one whose end is past u
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (ends[mid] > u) hi = mid;
+        else lo = mid + 1;
+      }
+      const Cut c = cuts[lo];
+      use(c, u - (ends[lo] - c.units));
+    }
   };
   const auto edge = [&](const Cut& c, int j) {  // where unit j begins
     return c.tiles / c.units * j + min(j, c.tiles % c.units);
@@ -369,13 +393,11 @@ __global__ __launch_bounds__(kPlanThreads) void kv_weigh_plan_kernel(KvWeighArgs
     const float cost = (float)(to - from) + 0.3f * (float)min(max(c.masked - from, 0), to - from);
     return (int)((float)(kClasses - 1) * max(0.0f, 1.0f - cost / (1.3f * (float)piece)));
   };
-  // (a wavefront a chunk, a lane a unit, but for many chunks)
-  const int lanes = chunks <= kPlanThreads ? 64 : 1;
-  const int first = threadIdx.x / lanes, step = kPlanThreads / lanes, mine = threadIdx.x % lanes;
-  for (int i = first; i < chunks; i += step) {
-    const Cut c = cut(part(i));
-    for (int j = mine; j < c.units; j += lanes)
-      atomicAdd(&at[class_of(c, edge(c, j), edge(c, j + 1))], 1);
+  int units = 0;
+  for (int i0 = 0; i0 < chunks; i0 += kPlanThreads) {
+    if (i0 > 0) __syncthreads();  // (the last ones are done with)
+    units = fill(i0, chunks <= kPlanThreads);
+    each(units, [&](const Cut& c, int j) { atomicAdd(&at[class_of(c, edge(c, j), edge(c, j + 1))], 1); });
   }
   __syncthreads();
   if (wave == 0) {
@@ -391,26 +413,18 @@ __global__ __launch_bounds__(kPlanThreads) void kv_weigh_plan_kernel(KvWeighArgs
   }
   __syncthreads();
   // (which of a class comes first only changes where its sums are)
-  for (int i = first; i < chunks; i += step) {
-    const Part p = part(i);
-    const Cut c = cut(p);
-    Unit u{p.request, p.chunk, 0, 0, -1, p.sp.first - p.sp.begin, p.sp.last, c.units};
-    int slot = 0, place = 0;
-    if (c.units > 1) {
-      if (mine == 0) {
-        slot = atomicAdd(&slots, c.units);
-        place = atomicAdd(&several, 1);
-      }
-      if (lanes > 1) slot = uniform(slot);
-    }
-    for (int j = mine; j < c.units; j += lanes) {
+  for (int i0 = 0; i0 < chunks; i0 += kPlanThreads) {
+    if (i0 > 0) __syncthreads();
+    if (chunks > kPlanThreads) units = fill(i0, true);
+    each(units, [&](const Cut& c, int j) {
+      const Span sp = few ? spans[c.request] : span_of(a, c.request);
       const int from = edge(c, j), to = edge(c, j + 1);
-      u.begin = p.sp.begin + p.from + from * a.tile;
-      u.end = p.sp.begin + min(p.sp.tokens, p.from + to * a.tile);
-      u.slot = c.units > 1 ? slot + j : -1;
+      const Unit u{c.request, c.chunk, sp.begin + c.from + from * a.tile,
+                   sp.begin + min(sp.tokens, c.from + to * a.tile), c.units > 1 ? c.slot + j : -1,
+                   sp.first - sp.begin, sp.last, c.units};
       work.unit[atomicAdd(&at[class_of(c, from, to)], 1)] = u;
-      if (j == 0 && c.units > 1) work.several[place] = u;
-    }
+      if (j == 0 && c.units > 1) work.several[atomicAdd(&several, 1)] = u;
+    });
   }
   __syncthreads();
   if (threadIdx.x == 0) work.shared[0] = several;
