@@ -14,20 +14,22 @@
 // (a token's query head each) come through LDS by direct loads, whole tokens of up
 // to 64 rows at a time, three tiles ahead, for all four wavefronts.  A lane adds up
 // its column's weights of each of its 32 keys over all rows, and the columns meet
-// once at the end.  A product of 32 x 32 takes as long as the 6 vector instructions
-// for its 2 weights a lane (fma, exp, add), so both kinds are written side by side:
-// a block's products next to the weights of the one before.
+// once at the end.  A product of 32 x 32 takes 33 cycles of a SIMD, the 6 vector
+// instructions of its 2 weights a lane (fma, exp, add) 21, so both kinds are written
+// side by side, a block's products next to the weights of the one before: 41 cycles,
+// 59 if four of each follow one another.
 //
 // Measured: single tokens over 64 requests of up to 8,192 keys in 8 heads of 128
 // values 122 us, 5.1 TB/s of keys, masses and their return (a copy: 4.95); chunks of
 // 1,500 tokens in 3 requests of up to 8,192, 32 heads on 8, 138 us, 836 TFLOP/s, and
-// a prompt of 4,001 tokens, 28 heads on 4, 86 us, 667 (16 long prompts together 877).  Two workgroups on a CU take
-// 28 ns a product and SIMD, as a large library product does (27, the card's power); the
-// rest are some 4 us at a unit's begin, until its keys and first rows are there, the
-// end, where CUs run dry, masked tiles, and 12 us of plan and joining.  Tried: 128
-// keys a wavefront and 128 rows a tile, with one wavefront a SIMD, 181 and 144; one
-// share of all tiles for each workgroup, which may go on in another chunk, 211 and 103
-// (the rows of Q then miss in L2); a fifth of the tiles in small units, the same.
+// a prompt of 4,001 tokens, 28 heads on 4, 86 us, 667 (16 prompts of up to 32,768
+// together 877).  Two workgroups on a CU take 28 ns a product and SIMD, as a large
+// library product does (27, the card's power); the rest are some 4 us at a unit's
+// begin, until its keys and first rows are there, the end, where CUs run dry, masked
+// tiles, and 12 us of plan and joining.  Tried: 128 keys a wavefront and 128 rows a
+// tile, with one wavefront a SIMD, 181 and 144; one share of all tiles for each
+// workgroup, which may go on in another chunk, 211 and 103 (the rows of Q then miss
+// in L2); a fifth of the tiles in small units, the same.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
