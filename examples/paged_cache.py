@@ -62,17 +62,18 @@ def run(requests=8, context=16384, steps=32, blocks=32, seed=0, budget=0):
     lengths = torch.zeros(requests, **ints)
     rotary = mlxvs.Rotary(DIM)
     evicted = torch.zeros(requests, **ints)  # tokens of a request that the cache has lost
+    longest = max(prompts) + (0 if budget else steps)  # tokens that a request holds at most
     mass = torch.zeros(requests, KV_HEADS, columns * PAGE, device="cuda") if budget else None
 
     def cut(q, plan, lse):
         """The step's attention counted, and the requests cut that hold a page too many."""
-        nonlocal lengths, cursor, evicted
-        cache.weigh(q, table, plan.starts, plan.positions, lse, mass,
-                    longest=max(prompts) + steps)
+        nonlocal lengths, cursor, evicted, longest
+        cache.weigh(q, table, plan.starts, plan.positions, lse, mass, longest=longest)
         kept = cache.keep(mass, plan.lengths, budget, first=min(4, budget // 2),
                           recent=min(2 * PAGE, budget // 2), above=budget + PAGE - 1)
         lengths, cursor = cache.compact(table, plan.lengths, kept, free, plan.cursor, mass=mass)
         evicted = evicted + plan.lengths - lengths
+        longest = budget + PAGE
 
     # the prompts, all tokens in one step
     total = sum(prompts)
@@ -81,8 +82,7 @@ def run(requests=8, context=16384, steps=32, blocks=32, seed=0, budget=0):
     q, k, v = layer.project(x)
     q, k = rotary.rotate(q, k, plan.positions)
     cache.append(k, v, plan.slots)
-    out, lse = cache.attend(q, table, plan.requests, plan.positions, longest=max(prompts),
-                            lse=True)
+    out, lse = cache.attend(q, table, plan.requests, plan.positions, longest=longest, lse=True)
     last = torch.tensor(prompts, device="cuda").cumsum(0) - 1  # the prompts' last tokens
     x = torch.tanh(out[last].flatten(1) @ layer.out)
     lengths, cursor = plan.lengths, plan.cursor
@@ -104,8 +104,7 @@ def run(requests=8, context=16384, steps=32, blocks=32, seed=0, budget=0):
         lengths, cursor = plan.lengths, plan.cursor
         torch.cuda.synchronize()
         spent += time.perf_counter() - start if i else 0.0  # (the first one warms up)
-        full, lse = cache.attend(q, table, plan.requests, plan.positions,
-                                 longest=max(prompts) + steps, lse=True)
+        full, lse = cache.attend(q, table, plan.requests, plan.positions, longest=longest, lse=True)
         if budget:
             cut(q, plan, lse)
         close += torch.cosine_similarity(out.float().flatten(1), full.float().flatten(1)).mean() \
