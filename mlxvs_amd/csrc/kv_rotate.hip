@@ -141,9 +141,9 @@ __global__ __launch_bounds__(256) void kv_rotate_any_kernel(KvRotateArgs a) {
   }
 }
 
-// `rotated` a multiple of 16 (a value a lane is 300 instead of 72 us, above): a lane has 16 values of a head, two pieces of 16 bytes
-// that are turned with one another (halves) or within themselves (pairs), or that
-// pass.  LANES lanes have a head, a wavefront 64 / LANES heads of one token at a
+// `rotated` a multiple of 16 (a value a lane is 300 instead of 72 us, above): a lane has
+// 16 values of a head, two pieces of 16 bytes that are turned with one another (halves)
+// or within themselves (pairs), or that pass.  LANES lanes have a head, a wavefront 64 / LANES heads of one token at a
 // time, with the same angles for all of them.
 template <bool BF16, bool PAIRS, bool NORM, int LANES>
 __global__ __launch_bounds__(256) void kv_rotate_kernel(KvRotateArgs a, int parts) {

@@ -631,7 +631,9 @@ class PagedKVCache:
         other).  A request of at most ``above`` keeps all: its list is -1
         throughout.  ``lengths`` int32 [requests]."""
         op = "kv_keep"
-        n = int(n)
+        n, first, recent = int(n), int(first), int(recent)
+        above = n if above is None else min(int(above), (1 << 31) - 1)
+        _need(max(n, first, recent) < 1 << 31, op, "n, first and recent must be below 2^31.")
         device = self._device
         pl = _ints(lengths, "lengths", op, device)
         requests = lengths.numel()
@@ -642,8 +644,7 @@ class PagedKVCache:
             work, size = self._scratch("mlxvs_kv_keep_workspace", mass, requests, self.kv_heads,
                                        mass.shape[2])
             _check(_L().mlxvs_kv_keep_device(pm, requests, self.kv_heads, mass.shape[2], pl, n,
-                                             int(first), int(recent),
-                                             n if above is None else int(above), kept.data_ptr(),
+                                             first, recent, above, kept.data_ptr(),
                                              None if work is None else work.data_ptr(), size,
                                              stream))
         return kept

@@ -883,3 +883,75 @@ def test_the_example_within_a_budget(engine):
     # (prompts of 593 and 886 tokens cut to 256, and again after 64; one of 300 after 20)
     assert lengths == [256 + 50, 256 + 6, 256 + 6] and math.isfinite(close) and ms > 0
     assert example.run(requests=2, context=100, steps=3, blocks=4, budget=1)[0] == [53, 4]
+
+
+def test_budgets_of_numbers_past_32_bits(engine):
+    c = engine.PagedKVCache.empty(1, 2, 16, 64)
+    mass, lengths = torch.rand(1, 2, 64, device="cuda"), dev([50], torch.int32)
+    assert (c.keep(mass, lengths, 8, above=2 ** 33) == -1).all()
+    for k in (dict(first=2 ** 32), dict(recent=2 ** 32 + 1)):
+        with pytest.raises(ValueError, match="below 2"):
+            c.keep(mass, lengths, 8, **k)
+
+
+def test_offsets_past_32_bits_of_rows(engine):
+    # places 2^30 values apart
+    rng = np.random.default_rng(0)
+    room = torch.empty(5 * 2 ** 29 + 1024, dtype=torch.bfloat16, device="cuda")
+    q, k = rows(rng, 3, 4, 64, "bf16"), rows(rng, 3, 2, 64, "bf16")
+    far = room.as_strided((3, 4, 64), (2 ** 30, 64, 1))
+    far_k = room.as_strided((3, 2, 64), (2 ** 30, 64, 1), 512)
+    far.copy_(q)
+    far_k.copy_(k)
+    pos = dev([5, 70_000, 2 ** 31 - 1], torch.int32)
+    for rotated in (64, 20):
+        rot = engine.Rotary(64, rotated=rotated)
+        want = rot.rotate(q, k, pos)
+        got = rot.rotate(far, far_k, pos)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    rot.rotate(far, far_k, pos, out=(far, far_k))
+    assert torch.equal(far, want[0]) and torch.equal(far_k, want[1])
+
+
+def test_offsets_past_32_bits_of_a_cache(engine):
+    # the same step over pages at both ends of a cache of more than 2^31 values
+    heads, page, dim = 8, 64, 128
+    lengths, counts = [500, 300], [200, 1]
+    pages = 2 ** 31 // (heads * page * dim) + 40
+    near = Step(engine, lengths, counts, page=page, heads=heads, group=2, dim=dim, seed=2).attend()
+    cache = engine.PagedKVCache.empty(pages, heads, page, dim)
+    held = near.cache.keys.shape[0]
+    for name in ("keys", "values", "summaries", "scales"):
+        getattr(cache, name)[pages - held:].copy_(getattr(near.cache, name))
+    table = torch.where(near.table >= 0, near.table + (pages - held), near.table)
+    for n in (201, 2):  # prompts, and a token each
+        s = near
+        if n == 2:
+            s = Step(engine, lengths, [1, 1], page=page, heads=heads, group=2, dim=dim, seed=2).attend()
+        want, mass = s.mass.clone(), s.mass.clone()
+        s.cache.weigh(s.q, s.table, s.starts, s.positions, s.lse, want)
+        cache.weigh(s.q, table, s.starts, s.positions, s.lse, mass)
+        assert len(s.q) == n and torch.equal(mass, want)
+    kept = near.cache.keep(want, dev(lengths, torch.int32), 130)
+    i = dict(dtype=torch.int32, device="cuda")
+    for c, t, m in ((near.cache, near.table, want), (cache, table, mass)):
+        free = torch.full((40,), -7, **i)
+        out = c.compact(t, dev(lengths, torch.int32), kept, free, dev([30], torch.int32), mass=m)
+        assert out.lengths.tolist() == [130, 130] and out.cursor.tolist() == [30 - 5 - 2]
+    assert torch.equal(mass, want)
+    for name in ("keys", "values", "summaries", "scales"):
+        a, b = getattr(cache, name)[pages - held:], getattr(near.cache, name)
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)), name
+
+
+def test_offsets_past_32_bits_of_masses(engine):
+    requests, heads, slots = 4_200, 8, 65_536
+    c = engine.PagedKVCache.empty(1, heads, 16, 64)
+    mass = torch.empty(requests, heads, slots, device="cuda")
+    lengths = torch.zeros(requests, dtype=torch.int32, device="cuda")
+    lengths[-1] = 6_000
+    row = torch.rand(1, heads, slots, device="cuda")
+    mass[-1].copy_(row[0])
+    want = c.keep(row, lengths[-1:], 100)
+    got = c.keep(mass, lengths, 100)
+    assert torch.equal(got[-1], want[0]) and (got[:-1] == -1).all()
