@@ -88,12 +88,12 @@ def _ints(x, name: str, op: str, device, dtype=torch.int32, size: Optional[int] 
 
 
 def _table(table, op: str, device):
-    _need(isinstance(table, torch.Tensor) and table.dtype == torch.int32 and table.dim() == 2
-          and table.device == device
-          and (table.shape[1] <= 1 or table.stride(1) == 1 or table.numel() == 0)
-          and (table.shape[0] <= 1 or table.stride(0) >= table.shape[1]), op,
-          f"table must be an int32 [requests, columns] tensor on {device} with contiguous rows "
-          "that do not overlap.")
+    if not (isinstance(table, torch.Tensor) and table.dtype == torch.int32 and table.dim() == 2
+            and table.device == device
+            and (table.shape[1] <= 1 or table.stride(1) == 1 or table.numel() == 0)
+            and (table.shape[0] <= 1 or table.stride(0) >= table.shape[1])):
+        raise ValueError(f"[mlxvs::{op}] table must be an int32 [requests, columns] tensor on "
+                         f"{device} with contiguous rows that do not overlap.")
     return table.data_ptr(), max(table.stride(0), table.shape[1])
 
 
@@ -278,20 +278,21 @@ class Rotary:
             raise ValueError(f"[mlxvs::{op}] {name} must be a float16 or bfloat16 [tokens, heads, "
                              f"{self.dim}] tensor on {device}, as many tokens and of one type.")
         if norm is not None:
-            _need(isinstance(norm, torch.Tensor) and norm.shape == (self.dim,)
-                  and norm.dtype in (x.dtype, torch.float32) and norm.device == device
-                  and norm.is_contiguous(), op,
-                  f"{name}_norm must be a contiguous {x.dtype} or float32 [{self.dim}] tensor on "
-                  f"{device}.")
+            if not (isinstance(norm, torch.Tensor) and norm.shape == (self.dim,)
+                    and norm.dtype in (x.dtype, torch.float32) and norm.device == device
+                    and norm.is_contiguous()):
+                raise ValueError(f"[mlxvs::{op}] {name}_norm must be a contiguous {x.dtype} or "
+                                 f"float32 [{self.dim}] tensor on {device}.")
             if norm.data_ptr() & 15:
                 norm = norm.clone()
         if out is None:
             out = torch.empty_like(x, memory_format=torch.contiguous_format)
         else:
-            _need(isinstance(out, torch.Tensor) and out.shape == x.shape and out.dtype == x.dtype
-                  and out.device == device and _aligned(out), op,
-                  f"out of {name} must be a {x.dtype} {list(x.shape)} tensor on {device}, 16-byte "
-                  "aligned with contiguous heads.")
+            if not (isinstance(out, torch.Tensor) and out.shape == x.shape
+                    and out.dtype == x.dtype and out.device == device and _aligned(out)):
+                raise ValueError(f"[mlxvs::{op}] out of {name} must be a {x.dtype} "
+                                 f"{list(x.shape)} tensor on {device}, 16-byte aligned with "
+                                 "contiguous heads.")
         if not _aligned(x):
             x = x.clone(memory_format=torch.contiguous_format)
         st, so = x.stride(), out.stride()
@@ -607,10 +608,11 @@ class PagedKVCache:
         q, qs = self._queries(q, table, None, positions, op)
         tokens, heads, dim = q.shape
         ps = _ints(starts, "starts", op, self._device, size=qs.requests + 1)
-        _need(isinstance(lse, torch.Tensor) and lse.shape == (tokens, heads)
-              and lse.dtype == torch.float32 and lse.device == self._device
-              and lse.is_contiguous(), op,
-              f"lse must be a contiguous float32 [tokens, q_heads] tensor on {self._device}.")
+        if not (isinstance(lse, torch.Tensor) and lse.shape == (tokens, heads)
+                and lse.dtype == torch.float32 and lse.device == self._device
+                and lse.is_contiguous()):
+            raise ValueError(f"[mlxvs::{op}] lse must be a contiguous float32 [tokens, q_heads] "
+                             f"tensor on {self._device}.")
         pm = self._mass(mass, op, qs.requests, qs.columns * self.page_size)
         if scale is None:
             scale = 1.0 / math.sqrt(dim)
