@@ -9,13 +9,13 @@
 // and the first of those that equal it.
 //
 // A row of up to 65,536 slots is a workgroup's and read once: its ranks stay in
-// registers.  A longer one is split into parts of 16,384, a workgroup each, with a
+// registers.  A longer one is split into parts of 8,192 or more, a workgroup each, with a
 // launch for every histogram and one for the list: the parts' histograms are summed
 // by whoever needs them, so that nothing is counted by atomics in memory.
 //
 // Chains of small steps, far from the bytes' 2 us: 256 rows of 16,384 slots 15 us (53
 // if all masses are equal, whose counts meet in one place; 20 if half of them are),
-// 8 rows of 262,144 38 us in four launches.
+// 8 rows of 262,144 32 us in four launches.
 #include <hip/hip_runtime.h>
 
 #include "kv_cache.h"
@@ -26,9 +26,9 @@ namespace {
 constexpr uint32_t kAlways = 0xFFFFFFFFu;
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kBins = 2048, kDigits = 3;
-constexpr int kPart = 16384;       // slots of a part
 
 __device__ __forceinline__ int shift_of(int digit) { return digit == 0 ? 21 : digit == 1 ? 10 : 0; }
+__device__ __forceinline__ int bins_of(int digit) { return digit == 2 ? 1024 : kBins; }
 __device__ __forceinline__ uint32_t digit_of(uint32_t rank, int digit) {
   return digit == 2 ? rank & 1023 : rank >> shift_of(digit) & 2047;
 }
@@ -49,17 +49,20 @@ struct Ranks {
   uint32_t k[R];
   int from;  // this lane's first token
 
-  __device__ __forceinline__ Ranks(const KvKeepArgs& a, const float* mass, int start, int length) {
+  // (read first, ranked once something else has been read, too)
+  __device__ __forceinline__ Ranks(const float* mass, int start, int length) {
     from = start + (threadIdx.x >> 6) * 64 * R + (threadIdx.x & 63);
-    float x[R];
 #pragma unroll
-    for (int i = 0; i < R; ++i) x[i] = from + 64 * i < length ? mass[from + 64 * i] : 0.0f;
+    for (int i = 0; i < R; ++i)
+      k[i] = __builtin_bit_cast(uint32_t, from + 64 * i < length ? mass[from + 64 * i] : 0.0f);
+  }
+  __device__ __forceinline__ void rank(const KvKeepArgs& a, int length) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int t = from + 64 * i;
-      k[i] = t >= length                                 ? 0
+      k[i] = t >= length                             ? 0
              : t < a.first || t >= length - a.recent ? kAlways
-                                                         : rank_of(x[i]);
+                                                     : rank_of(__builtin_bit_cast(float, k[i]));
     }
   }
 
@@ -152,7 +155,8 @@ __global__ __launch_bounds__(kThreads) void kv_keep_kernel(KvKeepArgs a) {
   const int length = length_of(a, row), tid = threadIdx.x;
   int32_t* out = a.kept + row * a.n;
   if (length <= a.above) return none(a, out);
-  const Ranks<R> ranks(a, a.mass + row * a.slots, 0, length);
+  Ranks<R> ranks(a.mass + row * a.slots, 0, length);
+  ranks.rank(a, length);
   uint32_t cut = 0;
   int left = a.n;
 #pragma unroll 1
@@ -184,8 +188,17 @@ struct Work {
   int* above;      // [rows][parts][2]: by the first digit, by the second
   uint32_t* known; // [rows][2][2]: after the first and second digit: prefix, left
 };
+// Slots of a part for each of its threads: few, but no more than 32 parts if that can
+// be, since each reads the histograms of all.  8 rows of 262,144 slots with 4, 8, 16, 32:
+// 59, 34, 37, 51 us; of 1,048,576 with 16, 32, 64: 97, 78, 139.
+__host__ __device__ __forceinline__ int each_of(const KvKeepArgs& a) {
+  int each = 8;
+  while (each < 64 && a.slots > (int64_t)32 * kThreads * each) each *= 2;
+  return each;
+}
 __host__ __device__ __forceinline__ int64_t parts_of(const KvKeepArgs& a) {
-  return (a.slots + kPart - 1) / kPart;
+  const int part = kThreads * each_of(a);
+  return (a.slots + part - 1) / part;
 }
 __device__ __forceinline__ Work work_of(const KvKeepArgs& a) {
   const int64_t rows = a.requests * a.heads, units = rows * parts_of(a);
@@ -195,12 +208,13 @@ __device__ __forceinline__ Work work_of(const KvKeepArgs& a) {
 
 // STEP 0, 1, 2: the part's histogram of that digit, the one before it being found
 // first.  STEP 3: the list.
-template <int STEP>
+template <int STEP, int R>
 __global__ __launch_bounds__(kThreads) void kv_keep_part_kernel(KvKeepArgs a) {
+  constexpr int kPart = kThreads * R;
   __shared__ uint32_t hist[kBins];
   __shared__ Pick s;
   __shared__ int waves[kWaves][2];
-  __shared__ int sums[kWaves];
+  __shared__ int sums[kWaves], same;
   const int parts = (int)parts_of(a), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x / parts;
   const int part = (int)(blockIdx.x % parts), length = length_of(a, row);
@@ -212,7 +226,8 @@ __global__ __launch_bounds__(kThreads) void kv_keep_part_kernel(KvKeepArgs a) {
   const int some = (length + kPart - 1) / kPart;  // parts that hold tokens
   if (part >= some) return;
   const Work work = work_of(a);
-  const Ranks<kPart / kThreads> ranks(a, a.mass + row * a.slots, part * kPart, length);
+  Ranks<R> ranks(a.mass + row * a.slots, part * kPart, length);
+  if (STEP == 0) ranks.rank(a, length);
   const auto hist_of = [&](int p, int digit) {
     return work.hist + ((row * parts + p) * kDigits + digit) * kBins;
   };
@@ -225,22 +240,27 @@ __global__ __launch_bounds__(kThreads) void kv_keep_part_kernel(KvKeepArgs a) {
       prefix = work.known[row * 4 + (STEP - 2) * 2];
       left = (int)work.known[row * 4 + (STEP - 2) * 2 + 1];
     }
-    int hi = 0, lo = 0;
-#pragma unroll 8
-    for (int p = 0; p < some; ++p) {
-      const uint2 x = *(const uint2*)(hist_of(p, kDigit) + b0);
-      lo += (int)x.x;
-      hi += (int)x.y;
+    int hi = 0, lo = 0;  // over all parts; and of this one, or for the list of those before it
+    int hi_here = 0, lo_here = 0;
+    if (b0 < bins_of(kDigit)) {
+#pragma unroll 16
+      for (int p = 0; p < some; ++p) {
+        const uint2 x = *(const uint2*)(hist_of(p, kDigit) + b0);
+        lo += (int)x.x;
+        hi += (int)x.y;
+        if (STEP == 3 ? p < part : p == part) {
+          lo_here += (int)x.x;
+          hi_here += (int)x.y;
+        }
+      }
     }
+    ranks.rank(a, length);
     pick(hi, lo, left, s);
     const uint32_t bin = s.bin;
     prefix |= bin << shift_of(kDigit);
     left = s.left;
-    // how many of a part are above the bin
-    const auto over = [&](int p) {
-      const uint2 x = *(const uint2*)(hist_of(p, kDigit) + b0);
-      return (b0 + 1 > (int)bin ? (int)x.y : 0) + (b0 > (int)bin ? (int)x.x : 0);
-    };
+    // how many of those are above the bin
+    const int over = (b0 + 1 > (int)bin ? hi_here : 0) + (b0 > (int)bin ? lo_here : 0);
     const auto total = [&](int x) {
 #pragma unroll
       for (int i = 32; i >= 1; i >>= 1) x += __shfl_xor(x, i);
@@ -251,7 +271,7 @@ __global__ __launch_bounds__(kThreads) void kv_keep_part_kernel(KvKeepArgs a) {
       return x;
     };
     if constexpr (STEP < 3) {
-      const int mine = total(over(part));
+      const int mine = total(over);
       if (tid == 0) {
         work.above[(row * parts + part) * 2 + kDigit] = mine;
         if (part == 0) {
@@ -261,15 +281,12 @@ __global__ __launch_bounds__(kThreads) void kv_keep_part_kernel(KvKeepArgs a) {
       }
     } else {
       // where this part's tokens go: after those of the parts before it
-      int gt = 0, eq = 0;
-      for (int p = 0; p < part; ++p) gt += over(p);
-      for (int p = tid; p < part; p += kThreads) {
+      int gt = over;
+      for (int p = tid; p < part; p += kThreads)
         gt += work.above[(row * parts + p) * 2] + work.above[(row * parts + p) * 2 + 1];
-        eq += (int)hist_of(p, kDigit)[bin];
-      }
+      if (b0 == (int)bin || b0 + 1 == (int)bin) same = b0 == (int)bin ? lo_here : hi_here;
       gt = total(gt);
-      __syncthreads();
-      eq = total(eq);
+      const int eq = same;
       ranks.take(prefix, max(0, left - eq), out + gt + min(eq, left), waves);
       return;
     }
@@ -279,17 +296,23 @@ __global__ __launch_bounds__(kThreads) void kv_keep_part_kernel(KvKeepArgs a) {
   ranks.count(hist, STEP, prefix);
   __syncthreads();
   uint2* to = (uint2*)hist_of(part, STEP);
-  to[tid] = *(const uint2*)(hist + 2 * tid);
+  if (2 * tid < bins_of(STEP)) to[tid] = *(const uint2*)(hist + 2 * tid);
 }
 
 template <int STEP>
 hipError_t launch_step(const KvKeepArgs& a, hipStream_t s) {
-  kv_keep_part_kernel<STEP><<<dim3((unsigned)kv_keep_grid(a)), kThreads, 0, s>>>(a);
+  const dim3 grid((unsigned)kv_keep_grid(a));
+  switch (each_of(a)) {
+    case 8: kv_keep_part_kernel<STEP, 8><<<grid, kThreads, 0, s>>>(a); break;
+    case 16: kv_keep_part_kernel<STEP, 16><<<grid, kThreads, 0, s>>>(a); break;
+    case 32: kv_keep_part_kernel<STEP, 32><<<grid, kThreads, 0, s>>>(a); break;
+    default: kv_keep_part_kernel<STEP, 64><<<grid, kThreads, 0, s>>>(a);
+  }
   return hipGetLastError();
 }
 
-// Whether rows are split.  Whole / in parts: 8 rows of 32,768 slots 23 / 33 us, of
-// 65,536 48 / 33; 256 rows of 65,536 64 / 123.
+// Whether rows are split.  Whole / in parts: 8 rows of 32,768 slots 25 / 27 us, of
+// 65,536 51 / 31; 64 rows of 65,536 53 / 45, 256 of them 68 / 150.
 bool in_parts(const KvKeepArgs& a) {
   return a.slots > 65536 || (a.slots > 32768 && a.requests * a.heads <= 64);
 }
