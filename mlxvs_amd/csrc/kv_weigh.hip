@@ -23,7 +23,7 @@
 // values 122 us, 5.1 TB/s of keys, masses and their return (a copy: 4.95); chunks of
 // 1,500 tokens in 3 requests of up to 8,192, 32 heads on 8, 138 us, 836 TFLOP/s, and
 // a prompt of 4,001 tokens, 28 heads on 4, 86 us, 667 (16 prompts of up to 32,768
-// together 877).  Two workgroups on a CU take 28 ns a product and SIMD, as a large
+// together 875 to 891).  Two workgroups on a CU take 28 ns a product and SIMD, as a large
 // library product does (27, the card's power); the rest are some 4 us at a unit's
 // begin, until its keys and first rows are there, the end, where CUs run dry, masked
 // tiles, and 12 us of plan and joining.  Tried: 128 keys a wavefront and 128 rows a
