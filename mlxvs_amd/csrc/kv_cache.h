@@ -140,7 +140,8 @@ struct KvWeighArgs {
   float* mass;      // [requests][heads][slots]
   int64_t slots;
   // from kv_weigh_plan
-  bool prompts;  // else single tokens
+  bool prompts;      // some requests have many rows of queries
+  int64_t few_rows;  // those that have no more are taken like single tokens
   int tile;      // tokens that a workgroup takes at a time
   int64_t most_units, most_several, most_slots;  // shares, and partial sums of them
   int32_t* work;  // kv_weigh_workspace bytes

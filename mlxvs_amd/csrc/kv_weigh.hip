@@ -87,7 +87,7 @@ __device__ __forceinline__ float row_sum(float x) {
   return x;
 }
 
-// kSpan keys of a request and head a workgroup, 32 a wavefront at a time, the next
+// Requests of up to few_rows rows.  kSpan keys of a request and head a workgroup, 32 a wavefront at a time, the next
 // ones on their way; with more requests' keys than the spans hold it comes again.
 // The rows of up to 16 query heads stay in registers.
 template <int DP, bool BF16>
@@ -115,6 +115,7 @@ __global__ __launch_bounds__(256) void kv_weigh_few_kernel(KvWeighArgs a, int sp
   const int32_t* table = a.q.table + (int64_t)r * a.q.table_stride;
   float* mass = a.mass + ((int64_t)r * a.c.heads + h) * a.slots;
   const int64_t rows = (int64_t)sp.tokens * group;
+  if (rows > a.few_rows) return;
 
   const auto load_rows = [&](int64_t x0, Rows& y) {
     const int64_t x = x0 + col;
@@ -335,7 +336,8 @@ __global__ __launch_bounds__(kPlanThreads) void kv_weigh_plan_kernel(KvWeighArgs
     if (r < a.q.requests) {
       const Span sp = span_of(a, r);
       if (few) spans[r] = sp;
-      n = sp.last < 0 ? 0 : sp.last / kChunk + 1;
+      const bool mine = sp.last >= 0 && (int64_t)sp.tokens * a.q.group > a.few_rows;
+      n = mine ? sp.last / kChunk + 1 : 0;
     }
     n = running(n, all, waves);
     if (r < a.q.requests) {
@@ -808,13 +810,28 @@ int64_t chunks_of(const KvWeighArgs& a, int64_t chunk, int64_t most) {
   return std::max<int64_t>(1, (most + chunk - 1) / chunk);
 }
 
+// Where there are more tokens than requests, at least 16 requests are dealt by their
+// rows, those of up to 32 to the kernel of single tokens (a launch more).  All by the
+// kernel of prompts / dealt: 64 requests of up to 8,192 keys, group 4, with 2 tokens each
+// 217 / 151 us, with 8 214 / 193, with 12 215 / 227, 63 single tokens and a prompt of 512
+// 233 / 185; 3 and that 48 / 55.
+constexpr int kSomeRequests = 16, kFewRows = 32;
+
 constexpr int64_t kGrid = 2048;  // workgroups at most
+
+int64_t few_grid(const KvWeighArgs& a) {
+  return a.q.requests * a.c.heads * chunks_of(a, kSpan, a.longest);
+}
+int64_t prompts_grid(const KvWeighArgs& a) {
+  return std::min(a.most_units, std::max<int64_t>(1, kGrid / a.c.heads)) * a.c.heads;
+}
 
 template <int DP, bool BF16>
 void launch_dim(const KvWeighArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)kv_weigh_grid(a));
-  if (a.prompts) kv_weigh_kernel<DP, BF16><<<grid, 256, 0, s>>>(a);
-  else kv_weigh_few_kernel<DP, BF16><<<grid, 256, 0, s>>>(a, (int)chunks_of(a, kSpan, a.longest));
+  if (a.prompts) kv_weigh_kernel<DP, BF16><<<dim3((unsigned)prompts_grid(a)), 256, 0, s>>>(a);
+  if (a.few_rows > 0)
+    kv_weigh_few_kernel<DP, BF16>
+        <<<dim3((unsigned)few_grid(a)), 256, 0, s>>>(a, (int)chunks_of(a, kSpan, a.longest));
 }
 
 template <bool BF16>
@@ -830,6 +847,7 @@ void launch_type(const KvWeighArgs& a, hipStream_t s) {
 
 void kv_weigh_plan(KvWeighArgs& a) {
   a.prompts = a.q.tokens > a.q.requests && a.q.cols > 0 && a.q.group <= kRows;
+  a.few_rows = !a.prompts ? INT64_MAX : a.q.requests >= kSomeRequests ? kFewRows : 0;
   a.most_units = a.most_several = a.most_slots = 0;
   if (!a.prompts) return;
   a.tile = kRows / a.q.group;
@@ -847,8 +865,7 @@ int64_t kv_weigh_workspace(const KvWeighArgs& a) {
 }
 
 int64_t kv_weigh_grid(const KvWeighArgs& a) {
-  if (!a.prompts) return a.q.requests * a.c.heads * chunks_of(a, kSpan, a.longest);
-  return std::min(a.most_units, std::max<int64_t>(1, kGrid / a.c.heads)) * a.c.heads;
+  return std::max(a.few_rows > 0 ? few_grid(a) : 0, a.prompts ? prompts_grid(a) : 0);
 }
 
 hipError_t launch_kv_weigh(const KvWeighArgs& a, hipStream_t s) {

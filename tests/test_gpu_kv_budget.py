@@ -321,6 +321,17 @@ def test_weights_of_many_requests(engine, most):
     Step(engine, lengths, counts, heads=1, group=2, dim=16, seed=most).attend().check()
 
 
+@pytest.mark.parametrize("group", [1, 4, 33])
+def test_weights_of_requests_with_few_and_many_rows(engine, group):
+    # 20 requests, dealt to two kernels: 1 to 33 rows, prompts, none
+    counts = [1, 8, 9, 31, 32, 33, 0, 70, 1, 1, 2, 3, 4, 5, 6, 7, 8, 9, 0, 1]
+    lengths = [n + 13 * i for i, n in enumerate(counts)]
+    s = Step(engine, lengths, counts, heads=2, group=group, dim=48, seed=group).attend()
+    s.positions[s.starts[5]:s.starts[6]] = -1  # (one was not admitted)
+    s.positions[s.starts[2]:s.starts[3]] = -1
+    s.check(decay=0.5)
+
+
 @pytest.mark.parametrize("longest", [0, 1, 1_000])
 def test_weights_of_prompts_of_other_sizes_together(engine, longest):
     # units of many sizes, keys that few of the tokens see, masked tiles in between
