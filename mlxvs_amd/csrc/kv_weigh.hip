@@ -521,7 +521,7 @@ struct Weigh {
   }
 
   // The keys from k0 on of a table's row.  (Where there is none some key of the cache
-  // is read, whose sum is left out.)
+  // is read, whose sum is left out: a cache without pages does not come here.)
   __device__ __forceinline__ void keys(const int32_t* table, int k0, int upto) {
     const int d = a.c.dim, col = lane & 31, half = lane >> 5;
     int page[2];
@@ -846,7 +846,8 @@ void launch_type(const KvWeighArgs& a, hipStream_t s) {
 }  // namespace
 
 void kv_weigh_plan(KvWeighArgs& a) {
-  a.prompts = a.q.tokens > a.q.requests && a.q.cols > 0 && a.q.group <= kRows;
+  // (the kernel of prompts reads some key in place of an absent one: there has to be one)
+  a.prompts = a.q.tokens > a.q.requests && a.q.cols > 0 && a.q.group <= kRows && a.c.pages > 0;
   a.few_rows = !a.prompts ? INT64_MAX : a.q.requests >= kSomeRequests ? kFewRows : 0;
   a.most_units = a.most_several = a.most_slots = 0;
   if (!a.prompts) return;
