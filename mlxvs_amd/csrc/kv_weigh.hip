@@ -87,8 +87,9 @@ __device__ __forceinline__ float row_sum(float x) {
   return x;
 }
 
-// Requests of up to few_rows rows.  kSpan keys of a request and head a workgroup, 32 a wavefront at a time, the next
-// ones on their way; with more requests' keys than the spans hold it comes again.
+// Requests of up to few_rows rows.  kSpan keys of a request and head a workgroup, 32 a
+// wavefront at a time, the next ones on their way; with more keys than the `spans`
+// workgroups of a request and head hold it comes again.
 // The rows of up to 16 query heads stay in registers.
 template <int DP, bool BF16>
 __global__ __launch_bounds__(256) void kv_weigh_few_kernel(KvWeighArgs a, int spans) {
@@ -819,9 +820,20 @@ constexpr int kSomeRequests = 16, kFewRows = 32;
 
 constexpr int64_t kGrid = 2048;  // workgroups at most
 
-int64_t few_grid(const KvWeighArgs& a) {
-  return a.q.requests * a.c.heads * chunks_of(a, kSpan, a.longest);
+// Workgroups of single tokens for each request and head: no more than make kFewGrid, as a
+// table may be far wider than its requests are long; the rest of the keys is come to
+// later.  Without a limit / with it (8 kv heads of 4, 128 values, longest not told): 256
+// requests of up to 2,048 tokens in a table for 131,072 838 / 148 us (in one for 2,048
+// 136), 1,024 of 1,000 in one for 32,768 1,117 / 423, 8 of up to 8,192 in one for
+// 1,048,576 193 / 27; 256 of 4,096 395 / 399.  (65,536: 178, 460, 60, 394; 32,768: 156,
+// 439, 38, 395; 8,192: 148, 415, 22, 413.)
+constexpr int64_t kFewGrid = 16384;
+
+int64_t few_spans(const KvWeighArgs& a) {
+  const int64_t rows = std::max<int64_t>(1, a.q.requests * a.c.heads);
+  return std::min(chunks_of(a, kSpan, a.longest), std::max<int64_t>(1, kFewGrid / rows));
 }
+int64_t few_grid(const KvWeighArgs& a) { return a.q.requests * a.c.heads * few_spans(a); }
 int64_t prompts_grid(const KvWeighArgs& a) {
   return std::min(a.most_units, std::max<int64_t>(1, kGrid / a.c.heads)) * a.c.heads;
 }
@@ -831,7 +843,7 @@ void launch_dim(const KvWeighArgs& a, hipStream_t s) {
   if (a.prompts) kv_weigh_kernel<DP, BF16><<<dim3((unsigned)prompts_grid(a)), 256, 0, s>>>(a);
   if (a.few_rows > 0)
     kv_weigh_few_kernel<DP, BF16>
-        <<<dim3((unsigned)few_grid(a)), 256, 0, s>>>(a, (int)chunks_of(a, kSpan, a.longest));
+        <<<dim3((unsigned)few_grid(a)), 256, 0, s>>>(a, (int)few_spans(a));
 }
 
 template <bool BF16>

@@ -10,8 +10,57 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from test_gpu_kv import dev  # noqa: E402
+from test_gpu_kv_budget import Step  # noqa: E402
 
 pytestmark = pytest.mark.gpu
+
+
+def weights(s, mass, decay=1.0):
+    """float64 (mass, err) of a Step: kv_budget_oracle.weigh's sums and bounds in
+    products over all keys of a request, for many of them."""
+    keys, table = s.cache.keys, s.table.long()
+    pages, heads, page, d = keys.shape
+    out, err = mass.double(), torch.zeros(mass.shape, dtype=torch.float64, device="cuda")
+    starts, positions = s.starts.tolist(), s.positions.tolist()
+    most, group = table.shape[1] * page, s.q.shape[1] // heads
+    for r in range(len(table)):
+        a, b = starts[r], starts[r + 1]
+        if a == b or positions[a] < 0:
+            continue
+        first, n = positions[a], min(positions[b - 1] + 1, most)
+        p = torch.arange(n, device="cuda")
+        pid = table[r, p // page]
+        there = (pid >= 0) & (pid < pages)
+        k = keys[torch.where(there, pid, 0), :, p % page].double().permute(1, 2, 0).contiguous()
+        got, off, sees = (torch.zeros(heads, n, dtype=torch.float64, device="cuda") for _ in range(3))
+        step = max(1, (1 << 25) // (heads * group * n))
+        for t in range(a, b, step):
+            u = min(b, t + step)
+            x = s.q[t:u].double().unflatten(1, (heads, group)).transpose(0, 1).flatten(1, 2)
+            lse = s.lse[t:u].double().unflatten(1, (heads, group)).transpose(0, 1).flatten(1, 2)[..., None]
+            see = (s.positions[t:u, None] >= p).repeat_interleave(group, 0)
+            score = x @ k * s.scale
+            e = torch.where(see, torch.exp(score - lse), 0.0)
+            w = e * ((d + 4) * (x.abs() @ k.abs()) * s.scale + 4 * (score.abs() + lse.abs()) + 16)
+            got += e.sum(1)
+            off += torch.where(see, w, 0.0).sum(1)
+            sees += see.sum(0)
+        off = torch.where(there, off + sees * got, 0.0)
+        got = torch.where(there, got, 0.0)
+        before = torch.where(p < first, decay * out[r, :, :n], 0.0) if decay else torch.zeros_like(got)
+        out[r, :, :n] = before + got
+        err[r, :, :n] = off + 2 * before.abs() + 2 * got.abs()
+    return out, err
+
+
+def check_weights(s, decay=1.0, **how):
+    want, err = weights(s, s.mass, decay)
+    again = s.mass.clone()
+    s.cache.weigh(s.q, s.table, s.starts, s.positions, s.lse, s.mass, decay=decay, **how)
+    s.cache.weigh(s.q, s.table, s.starts, s.positions, s.lse, again, decay=decay, **how)
+    bad = ~((s.mass.double() - want).abs() <= err * 2.0 ** -24 + 1e-37)
+    assert not bad.any(), (bad.nonzero()[:5], s.mass[bad][:5], want[bad][:5])
+    assert torch.equal(s.mass, again)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
@@ -33,3 +82,17 @@ def test_weights_of_a_cache_without_pages(engine, counts, dtype):
             want[r, :, past[r]:past[r] + counts[r]] = 0
         c.weigh(q, table, starts, positions, lse, mass, decay=0.5)
         assert torch.equal(mass, want)
+
+
+@pytest.mark.parametrize("longest", [0, 100, 1_800])
+def test_weights_of_more_keys_than_a_call_has_workgroups_for(engine, longest):
+    # 70 x 64 rows of keys, 3 workgroups of 256 keys each; and one for each of 300 x 64
+    rng = np.random.default_rng(longest)
+    lengths = rng.integers(1, 1_800, 70)
+    lengths[[3, 69]] = 1_800, 769
+    s = Step(engine, lengths, [1] * 70, page=64, heads=64, group=1, dim=8, spare=30, seed=1).attend()
+    check_weights(s, decay=0.5, longest=longest)
+    lengths = rng.integers(0, 600, 300)
+    counts = np.minimum(lengths, rng.integers(0, 2, 300))
+    check_weights(Step(engine, lengths, counts, page=64, heads=64, group=2, dim=8, seed=2).attend(),
+                  longest=longest)

@@ -20,3 +20,27 @@ def test_a_cache_without_pages_has_no_prompts(engine, requests):
     assert weigh_workspace(engine, cache(), q) > 0
     assert weigh_workspace(engine, cache(pages=0, keys=None, values=None), q) == 0
     assert weigh_workspace(engine, cache(pages=0), q) == 0
+
+
+@pytest.mark.parametrize("requests,held", [(512, 1 << 20), (4_096, 1 << 17), (300_000, 1 << 20),
+                                           (2_000_000, 5 * 64)])
+def test_weights_of_single_tokens_in_wide_tables(engine, requests, held):
+    # what attention over the same cache serves, whatever the table has room for
+    q = queries(tokens=requests, requests=requests, columns=held // 64, table_stride=held // 64)
+    c = cache(heads=8, page_size=64)
+    lib = engine._L()
+    assert weigh_workspace(engine, c, q) == 0, lib.mlxvs_last_error()
+    assert weigh_workspace(engine, c, q, 1_000) == 0
+    assert lib.mlxvs_kv_attend_workspace(ctypes.byref(c), ctypes.byref(q), 0, 1_000) >= 0
+    # prompts beside them
+    q = queries(tokens=requests + 300, requests=requests, columns=5, table_stride=5)
+    assert weigh_workspace(engine, c, q) > 0
+
+
+def test_weights_of_too_many_requests(engine):
+    # a workgroup of 256 threads for each request and head: past 2^32
+    q = queries(tokens=2_200_000, requests=2_200_000)
+    assert weigh_workspace(engine, cache(heads=8), q) == -1
+    assert b"too many tokens" in engine._L().mlxvs_last_error()
+    assert weigh_workspace(engine, cache(heads=8), queries(tokens=0, requests=0)) == 0
+    assert weigh_workspace(engine, cache(heads=8), queries(tokens=9, requests=0)) >= 0
