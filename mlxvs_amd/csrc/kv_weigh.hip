@@ -828,10 +828,16 @@ constexpr int64_t kGrid = 2048;  // workgroups at most
 // 1,048,576 193 / 27; 256 of 4,096 395 / 399.  (65,536: 178, 460, 60, 394; 32,768: 156,
 // 439, 38, 395; 8,192: 148, 415, 22, 413.)
 constexpr int64_t kFewGrid = 16384;
+// Half as many beside prompts, where all may find nothing: 64 requests of up to 8,192
+// keys with 12 tokens each 228 / 224 us (without this launch 215), with 32 260 / 256
+// (248), with 2 151 / 153, 63 single tokens and a prompt of 512 185 / 185.  (4,096: 221,
+// 253, 157, 189.)
+constexpr int64_t kFewGridBeside = 8192;
 
 int64_t few_spans(const KvWeighArgs& a) {
   const int64_t rows = std::max<int64_t>(1, a.q.requests * a.c.heads);
-  return std::min(chunks_of(a, kSpan, a.longest), std::max<int64_t>(1, kFewGrid / rows));
+  const int64_t most = a.prompts ? kFewGridBeside : kFewGrid;
+  return std::min(chunks_of(a, kSpan, a.longest), std::max<int64_t>(1, most / rows));
 }
 int64_t few_grid(const KvWeighArgs& a) { return a.q.requests * a.c.heads * few_spans(a); }
 int64_t prompts_grid(const KvWeighArgs& a) {

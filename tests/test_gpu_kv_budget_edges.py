@@ -96,3 +96,11 @@ def test_weights_of_more_keys_than_a_call_has_workgroups_for(engine, longest):
     counts = np.minimum(lengths, rng.integers(0, 2, 300))
     check_weights(Step(engine, lengths, counts, page=64, heads=64, group=2, dim=8, seed=2).attend(),
                   longest=longest)
+
+
+def test_weights_of_few_tokens_beside_prompts_in_many_keys(engine):
+    # 20 x 64 rows, 6 workgroups of 256 keys each for the requests of up to 32 rows
+    lengths = [2_500, 1_537, 1, 40, 0, 1_900] + [300 + 7 * i for i in range(14)]
+    counts = [1, 32, 1, 40, 0, 33] + [i % 3 for i in range(14)]
+    check_weights(Step(engine, lengths, counts, page=64, heads=64, group=1, dim=8, spare=9,
+                       seed=3).attend(), decay=0.5)
