@@ -104,3 +104,20 @@ def test_weights_of_few_tokens_beside_prompts_in_many_keys(engine):
     counts = [1, 32, 1, 40, 0, 33] + [i % 3 for i in range(14)]
     check_weights(Step(engine, lengths, counts, page=64, heads=64, group=1, dim=8, spare=9,
                        seed=3).attend(), decay=0.5)
+
+
+@pytest.mark.parametrize("group,dim,dtype", [(1, 8, "bf16"), (3, 72, "f16"), (64, 16, "bf16")])
+def test_weights_of_a_prompt_among_idle_rows(engine, group, dim, dtype):
+    # a table with room for 8 million keys: the rows are idle, have a token each, or are
+    # few and many tokens', with fewer tokens than rows
+    n = 600
+    idle = [0] * (n - 1)
+    for lengths, counts in (([900] + idle, [n] + idle),
+                            ([300] + [20] * 500 + [0] * 99, [77] + [1] * 500 + [0] * 99),
+                            ([40] * 10 + [1_300] * 3 + idle[:-11], [2] * 10 + [34, 190, 1] + idle[:-11])):
+        s = Step(engine, lengths, counts, page=64, heads=2, group=group, dim=dim, dtype=dtype,
+                 spare=-(-8_192 // 64) - -(-max(lengths) // 64), seed=dim).attend()
+        assert sum(counts) <= len(lengths) and s.mass.numel() >= 8 << 20
+        check_weights(s, decay=0.5)
+        s.positions[:s.starts[1].item()] = -1  # (the first one was not admitted)
+        check_weights(s)
