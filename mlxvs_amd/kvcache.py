@@ -124,6 +124,12 @@ class _On:
             self.guard.__exit__(*a)
 
 
+# What the kernels have written is told to autograd, as by any operation in place: a
+# backward pass that saved what was there before is an error then, not wrong.  (Tensors;
+# a cheaper way to torch.autograd.graph.increment_version: 0.1 instead of 0.3 us)
+_written = getattr(torch._C, "_increment_version", torch.autograd.graph.increment_version)
+
+
 class _NoGradient(torch.autograd.Function):
     """Marks results as depending on inputs that want a gradient: asking for it is
     an error then, not a gradient that is silently missing."""
@@ -198,6 +204,7 @@ def kv_plan(past, new, table, free_pages, cursor, page_size, tokens, *, out=None
         _check(_L().mlxvs_kv_plan_device(pp, pn, requests, pt, stride, table.shape[1], pf,
                                          free_pages.numel(), pc, int(page_size), tokens, *ptrs,
                                          stream))
+    _written((table, *out))
     return out
 
 
@@ -342,6 +349,8 @@ class Rotary:
             _check(_L().mlxvs_kv_rotate_device(
                 ctypes.byref(self._c[q.dtype]), ctypes.byref(hq), hk and ctypes.byref(hk), tokens,
                 pp, pr, pe, 0 if evicted is None else evicted.numel(), float(eps), stream))
+        if out is not None:
+            _written((q_out,) if k is None else (q_out, k_out))
         if wanted:
             some = (q_out,) if k is None else (q_out, k_out)
             some = _NoGradient.apply(op, some, *(x for x in given if x is not None))
@@ -463,6 +472,7 @@ class PagedKVCache:
         with _On(self._device) as stream:
             _check(_L().mlxvs_kv_append_device(cache, pk, ks[0], ks[1], pv, vs[0], vs[1], ps,
                                                tokens, stream))
+        _written(self._held)
 
     def _queries(self, q, table, requests, positions, op: str):
         q, pq, st = self._rows(q, "q", op)
@@ -559,6 +569,7 @@ class PagedKVCache:
         longest = int(longest)
         with _On(self._device) as stream:
             work, size = self._workspace("mlxvs_kv_attend_workspace", q, qs, n, longest)
+            given = out
             if out is None:
                 out = q.new_empty((tokens, heads, dim))
             else:
@@ -574,6 +585,8 @@ class PagedKVCache:
                     cache, ctypes.byref(qs), pb, n, float(scale), longest, out.data_ptr(),
                     None if sums is None else sums.data_ptr(),
                     None if work is None else work.data_ptr(), size, stream))
+        if given is not None:
+            _written((given,))
         if wanted:
             results = _NoGradient.apply(op, (out, sums) if lse else (out,), q, keys, values)
             return results if lse else results[0]
@@ -589,6 +602,12 @@ class PagedKVCache:
                              f"{slots} slots.")
         return mass.data_ptr()
 
+    def _mass_to_write(self, mass, op: str, requests: int, slots: int):
+        at = self._mass(mass, op, requests, slots)
+        _need(not (mass.requires_grad and torch.is_grad_enabled()), op,
+              "mass is written: it takes no result that wants a gradient.")
+        return at
+
     def weigh(self, q, table, starts, positions, lse, mass, *, scale=None, decay=1.0,
               longest=0) -> None:
         """Add the attention that each key gets from the step's tokens to ``mass``
@@ -602,6 +621,8 @@ class PagedKVCache:
         needs no clearing before a new request gets it; what the others had is
         multiplied by ``decay`` (0: not read).  Masses past a request's last token,
         and of requests without tokens, stay as they are.  The same bits every time.
+        What is added are values: no gradient goes back to ``q`` and ``lse``, and
+        ``mass`` must not want one.
         """
         op = "kv_weigh"
         cache = self._cache(op)
@@ -613,7 +634,7 @@ class PagedKVCache:
                 and lse.is_contiguous()):
             raise ValueError(f"[mlxvs::{op}] lse must be a contiguous float32 [tokens, q_heads] "
                              f"tensor on {self._device}.")
-        pm = self._mass(mass, op, qs.requests, qs.columns * self.page_size)
+        pm = self._mass_to_write(mass, op, qs.requests, qs.columns * self.page_size)
         if scale is None:
             scale = 1.0 / math.sqrt(dim)
         longest = int(longest)
@@ -622,6 +643,7 @@ class PagedKVCache:
             _check(_L().mlxvs_kv_weigh_device(
                 cache, ctypes.byref(qs), ps, lse.data_ptr(), float(scale), float(decay), longest,
                 pm, mass.shape[2], None if work is None else work.data_ptr(), size, stream))
+        _written((mass,))
 
     def keep(self, mass, lengths, n, *, first=1, recent=1, above=None):
         """The ``n`` tokens of each request and kv head that a budget leaves: int32
@@ -684,7 +706,8 @@ class PagedKVCache:
         pf = _ints(free_pages, "free_pages", op, device)
         pc = _ints(cursor, "cursor", op, device, size=1)
         slots = columns * self.page_size if mass is None else mass.shape[-1]
-        pm = None if mass is None else self._mass(mass, op, requests, columns * self.page_size)
+        pm = None if mass is None \
+            else self._mass_to_write(mass, op, requests, columns * self.page_size)
         n = kept.shape[2]
         with _On(device) as stream:
             if out is None:
@@ -699,4 +722,6 @@ class PagedKVCache:
                 cache, pt, stride, columns, requests, pl, kept.data_ptr(), n, pf,
                 free_pages.numel(), pc, pm, slots, po, pn,
                 None if work is None else work.data_ptr(), need, stream))
+        _written((*self._held, free_pages, *out) if mass is None
+                 else (*self._held, free_pages, mass, *out))
         return out

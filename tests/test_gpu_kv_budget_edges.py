@@ -121,3 +121,82 @@ def test_weights_of_a_prompt_among_idle_rows(engine, group, dim, dtype):
         check_weights(s, decay=0.5)
         s.positions[:s.starts[1].item()] = -1  # (the first one was not admitted)
         check_weights(s)
+
+
+def step_in_place(engine, requests=2, heads=2, dim=64, page=16):
+    """Everything that a step with a budget writes, by name, and the step."""
+    i = dict(dtype=torch.int32, device="cuda")
+    c = engine.PagedKVCache.empty(20, heads, page, dim)
+    t = dict(keys=c.keys, values=c.values, summaries=c.summaries, scales=c.scales,
+             table=torch.full((requests, 6), -1, **i), free=torch.arange(20, **i),
+             mass=torch.zeros(requests, heads, 6 * page, device="cuda"),
+             q=torch.randn(90, 2 * heads, dim, device="cuda").bfloat16(),
+             k=torch.randn(90, heads, dim, device="cuda").bfloat16(),
+             out=torch.zeros(90, 2 * heads, dim, device="cuda").bfloat16(),
+             lengths=torch.zeros(requests, **i), cursor=torch.zeros(1, **i))
+    zero = torch.zeros(requests, **i)
+
+    def step():
+        plan = engine.kv_plan(zero, torch.tensor([60, 30], **i), t["table"], t["free"],
+                              torch.zeros(1, **i), page, 90)
+        engine.Rotary(dim).rotate(t["q"], t["k"], plan.positions, out=(t["q"], t["k"]))
+        c.append(t["k"], t["k"], plan.slots)
+        _, lse = c.attend(t["q"], t["table"], plan.requests, plan.positions, lse=True, out=t["out"])
+        c.weigh(t["q"], t["table"], plan.starts, plan.positions, lse, t["mass"])
+        kept = c.keep(t["mass"], plan.lengths, 20)
+        c.compact(t["table"], plan.lengths, kept, t["free"], plan.cursor, mass=t["mass"],
+                  out=engine.KvCompact(t["lengths"], t["cursor"]))
+
+    return t, step
+
+
+def test_what_is_written_in_place_is_told_to_autograd(engine):
+    t, step = step_in_place(engine)
+    before = {name: x._version for name, x in t.items()}
+    step()
+    assert all(x._version > before[name] for name, x in t.items()), before
+    assert t["lengths"].tolist() == [20, 20]
+    # a backward pass that needs what was there before is an error
+    for name in ("keys", "mass", "q", "k", "out"):
+        w = torch.ones((), device="cuda", requires_grad=True)
+        y = (w * t[name]).sum()
+        step()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    # what is only read is not
+    t, step = step_in_place(engine)
+    q, pos = t["q"], torch.arange(90, dtype=torch.int32, device="cuda")
+    at = q._version, pos._version
+    engine.Rotary(64).rotate(q, t["k"], pos)
+    assert (q._version, pos._version) == at
+
+
+def test_steps_in_place_in_inference_mode(engine):
+    with torch.inference_mode():
+        t, step = step_in_place(engine)
+        step()
+    step()  # (tensors made there have no versions)
+    assert t["lengths"].tolist() == [20, 20]
+
+
+def test_masses_that_want_a_gradient(engine):
+    s = Step(engine, [20, 30], [2, 3]).attend()
+    args = s.q, s.table, s.starts, s.positions, s.lse
+    want = s.mass.clone()
+    s.cache.weigh(*args, want)
+    lengths, kept = dev([20, 30], torch.int32), s.cache.keep(want, dev([20, 30], torch.int32), 9)
+    free, cursor = dev(np.arange(9), torch.int32), dev([5], torch.int32)
+    mass = s.mass.clone().requires_grad_()
+    for m in (mass, mass * 1):
+        with pytest.raises(ValueError, match="gradient"):
+            s.cache.weigh(*args, m)
+        with pytest.raises(ValueError, match="gradient"):
+            s.cache.compact(s.table, lengths, kept, free, cursor, mass=m)
+        assert torch.equal(m, s.mass)
+    with torch.no_grad():
+        s.cache.weigh(*args, mass)
+    assert torch.equal(mass, want)
+    # values are added: no gradient goes back to queries
+    again = s.mass.clone()
+    s.cache.weigh(s.q.requires_grad_(), *args[1:], again)
+    assert torch.equal(again, want) and not again.requires_grad
