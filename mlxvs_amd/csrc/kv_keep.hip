@@ -223,7 +223,7 @@ __global__ __launch_bounds__(kThreads) void kv_keep_part_kernel(KvKeepArgs a) {
     if (STEP == 3 && part == 0) none(a, out);
     return;
   }
-  const int some = (length + kPart - 1) / kPart;  // parts that hold tokens
+  const int some = (length - 1) / kPart + 1;  // parts that hold tokens
   if (part >= some) return;
   const Work work = work_of(a);
   Ranks<R> ranks(a.mass + row * a.slots, part * kPart, length);

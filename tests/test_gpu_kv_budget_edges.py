@@ -200,3 +200,17 @@ def test_masses_that_want_a_gradient(engine):
     again = s.mass.clone()
     s.cache.weigh(s.q.requires_grad_(), *args[1:], again)
     assert torch.equal(again, want) and not again.requires_grad
+
+
+def test_budget_of_a_row_of_nearly_two_to_the_31_slots(engine):
+    # its last part ends at 2^31: ties go to the lowest, marks lie in the first and last parts
+    slots = 2 ** 31 - 1
+    c = engine.PagedKVCache.empty(1, 1, 16, 16)
+    mass = torch.zeros(1, 1, slots, device="cuda")
+    marks = [70_000, 2 ** 30 + 1, slots - 65_535, slots - 3]
+    mass[0, 0, torch.tensor(marks, device="cuda")] = dev([1.0, 3.0, 2.0, 4.0], torch.float32)
+    for length, want in ((slots, [0, 1, 2, *marks, slots - 1]),
+                         (slots - 2, [0, 1, 2, *marks]),
+                         (slots - 65_536, [0, 1, 2, 3, 4, *marks[:2], slots - 65_537])):
+        kept = c.keep(mass, dev([length], torch.int32), len(want), first=1, recent=1)
+        assert kept.flatten().tolist() == want, length
