@@ -214,3 +214,65 @@ def test_budget_of_a_row_of_nearly_two_to_the_31_slots(engine):
                          (slots - 65_536, [0, 1, 2, 3, 4, *marks[:2], slots - 65_537])):
         kept = c.keep(mass, dev([length], torch.int32), len(want), first=1, recent=1)
         assert kept.flatten().tolist() == want, length
+
+
+def check_keep(engine, mass, lengths, n, first, recent):
+    """kept against a stable sort of float64 masses, for long rows."""
+    c = engine.PagedKVCache.empty(1, mass.shape[1], 16, 16)
+    got = c.keep(dev(mass), dev(lengths, torch.int32), n, first=first, recent=recent).cpu().numpy()
+    for r, length in enumerate(lengths):
+        for h in range(mass.shape[1]):
+            if length <= n:
+                assert (got[r, h] == -1).all()
+                continue
+            # (lexsort's last key counts most: NaN at the end, then the greatest first, then
+            # the lowest position)
+            x = mass[r, h, first:length - recent].astype(np.float64)
+            best = np.lexsort((np.arange(len(x)), -np.nan_to_num(x), np.isnan(x)))
+            want = np.concatenate([np.arange(first), first + np.sort(best[:n - first - recent]),
+                                   np.arange(length - recent, length)])
+            assert np.array_equal(got[r, h], want), (r, h)
+
+
+@pytest.mark.parametrize("slots,part", [(262_144, 8_192), (262_145, 16_384), (524_288, 16_384),
+                                        (524_289, 32_768), (1_048_577, 65_536), (2_500_000, 65_536)])
+def test_budgets_of_rows_in_parts_of_any_size(engine, slots, part):
+    # ties of the cut over several parts' borders, rows that end within a part or at its
+    # border, parts without tokens
+    rng = np.random.default_rng(slots)
+    mass = rng.integers(0, 40, (4, 1, slots)).astype(np.float32)
+    mass[1] = rng.lognormal(0, 2, (1, slots))
+    mass[2, :, part - 300:part + 300] = 100.0
+    mass[3, :, ::5], mass[3, :, 1::7] = math.nan, -math.inf
+    lengths = [slots, slots - 1, 3 * part, part + 1]
+    for n in (1, 500, part, part + 7, slots // 2, slots - 2):
+        check_keep(engine, mass, lengths, n, min(4, n // 2), min(128, n // 3))
+
+
+def test_weights_of_more_shares_than_workgroups(engine):
+    # 64 heads leave 32 workgroups to each, which take several shares one after another
+    s = Step(engine, [2_100, 3_000, 1_500, 700, 4_500], [2_100, 1_000, 1, 700, 300], page=64, heads=64,
+             group=1, dim=8, seed=1).attend()
+    check_weights(s, decay=0.5)
+    s = Step(engine, [1_300, 1_024, 2_000], [1_200, 1_024, 7], page=128, heads=128, group=2, dim=16,
+             dtype="f16", seed=2).attend()
+    check_weights(s)
+
+
+@pytest.mark.parametrize("dim", [16, 192])
+def test_weights_of_more_chunks_than_the_plan_takes_at_a_time(engine, dim):
+    # 14 requests over the same pages: 1,024 chunks of 256 keys and more, some in several
+    # shares, the last ones in a pass of their own
+    long, page = 20_480, 256
+    s = Step(engine, [long], [0], page=page, heads=1, group=2, dim=dim, seed=dim)
+    s.cache.keys[:long // page] = torch.randn(long // page, 1, page, dim, device="cuda").bfloat16()
+    lengths = np.array([long - 250 * i for i in range(14)])
+    counts = np.array([3, 1, 900, 40, 5, 300, 64, 1, 2, 33, 1, 450, 7, 1_200])
+    s.table = torch.randperm(long // page, device="cuda").int().expand(14, -1).contiguous()
+    s.starts = dev(np.concatenate([[0], np.cumsum(counts)]), torch.int32)
+    s.positions = dev(np.concatenate([np.arange(n - m, n) for n, m in zip(lengths, counts)]), torch.int32)
+    s.requests = dev(np.repeat(np.arange(14), counts), torch.int32)
+    s.q = torch.randn(counts.sum(), 2, dim, device="cuda").bfloat16()
+    s.mass = torch.rand(14, 1, long, device="cuda")
+    assert sum(-(-n // 256) for n in lengths) > 1_024
+    check_weights(s.attend(), decay=0.5)
