@@ -324,20 +324,18 @@ class Rotary:
         It has no gradient: the result of inputs that want one can be used, but not
         differentiated, and not written into ``out``."""
         op = "kv_rotate"
-        wanted = (q.requires_grad or (k is not None and k.requires_grad)
-                  or (q_norm is not None and q_norm.requires_grad)
-                  or (k_norm is not None and k_norm.requires_grad)) and torch.is_grad_enabled()
-        _need(out is None or not wanted, op, "out takes no result that wants a gradient.")
         _need(out is None or (isinstance(out, (tuple, list)) and len(out) == 2), op,
               "out must be (q, k).")
         _need(k is not None or k_norm is None, op, "k_norm needs k.")
         to_q, to_k = (None, None) if out is None else out
-        given = (q, k, q_norm, k_norm)
+        given = [x for x in (q, k, q_norm, k_norm) if x is not None]
         # (what is copied for the kernel has to live until the call is made)
         q, q_norm, q_out, hq = self._heads(q, "q", q_norm, to_q, None)
         k_out, hk = None, None
         if k is not None:
             k, k_norm, k_out, hk = self._heads(k, "k", k_norm, to_k, q)
+        wanted = torch.is_grad_enabled() and any(x.requires_grad for x in given)
+        _need(out is None or not wanted, op, "out takes no result that wants a gradient.")
         device, tokens = q.device, q.shape[0]
         pp = _ints(positions, "positions", op, device, size=tokens)
         pr = pe = None
@@ -353,7 +351,7 @@ class Rotary:
             _written((q_out,) if k is None else (q_out, k_out))
         if wanted:
             some = (q_out,) if k is None else (q_out, k_out)
-            some = _NoGradient.apply(op, some, *(x for x in given if x is not None))
+            some = _NoGradient.apply(op, some, *given)
             return some[0], (None if k is None else some[1])
         return q_out, k_out
 
@@ -705,9 +703,10 @@ class PagedKVCache:
                              f"n] tensor on {device}.")
         pf = _ints(free_pages, "free_pages", op, device)
         pc = _ints(cursor, "cursor", op, device, size=1)
-        slots = columns * self.page_size if mass is None else mass.shape[-1]
-        pm = None if mass is None \
-            else self._mass_to_write(mass, op, requests, columns * self.page_size)
+        slots, pm = columns * self.page_size, None
+        if mass is not None:
+            pm = self._mass_to_write(mass, op, requests, slots)
+            slots = mass.shape[2]
         n = kept.shape[2]
         with _On(device) as stream:
             if out is None:

@@ -276,3 +276,39 @@ def test_weights_of_more_chunks_than_the_plan_takes_at_a_time(engine, dim):
     s.mass = torch.rand(14, 1, long, device="cuda")
     assert sum(-(-n // 256) for n in lengths) > 1_024
     check_weights(s.attend(), decay=0.5)
+
+
+@pytest.mark.parametrize("bad", [None, 3, [1.0, 2.0], np.zeros((3, 4, 64), np.float32)])
+def test_what_is_no_tensor_is_refused(engine, bad):
+    rot, s = engine.Rotary(64), Step(engine, [20, 30], [2, 3]).attend()
+    q, pos = s.q[:, :, :64], s.positions
+    lengths, kept = dev([20, 30], torch.int32), torch.full((2, 2, 4), -1, dtype=torch.int32, device="cuda")
+    free, cursor = dev(np.arange(9), torch.int32), dev([5], torch.int32)
+    calls = [lambda: rot.rotate(bad, q, pos), lambda: rot.rotate(q, q, bad),
+             lambda: rot.rotate(q, q, pos, evicted=pos, requests=bad),
+             lambda: s.cache.weigh(bad, s.table, s.starts, pos, s.lse, s.mass),
+             lambda: s.cache.weigh(q, bad, s.starts, pos, s.lse, s.mass),
+             lambda: s.cache.weigh(q, s.table, bad, pos, s.lse, s.mass),
+             lambda: s.cache.weigh(q, s.table, s.starts, bad, s.lse, s.mass),
+             lambda: s.cache.weigh(q, s.table, s.starts, pos, bad, s.mass),
+             lambda: s.cache.weigh(q, s.table, s.starts, pos, s.lse, bad),
+             lambda: s.cache.keep(bad, lengths, 4), lambda: s.cache.keep(s.mass, bad, 4),
+             lambda: s.cache.compact(bad, lengths, kept, free, cursor),
+             lambda: s.cache.compact(s.table, bad, kept, free, cursor),
+             lambda: s.cache.compact(s.table, lengths, bad, free, cursor),
+             lambda: s.cache.compact(s.table, lengths, kept, bad, cursor),
+             lambda: s.cache.compact(s.table, lengths, kept, free, bad)]
+    if bad is not None:
+        calls += [lambda: rot.rotate(q, bad, pos), lambda: rot.rotate(q, q, pos, q_norm=bad),
+                  lambda: rot.rotate(q, q, pos, k_norm=bad), lambda: rot.rotate(q, q, pos, out=bad),
+                  lambda: rot.rotate(q, q, pos, out=(q, bad)),
+                  lambda: rot.rotate(q, q, pos, evicted=bad, requests=pos),
+                  lambda: s.cache.compact(s.table, lengths, kept, free, cursor, mass=bad),
+                  lambda: s.cache.compact(s.table, lengths, kept, free, cursor, out=bad)]
+    for call in calls:
+        with pytest.raises(ValueError, match="mlxvs::kv_"):
+            call()
+    # (of no, one or two axes)
+    for mass in (s.mass[0, 0, 0], s.mass[0, 0], s.mass[0]):
+        with pytest.raises(ValueError, match="mass must be"):
+            s.cache.compact(s.table, lengths, kept, free, cursor, mass=mass)
