@@ -884,10 +884,13 @@ void launch_type(const KvWeighArgs& a, hipStream_t s) {
 
 void kv_weigh_plan(KvWeighArgs& a) {
   // (the kernel of prompts reads some key in place of an absent one: there has to be one)
+  // (a single token is few, whatever its rows are: 256 of 33 and 64 query heads over 32,768
+  // keys of one kv head 565 and 685 us, by the kernel of prompts 899 and 902)
+  const int64_t few = idle_rows(a) ? std::max(kFewRows, a.q.group) : kFewRows;
   a.prompts = a.q.tokens > 0 && a.q.cols > 0 && a.q.group <= kRows && a.c.pages > 0 &&
-              (!idle_rows(a) || (room_of(a) >= kDealt && a.q.tokens * a.q.group > kFewRows));
+              (!idle_rows(a) || (room_of(a) >= kDealt && a.q.tokens * a.q.group > few));
   a.few_rows = !a.prompts                                      ? INT64_MAX
-               : idle_rows(a) || a.q.requests >= kSomeRequests ? kFewRows
+               : idle_rows(a) || a.q.requests >= kSomeRequests ? few
                                                                : 0;
   a.most_units = a.most_several = a.most_slots = 0;
   if (!a.prompts) return;

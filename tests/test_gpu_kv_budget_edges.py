@@ -106,7 +106,8 @@ def test_weights_of_few_tokens_beside_prompts_in_many_keys(engine):
                        seed=3).attend(), decay=0.5)
 
 
-@pytest.mark.parametrize("group,dim,dtype", [(1, 8, "bf16"), (3, 72, "f16"), (64, 16, "bf16")])
+@pytest.mark.parametrize("group,dim,dtype", [(1, 8, "bf16"), (3, 72, "f16"), (40, 24, "f16"),
+                                             (64, 16, "bf16")])
 def test_weights_of_a_prompt_among_idle_rows(engine, group, dim, dtype):
     # a table with room for 8 million keys: the rows are idle, have a token each, or are
     # few and many tokens', with fewer tokens than rows

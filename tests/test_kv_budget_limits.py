@@ -67,3 +67,12 @@ def test_which_requests_are_dealt(engine, tokens, requests, held, longest, dealt
     # (64 rows of Q are a tile: more query heads than that are always taken one by one)
     q = queries(tokens=tokens, requests=requests, columns=columns, table_stride=columns, q_heads=8 * 65)
     assert weigh_workspace(engine, cache(heads=8, page_size=64), q, longest) == 0
+
+
+@pytest.mark.parametrize("group", [33, 64])
+def test_single_tokens_of_many_query_heads_are_not_dealt(engine, group):
+    # one token's rows are no prompt: there has to be another one
+    c = cache(heads=8, page_size=64)
+    for tokens, dealt in ((1, False), (2, True)):
+        q = queries(tokens=tokens, requests=512, columns=64, table_stride=64, q_heads=8 * group)
+        assert (weigh_workspace(engine, c, q) > 0) == dealt
