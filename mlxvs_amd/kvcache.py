@@ -328,13 +328,16 @@ class Rotary:
               "out must be (q, k).")
         _need(k is not None or k_norm is None, op, "k_norm needs k.")
         to_q, to_k = (None, None) if out is None else out
-        given = [x for x in (q, k, q_norm, k_norm) if x is not None]
+        given = q, k, q_norm, k_norm
         # (what is copied for the kernel has to live until the call is made)
         q, q_norm, q_out, hq = self._heads(q, "q", q_norm, to_q, None)
         k_out, hk = None, None
         if k is not None:
             k, k_norm, k_out, hk = self._heads(k, "k", k_norm, to_k, q)
-        wanted = torch.is_grad_enabled() and any(x.requires_grad for x in given)
+        # (copies want a gradient where what they are copies of does)
+        wanted = (q.requires_grad or (k is not None and k.requires_grad)
+                  or (q_norm is not None and q_norm.requires_grad)
+                  or (k_norm is not None and k_norm.requires_grad)) and torch.is_grad_enabled()
         _need(out is None or not wanted, op, "out takes no result that wants a gradient.")
         device, tokens = q.device, q.shape[0]
         pp = _ints(positions, "positions", op, device, size=tokens)
@@ -351,7 +354,7 @@ class Rotary:
             _written((q_out,) if k is None else (q_out, k_out))
         if wanted:
             some = (q_out,) if k is None else (q_out, k_out)
-            some = _NoGradient.apply(op, some, *given)
+            some = _NoGradient.apply(op, some, *(x for x in given if x is not None))
             return some[0], (None if k is None else some[1])
         return q_out, k_out
 
