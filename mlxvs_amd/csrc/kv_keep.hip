@@ -8,14 +8,18 @@
 // bits, a histogram of 2,048 bins in LDS each; then the tokens above it are taken,
 // and the first of those that equal it.
 //
-// A row of up to 65,536 slots is a workgroup's and read once: its ranks stay in
-// registers.  A longer one is split into parts of 8,192 or more, a workgroup each, with a
-// launch for every histogram and one for the list: the parts' histograms are summed
-// by whoever needs them, so that nothing is counted by atomics in memory.
+// A row of up to 32,768 slots is a workgroup's and read once: its ranks stay in
+// registers; so is one of up to 65,536 where there are more than 64 rows.  Others are
+// split into parts of 8,192 or more, a workgroup each, with a launch for every histogram
+// and one for the list: the parts' histograms are summed by whoever needs them, so that
+// nothing is counted by atomics in memory.  (With 64 ranks a lane, rows of more than
+// 32,768 slots and parts of rows of more than 1,048,576, not all stay in registers: 33 to
+// 76 of 128 are spilled.)
 //
 // Chains of small steps, far from the bytes' 2 us: 256 rows of 16,384 slots 15 us (53
-// if all masses are equal, whose counts meet in one place; 20 if half of them are),
-// 8 rows of 262,144 32 us in four launches.
+// if all masses are equal, whose counts meet in one place; 20 if half of them are), 8
+// rows of 262,144 33 us (53) in four launches of 5, 11, 10 and 10: each workgroup of the
+// later ones sums all parts' histograms.
 #include <hip/hip_runtime.h>
 
 #include "kv_cache.h"

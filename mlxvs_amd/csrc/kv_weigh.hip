@@ -829,10 +829,11 @@ int64_t room_of(const KvWeighArgs& a) {
 
 // No more tokens than rows of the table are a token each, or a prompt among idle rows,
 // which the device finds: where single tokens could take 0.4 ms or more, and one request
-// have rows enough, requests are dealt here, too.  By the kernel of single tokens / dealt (8 kv heads of 4, 128 values):
-// a prompt of 200 tokens over 4,096 keys in a table of 512 rows 179 / 42 us (29 in one of
-// its own), with a token in each other one, 1,000 keys, 377 / 231; 512 tokens over 16,384
-// 1,134 / 106 (93).  No prompt, 256 rows of 4,096 keys 397 / 408, 1,024 1,612 / 1,623.
+// have rows enough, requests are dealt here, too.  By the kernel of single tokens / dealt
+// (8 kv heads of 4, 128 values): a prompt of 200 tokens over 4,096 keys in a table of 512
+// rows 179 / 41 us (29 in one of its own), with a token in each other one, 1,000 keys, 377
+// / 233; 512 tokens over 16,384 1,134 / 105 (93).  No prompt, 256 rows of 4,096 keys 397 /
+// 408, 1,024 1,612 / 1,622.
 constexpr int64_t kDealt = 8 << 20;
 
 bool idle_rows(const KvWeighArgs& a) { return a.q.tokens <= a.q.requests; }

@@ -232,10 +232,13 @@ class Rotary:
             make 32 or more kept, a straight line between them; rotated values
             times 0.1 ln(factor) + 1).
         frequencies, magnitude: radians a position of each pair and the factor
-            of rotated values, instead of all that.
+            of rotated values, instead of all that: models whose ramp has other
+            bounds, runs over the pairs instead of their turns or has no factor
+            come with these.
 
-    An angle is the exact product of the position and a 64-bit frequency, at
-    every position.  ``frequencies`` and ``magnitude`` can be read back.
+    A position times a frequency (64 bits, of a turn) is exact modulo a turn, at
+    every position; the angle is then rounded to 2^-26 of a turn.  ``frequencies``
+    and ``magnitude`` can be read back.
     """
 
     _LAYOUTS = {"halves": 0, "pairs": 1}
@@ -313,8 +316,8 @@ class Rotary:
         """Queries [tokens, q_heads, dim] and keys [tokens, kv_heads, dim] (any
         token and head strides; k may be None), normed and turned.
 
-        ``positions`` int32 [tokens] (KvPlan's); a token without one (-1) is not
-        turned.  ``evicted`` int32 [requests]: how many tokens a request's cache has
+        ``positions`` int32 [tokens] (KvPlan's); a token without one (-1) is
+        turned by nothing, as at position 0.  ``evicted`` int32 [requests]: how many tokens a request's cache has
         lost, added to its tokens' positions; ``requests`` int32 [tokens] (KvPlan's)
         says whose they are.  ``q_norm`` / ``k_norm`` [dim]: weights of a norm of
         each head before that, x / sqrt(mean(x^2) + eps) x weight, over the whole
@@ -621,7 +624,8 @@ class PagedKVCache:
         of its kv head.  The step's own keys start from zero, so a row of ``mass``
         needs no clearing before a new request gets it; what the others had is
         multiplied by ``decay`` (0: not read).  Masses past a request's last token,
-        and of requests without tokens, stay as they are.  The same bits every time.
+        and of requests without tokens, stay as they are; so do those of a step that
+        is left out, whose keys have what their places held before.  The same bits every time.
         What is added are values: no gradient goes back to ``q`` and ``lse``, and
         ``mass`` must not want one.
         """
