@@ -828,36 +828,48 @@ int64_t room_of(const KvWeighArgs& a) {
 }
 
 // No more tokens than rows of the table are a token each, or a prompt among idle rows,
-// which the device finds: where single tokens could take 0.4 ms or more, and one request
-// have rows enough, requests are dealt here, too.  By the kernel of single tokens / dealt
-// (8 kv heads of 4, 128 values): a prompt of 200 tokens over 4,096 keys in a table of 512
-// rows 179 / 41 us (29 in one of its own), with a token in each other one, 1,000 keys, 377
-// / 233; 512 tokens over 16,384 1,134 / 105 (93).  No prompt, 256 rows of 4,096 keys 397 /
-// 408, 1,024 1,612 / 1,622.
-constexpr int64_t kDealt = 8 << 20;
+// which the device finds: where single tokens could take 0.4 ms or more, requests are
+// dealt here, too.  By the kernel of single tokens / dealt (8 kv heads of 4, 128 values):
+// a prompt of 200 tokens over 4,096 keys in a table of 512 rows 179 / 41 us (29 in one of
+// its own), with a token in each other one, 1,000 keys, 377 / 233; 512 tokens over 16,384
+// 1,134 / 105 (93).  No prompt, 256 rows of 4,096 keys 397 / 408, 1,024 1,612 / 1,622.
+// More requests than these take the plan too long, 2 us for each turn: 131,072 of 64 keys
+// 4,287 / 4,527, 16,384 538 / 576, 2,048 of 512 398 / 415.
+constexpr int64_t kDealt = 8 << 20, kDealtRequests = kPlanSpans;
 
 bool idle_rows(const KvWeighArgs& a) { return a.q.tokens <= a.q.requests; }
 
-// Workgroups of single tokens for each request and head: no more than make kFewGrid where
-// there is room for as many keys as above, as a table may be far wider than its requests
-// are long; the rest of the keys is come to later.  Without a limit / with it, longest not
-// told: 256 requests of up to 2,048 tokens in a table for 131,072 838 / 158 us (in one for
-// 2,048 137), 1,024 of 1,000 in one for 32,768 1,117 / 432, 8 of up to 8,192 in one for
-// 1,048,576 193 / 27.  (32,768: 165, 450, 38, and 1,024 of 4,096 1,649 instead of 1,623.
-// A prompt that is not dealt would have to do with a few: 512 tokens over 16,384 keys in a
-// table of 512 rows 3,986 us instead of 1,134.)
+// Rows of queries that are few; of idle rows' tables a single token's, whatever they are
+// (256 of 33 and 64 query heads over 32,768 keys of one kv head 565 and 685 us, by the
+// kernel of prompts 899 and 902).
+int64_t few_rows_of(const KvWeighArgs& a) {
+  return idle_rows(a) ? std::max(kFewRows, a.q.group) : kFewRows;
+}
+
+// Whether a request may have more.
+bool some_many(const KvWeighArgs& a) { return a.q.tokens * a.q.group > few_rows_of(a); }
+
+// Workgroups of single tokens for each request and head: no more than make kFewGrid, as a
+// table may be far wider than its requests are long; the rest of the keys is come to
+// later.  Without a limit / with it, longest not told: 256 requests of up to 2,048 tokens
+// in a table for 131,072 838 / 158 us (in one for 2,048 137), 1,024 of 1,000 in one for
+// 32,768 1,117 / 432, 8 of up to 8,192 in one for 1,048,576 193 / 27.  (32,768: 165, 450,
+// 38, and 1,024 of 4,096 1,649 instead of 1,623.)
 constexpr int64_t kFewGrid = 16384;
+// Many where there may be a prompt that is not dealt, which would have to do with a few:
+// 512 tokens over 16,384 keys in a table of 512 rows 1,134 / 3,986 us.
+constexpr int64_t kFewGridAlone = 1 << 20;
 // Fewer beside prompts, where all may find nothing: 64 requests of up to 8,192 keys with
 // 12 tokens each 228 / 224 us (without this launch 215), with 32 260 / 256 (248), with 2
 // 151 / 153, 63 single tokens and a prompt of 512 185 / 185.  (4,096: 221, 253, 157, 189.)
 constexpr int64_t kFewGridBeside = 8192;
 
 int64_t few_spans(const KvWeighArgs& a) {
-  const int64_t spans = chunks_of(a, kSpan, a.longest);
+  const int64_t most = a.prompts && !idle_rows(a)      ? kFewGridBeside
+                       : a.prompts || !some_many(a) ? kFewGrid
+                                                    : kFewGridAlone;
   const int64_t rows = std::max<int64_t>(1, a.q.requests * a.c.heads);
-  const bool beside = a.prompts && !idle_rows(a);
-  if (!beside && room_of(a) < kDealt) return spans;
-  return std::min(spans, std::max<int64_t>(1, (beside ? kFewGridBeside : kFewGrid) / rows));
+  return std::min(chunks_of(a, kSpan, a.longest), std::max<int64_t>(1, most / rows));
 }
 int64_t few_grid(const KvWeighArgs& a) { return a.q.requests * a.c.heads * few_spans(a); }
 int64_t prompts_grid(const KvWeighArgs& a) {
@@ -885,13 +897,10 @@ void launch_type(const KvWeighArgs& a, hipStream_t s) {
 
 void kv_weigh_plan(KvWeighArgs& a) {
   // (the kernel of prompts reads some key in place of an absent one: there has to be one)
-  // (a single token is few, whatever its rows are: 256 of 33 and 64 query heads over 32,768
-  // keys of one kv head 565 and 685 us, by the kernel of prompts 899 and 902)
-  const int64_t few = idle_rows(a) ? std::max(kFewRows, a.q.group) : kFewRows;
   a.prompts = a.q.tokens > 0 && a.q.cols > 0 && a.q.group <= kRows && a.c.pages > 0 &&
-              (!idle_rows(a) || (room_of(a) >= kDealt && a.q.tokens * a.q.group > few));
+              (!idle_rows(a) || (some_many(a) && a.q.requests <= kDealtRequests && room_of(a) >= kDealt));
   a.few_rows = !a.prompts                                      ? INT64_MAX
-               : idle_rows(a) || a.q.requests >= kSomeRequests ? few
+               : idle_rows(a) || a.q.requests >= kSomeRequests ? few_rows_of(a)
                                                                : 0;
   a.most_units = a.most_several = a.most_slots = 0;
   if (!a.prompts) return;

@@ -56,6 +56,7 @@ def test_weights_of_too_many_requests(engine):
     (32, 32, 1 << 20, 0, False), (33, 33, 1 << 20, 0, True),  # (up to 32 rows are few)
     (200, 512, 4_096, 0, True),       # fewer tokens than rows
     (200, 512, 2_047, 2_000, False),
+    (1_024, 1_024, 4_096, 0, True), (1_025, 1_025, 4_096, 0, False),  # (the plan takes too long)
     (3, 2, 64, 0, True), (2, 2, 64, 0, False), (0, 512, 1 << 17, 0, False)])
 def test_which_requests_are_dealt(engine, tokens, requests, held, longest, dealt):
     # the device finds the prompts among them (and needs a workspace) where single tokens
