@@ -740,8 +740,8 @@ typedef struct {
  * rounded once.  A position times the given turns is exact modulo a turn, at every
  * position; the angle is then rounded to 2^-26 of a turn.  (What a frequency was rounded
  * by as a double grows with the position: for one just below a radian it is 2^-25.6 of a
- * turn at position 2^31.)  out may be x with its strides; otherwise what is written may overlap neither
- * what is read nor the other results.
+ * turn at position 2^31.)  out may be x with its strides; otherwise what is written may
+ * overlap neither what is read nor the other results.
  */
 MLXVS_C_API int mlxvs_kv_rotate_device(const mlxvs_kv_rotary* rotary, const mlxvs_kv_heads* q,
                                        const mlxvs_kv_heads* k, int64_t tokens,
@@ -763,10 +763,10 @@ MLXVS_C_API int mlxvs_kv_rotate_device(const mlxvs_kv_rotary* rotary, const mlxv
  * first being the first token's position: the step's own keys start from zero.  The
  * others, and requests without tokens (or with position -1), stay as they are: the
  * keys of a step that is left out have what their places held before.  A key of an
- * absent page gets nothing, and one with values that are not finite may get NaN.  decay in [0, 1]; with 0 masses are not read.
- * A page that several rows share has a mass in each.  longest guides how work is
- * split, as in mlxvs_kv_attend_device.  The same bits every time.  workspace:
- * mlxvs_kv_weigh_workspace bytes (may be 0).
+ * absent page gets nothing, and one with values that are not finite may get NaN.
+ * decay in [0, 1]; with 0 masses are not read.  A page that several rows share has a
+ * mass in each.  longest guides how work is split, as in mlxvs_kv_attend_device.  The
+ * same bits every time.  workspace: mlxvs_kv_weigh_workspace bytes (may be 0).
  */
 MLXVS_C_API int mlxvs_kv_weigh_device(const mlxvs_kv_cache* cache,
                                       const mlxvs_kv_queries* queries, const int32_t* starts,

@@ -865,7 +865,7 @@ constexpr int64_t kFewGridAlone = 1 << 20;
 constexpr int64_t kFewGridBeside = 8192;
 
 int64_t few_spans(const KvWeighArgs& a) {
-  const int64_t most = a.prompts && !idle_rows(a)      ? kFewGridBeside
+  const int64_t most = a.prompts && !idle_rows(a)   ? kFewGridBeside
                        : a.prompts || !some_many(a) ? kFewGrid
                                                     : kFewGridAlone;
   const int64_t rows = std::max<int64_t>(1, a.q.requests * a.c.heads);

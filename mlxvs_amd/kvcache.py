@@ -317,9 +317,9 @@ class Rotary:
         token and head strides; k may be None), normed and turned.
 
         ``positions`` int32 [tokens] (KvPlan's); a token without one (-1) is
-        turned by nothing, as at position 0.  ``evicted`` int32 [requests]: how many tokens a request's cache has
-        lost, added to its tokens' positions; ``requests`` int32 [tokens] (KvPlan's)
-        says whose they are.  ``q_norm`` / ``k_norm`` [dim]: weights of a norm of
+        turned by nothing, as at position 0.  ``evicted`` int32 [requests]: how many
+        tokens a request's cache has lost, added to its tokens' positions;
+        ``requests`` int32 [tokens] (KvPlan's) says whose they are.  ``q_norm`` / ``k_norm`` [dim]: weights of a norm of
         each head before that, x / sqrt(mean(x^2) + eps) x weight, over the whole
         head.  ``out``: (q, k) tensors to write into, which may be q and k
         themselves.  Returns (q, k).
@@ -625,9 +625,9 @@ class PagedKVCache:
         needs no clearing before a new request gets it; what the others had is
         multiplied by ``decay`` (0: not read).  Masses past a request's last token,
         and of requests without tokens, stay as they are; so do those of a step that
-        is left out, whose keys have what their places held before.  The same bits every time.
-        What is added are values: no gradient goes back to ``q`` and ``lse``, and
-        ``mass`` must not want one.
+        is left out, whose keys have what their places held before.  The same bits
+        every time.  What is added are values: no gradient goes back to ``q`` and
+        ``lse``, and ``mass`` must not want one.
         """
         op = "kv_weigh"
         cache = self._cache(op)
